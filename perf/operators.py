@@ -179,7 +179,7 @@ def _grown(x, mask, scale, codes):
     """The scale after tokens x [page, token, head, dim] (those in mask [page, token]) have come: [page, head]."""
     amax = torch.where(mask[:, :, None, None], x.abs(), torch.zeros_like(x)).amax(dim=(1, 3)).float()
     limit = torch.full_like(amax, LIMIT[codes])
-    s = torch.where(amax > 0, torch.clamp(amax / limit, min=2.0 ** -126), amax)
+    s = torch.where(amax > 0, torch.clamp(amax / limit, min=2.0 ** -100), amax)
     return torch.maximum(scale, s)
 
 
