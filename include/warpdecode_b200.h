@@ -32,11 +32,13 @@ extern "C" {
 
 /* ggml tensor type ids (src/gguf.hpp:26-44). */
 #define WD_TYPE_F32 0
+#define WD_TYPE_F16 1
 #define WD_TYPE_Q4_0 2
 #define WD_TYPE_Q8_0 8
 #define WD_TYPE_IQ4_NL 20
 #define WD_TYPE_IQ3_S 21
 #define WD_TYPE_IQ2_S 22
+#define WD_TYPE_BF16 30
 
 typedef struct wd_engine wd_engine;
 
@@ -357,6 +359,85 @@ int wd_dense_pack_q8_0_device(const void *w_ggml_dev, int rows, int cols, void *
 int wd_embed_q8_0(const void *table_ggml_dev, int rows, int cols, const int *token_dev, float *out_dev, void *stream);
 int wd_head_argmax_q8_0(void *packed_dev, int rows, int cols, const float *x_dev, float *logits_dev, int *token_dev,
                         int *nonfinite_dev, void *stream);
+
+/* ---- key/value cache in 8 bits and attention over it ------------------------------------------- */
+/* For programs that put their own layers together (embedding row, dense products, MoE block, head) or whose host engine has mixers of
+ * its own beside the MoE blocks. The reference keeps F16 keys and values, one contiguous run of positions (the plain decoder's
+ * attention, src/warodecode.cu:1211-2150); here a cache is pages of tokens shared by sequences.
+ *
+ * Codes are 8 bits (int8, or e4m3), with one F32 scale for each page of tokens, kv head, and keys or values:
+ *   number = code * scale;   scale = max(largest finite magnitude / (127 or 448), 2^-100), 0 where every number is 0.
+ * Tokens that come into a page that holds some already keep its scale s unless they need a larger one, s'; then the codes c that are
+ * there become round(c s / s'). All roundings of codes are exact: the nearest code of the real quotient, ties to even. An infinity
+ * becomes the largest code, a NaN zero, and either raises bit 32 of the status.
+ *
+ * Which sequence holds which pages is kept on the host (calls fail there, with nothing changed) and sent to the device in the
+ * stream's order: calls of one cache are made from one host thread at a time and on one stream, or on streams that the caller orders.
+ * stream: a cudaStream_t of the cache's device, NULL = its default stream. wd_kv_append, wd_kv_attend and wd_kv_read can be captured;
+ * the others cannot (they are refused), but may come between replays: a replayed append or attend works on the step that is current
+ * then, with the launches of the captured one (any step is answered rightly; the captured rows should be about as many).
+ *
+ * Rows: [rows][heads][head_dim] of F32, F16 or BF16 (WD_TYPE_*); a stride is the elements from one row to the next, 0 = rows lie
+ * one behind the other, so that the parts of a fused q/k/v row can be used where they are. Sums, maxima and scores are F32; F32 rows
+ * are answered to about 2^-20 of the values' size, F16 and BF16 rows to their own rounding. */
+#define WD_KV_INT8 0
+#define WD_KV_E4M3 1
+typedef struct {
+    int32_t n_layers;
+    int32_t n_heads;        /* query heads: a multiple of n_kv_heads */
+    int32_t n_kv_heads;
+    int32_t head_dim;       /* 32, 64, 96, 128 or 256 */
+    int32_t page_tokens;    /* 16, 32, 64 or 128 */
+    int32_t n_pages;        /* for all sequences; a page holds its tokens in every layer */
+    int32_t max_seqs;       /* sequences 0 .. max_seqs - 1, at most 1024 */
+    int32_t max_context;    /* tokens of a sequence */
+    int32_t codes;          /* WD_KV_INT8 or WD_KV_E4M3 */
+    int32_t device;         /* -1: the host's part alone, without a GPU (plans, tests): appends, attention and reads are refused */
+} wd_kv_config;
+typedef struct wd_kv_cache wd_kv_cache;
+int wd_kv_create(const wd_kv_config *cfg, wd_kv_cache **out);
+void wd_kv_destroy(wd_kv_cache *c);
+/* Begins a step: sequence seqs[i] gets room for counts[i] more tokens (0: none; a sequence at most once). The rows of the step are those
+ * tokens, sequence by sequence. Pages come from the free ones, and a last page that other sequences hold too is copied first.
+ * WD_E_NOMEM, with nothing changed, where there are not enough pages. A step lasts until the next one, or until wd_kv_truncate,
+ * wd_kv_free or wd_kv_keep ends it. */
+int wd_kv_begin(wd_kv_cache *c, int n, const int *seqs, const int *counts, void *stream);
+/* Keys and values of the step's rows into a layer. The same rows again leave the cache as it is. */
+int wd_kv_append(wd_kv_cache *c, int layer, const void *k_dev, const void *v_dev, int type, int64_t k_stride, int64_t v_stride, void *stream);
+/* out = softmax(scale q k) v of the step's rows, each against the tokens up to its own (which must have been appended), or the last
+ * `window` of them (0 = all). Row i of a sequence's n rows is the token n - 1 - i before its last. out may be q. */
+int wd_kv_attend(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, int type, float scale, int window, int64_t q_stride,
+                 int64_t out_stride, void *stream);
+/* Tokens firsts[i] .. firsts[i] + counts[i] - 1 of the sequences as numbers, one behind the other: [rows][n_kv_heads][head_dim], for
+ * layer -1 [n_layers][rows][n_kv_heads][head_dim]. Either output may be null. */
+int wd_kv_read(wd_kv_cache *c, int layer, int n, const int *seqs, const int *firsts, const int *counts, void *k_dev, void *v_dev, int type, void *stream);
+/* Sequences dsts (empty ones) become what src is, on the same pages; a page is copied when one of its holders comes to write into it. */
+int wd_kv_fork(wd_kv_cache *c, int src, int n, const int *dsts, void *stream);
+/* Of the tokens from `first` on only first + index[0], first + index[1], ... stay (index goes up) and move together: the accepted path
+ * of a tree of drafts, or what an eviction leaves. A page takes the largest scale among the pages that its tokens come from, and codes
+ * of smaller ones are rounded anew. Positions inside keys (a rotary embedding) are the caller's. */
+int wd_kv_keep(wd_kv_cache *c, int seq, int first, int n, const int *index, void *stream);
+/* The first `length` tokens stay (a rejected draft); pages behind them become free. wd_kv_free: no token stays. */
+int wd_kv_truncate(wd_kv_cache *c, int seq, int length, void *stream);
+int wd_kv_free(wd_kv_cache *c, int n, const int *seqs, void *stream);
+/* Tokens of a sequence; pages nobody holds; a sequence's pages (returns how many, writes at most cap). Negative: an error code. */
+int wd_kv_length(const wd_kv_cache *c, int seq);
+int wd_kv_free_pages(const wd_kv_cache *c);
+int wd_kv_pages(const wd_kv_cache *c, int seq, int *pages, int cap);
+/* Waits for the device, returns its status word and clears it: 0, or 32 where a NaN or an infinity was appended. */
+int wd_kv_status(wd_kv_cache *c, int *status);
+
+/* ---- scoring of tokens ----------------------------------------------------------------------- */
+/* From logits [rows][vocab] (F32, F16 or BF16; `stride` elements from row to row, 0 = vocab), as wd_head_argmax_q8_0 writes them, the
+ * natural logarithms of probabilities:
+ *   logprob_dev[r] (nullable, with tokens_dev)  of the token tokens_dev[r]; NaN where that is no token of the vocabulary
+ *   entropy_dev[r] (nullable)                   - sum p log p
+ *   top_ids_dev, top_logprobs_dev [r][n_top]    the n_top (0 to 32) likeliest tokens, ties to the lowest id; -1 and -inf behind the
+ *                                               last token that has a probability
+ * A logit of -inf is a token that cannot come. A row with a NaN or +inf, or with nothing but -inf, has no distribution: NaN, and ids -1.
+ * Runs on the device of `logits_dev`, without a workspace. */
+int wd_token_logprobs(const void *logits_dev, int type, int rows, int vocab, int64_t stride, const int *tokens_dev, float *logprob_dev,
+                      float *entropy_dev, int n_top, int *top_ids_dev, float *top_logprobs_dev, void *stream);
 
 /* Has no counterpart in the reference. y = W x for one IQ3_S matrix like wd_matvec_host, for callers
  * that must not allocate device memory (HBM already handed to the expert pool, a latency-critical

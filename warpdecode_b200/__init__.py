@@ -18,8 +18,14 @@ SOURCES = [os.path.join(HERE, "csrc", f) for f in
            ("wd_engine.cu", "wd_aux_kernels.cuh", "wd_moe_kernel.cuh", "wd_moe_kernel_phases.inc", "wd_moe_fast.cuh", "wd_moe_batch.cuh", "wd_dense_decoder.cuh", "wd_dense_decoder.inc", "wd_dense_token.cuh", "wd_dense_prefill.cuh", "wd_dense_prompt_tc.cuh",
             "wd_plain_moe.cuh", "wd_plain_wide.cuh", "wd_plain_moe.inc", "wd_blocks.cuh", "wd_router.cuh",
             "wd_formats.cuh", "wd_device.cuh", "wd_dense.cuh", "wd_gguf.inc",
-            "wd_grids.h")] + [os.path.join(ROOT, "include", "warpdecode_b200.h")]
+            "wd_grids.h", "wd_host.h", "wd_kv.cu", "wd_kv_layout.cuh", "wd_kv_kernels.cuh", "wd_kv_attend.cuh", "wd_score.cu")] + [
+               os.path.join(ROOT, "include", "warpdecode_b200.h")]
+UNITS = {"wd_engine": [s for s in SOURCES if not os.path.basename(s).startswith(("wd_kv", "wd_score"))],        # translation units, and what they include
+         "wd_kv": [s for s in SOURCES if os.path.basename(s).startswith(("wd_kv", "wd_device", "wd_host", "warpdecode"))],
+         "wd_score": [s for s in SOURCES if os.path.basename(s).startswith(("wd_score", "wd_device", "wd_host", "warpdecode"))]}
 
+TYPE_F16, TYPE_BF16 = 1, 30
+KV_INT8, KV_E4M3 = 0, 1
 TYPE_F32, TYPE_Q4_0, TYPE_Q8_0, TYPE_IQ4_NL, TYPE_IQ3_S, TYPE_IQ2_S = 0, 2, 8, 20, 21, 22
 TAPS = dict(logits=0, ids=1, weights=2, act=3, expert_out=4, routed=5, shared=6, shared_gate=7, shared_act=8)
 
@@ -34,12 +40,27 @@ def build(force=False, verbose=False):
         if os.path.getmtime(LIB_PATH) >= newest:
             return LIB_PATH
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-    cmd = [nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-o", LIB_PATH, SOURCES[0]]
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    objects = os.path.join(HERE, "build")
+    os.makedirs(objects, exist_ok=True)
+    jobs, out = [], ""
+    for unit, files in UNITS.items():           # side by side; a unit is compiled again when one of its files is newer
+        obj = os.path.join(objects, unit + ".o")
+        if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(f) for f in files):
+            continue
+        cmd = [nvcc] + [f for f in NVCC_FLAGS if f != "-shared"] + (["-Xptxas", "-v"] if verbose else []) + ["-c", "-o", obj, os.path.join(HERE, "csrc", unit + ".cu")]
+        jobs.append((obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    for obj, job in jobs:
+        text, _ = job.communicate()
+        out += text
+        if job.returncode != 0 and os.path.exists(obj):
+            os.remove(obj)
+    if any(job.returncode for _, job in jobs):
+        raise RuntimeError("nvcc failed:\n" + out)
+    r = subprocess.run([nvcc] + NVCC_FLAGS + ["-o", LIB_PATH] + [os.path.join(objects, unit + ".o") for unit in UNITS], capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("nvcc failed:\n" + r.stdout + r.stderr)
     if verbose:
-        print(r.stderr)
+        print(out)
     return LIB_PATH
 
 
@@ -56,6 +77,11 @@ class DenseConfig(C.Structure):
     _fields_ = [("hidden", C.c_int32), ("n_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32),
                 ("ffn", C.c_int32), ("vocab", C.c_int32), ("n_layers", C.c_int32), ("max_ctx", C.c_int32),
                 ("rms_eps", C.c_float), ("rope_theta", C.c_float), ("device", C.c_int32)]
+
+
+class KvConfig(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_layers", "n_heads", "n_kv_heads", "head_dim", "page_tokens", "n_pages", "max_seqs", "max_context",
+                                         "codes", "device")]
 
 
 _lib = None
@@ -142,6 +168,23 @@ def lib():
         L.wd_dense_pack_q8_0_device.argtypes = [vp, i, i, C.POINTER(vp), vp]
         L.wd_head_argmax_q8_0.argtypes = [vp, i, i, vp, vp, vp, vp, vp]
         L.wd_embed_q8_0.argtypes = [vp, i, i, vp, vp, vp]
+        i64 = C.c_int64
+        L.wd_kv_create.argtypes = [C.POINTER(KvConfig), C.POINTER(vp)]
+        L.wd_kv_destroy.argtypes = [vp]
+        L.wd_kv_destroy.restype = None
+        L.wd_kv_begin.argtypes = [vp, i, vp, vp, vp]
+        L.wd_kv_append.argtypes = [vp, i, vp, vp, i, i64, i64, vp]
+        L.wd_kv_attend.argtypes = [vp, i, vp, vp, i, C.c_float, i, i64, i64, vp]
+        L.wd_kv_read.argtypes = [vp, i, i, vp, vp, vp, vp, vp, i, vp]
+        L.wd_kv_fork.argtypes = [vp, i, i, vp, vp]
+        L.wd_kv_keep.argtypes = [vp, i, i, i, vp, vp]
+        L.wd_kv_truncate.argtypes = [vp, i, i, vp]
+        L.wd_kv_free.argtypes = [vp, i, vp, vp]
+        L.wd_kv_length.argtypes = [vp, i]
+        L.wd_kv_free_pages.argtypes = [vp]
+        L.wd_kv_pages.argtypes = [vp, i, vp, i]
+        L.wd_kv_status.argtypes = [vp, C.POINTER(i)]
+        L.wd_token_logprobs.argtypes = [vp, i, i, i, i64, vp, vp, vp, i, vp, vp, vp]
         L.wd_gguf_open.argtypes = [C.c_char_p, C.POINTER(vp)]
         L.wd_gguf_close.argtypes = [vp]
         L.wd_gguf_close.restype = None
@@ -552,6 +595,105 @@ class DenseDecoder:
             self.close()
         except Exception:
             pass
+
+
+def _ints(values):
+    return np.ascontiguousarray(values, np.int32)
+
+
+class KvCache:
+    """Keys and values in 8 bits, in pages that sequences share, and attention over them (wd_kv_*). device=-1: the host's part alone.
+
+    A step: begin(seqs, counts), then append and attend for every layer. Pointers are device addresses of rows [rows][heads][head_dim]
+    of F32, F16 or BF16; a stride is in elements, 0 = rows lie one behind the other."""
+
+    def __init__(self, n_layers, n_heads, n_kv_heads, head_dim, n_pages, max_seqs, max_context, page_tokens=64, codes=KV_INT8, device=0):
+        self.cfg = KvConfig(n_layers, n_heads, n_kv_heads, head_dim, page_tokens, n_pages, max_seqs, max_context, codes, device)
+        self.h = C.c_void_p()
+        _check(lib().wd_kv_create(C.byref(self.cfg), C.byref(self.h)))
+
+    def begin(self, seqs, counts, stream=None):
+        """Room for counts[i] more tokens of sequence seqs[i]; these tokens are the rows of the step."""
+        s, n = _ints(seqs), _ints(counts)
+        if s.ndim != 1 or s.shape != n.shape:
+            raise ValueError("one count for each sequence")
+        _check(lib().wd_kv_begin(self.h, s.size, _ptr(s), _ptr(n), stream))
+
+    def append(self, layer, k_ptr, v_ptr, type=TYPE_F32, k_stride=0, v_stride=0, stream=None):
+        rc = lib().wd_kv_append(self.h, layer, k_ptr, v_ptr, type, k_stride, v_stride, stream)
+        if rc:
+            _check(rc)
+
+    def attend(self, layer, q_ptr, out_ptr, type=TYPE_F32, scale=None, window=0, q_stride=0, out_stride=0, stream=None):
+        """out = softmax(scale q k) v of the step's rows (scale: 1 / sqrt(head_dim) by default)."""
+        rc = lib().wd_kv_attend(self.h, layer, q_ptr, out_ptr, type, self.cfg.head_dim ** -0.5 if scale is None else scale, window, q_stride, out_stride, stream)
+        if rc:
+            _check(rc)
+
+    def read(self, layer, seqs, firsts, counts, k_ptr, v_ptr, type=TYPE_F32, stream=None):
+        """Tokens of sequences as numbers; layer -1: of every layer, one behind the other."""
+        s, f, n = _ints(seqs), _ints(firsts), _ints(counts)
+        if s.ndim != 1 or not s.shape == f.shape == n.shape:
+            raise ValueError("one first token and one count for each sequence")
+        _check(lib().wd_kv_read(self.h, layer, s.size, _ptr(s), _ptr(f), _ptr(n), k_ptr, v_ptr, type, stream))
+
+    def fork(self, src, dsts, stream=None):
+        d = _ints(dsts)
+        _check(lib().wd_kv_fork(self.h, src, d.size, _ptr(d), stream))
+
+    def keep(self, seq, first, index, stream=None):
+        """Of the tokens from `first` on those at `index` (relative to it, going up) stay and move together."""
+        x = _ints(index)
+        _check(lib().wd_kv_keep(self.h, seq, first, x.size, _ptr(x), stream))
+
+    def truncate(self, seq, length, stream=None):
+        _check(lib().wd_kv_truncate(self.h, seq, length, stream))
+
+    def free(self, seqs, stream=None):
+        s = _ints(seqs)
+        _check(lib().wd_kv_free(self.h, s.size, _ptr(s), stream))
+
+    def length(self, seq):
+        n = lib().wd_kv_length(self.h, seq)
+        _check(0 if n >= 0 else n)
+        return n
+
+    def free_pages(self):
+        n = lib().wd_kv_free_pages(self.h)
+        _check(0 if n >= 0 else n)
+        return n
+
+    def pages(self, seq):
+        n = lib().wd_kv_pages(self.h, seq, None, 0)
+        _check(0 if n >= 0 else n)
+        a = np.zeros(n, np.int32)
+        lib().wd_kv_pages(self.h, seq, _ptr(a), n)
+        return a
+
+    def status(self):
+        """Waits for the device; 0, or 32 where a NaN or an infinity was appended since the last call."""
+        st = C.c_int()
+        _check(lib().wd_kv_status(self.h, C.byref(st)))
+        return st.value
+
+    def close(self):
+        if self.h:
+            lib().wd_kv_destroy(self.h)
+            self.h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def token_logprobs(logits_ptr, rows, vocab, tokens_ptr=None, logprob_ptr=None, entropy_ptr=None, n_top=0, top_ids_ptr=None, top_logprobs_ptr=None,
+                   type=TYPE_F32, stride=0, stream=None):
+    """Log probabilities of given tokens, the entropy and the likeliest alternatives of rows of logits, on device buffers (wd_token_logprobs)."""
+    rc = lib().wd_token_logprobs(logits_ptr, type, rows, vocab, stride, tokens_ptr, logprob_ptr, entropy_ptr, n_top, top_ids_ptr, top_logprobs_ptr, stream)
+    if rc:
+        _check(rc)
 
 
 def measure_tile_decoder(nsb=8, warps=16, unroll=1, device=0):

@@ -80,7 +80,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
 // while), or 64 more polls once another wait of this launch has failed, so that a broken launch ends quickly. On
 // timeout raises kErrCopyTimeout, leaves the barrier's shared-memory address in err[2] (first failure only, for
 // diagnosis) and returns false; the caller carries on with whatever is in shared memory so that the kernel terminates.
-__device__ __noinline__ bool mbar_wait_slow(uint64_t *bar, uint32_t parity, unsigned *err) {
+static __device__ __noinline__ bool mbar_wait_slow(uint64_t *bar, uint32_t parity, unsigned *err) {
     const unsigned long long t0 = global_timer_ns();
 #pragma unroll 1
     for (unsigned i = 0;; ++i) {
@@ -136,12 +136,12 @@ typedef unsigned long long tagged_t;
 // over NVLink), or some other wait of this launch already failed (then the remaining waits end after
 // 1024 polls, so that a broken launch still terminates quickly). Raises kErrBarrierTimeout. `t0` is
 // the caller's loop-local start time, 0 before the loop.
-__device__ __noinline__ bool wait_expired_slow(unsigned it, unsigned long long &t0, unsigned *err);
+static __device__ __noinline__ bool wait_expired_slow(unsigned it, unsigned long long &t0, unsigned *err);
 __device__ __forceinline__ bool wait_expired(unsigned it, unsigned long long &t0, unsigned *err) {
     if ((it & 0x3ffu) != 0x3ffu) return false;
     return wait_expired_slow(it, t0, err);
 }
-__device__ __noinline__ bool wait_expired_slow(unsigned it, unsigned long long &t0, unsigned *err) {
+static __device__ __noinline__ bool wait_expired_slow(unsigned it, unsigned long long &t0, unsigned *err) {
     const unsigned long long now = global_timer_ns();
     if (t0 == 0ull) t0 = now;
     if (now - t0 > kWaitLimitNs || it >= 0xfffffc00u ||
@@ -161,7 +161,7 @@ __device__ __forceinline__ unsigned tag_behind(tagged_t w, uint32_t tag) {
 __device__ __forceinline__ unsigned tag_ahead(tagged_t w, uint32_t tag) {
     return static_cast<int32_t>(static_cast<uint32_t>(w >> 32) - tag) > 0;
 }
-__device__ __noinline__ void report_overrun_slow(unsigned *err) { atomicOr(err, kErrOverrun); }
+static __device__ __noinline__ void report_overrun_slow(unsigned *err) { atomicOr(err, kErrOverrun); }
 __device__ __forceinline__ void report_overrun(unsigned over, unsigned *err) {
     if (over) report_overrun_slow(err);
 }
@@ -297,7 +297,7 @@ __device__ __forceinline__ float hsum8_lanes(float v) {
 // round to the same float unless a midpoint between two floats lies within those units, which the 29 bits that the conversion drops show (64
 // units are allowed for): then, and outside 2^-100 .. 2^100 (zero, infinity and NaN among them), the expression is evaluated as it stands.
 __device__ __forceinline__ float inv_sqrt_as_written(double z) { return __double2float_rn(__ddiv_rn(1.0, __dsqrt_rn(z))); }
-__device__ __noinline__ float inv_sqrt_rare(double z) { return inv_sqrt_as_written(z); }       // out of the way of the code that runs
+static __device__ __noinline__ float inv_sqrt_rare(double z) { return inv_sqrt_as_written(z); }       // out of the way of the code that runs
 __device__ __forceinline__ bool rounds_alike(double v) { return (static_cast<unsigned>(__double2loint(v)) & 0x1fffffffu) - (0x10000000u - 64u) > 128u; }
 __device__ __forceinline__ float inv_sqrt_to_float(double z) {
     const float zf = __double2float_rn(z);

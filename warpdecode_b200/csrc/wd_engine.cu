@@ -30,6 +30,7 @@
 #include "wd_plain_moe.cuh"
 #include "wd_plain_wide.cuh"
 #include "wd_grids.h"
+#include "wd_host.h"
 
 namespace {
 
@@ -955,6 +956,8 @@ int check_device_status(wd_engine *e) {
 
 #define WD_TILED_ONLY(e)                                                                                              \
     if ((e) && (e)->plain) return fail(WD_E_INVALID, "not available on an engine that runs the plain-layout path (wd_engine_create)")
+
+int wd_host::set_error(int code, const std::string &msg) { return fail(code, msg); }
 
 extern "C" {
 

@@ -1,0 +1,139 @@
+// The 8-bit key/value cache: how a page lies in memory, how numbers become codes and codes numbers.
+//
+// pool    [layer][page][kv head][K: page_tokens D bytes | V: page_tokens D bytes]
+// scales  [layer][page][kv head][2]  (F32; keys, values)
+// book    int32 words: the step's header and entries, then the page table [max_seqs][max_pages]
+//
+// K and V are sub-blocks of 16 tokens, 16 D bytes each, laid out as the A operands of a matrix instruction of 16 x 8 x 16 want them: a lane
+// (g = lane / 4, t = lane % 4) reads 16 bytes, a warp 512 bytes in a row.
+//   K   rows are tokens:  [D / CW][16 tokens][CW], CW = 64 elements (32 where head_dim is no multiple of 64)
+//   V   rows are elements of the head, the contraction runs over tokens: [D / 32][g][t][i][b] is element 8 i + g of the 32, token
+//       2 t + (b & 1) + 8 (b >> 1)
+// An int8 code c is held as the byte c + 128 (an f16 is made of it with one byte permutation and one subtraction), an e4m3 code as it is.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "wd_device.cuh"
+
+namespace wd {
+
+constexpr int kKvSub = 16;              // tokens of a sub-block
+constexpr int kKvStepWords = 8;         // words of a step's entry: sequence, first row, rows, length with the step's tokens, first page item
+constexpr int kKvHead = 8;              // words in front of the entries: sequences, rows, page items
+constexpr float kKvLeastScale = 7.888609052210118e-31f;     // 2^-100: keeps 1 / scale and sums of it far inside F32
+
+enum : unsigned { kKvNonFinite = 32u };     // status bit: a NaN or an infinity was appended
+
+struct KvShape {
+    int heads, kv_heads, head_dim, page_shift, e4m3, max_pages;
+};
+__host__ __device__ inline int kv_cw(int d) { return d % 64 == 0 ? 64 : 32; }
+__host__ __device__ inline size_t kv_sub_bytes(int d) { return static_cast<size_t>(d) * 16; }
+__host__ __device__ inline size_t kv_half_bytes(const KvShape &s) { return static_cast<size_t>(s.head_dim) << s.page_shift; }       // keys or values of a page's head
+__host__ __device__ inline size_t kv_head_bytes(const KvShape &s) { return 2 * kv_half_bytes(s); }
+__host__ __device__ inline size_t kv_page_bytes(const KvShape &s) { return kv_head_bytes(s) * s.kv_heads; }
+// offset in a sub-block of the 16 bytes of token t (0 .. 15) that hold the elements k .. k + 15 (k a multiple of 16) of a key
+__host__ __device__ inline int kv_k_offset(int d, int t, int k) {
+    const int cw = kv_cw(d);
+    return (k / cw) * (16 * cw) + t * cw + k % cw;
+}
+// offset of one element of a value, and the token and element that byte j of the v-th 16 bytes stands for
+__host__ __device__ inline int kv_v_offset(int t, int d) { return (d >> 5) * 512 + ((d & 7) * 4 + ((t & 7) >> 1)) * 16 + ((d & 31) >> 3) * 4 + (t & 1) + (t >> 3) * 2; }
+__host__ __device__ inline int kv_v_token(int v, int j) { return (v & 3) * 2 + (j & 1) + ((j & 2) << 2); }
+__host__ __device__ inline int kv_v_element(int v, int j) { return (v >> 5) * 32 + (j >> 2) * 8 + ((v & 31) >> 2); }
+
+// ---- numbers of the rows ------------------------------------------------------------------------------------------------
+enum { kRowsF32 = 0, kRowsF16 = 1, kRowsBF16 = 2 };
+__device__ __forceinline__ float row_load(const void *p, int type, size_t i) {
+    if (type == kRowsF32) return static_cast<const float *>(p)[i];
+    if (type == kRowsF16) return __half2float(static_cast<const __half *>(p)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+}
+__device__ __forceinline__ void row_store(void *p, int type, size_t i, float v) {
+    if (type == kRowsF32) static_cast<float *>(p)[i] = v;
+    else if (type == kRowsF16) static_cast<__half *>(p)[i] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// ---- codes --------------------------------------------------------------------------------------------------------------
+// The code of the quotient n / s, to the nearest, ties to even, and exactly so: a quotient that F32 rounds onto the middle between two codes is
+// told apart in 64 bits. (n = x, or an older code times its scale, has at most 32 significant bits and a middle at most 9, so that a quotient of
+// 64 bits lies on a middle only where n / s does.)
+__device__ __forceinline__ int e4m3_of(double q) {
+    float f = __double2float_rz(q);
+    if (static_cast<double>(f) != q) f = __uint_as_float(__float_as_uint(f) | 1u);        // to odd: the one rounding to come sees what was cut off
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.0f), "f"(f));
+    return r & 0xff;
+}
+template <bool E4M3>
+__device__ __forceinline__ int kv_code_exact(double n, float s) {
+    const double q = n / static_cast<double>(s);
+    if (E4M3) return e4m3_of(q);
+    return max(-127, min(127, __double2int_rn(q))) + 128;
+}
+// x finite or not (an infinity becomes the largest code, a NaN zero); r = 1 / s. The product x r is off by at most 2^-22 of itself, so that only
+// quotients that near to a middle are worked out in 64 bits.
+template <bool E4M3>
+__device__ __forceinline__ int kv_code(float x, float s, float r) {
+    const float q = x * r;
+    if (E4M3) {
+        const uint32_t b = __float_as_uint(q) & 0x7fffffffu;
+        const uint32_t off = (b & 0xfffffu) - 0x80000u + 16u;
+        if (off <= 32u || (b < 0x3c800000u && b > 0x3a000000u) || b > 0x43e00000u) {     // a middle; between 2^-11 and 2^-6 (codes without leading bit); over 448
+            if (!(fabsf(x) <= 3.402823466e38f)) return x != x ? 0 : x > 0.0f ? 0x7e : 0xfe;
+            return kv_code_exact<true>(static_cast<double>(x), s);
+        }
+        uint16_t c;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(0.0f), "f"(q));
+        return c & 0xff;
+    }
+    const float k = rintf(q);
+    if (fabsf(fabsf(q - k) - 0.5f) < 1e-4f || !(fabsf(q) <= 127.0f)) {
+        if (!(fabsf(x) <= 3.402823466e38f)) return x != x ? 128 : x > 0.0f ? 255 : 1;
+        return kv_code_exact<false>(static_cast<double>(x), s);
+    }
+    return static_cast<int>(k) + 128;
+}
+template <bool E4M3>
+__device__ __forceinline__ float kv_value(int byte) {
+    if (E4M3) {
+        uint32_t h2;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(byte)));
+        return __half2float(__ushort_as_half(static_cast<unsigned short>(h2 & 0xffff)));
+    }
+    return static_cast<float>(byte - 128);
+}
+// a code under scale s0 as a code under s1 >= s0
+template <bool E4M3>
+__device__ __forceinline__ int kv_recode(int byte, float s0, float s1) {
+    return kv_code_exact<E4M3>(static_cast<double>(kv_value<E4M3>(byte)) * static_cast<double>(s0), s1);
+}
+// four codes -> their values as f16 pairs (exact: both code sets are subsets of f16)
+template <bool E4M3>
+__device__ __forceinline__ void kv_halves(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    if (E4M3) {
+        asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(w));
+    } else {        // 0x6400 | byte is 1024 + byte
+        const __half2 off = __half2half2(__ushort_as_half(0x6480));
+        uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+        const __half2 x = __hsub2(*reinterpret_cast<__half2 *>(&a), off), y = __hsub2(*reinterpret_cast<__half2 *>(&b), off);
+        lo = *reinterpret_cast<const uint32_t *>(&x);
+        hi = *reinterpret_cast<const uint32_t *>(&y);
+    }
+}
+
+// the entry of the step that page item `item` belongs to (its page items are first .. first + pages - 1)
+__device__ __forceinline__ int kv_entry_of_item(const int *entries, int n, int item) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (entries[mid * kKvStepWords + 4] <= item) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+}  // namespace wd
