@@ -8,6 +8,7 @@ library's own error text.
 import ctypes as C
 import os
 import subprocess
+from array import array
 
 import numpy as np
 
@@ -598,7 +599,15 @@ class DenseDecoder:
 
 
 def _ints(values):
-    return np.ascontiguousarray(values, np.int32)
+    """(what holds the whole numbers as int32, their address, how many)"""
+    if isinstance(values, np.ndarray):
+        a = np.ascontiguousarray(values, np.int32)
+        if a.ndim != 1:
+            raise ValueError("a list of whole numbers is wanted")
+        return a, a.ctypes.data, a.size
+    a = array("i", values)
+    at, n = a.buffer_info()
+    return a, at, n
 
 
 class KvCache:
@@ -614,10 +623,11 @@ class KvCache:
 
     def begin(self, seqs, counts, stream=None):
         """Room for counts[i] more tokens of sequence seqs[i]; these tokens are the rows of the step."""
-        s, n = _ints(seqs), _ints(counts)
-        if s.ndim != 1 or s.shape != n.shape:
+        s, s_at, n = _ints(seqs)
+        c, c_at, m = _ints(counts)
+        if n != m:
             raise ValueError("one count for each sequence")
-        _check(lib().wd_kv_begin(self.h, s.size, _ptr(s), _ptr(n), stream))
+        _check(lib().wd_kv_begin(self.h, n, s_at, c_at, stream))
 
     def append(self, layer, k_ptr, v_ptr, type=TYPE_F32, k_stride=0, v_stride=0, stream=None):
         rc = lib().wd_kv_append(self.h, layer, k_ptr, v_ptr, type, k_stride, v_stride, stream)
@@ -632,26 +642,28 @@ class KvCache:
 
     def read(self, layer, seqs, firsts, counts, k_ptr, v_ptr, type=TYPE_F32, stream=None):
         """Tokens of sequences as numbers; layer -1: of every layer, one behind the other."""
-        s, f, n = _ints(seqs), _ints(firsts), _ints(counts)
-        if s.ndim != 1 or not s.shape == f.shape == n.shape:
+        s, s_at, n = _ints(seqs)
+        f, f_at, nf = _ints(firsts)
+        c, c_at, nc = _ints(counts)
+        if not n == nf == nc:
             raise ValueError("one first token and one count for each sequence")
-        _check(lib().wd_kv_read(self.h, layer, s.size, _ptr(s), _ptr(f), _ptr(n), k_ptr, v_ptr, type, stream))
+        _check(lib().wd_kv_read(self.h, layer, n, s_at, f_at, c_at, k_ptr, v_ptr, type, stream))
 
     def fork(self, src, dsts, stream=None):
-        d = _ints(dsts)
-        _check(lib().wd_kv_fork(self.h, src, d.size, _ptr(d), stream))
+        d, at, n = _ints(dsts)
+        _check(lib().wd_kv_fork(self.h, src, n, at, stream))
 
     def keep(self, seq, first, index, stream=None):
         """Of the tokens from `first` on those at `index` (relative to it, going up) stay and move together."""
-        x = _ints(index)
-        _check(lib().wd_kv_keep(self.h, seq, first, x.size, _ptr(x), stream))
+        x, at, n = _ints(index)
+        _check(lib().wd_kv_keep(self.h, seq, first, n, at, stream))
 
     def truncate(self, seq, length, stream=None):
         _check(lib().wd_kv_truncate(self.h, seq, length, stream))
 
     def free(self, seqs, stream=None):
-        s = _ints(seqs)
-        _check(lib().wd_kv_free(self.h, s.size, _ptr(s), stream))
+        s, at, n = _ints(seqs)
+        _check(lib().wd_kv_free(self.h, n, at, stream))
 
     def length(self, seq):
         n = lib().wd_kv_length(self.h, seq)

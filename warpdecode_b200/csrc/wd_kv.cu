@@ -32,7 +32,8 @@ struct wd_kv_cache {
     std::vector<int> holders;               // of each page
     std::vector<int> free_pages;            // last one goes first
     std::vector<int> book;
-    std::vector<int2> changed;              // words to send
+    std::vector<int> changed;               // words to send, each of them once
+    std::vector<char> dirty;                // those in `changed`
     std::vector<int2> copies;               // pages to copy: from, to
     int table_at = 0, rows = 0, max_rows = 0, items = 0;        // rows of the step, the most of one sequence's, page items
 
@@ -51,7 +52,9 @@ struct wd_kv_cache {
     void set(size_t at, int value) {
         if (book[at] == value) return;
         book[at] = value;
-        changed.push_back(make_int2(static_cast<int>(at), value));
+        if (dirty[at]) return;
+        dirty[at] = 1;
+        changed.push_back(static_cast<int>(at));
     }
     void set_page(int seq, int i, int page) { set(table_at + static_cast<size_t>(seq) * shape.max_pages + i, page); }
     int take_page() {
@@ -124,20 +127,32 @@ int check_device(const wd_kv_cache *c) {
     return WD_OK;
 }
 
+// Changes that no kernel reads before the next begin, read or keep wait for it: pages change hands only there.
+int later(wd_kv_cache *c) {
+    if (c->host_only()) {
+        for (int at : c->changed) c->dirty[at] = 0;
+        c->changed.clear();
+    }
+    return WD_OK;
+}
+
 template <int N>
 void send_words(wd_kv_cache *c, size_t from, cudaStream_t s) {
     wd::KvWords<N> w;
     w.n = static_cast<int>(std::min<size_t>(N, c->changed.size() - from));
     w.pad = 0;
-    std::memcpy(w.w, c->changed.data() + from, static_cast<size_t>(w.n) * sizeof(int2));
+    for (int i = 0; i < w.n; ++i) {
+        const int at = c->changed[from + i];
+        w.w[i] = make_int2(at, c->book[at]);
+        c->dirty[at] = 0;
+    }
     wd::kv_words_kernel<N><<<1, 256, 0, s>>>(w, c->d_book);
 }
 // What the call changed goes to the device: pages first, then the words that name them.
 int flush(wd_kv_cache *c, cudaStream_t s) {
     if (c->host_only()) {
-        c->changed.clear();
         c->copies.clear();
-        return WD_OK;
+        return later(c);
     }
     c->broken = true;
     const size_t page_bytes = wd::kv_page_bytes(c->shape);
@@ -171,6 +186,13 @@ int flush(wd_kv_cache *c, cudaStream_t s) {
 template <class F>
 int by_codes(const wd_kv_cache *c, F &&f) {
     return c->shape.e4m3 ? f(std::true_type{}) : f(std::false_type{});
+}
+
+template <class F>
+int by_rows_and_codes(const wd_kv_cache *c, int rows, F &&f) {
+    return by_codes(c, [&](auto e4m3) {
+        return rows == wd::kRowsF32 ? f(0.0f, e4m3) : rows == wd::kRowsF16 ? f(__half(), e4m3) : f(__nv_bfloat16(), e4m3);
+    });
 }
 
 template <int D, int N8, bool SPLIT>
@@ -226,6 +248,7 @@ int wd_kv_create(const wd_kv_config *cfg, wd_kv_cache **out) {
         const size_t words = k->table_at + static_cast<size_t>(c.max_seqs) * k->shape.max_pages;
         if (words > INT_MAX / 2) return set_error(WD_E_INVALID, "key/value cache: max_seqs times max_context is too large for one table");
         k->book.assign(words, 0);
+        k->dirty.assign(words, 0);
         k->seqs.resize(c.max_seqs);
         k->holders.assign(c.n_pages, 0);
         k->free_pages.resize(c.n_pages);
@@ -336,12 +359,14 @@ int wd_kv_append(wd_kv_cache *c, int layer, const void *k_dev, const void *v_dev
         if (int rc = check_device(c)) return rc;
         if (layer < 0 || layer >= c->cfg.n_layers) return set_error(WD_E_INVALID, "key/value cache: layer out of range");
         wd::KvAppend p;
-        if (int rc = rows_type(type, &p.type)) return rc;
+        int rows_of = 0;
+        if (int rc = rows_type(type, &rows_of)) return rc;
+        const size_t size = rows_size(rows_of);
         p.stride[0] = k_stride;
         p.stride[1] = v_stride;
         const long long width = static_cast<long long>(c->cfg.n_kv_heads) * c->cfg.head_dim;
-        if (int rc = check_rows(k_dev, rows_size(p.type), &p.stride[0], width, "k")) return rc;
-        if (int rc = check_rows(v_dev, rows_size(p.type), &p.stride[1], width, "v")) return rc;
+        if (int rc = check_rows(k_dev, size, &p.stride[0], width, "k")) return rc;
+        if (int rc = check_rows(v_dev, size, &p.stride[1], width, "v")) return rc;
         if (c->book[0] == 0) return set_error(WD_E_STATE, "key/value cache: no step has begun");
         if (c->items == 0) return WD_OK;
         OnDevice on(c->cfg.device);
@@ -353,9 +378,16 @@ int wd_kv_append(wd_kv_cache *c, int layer, const void *k_dev, const void *v_dev
         p.rows[1] = v_dev;
         p.status = c->d_status;
         p.s = c->shape;
+        for (int i = 0; i < 2; ++i) p.vec[i] = reinterpret_cast<uintptr_t>(p.rows[i]) % 16 == 0 && p.stride[i] * size % 16 == 0;
         const dim3 grid(static_cast<unsigned>(c->items), c->cfg.n_kv_heads, 2);
-        return by_codes(c, [&](auto e4m3) {
-            wd::kv_append_kernel<decltype(e4m3)::value><<<grid, wd::kAppendThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+        const size_t smem = static_cast<size_t>(c->cfg.page_tokens) * c->cfg.head_dim;
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        // few tokens a page: a warp reads them at once, and more threads would only meet at the barriers
+        const bool small = static_cast<long long>(std::min(c->max_rows, c->cfg.page_tokens)) * c->cfg.head_dim <= 2048;
+        return by_rows_and_codes(c, rows_of, [&](auto t, auto e4m3) {
+            using T = decltype(t);
+            if (small) wd::kv_append_kernel<T, decltype(e4m3)::value, 64><<<grid, 64, smem, s>>>(p);
+            else wd::kv_append_kernel<T, decltype(e4m3)::value, 256><<<grid, 256, smem, s>>>(p);
             WD_TRY_CUDA(cudaGetLastError());
             return WD_OK;
         });
@@ -409,9 +441,11 @@ int wd_kv_read(wd_kv_cache *c, int layer, int n, const int *seqs, const int *fir
         if (layer < -1 || layer >= c->cfg.n_layers) return set_error(WD_E_INVALID, "key/value cache: layer out of range");
         if (n < 0 || (n > 0 && (!seqs || !firsts || !counts)) || (!k_dev && !v_dev)) return set_error(WD_E_INVALID, "null argument");
         wd::KvRead p;
-        if (int rc = rows_type(type, &p.type)) return rc;
+        int rows_of = 0;
+        if (int rc = rows_type(type, &rows_of)) return rc;
+        const size_t size = rows_size(rows_of);
         for (const void *o : {k_dev, v_dev})
-            if (reinterpret_cast<uintptr_t>(o) % rows_size(p.type)) return set_error(WD_E_INVALID, "key/value cache: an output is not aligned to its type");
+            if (reinterpret_cast<uintptr_t>(o) % size) return set_error(WD_E_INVALID, "key/value cache: an output is not aligned to its type");
         long long rows = 0;
         for (int i = 0; i < n; ++i) {
             if (int rc = check_seq(c, seqs[i])) return rc;
@@ -423,7 +457,11 @@ int wd_kv_read(wd_kv_cache *c, int layer, int n, const int *seqs, const int *fir
         }
         if (rows > INT_MAX / 2) return set_error(WD_E_INVALID, "key/value cache: too many rows in a read");
         if (rows == 0) return WD_OK;
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        if (!c->changed.empty())
+            if (int rc = check_not_captured(c, s)) return rc;
         OnDevice on(c->cfg.device);
+        if (int rc = flush(c, s)) return rc;
         const size_t width = static_cast<size_t>(c->cfg.n_kv_heads) * c->cfg.head_dim;
         const int layers = layer < 0 ? c->cfg.n_layers : 1;
         p.pool = c->d_pool + (layer < 0 ? 0 : layer) * c->pool_layer;
@@ -434,7 +472,7 @@ int wd_kv_read(wd_kv_cache *c, int layer, int n, const int *seqs, const int *fir
         p.pool_layer = c->pool_layer;
         p.scales_layer = c->scales_layer;
         p.out_layer = static_cast<size_t>(rows) * width;
-        p.n_rows_pad = 0;
+        p.vec = (reinterpret_cast<uintptr_t>(k_dev) | reinterpret_cast<uintptr_t>(v_dev)) % 16 == 0;       // (a row is a multiple of 64 bytes)
         p.s = c->shape;
         int row = 0;
         for (int i = 0; i < n;) {
@@ -447,24 +485,13 @@ int wd_kv_read(wd_kv_cache *c, int layer, int n, const int *seqs, const int *fir
                 row += counts[i];
             }
             if (p.n == 0) continue;
-            // (the second index of a grid ends at 65,535)
-            const int per = std::max(1, 65535 / c->cfg.n_kv_heads);
-            const wd::KvRead whole = p;
-            for (int l = 0; l < layers; l += per) {
-                p = whole;
-                p.pool += l * c->pool_layer;
-                p.scales += l * c->scales_layer;
-                for (int kv = 0; kv < 2; ++kv)
-                    if (p.out[kv]) p.out[kv] = static_cast<char *>(p.out[kv]) + static_cast<size_t>(l) * p.out_layer * rows_size(p.type);
-                const dim3 grid(static_cast<unsigned>(items), static_cast<unsigned>(std::min(per, layers - l) * c->cfg.n_kv_heads), 2);
-                const int rc = by_codes(c, [&](auto e4m3) {
-                    wd::kv_read_kernel<decltype(e4m3)::value><<<grid, wd::kReadThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
-                    WD_TRY_CUDA(cudaGetLastError());
-                    return WD_OK;
-                });
-                if (rc) return rc;
-            }
-            p = whole;
+            const dim3 grid(static_cast<unsigned>(items), static_cast<unsigned>(layers));
+            const int rc = by_rows_and_codes(c, rows_of, [&](auto t, auto e4m3) {
+                wd::kv_read_kernel<decltype(t), decltype(e4m3)::value><<<grid, wd::kReadThreads, 0, s>>>(p);
+                WD_TRY_CUDA(cudaGetLastError());
+                return WD_OK;
+            });
+            if (rc) return rc;
         }
         return WD_OK;
     });
@@ -490,8 +517,7 @@ int wd_kv_fork(wd_kv_cache *c, int src, int n, const int *dsts, void *stream) {
                 c->set_page(dsts[i], static_cast<int>(j), from.pages[j]);
             }
         }
-        OnDevice on(c->host_only() ? 0 : c->cfg.device);
-        return flush(c, s);
+        return later(c);
     });
 }
 
@@ -504,8 +530,7 @@ int wd_kv_truncate(wd_kv_cache *c, int seq, int length, void *stream) {
         if (int rc = check_not_captured(c, s)) return rc;
         c->cut(c->seqs[seq], length);
         c->end_step();
-        OnDevice on(c->host_only() ? 0 : c->cfg.device);
-        return flush(c, s);
+        return later(c);
     });
 }
 
@@ -518,8 +543,7 @@ int wd_kv_free(wd_kv_cache *c, int n, const int *seqs, void *stream) {
         if (int rc = check_not_captured(c, s)) return rc;
         for (int i = 0; i < n; ++i) c->cut(c->seqs[seqs[i]], 0);
         c->end_step();
-        OnDevice on(c->host_only() ? 0 : c->cfg.device);
-        return flush(c, s);
+        return later(c);
     });
 }
 
@@ -540,8 +564,7 @@ int wd_kv_keep(wd_kv_cache *c, int seq, int first, int n, const int *index, void
         if (kept == 0) {
             c->cut(q, end);
             c->end_step();
-            OnDevice on(c->host_only() ? 0 : c->cfg.device);
-            return flush(c, s);
+            return later(c);
         }
         const int page0 = from / c->page_tokens(), pages = c->pages_for(end) - page0;
         // Into new pages, all at once, where there are enough of them; else in place, page by page, but never into a page that others hold.
@@ -555,6 +578,7 @@ int wd_kv_keep(wd_kv_cache *c, int seq, int first, int n, const int *index, void
         for (int i = 0; i < pages; ++i) to[i] = fresh || c->holders[q.pages[page0 + i]] > 1 ? c->take_page() : q.pages[page0 + i];
         OnDevice on(c->host_only() ? 0 : c->cfg.device);
         if (!c->host_only()) {
+            if (int rc = flush(c, s)) return rc;        // the table as it was
             c->broken = true;
             words.insert(words.end(), to.begin(), to.end());
             for (size_t at = 0; at < words.size();) {
@@ -609,7 +633,7 @@ int wd_kv_keep(wd_kv_cache *c, int seq, int first, int n, const int *index, void
         }
         c->cut(q, end);
         c->end_step();
-        return flush(c, s);
+        return c->host_only() ? later(c) : flush(c, s);
     });
 }
 

@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(256) kv_run_kernel(const __grid_constant__ KvR
 // ---- append ---------------------------------------------------------------------------------------------------------------
 // A block takes the step's tokens that lie in one page, one kv head, keys (blockIdx.z = 0) or values. Two passes over its rows: the largest
 // magnitude, from which the scale follows, then the codes (the rows come from the caches the second time). A page that held tokens before keeps its
-// scale unless the new ones need a larger one; then the codes that are there are rounded anew.
+// scale unless the new ones need a larger one; then the codes that are there are rounded anew. Values are turned in shared memory.
 struct KvAppend {
     uint8_t *pool;              // of the layer
     float *scales;              // of the layer
@@ -37,42 +37,46 @@ struct KvAppend {
     const void *rows[2];
     long long stride[2];
     unsigned *status;
-    int type;
+    int vec[2];                 // rows lie on boundaries of 16 bytes
     KvShape s;
 };
-constexpr int kAppendThreads = 128;
 
-template <bool E4M3>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ KvAppend P) {
-    __shared__ float part[kAppendThreads / 32];
+template <class T, bool E4M3, int THREADS>
+__global__ void __launch_bounds__(THREADS) kv_append_kernel(const __grid_constant__ KvAppend P) {
+    extern __shared__ __align__(16) uint8_t app_sm[];           // values: the codes of the sub-blocks that the rows touch
+    __shared__ float part[THREADS / 32];
     __shared__ int bad_any;
     const int n_seq = P.book[0], n_items = P.book[2], tid = threadIdx.x, h = blockIdx.y, kv = blockIdx.z, D = P.s.head_dim;
     const int *entries = P.book + kKvHead;
     const int page_tokens = 1 << P.s.page_shift;
     const size_t stride = static_cast<size_t>(P.stride[kv]);
-    const void *rows = P.rows[kv];
+    const bool vec = P.vec[kv] != 0;
 #pragma unroll 1
     for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
         const int *e = entries + kv_entry_of_item(entries, n_seq, item) * kKvStepWords;
-        const int seq = e[0], row0 = e[1], count = e[2], length = e[3], begin = length - count;
+        const int4 e0 = *reinterpret_cast<const int4 *>(e);
+        const int seq = e0.x, row0 = e0.y, count = e0.z, length = e0.w, begin = length - count;
         const int logical = (begin >> P.s.page_shift) + item - e[4], page0 = logical << P.s.page_shift;
         const int a = max(begin - page0, 0), b = min(length - page0, page_tokens);       // the step's tokens in this page: a .. b - 1
         const int page = P.table[static_cast<size_t>(seq) * P.s.max_pages + logical];
-        const size_t first = static_cast<size_t>(row0 + page0 + a - begin);
+        const T *rows = static_cast<const T *>(P.rows[kv]) + static_cast<size_t>(row0 + page0 + a - begin) * stride + static_cast<size_t>(h) * D;
         uint8_t *base = P.pool + static_cast<size_t>(page) * kv_page_bytes(P.s) + h * kv_head_bytes(P.s) + kv * kv_half_bytes(P.s);
         float *scale = P.scales + (static_cast<size_t>(page) * P.s.kv_heads + h) * 2 + kv;
         const float s0 = a > 0 ? *scale : 0.0f;
-        const size_t col = static_cast<size_t>(h) * D;
+        const int per = D / 16, groups = (b - a) * per;
         // the largest finite magnitude
         float top = 0.0f;
         int bad = 0;
-        const int total = (b - a) * D;
-#pragma unroll 4
-        for (int i = tid; i < total; i += kAppendThreads) {
-            const int t = i / D, d = i - t * D;
-            const float x = fabsf(row_load(rows, P.type, (first + t) * stride + col + d));
-            if (x <= 3.402823466e38f) top = fmaxf(top, x);
-            else bad = 1;
+        for (int i = tid; i < groups; i += THREADS) {
+            const int t = i / per, k = (i - t * per) * 16;
+            float x[16];
+            row_load16(rows + t * stride + k, vec, x);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float y = fabsf(x[j]);
+                if (y <= 3.402823466e38f) top = fmaxf(top, y);
+                else bad = 1;
+            }
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -82,49 +86,50 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
         if (bad) bad_any = 1;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kAppendThreads / 32; ++w) top = fmaxf(top, part[w]);
+        for (int w = 0; w < THREADS / 32; ++w) top = fmaxf(top, part[w]);
         if (tid == 0 && bad_any) atomicOr(P.status, kKvNonFinite);
         const float need = top > 0.0f ? fmaxf(__fdiv_rn(top, E4M3 ? 448.0f : 127.0f), kKvLeastScale) : 0.0f;
         const float s1 = fmaxf(s0, need), r = s1 > 0.0f ? __fdiv_rn(1.0f, s1) : 0.0f;
         if (a > 0 && s1 != s0) {        // the codes of the tokens 0 .. a - 1 under the larger scale
             const int vecs = ((a + kKvSub - 1) / kKvSub) * D;
-            for (int i = tid; i < vecs; i += kAppendThreads) {
-                const int sub = i / D, v = i - sub * D;
+            const float ratio = __fdiv_rn(s0, s1);
+            for (int i = tid; i < vecs; i += THREADS) {
+                const int sub = i / D, v = i - sub * D, cw = kv_cw(D), token = (v * 16 % (16 * cw)) / cw;      // (of keys)
+                if (kv == 0 && sub * kKvSub + token >= a) continue;        // another thread may have written its new codes already
                 uint4 *p = reinterpret_cast<uint4 *>(base + sub * kv_sub_bytes(D)) + v;
                 uint4 x = *p;
                 uint8_t *c = reinterpret_cast<uint8_t *>(&x);
-                const int cw = kv_cw(D), token = (v * 16 % (16 * cw)) / cw;      // (keys)
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
-                    if (sub * kKvSub + (kv ? kv_v_token(v, j) : token) < a) c[j] = static_cast<uint8_t>(kv_recode<E4M3>(c[j], s0, s1));
+                    if (sub * kKvSub + (kv ? kv_v_token(v, j) : token) < a) c[j] = static_cast<uint8_t>(kv_recode<E4M3>(c[j], s0, s1, ratio));
                 *p = x;
             }
         }
-        __syncthreads();        // the values' old and new tokens may share 16 bytes
-        if (kv == 0) {
-            const int per = D / 16, vecs = (b - a) * per;
-            for (int i = tid; i < vecs; i += kAppendThreads) {
-                const int t = i / per, k = (i - t * per) * 16, token = a + t;
-                const size_t src = (first + t) * stride + col + k;
-                uint4 x;
-                uint8_t *c = reinterpret_cast<uint8_t *>(&x);
+        const int sub0 = a / kKvSub;
+        for (int i = tid; i < groups; i += THREADS) {
+            const int t = i / per, k = (i - t * per) * 16, token = a + t;
+            float y[16];
+            row_load16(rows + t * stride + k, vec, y);
+            uint4 x;
+            uint8_t *c = reinterpret_cast<uint8_t *>(&x);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) c[j] = static_cast<uint8_t>(kv_code<E4M3>(row_load(rows, P.type, src + j), s1, r));
+            for (int j = 0; j < 16; ++j) c[j] = static_cast<uint8_t>(kv_code<E4M3>(y[j], s1, r));
+            if (kv == 0) {
                 *reinterpret_cast<uint4 *>(base + (token / kKvSub) * kv_sub_bytes(D) + kv_k_offset(D, token % kKvSub, k)) = x;
+            } else {
+                uint8_t *to = app_sm + (token / kKvSub - sub0) * 16 * D + kv_v_offset(token % kKvSub, k);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) to[(j & 7) * 64 + (j >> 3) * 4] = c[j];       // element k + j: k is a multiple of 16, so that only j moves the byte
             }
-        } else {
-            const int sub0 = a / kKvSub, subs = (b - 1) / kKvSub + 1 - sub0;
-            for (int i = tid; i < subs * D; i += kAppendThreads) {
+        }
+        __syncthreads();        // the turned codes are there, and the older ones that share 16 bytes with them
+        if (kv == 1) {
+            const int vecs = ((b - 1) / kKvSub + 1 - sub0) * D;
+            for (int i = tid; i < vecs; i += THREADS) {
                 const int sub = sub0 + i / D, v = i % D, lo = a - sub * kKvSub, hi = b - sub * kKvSub;
                 uint8_t *to = base + sub * kv_sub_bytes(D) + v * 16;
-                uint4 x;
-                uint8_t *c = reinterpret_cast<uint8_t *>(&x);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int token = kv_v_token(v, j);
-                    if (token >= lo && token < hi)
-                        c[j] = static_cast<uint8_t>(kv_code<E4M3>(row_load(rows, P.type, (first + token - lo) * stride + col + kv_v_element(v, j)), s1, r));
-                }
+                const uint4 x = reinterpret_cast<const uint4 *>(app_sm)[i];
+                const uint8_t *c = reinterpret_cast<const uint8_t *>(&x);
                 if (lo <= 0 && hi >= kKvSub) {
                     *reinterpret_cast<uint4 *>(to) = x;
                 } else {
@@ -141,7 +146,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
 
 // ---- read -----------------------------------------------------------------------------------------------------------------
 // Tokens first .. first + count - 1 of sequences as numbers, rows one after the other: [layer][row][kv head][D]. A block takes a sub-block of
-// 16 tokens, one head, keys or values of one layer.
+// 16 tokens of a layer, all heads, keys and values; a warp 512 bytes, which are 16 tokens of 32 elements of a value's head (turned in shared
+// memory, so that rows are written in pieces of 64 bytes and more).
 struct KvReadEntry {
     int seq, first, count, row0, item0;         // items: sub-blocks that the range touches
 };
@@ -152,16 +158,17 @@ struct KvRead {
     const int *table;
     void *out[2];
     size_t pool_layer, scales_layer, out_layer;         // bytes, floats, elements from a layer to the next
-    int type, n, n_rows_pad;
+    int n, vec;
     KvShape s;
     KvReadEntry e[kReadEntries];
 };
-constexpr int kReadThreads = 128;
+constexpr int kReadThreads = 256;
 
-template <bool E4M3>
+template <class T, bool E4M3>
 __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const __grid_constant__ KvRead P) {
-    const int item = blockIdx.x, h = blockIdx.y % P.s.kv_heads, layer = blockIdx.y / P.s.kv_heads, kv = blockIdx.z, D = P.s.head_dim, tid = threadIdx.x;
-    if (P.out[kv] == nullptr) return;
+    constexpr int PITCH = 32 + 16 / sizeof(T);
+    __shared__ __align__(16) T turned[kReadThreads / 32][kKvSub][PITCH];
+    const int item = blockIdx.x, layer = blockIdx.y, D = P.s.head_dim, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int lo = 0, hi = P.n - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -172,29 +179,48 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const __grid_cons
     const int sub = e.first / kKvSub + item - e.item0, t0 = sub * kKvSub;
     const int a = max(e.first - t0, 0), b = min(e.first + e.count - t0, kKvSub), shift = P.s.page_shift;
     const int page = P.table[static_cast<size_t>(e.seq) * P.s.max_pages + (t0 >> shift)];
-    const uint8_t *base = P.pool + layer * P.pool_layer + static_cast<size_t>(page) * kv_page_bytes(P.s) + h * kv_head_bytes(P.s) +
-                          ((t0 & ((1 << shift) - 1)) / kKvSub) * kv_sub_bytes(D) + kv * kv_half_bytes(P.s);
-    const float s = P.scales[layer * P.scales_layer + (static_cast<size_t>(page) * P.s.kv_heads + h) * 2 + kv];
-    const size_t pitch = static_cast<size_t>(P.s.kv_heads) * D;
-    const size_t out0 = layer * P.out_layer + static_cast<size_t>(e.row0 + t0 - e.first) * pitch + static_cast<size_t>(h) * D;     // (of token 0, which may lie in front of the rows)
-    if (kv == 0) {
-        const int per = D / 16;
-        for (int i = a * per + tid; i < b * per; i += kReadThreads) {
-            const int t = i / per, k = (i - t * per) * 16;
-            const uint4 x = *reinterpret_cast<const uint4 *>(base + kv_k_offset(D, t, k));
-            const uint8_t *c = reinterpret_cast<const uint8_t *>(&x);
-            const size_t to = out0 + t * pitch + k;
+    const uint8_t *base = P.pool + layer * P.pool_layer + static_cast<size_t>(page) * kv_page_bytes(P.s) + ((t0 & ((1 << shift) - 1)) / kKvSub) * kv_sub_bytes(D);
+    const float *scales = P.scales + layer * P.scales_layer + static_cast<size_t>(page) * P.s.kv_heads * 2;
+    const size_t pitch = static_cast<size_t>(P.s.kv_heads) * D, head_bytes = kv_head_bytes(P.s), half = kv_half_bytes(P.s);
+    T *ko = static_cast<T *>(P.out[0]), *vo = static_cast<T *>(P.out[1]);
+    const size_t row0 = static_cast<size_t>(e.row0 + t0 - e.first);        // of token 0, which may lie in front of the rows
+    const int per_head = D / 32, units = P.s.kv_heads * per_head, cw = kv_cw(D);         // a unit is 512 bytes
+    constexpr int N = 16 / sizeof(T);
+#pragma unroll 2
+    for (int u = warp; u < 2 * units; u += kReadThreads / 32) {
+        const int kv = u >= units, in = u - kv * units, h = in / per_head, blk = in - h * per_head;
+        if ((kv ? vo : ko) == nullptr) continue;
+        const uint4 x = *reinterpret_cast<const uint4 *>(base + h * head_bytes + kv * half + blk * 512 + lane * 16);
+        const uint8_t *c = reinterpret_cast<const uint8_t *>(&x);
+        const float s = scales[h * 2 + kv];
+        if (kv == 0) {
+            const int at = blk * 512 + lane * 16, token = at % (16 * cw) / cw, k = at / (16 * cw) * cw + at % cw;
+            if (token < a || token >= b) continue;
+            T *to = ko + layer * P.out_layer + (row0 + token) * pitch + static_cast<size_t>(h) * D + k;
+            __align__(16) T y[16];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) row_store(P.out[0], P.type, to + j, __fmul_rn(kv_value<E4M3>(c[j]), s));
-        }
-    } else {
-        for (int v = tid; v < D; v += kReadThreads) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(base + v * 16);
-            const uint8_t *c = reinterpret_cast<const uint8_t *>(&x);
+            for (int j = 0; j < 16; ++j) y[j] = row_number<T>(__fmul_rn(kv_value<E4M3>(c[j]), s));
+            if (P.vec) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int token = kv_v_token(v, j);
-                if (token >= a && token < b) row_store(P.out[1], P.type, out0 + token * pitch + kv_v_element(v, j), __fmul_rn(kv_value<E4M3>(c[j]), s));
+                for (int j = 0; j < 16; j += N) *reinterpret_cast<uint4 *>(to + j) = *reinterpret_cast<const uint4 *>(y + j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) to[j] = y[j];
+            }
+        } else {
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) turned[warp][kv_v_token(lane, j)][kv_v_element(lane, j)] = row_number<T>(__fmul_rn(kv_value<E4M3>(c[j]), s));
+            __syncwarp();
+            T *to = vo + layer * P.out_layer + row0 * pitch + static_cast<size_t>(h) * D + blk * 32;
+            if (P.vec) {
+#pragma unroll
+                for (int i = lane; i < kKvSub * 32 / N; i += 32) {
+                    const int token = i / (32 / N), d = i % (32 / N) * N;
+                    if (token >= a && token < b) *reinterpret_cast<uint4 *>(to + token * pitch + d) = *reinterpret_cast<const uint4 *>(&turned[warp][token][d]);
+                }
+            } else {
+                for (int token = a; token < b; ++token) to[token * pitch + lane] = turned[warp][token][lane];
             }
         }
     }
@@ -245,6 +271,7 @@ __global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(const __grid_cons
     extern __shared__ __align__(16) uint8_t keep_sm[];        // the page's codes
     __shared__ int source[128];                               // position of each token, -1 behind the last
     __shared__ float from_scale[128], top;
+    __shared__ size_t from_page[128];
     const int h = blockIdx.y % P.s.kv_heads, layer = blockIdx.y / P.s.kv_heads, kv = blockIdx.z, D = P.s.head_dim, tid = threadIdx.x;
     const int shift = P.s.page_shift, tokens = 1 << shift, mask = tokens - 1;
     uint8_t *pool = P.pool + layer * P.pool_layer + h * kv_head_bytes(P.s) + kv * kv_half_bytes(P.s);
@@ -258,7 +285,9 @@ __global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(const __grid_cons
             const int pos = p0 + tid;
             const int src = pos < P.first ? pos : pos < P.first + P.kept ? P.first + P.index[pos - P.first] : -1;
             source[tid] = src;
-            from_scale[tid] = src < 0 ? 0.0f : scales[static_cast<size_t>(P.table[src >> shift]) * page_scales];
+            const size_t page = src < 0 ? 0 : static_cast<size_t>(P.table[src >> shift]);
+            from_page[tid] = page * page_bytes;
+            from_scale[tid] = src < 0 ? 0.0f : scales[page * page_scales];
         }
         __syncthreads();
         if (tid < 32) {
@@ -271,42 +300,51 @@ __global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(const __grid_cons
         __syncthreads();
         const float s1 = top;
         const int used = (min(P.first + P.kept - p0, tokens) + kKvSub - 1) / kKvSub;      // sub-blocks
-        if (kv == 0) {
-            const int per = D / 16;
-            for (int j = tid; j < used * kKvSub * per; j += kKeepThreads) {
-                const int t = j / per, k = (j - t * per) * 16, src = source[t];
-                uint4 x = make_uint4(0, 0, 0, 0);
-                uint8_t *c = reinterpret_cast<uint8_t *>(&x);
+        for (int j = tid; j < used * D; j += kKeepThreads) {         // 16 bytes each
+            const int sub = j / D, v = j - sub * D;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            uint8_t *c = reinterpret_cast<uint8_t *>(&x);
+            if (kv == 0) {
+                const int cw = kv_cw(D), at = v * 16, t = sub * kKvSub + at % (16 * cw) / cw, src = source[t];
                 if (src >= 0) {
                     const int o = src & mask;
-                    x = *reinterpret_cast<const uint4 *>(pool + static_cast<size_t>(P.table[src >> shift]) * page_bytes + (o / kKvSub) * kv_sub_bytes(D) +
-                                                         kv_k_offset(D, o % kKvSub, k));
+                    x = *reinterpret_cast<const uint4 *>(pool + from_page[t] + (o / kKvSub) * kv_sub_bytes(D) + (o % kKvSub) * cw + at / (16 * cw) * (16 * cw) + at % cw);
                     const float s0 = from_scale[t];
                     if (s0 != s1) {
+                        const float ratio = __fdiv_rn(s0, s1);
 #pragma unroll
-                        for (int b = 0; b < 16; ++b) c[b] = static_cast<uint8_t>(kv_recode<E4M3>(c[b], s0, s1));
+                        for (int k = 0; k < 16; ++k) c[k] = static_cast<uint8_t>(kv_recode<E4M3>(c[k], s0, s1, ratio));
                     }
                 }
-                *reinterpret_cast<uint4 *>(keep_sm + (t / kKvSub) * 16 * D + kv_k_offset(D, t % kKvSub, k)) = x;
-            }
-        } else {
-            for (int j = tid; j < used * kKvSub * D; j += kKeepThreads) {
-                const int sub = j / (kKvSub * D), in = j - sub * (kKvSub * D), v = in / 16, t = sub * kKvSub + kv_v_token(v, in % 16), src = source[t];
-                int c = 0;
-                if (src >= 0) {
+            } else {
+                // four tokens; of each one the four elements are at one place of the words of 16 bytes
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int t = sub * kKvSub + kv_v_token(v, q), src = source[t];
+                    if (src < 0) continue;
                     const int o = src & mask;
-                    c = pool[static_cast<size_t>(P.table[src >> shift]) * page_bytes + (o / kKvSub) * kv_sub_bytes(D) + kv_v_offset(o % kKvSub, kv_v_element(v, in % 16))];
+                    const uint8_t *p = pool + from_page[t] + (o / kKvSub) * kv_sub_bytes(D) + kv_v_offset(o % kKvSub, kv_v_element(v, 0));
+                    const uint4 y = *reinterpret_cast<const uint4 *>(reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(15));
+                    const int shift8 = 8 * static_cast<int>(reinterpret_cast<uintptr_t>(p) & 3);
+                    int z[4] = {static_cast<int>(y.x >> shift8 & 0xff), static_cast<int>(y.y >> shift8 & 0xff), static_cast<int>(y.z >> shift8 & 0xff),
+                                static_cast<int>(y.w >> shift8 & 0xff)};
                     const float s0 = from_scale[t];
-                    if (s0 != s1) c = kv_recode<E4M3>(c, s0, s1);
+                    if (s0 != s1) {
+                        const float ratio = __fdiv_rn(s0, s1);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) z[k] = kv_recode<E4M3>(z[k], s0, s1, ratio);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) c[4 * k + q] = static_cast<uint8_t>(z[k]);
                 }
-                keep_sm[j] = static_cast<uint8_t>(c);
             }
+            reinterpret_cast<uint4 *>(keep_sm)[j] = x;
         }
         __syncthreads();
         const int page = P.to[i];
         for (int j = tid; j < used * D; j += kKeepThreads) {
             const int sub = j / D, v = j - sub * D;
-            reinterpret_cast<uint4 *>(pool + static_cast<size_t>(page) * page_bytes + sub * kv_sub_bytes(D))[v] = reinterpret_cast<const uint4 *>(keep_sm + sub * 16 * D)[v];
+            reinterpret_cast<uint4 *>(pool + static_cast<size_t>(page) * page_bytes + sub * kv_sub_bytes(D))[v] = reinterpret_cast<const uint4 *>(keep_sm)[j];
         }
         if (tid == 0) scales[static_cast<size_t>(page) * page_scales] = s1;
         __syncthreads();

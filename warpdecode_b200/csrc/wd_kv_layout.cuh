@@ -57,6 +57,32 @@ __device__ __forceinline__ void row_store(void *p, int type, size_t i, float v) 
     else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
 }
 
+// 16 elements of a row, by reads of 16 bytes where `vec` says that they lie on such boundaries
+template <class T>
+__device__ __forceinline__ void row_load16(const T *p, bool vec, float *x) {
+    if (vec) {
+        constexpr int N = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 16; i += N) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p + i));
+            const T *e = reinterpret_cast<const T *>(&u);
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[i + j] = static_cast<float>(e[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = static_cast<float>(p[i]);
+    }
+}
+template <class T>
+__device__ __forceinline__ T row_number(float v);
+template <>
+__device__ __forceinline__ float row_number<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half row_number<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 row_number<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
 // ---- codes --------------------------------------------------------------------------------------------------------------
 // The code of the quotient n / s, to the nearest, ties to even, and exactly so: a quotient that F32 rounds onto the middle between two codes is
 // told apart in 64 bits. (n = x, or an older code times its scale, has at most 32 significant bits and a middle at most 9, so that a quotient of
@@ -106,10 +132,20 @@ __device__ __forceinline__ float kv_value(int byte) {
     }
     return static_cast<float>(byte - 128);
 }
-// a code under scale s0 as a code under s1 >= s0
+// a code under scale s0 as a code under s1 >= s0 (> 0), ratio = s0 / s1: the product with it is off by 2^-22, as in kv_code
 template <bool E4M3>
-__device__ __forceinline__ int kv_recode(int byte, float s0, float s1) {
-    return kv_code_exact<E4M3>(static_cast<double>(kv_value<E4M3>(byte)) * static_cast<double>(s0), s1);
+__device__ __forceinline__ int kv_recode(int byte, float s0, float s1, float ratio) {
+    const float v = kv_value<E4M3>(byte), q = v * ratio;
+    if (E4M3) {
+        const uint32_t b = __float_as_uint(q) & 0x7fffffffu, off = (b & 0xfffffu) - 0x80000u + 16u;
+        if (off <= 32u || (b < 0x3c800000u && b > 0x3a000000u)) return kv_code_exact<true>(static_cast<double>(v) * static_cast<double>(s0), s1);
+        uint16_t c;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(0.0f), "f"(q));
+        return c & 0xff;
+    }
+    const float k = rintf(q);
+    if (fabsf(fabsf(q - k) - 0.5f) < 1e-4f) return kv_code_exact<false>(static_cast<double>(v) * static_cast<double>(s0), s1);
+    return static_cast<int>(k) + 128;
 }
 // four codes -> their values as f16 pairs (exact: both code sets are subsets of f16)
 template <bool E4M3>
@@ -125,15 +161,14 @@ __device__ __forceinline__ void kv_halves(uint32_t w, uint32_t &lo, uint32_t &hi
     }
 }
 
-// the entry of the step that page item `item` belongs to (its page items are first .. first + pages - 1)
+// the entry of the step that page item `item` belongs to: the last one whose items begin at or in front of it (all threads of the block)
 __device__ __forceinline__ int kv_entry_of_item(const int *entries, int n, int item) {
-    int lo = 0, hi = n - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (entries[mid * kKvStepWords + 4] <= item) lo = mid;
-        else hi = mid - 1;
+    int at = -1;
+    for (int i = 0; i < n; i += blockDim.x) {
+        const int mine = i + static_cast<int>(threadIdx.x);
+        at += __syncthreads_count(mine < n && entries[mine * kKvStepWords + 4] <= item);
     }
-    return lo;
+    return at;
 }
 
 }  // namespace wd

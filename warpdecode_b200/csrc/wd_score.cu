@@ -2,16 +2,18 @@
 //
 //   m = max x,  s = sum e^(x - m),  t = sum (x - m) e^(x - m):   log p = x - m - log s,   H = log s - t / s
 //
-// One pass over the logits. A row is shared by the CTAs of a cluster where there are few rows (they meet in the first one's shared memory, so that no
-// workspace is needed). A thread keeps its own m, s, t over rounds of 16 elements. The alternatives are collected beside: a key is (order of the
-// value, lowest index first) in 64 bits, a candidate is what is not below the CTA's bar, and the bar comes from the first round (the n_top-th of the
-// threads' maxima) and rises when the list of candidates is cut to its n_top best. Behind the first rounds almost no element meets it.
+// One pass over the logits. A CTA an SM walks over the rows, and a ring of bulk copies runs ahead of it, over the rows' ends too; a row is shared by
+// the CTAs of a cluster where there are few rows (they meet in the first one's shared memory, so that no workspace is needed). A thread keeps its own
+// m, s, t over rounds of 16 elements. The alternatives are collected beside: a key is (order of the value, lowest index first) in 64 bits, a candidate
+// is what is not below the CTA's bar, and the bar comes from the first round (the n_top-th of the threads' maxima, to three bits behind the leading
+// one) and rises when the list of candidates is cut to its n_top best. Behind the first rounds almost no element meets it.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <climits>
 
+#include "wd_device.cuh"
 #include "wd_host.h"
 
 namespace cg = cooperative_groups;
@@ -21,13 +23,13 @@ using wd_host::set_error;
 namespace wd {
 namespace {
 
-constexpr int kScoreThreads = 512, kScoreTop = 32, kScoreList = 1024;
+constexpr int kScoreThreads = 1024, kScoreTop = 32, kScoreList = 1024, kScoreSlots = 6;
 typedef unsigned long long score_key;
 
 struct ScoreParams {
     const void *logits;
     long long stride;
-    int rows, vocab, n_top;
+    int rows, vocab, n_top, ctas;
     const int *tokens;
     float *logprob, *entropy;
     int *top_ids;
@@ -107,6 +109,7 @@ struct ScoreShared {
     float warp_max[kScoreThreads / 32];
     int count;
     score_key bar;
+    uint64_t full[kScoreSlots];
 };
 
 // The list is cut to its n best, in order, and the bar set to the last of them where there are n. All threads; keys are distinct.
@@ -130,191 +133,256 @@ __device__ void score_cut(ScoreShared &sh, int n) {
 }
 
 template <class T>
-__global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const __grid_constant__ ScoreParams P) {
+constexpr int kSlotsOf = sizeof(T) == 4 ? 3 : kScoreSlots;        // 192 KB of a round's 16 elements a thread each
+
+template <class T>
+__global__ void __launch_bounds__(kScoreThreads, 1) score_kernel(const __grid_constant__ ScoreParams P) {
+    extern __shared__ __align__(128) uint8_t score_ring[];
     __shared__ ScoreShared sh;
     cg::cluster_group cluster = cg::this_cluster();
-    const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank()), tid = threadIdx.x, n_top = P.n_top;
-    const int row = static_cast<int>(blockIdx.x) / ctas;        // (blocks of a cluster follow one another)
-    constexpr int VN = Vec<T>::kN, PER = 16 / VN;               // elements of a 16-byte read, reads of a round
-    const T *x = static_cast<const T *>(P.logits) + static_cast<size_t>(row) * P.stride;
-    // reads of 16 bytes from the first boundary on; what lies in front and behind are single elements of the first CTA's first round
-    const int lead = min(static_cast<int>(((16u - static_cast<unsigned>(reinterpret_cast<uintptr_t>(x) & 15u)) & 15u) / sizeof(T)), P.vocab);
-    const int n_vec = (P.vocab - lead) / VN, tail0 = lead + n_vec * VN, loose = lead + P.vocab - tail0;
-    const uint4 *xv = reinterpret_cast<const uint4 *>(x + lead);
-    const int per_cta = (n_vec + ctas - 1) / ctas, v0 = min(rank * per_cta, n_vec), v1 = min(v0 + per_cta, n_vec);
+    const int ctas = P.ctas, rank = ctas > 1 ? static_cast<int>(cluster.block_rank()) : 0, tid = threadIdx.x, n_top = P.n_top;
+    const int group = static_cast<int>(blockIdx.x) / ctas, groups = static_cast<int>(gridDim.x) / ctas;        // (blocks of a cluster follow one another)
+    constexpr int VN = Vec<T>::kN, PER = 16 / VN, ROUND = kScoreThreads * PER, SLOTS = kSlotsOf<T>;      // elements of 16 bytes, 16 bytes of a thread and of a round
+    // Where a row's reads of 16 bytes are: from the first boundary on. What lies in front and behind are single elements of the first CTA's first round.
+    struct Place {
+        const T *x;
+        int lead, n_vec, v0, v1;
+    };
+    auto place = [&](int row) {
+        Place p;
+        p.x = static_cast<const T *>(P.logits) + static_cast<size_t>(row) * P.stride;
+        p.lead = min(static_cast<int>(((16u - static_cast<unsigned>(reinterpret_cast<uintptr_t>(p.x) & 15u)) & 15u) / sizeof(T)), P.vocab);
+        p.n_vec = (P.vocab - p.lead) / VN;
+        const int per_cta = (p.n_vec + ctas - 1) / ctas;
+        p.v0 = min(rank * per_cta, p.n_vec);
+        p.v1 = min(p.v0 + per_cta, p.n_vec);
+        return p;
+    };
+    // the ring: the first thread asks for rounds in the order in which they are read
+    int ask_row = group, ask_base = -1, ask_slot = 0;
+    auto ask = [&]() {
+        while (ask_row < P.rows) {
+            const Place p = place(ask_row);
+            if (ask_base < 0) ask_base = p.v0;
+            if (ask_base >= p.v1) {
+                ask_row += groups;
+                ask_base = -1;
+                continue;
+            }
+            const uint32_t bytes = static_cast<uint32_t>(min(ROUND, p.v1 - ask_base)) * 16u;
+            mbar_expect_tx(&sh.full[ask_slot], bytes);
+            bulk_load(score_ring + static_cast<size_t>(ask_slot) * ROUND * 16, reinterpret_cast<const uint4 *>(p.x + p.lead) + ask_base, bytes, &sh.full[ask_slot]);
+            ask_base += ROUND;
+            ask_slot = ask_slot + 1 == SLOTS ? 0 : ask_slot + 1;
+            return;
+        }
+    };
     if (tid == 0) {
-        sh.count = 0;
-        sh.bar = 1;
+        for (int i = 0; i < SLOTS; ++i) mbar_init(&sh.full[i], 1);
+        mbar_fence_init();
+        for (int i = 0; i < SLOTS; ++i) ask();
     }
-    __syncthreads();
-    ScoreSums mine = {kScoreFloor, 0.0f, 0.0f, 0.0f};
-    auto add = [&](const float *v, int n, float top) {
-        if (!(top < INFINITY)) mine.bad = 1.0f;
-        if (top > mine.m) {
-            const float d = (mine.m - top) * 1.44269504f, f = ex2s(fmaxf(d, -200.0f));
-            mine.t = f > 0.0f ? (mine.t + d * mine.s) * f : 0.0f;
-            mine.s *= f;
-            mine.m = top;
+    int slot = 0;
+    uint32_t par = 0;
+#pragma unroll 1
+    for (int row = group; row < P.rows; row += groups) {
+        const Place at_row = place(row);
+        const T *x = at_row.x;
+        const int lead = at_row.lead, tail0 = lead + at_row.n_vec * VN, loose = lead + P.vocab - tail0, v0 = at_row.v0, v1 = at_row.v1;
+        if (tid == 0) {
+            sh.count = 0;
+            sh.bar = 1;
         }
-        float s = 0.0f, t = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (i < n) {
-                const float y = fmaxf((v[i] - mine.m) * 1.44269504f, -200.0f), e = ex2s(y);
-                s += e;
-                t = fmaf(e, y, t);
-            }
-        mine.s += s;
-        mine.t += t;
-    };
-    // candidates of a thread's elements; index(i) is the element's place in the row
-    auto offer = [&](const float *v, int n, float top, auto index) {
-        const score_key bar = sh.bar;
-        if (order_of(top) < static_cast<uint32_t>(bar >> 32)) return;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (i < n && v[i] > -INFINITY) {
-                const score_key k = key_of(v[i], index(i));
-                if (k >= bar) {
-                    const int at = atomicAdd(&sh.count, 1);
-                    if (at < kScoreList) sh.list[at] = k;
-                }
-            }
-    };
-    // after a round: a list that ran over is filled again above a higher bar, one that is half full is cut
-    auto settle = [&](int before, auto again) {
         __syncthreads();
-        int count = sh.count;
-        __syncthreads();
-        while (count > kScoreList) {
-            // the n_top-th best of what found room is a bar that the round's and the older candidates can be held to
-            const score_key keep = tid < before ? sh.list[tid] : 0;        // (before is at most kScoreList / 2, a thread for each)
-            score_cut(sh, n_top);
-            if (tid == 0) sh.count = 0;
-            __syncthreads();
-            if (keep != 0 && keep >= sh.bar) sh.list[atomicAdd(&sh.count, 1)] = keep;
-            __syncthreads();
-            before = sh.count;
-            __syncthreads();
-            again();
-            __syncthreads();
-            count = sh.count;
-            __syncthreads();
-        }
-        if (count <= kScoreList / 2) return count;
-        score_cut(sh, n_top);
-        return min(count, n_top);
-    };
-    int before = 0;
-    const int loose_n = rank == 0 ? loose : 0;
-    float lone = -INFINITY;
-    int lone_at = 0;
-    if (tid < loose_n) {
-        lone_at = tid < lead ? tid : tail0 + tid - lead;
-        lone = Vec<T>::one(x + lone_at);
-        add(&lone, 1, lone);
-    }
-    bool first = true;
-    for (int base = v0; base < v1 || first; base += kScoreThreads * PER) {
-        float v[16];
-        uint4 raw[PER];
-#pragma unroll
-        for (int p = 0; p < PER; ++p) {
-            const int i = base + p * kScoreThreads + tid;
-            if (i < v1) raw[p] = __ldcs(xv + i);
-        }
-#pragma unroll
-        for (int p = 0; p < PER; ++p) {
-            if (base + p * kScoreThreads + tid < v1) {
-                Vec<T>::get(raw[p], v + p * VN);
-            } else {
-#pragma unroll
-                for (int i = 0; i < VN; ++i) v[p * VN + i] = -INFINITY;
+        ScoreSums mine = {kScoreFloor, 0.0f, 0.0f, 0.0f};
+        auto add = [&](const float *v, int n, float top) {
+            if (!(top < INFINITY)) mine.bad = 1.0f;
+            if (top > mine.m) {
+                const float d = (mine.m - top) * 1.44269504f, f = ex2s(fmaxf(d, -200.0f));
+                mine.t = f > 0.0f ? (mine.t + d * mine.s) * f : 0.0f;
+                mine.s *= f;
+                mine.m = top;
             }
-        }
-        float top = v[0];
+            float s = 0.0f, t = 0.0f;
 #pragma unroll
-        for (int i = 1; i < 16; ++i) top = max_nan(top, v[i]);
-        if (top > -INFINITY || top != top) add(v, 16, top);
-        if (n_top > 0) {
-            auto index = [&](int i) { return lead + (base + (i / VN) * kScoreThreads + tid) * VN + i % VN; };
-            if (first) {
-                // the first bar: any value that at least n_top of the threads' maxima reach, as high as 16 halvings find
-                const float most = top == top ? fmaxf(top, lone) : lone;
-                const uint32_t o = most > -INFINITY ? order_of(most) : 0u;
-                uint32_t bar = 0;
-                for (int b = 31; b >= 16; --b) {
-                    const uint32_t with = bar | 1u << b;
-                    if (__syncthreads_count(o >= with) >= n_top) bar = with;
+            for (int i = 0; i < 16; ++i)
+                if (i < n) {
+                    const float y = fmaxf((v[i] - mine.m) * 1.44269504f, -200.0f), e = ex2s(y);
+                    s += e;
+                    t = fmaf(e, y, t);
                 }
-                if (tid == 0) sh.bar = max(static_cast<score_key>(1), static_cast<score_key>(bar) << 32);
+            mine.s += s;
+            mine.t += t;
+        };
+        // candidates of a thread's elements; index(i) is the element's place in the row
+        auto offer = [&](const float *v, int n, float top, auto index) {
+            const score_key bar = sh.bar;
+            if (order_of(top) < static_cast<uint32_t>(bar >> 32)) return;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (i < n && v[i] > -INFINITY) {
+                    const score_key k = key_of(v[i], index(i));
+                    if (k >= bar) {
+                        const int at = atomicAdd(&sh.count, 1);
+                        if (at < kScoreList) sh.list[at] = k;
+                    }
+                }
+        };
+        // after a round: a list that ran over is filled again above a higher bar, one that is half full is cut
+        auto settle = [&](int before, auto again) {
+            __syncthreads();
+            int count = sh.count;
+            __syncthreads();
+            while (count > kScoreList) {
+                // the n_top-th best of what found room is a bar that the round's and the older candidates can be held to
+                const score_key keep = tid < before ? sh.list[tid] : 0;        // (before is at most kScoreList / 2, a thread for each)
+                score_cut(sh, n_top);
+                if (tid == 0) sh.count = 0;
+                __syncthreads();
+                if (keep != 0 && keep >= sh.bar) sh.list[atomicAdd(&sh.count, 1)] = keep;
+                __syncthreads();
+                before = sh.count;
+                __syncthreads();
+                again();
+                __syncthreads();
+                count = sh.count;
                 __syncthreads();
             }
-            const bool with_lone = first && tid < loose_n;
-            auto round = [&]() {
-                offer(v, 16, top, index);
-                if (with_lone) offer(&lone, 1, lone, [&](int) { return lone_at; });
-            };
-            round();
-            before = settle(before, round);
-        }
-        first = false;
-    }
-    // the CTA's sums
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const ScoreSums other = {__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.s, o), __shfl_xor_sync(0xffffffffu, mine.t, o),
-                                 __shfl_xor_sync(0xffffffffu, mine.bad, o)};
-        mine = both(mine, other);
-    }
-    if ((tid & 31) == 0) sh.warp_sums[tid >> 5] = mine;
-    if (n_top > 0) score_cut(sh, n_top);
-    __syncthreads();
-    if (tid == 0) {
-        ScoreSums r = sh.warp_sums[0];
-        for (int w = 1; w < kScoreThreads / 32; ++w) r = both(r, sh.warp_sums[w]);
-        sh.sums = r;
-    }
-    cluster.sync();
-    if (rank == 0) {
-        ScoreSums r = sh.sums;
-        for (int c = 1; c < ctas; ++c) r = both(r, *cluster.map_shared_rank(&sh.sums, c));
-        if (n_top > 0 && ctas > 1) {
-            // at most 16 x 32 candidates of the others go behind the own ones
-            for (int i = tid; i < (ctas - 1) * n_top; i += kScoreThreads) {
-                ScoreShared *o = cluster.map_shared_rank(&sh, 1 + i / n_top);
-                if (i % n_top < o->count) sh.list[atomicAdd(&sh.count, 1)] = o->list[i % n_top];
-            }
-            __syncthreads();
+            if (count <= kScoreList / 2) return count;
             score_cut(sh, n_top);
+            return min(count, n_top);
+        };
+        int before = 0;
+        const int loose_n = rank == 0 ? loose : 0;
+        float lone = -INFINITY;
+        int lone_at = 0;
+        if (tid < loose_n) {
+            lone_at = tid < lead ? tid : tail0 + tid - lead;
+            lone = Vec<T>::one(x + lone_at);
+            add(&lone, 1, lone);
         }
-        const bool none = r.bad != 0.0f || !(r.s > 0.0f);
-        const float log_s = logf(r.s);
-        if (tid == 0 && P.entropy) P.entropy[row] = none ? NAN : fmaxf(0.0f, log_s - 0.69314718f * (r.t / r.s));
-        if (tid == 0 && P.logprob) {
-            const int token = P.tokens[row];
-            P.logprob[row] = none || token < 0 || token >= P.vocab ? NAN : (Vec<T>::one(x + token) - r.m) - log_s;
+        bool first = true;
+#pragma unroll 1
+        for (int base = v0; base < v1 || first; base += ROUND) {
+            float v[16];
+            if (base < v1) {
+                // (a copy that never lands makes its row NaN)
+                bool landed = false;
+#pragma unroll 1
+                for (unsigned i = 0; i < kSpinLimit && !landed; ++i) landed = mbar_try_wait(&sh.full[slot], par);
+                if (!landed) mine.bad = 1.0f;
+            }
+            const uint4 *from = reinterpret_cast<const uint4 *>(score_ring + static_cast<size_t>(slot) * ROUND * 16) + tid;
+#pragma unroll
+            for (int p = 0; p < PER; ++p) {
+                if (base + p * kScoreThreads + tid < v1) {
+                    Vec<T>::get(from[p * kScoreThreads], v + p * VN);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < VN; ++i) v[p * VN + i] = -INFINITY;
+                }
+            }
+            const bool filled = base < v1;
+            if (filled && ++slot == SLOTS) {
+                slot = 0;
+                par ^= 1;
+            }
+            float top = v[0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) top = max_nan(top, v[i]);
+            if (top > -INFINITY || top != top) add(v, 16, top);
+            if (n_top > 0) {
+                auto index = [&](int i) { return lead + (base + (i / VN) * kScoreThreads + tid) * VN + i % VN; };
+                if (first) {
+                    // the first bar: any value that at least n_top of the threads' maxima reach, as high as 12 halvings find
+                    const float most = top == top ? fmaxf(top, lone) : lone;
+                    const uint32_t o = most > -INFINITY ? order_of(most) : 0u;
+                    uint32_t bar = 0;
+                    for (int b = 31; b >= 20; --b) {
+                        const uint32_t with = bar | 1u << b;
+                        if (__syncthreads_count(o >= with) >= n_top) bar = with;
+                    }
+                    if (tid == 0) sh.bar = max(static_cast<score_key>(1), static_cast<score_key>(bar) << 32);
+                    __syncthreads();
+                }
+                const bool with_lone = first && tid < loose_n;
+                auto round = [&]() {
+                    offer(v, 16, top, index);
+                    if (with_lone) offer(&lone, 1, lone, [&](int) { return lone_at; });
+                };
+                round();
+                before = settle(before, round);
+            } else {
+                __syncthreads();
+            }
+            if (tid == 0 && filled) ask();         // all threads have read the slot
+            first = false;
         }
-        if (tid < n_top) {
-            const size_t to = static_cast<size_t>(row) * n_top + tid;
-            const bool is = !none && tid < sh.count;
-            const score_key k = is ? sh.list[tid] : 0;
-            P.top_ids[to] = is ? static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)) : -1;
-            P.top_logprobs[to] = none ? NAN : is ? (value_of(static_cast<uint32_t>(k >> 32)) - r.m) - log_s : -INFINITY;
+        // the CTA's sums
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            const ScoreSums other = {__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.s, o), __shfl_xor_sync(0xffffffffu, mine.t, o),
+                                     __shfl_xor_sync(0xffffffffu, mine.bad, o)};
+            mine = both(mine, other);
         }
+        if ((tid & 31) == 0) sh.warp_sums[tid >> 5] = mine;
+        if (n_top > 0) score_cut(sh, n_top);
+        __syncthreads();
+        if (tid == 0) {
+            ScoreSums r = sh.warp_sums[0];
+            for (int w = 1; w < kScoreThreads / 32; ++w) r = both(r, sh.warp_sums[w]);
+            sh.sums = r;
+        }
+        if (ctas > 1) cluster.sync();
+        else __syncthreads();
+        if (rank == 0) {
+            ScoreSums r = sh.sums;
+            for (int c = 1; c < ctas; ++c) r = both(r, *cluster.map_shared_rank(&sh.sums, c));
+            if (n_top > 0 && ctas > 1) {
+                // at most 16 x 32 candidates of the others go behind the own ones
+                for (int i = tid; i < (ctas - 1) * n_top; i += kScoreThreads) {
+                    ScoreShared *o = cluster.map_shared_rank(&sh, 1 + i / n_top);
+                    if (i % n_top < o->count) sh.list[atomicAdd(&sh.count, 1)] = o->list[i % n_top];
+                }
+                __syncthreads();
+                score_cut(sh, n_top);
+            }
+            const bool none = r.bad != 0.0f || !(r.s > 0.0f);
+            const float log_s = logf(r.s);
+            if (tid == 0 && P.entropy) P.entropy[row] = none ? NAN : fmaxf(0.0f, log_s - 0.69314718f * (r.t / r.s));
+            if (tid == 0 && P.logprob) {
+                const int token = P.tokens[row];
+                P.logprob[row] = none || token < 0 || token >= P.vocab ? NAN : (Vec<T>::one(x + token) - r.m) - log_s;
+            }
+            if (tid < n_top) {
+                const size_t to = static_cast<size_t>(row) * n_top + tid;
+                const bool is = !none && tid < sh.count;
+                const score_key k = is ? sh.list[tid] : 0;
+                P.top_ids[to] = is ? static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)) : -1;
+                P.top_logprobs[to] = none ? NAN : is ? (value_of(static_cast<uint32_t>(k >> 32)) - r.m) - log_s : -INFINITY;
+            }
+        }
+        // the others' shared memory, and one's own, stay until they have been read
+        if (ctas > 1) cluster.sync();
+        else __syncthreads();
     }
-    cluster.sync();         // the others' shared memory stays until it has been read
 }
 
 template <class T>
-int score_launch(const ScoreParams &p, int ctas, cudaStream_t s) {
+int score_launch(ScoreParams p, int n_sm, cudaStream_t s) {
+    // A row's CTAs: enough that few rows fill the SMs, none with less than a round.
+    p.ctas = 1;
+    while (p.ctas < 8 && static_cast<long long>(p.rows) * p.ctas * 2 <= n_sm && p.vocab >= p.ctas * 2 * kScoreThreads * 16) p.ctas *= 2;
+    const int smem = kSlotsOf<T> * kScoreThreads * 16 * static_cast<int>(sizeof(T));
+    WD_TRY_CUDA(cudaFuncSetAttribute(score_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * ctas);
+    cfg.gridDim = dim3(static_cast<unsigned>(p.rows < n_sm / p.ctas ? p.rows : n_sm / p.ctas) * p.ctas);
     cfg.blockDim = dim3(kScoreThreads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute a[1];
     a[0].id = cudaLaunchAttributeClusterDimension;
-    a[0].val.clusterDim.x = ctas;
+    a[0].val.clusterDim.x = p.ctas;
     a[0].val.clusterDim.y = a[0].val.clusterDim.z = 1;
     cfg.attrs = a;
     cfg.numAttrs = 1;
@@ -346,11 +414,10 @@ extern "C" int wd_token_logprobs(const void *logits_dev, int type, int rows, int
         }
         OnDevice on(at.device);
         if (!on.ok()) return set_error(WD_E_CUDA, "token logprobs: the logits' device");
-        wd::ScoreParams p{logits_dev, stride, rows, vocab, n_top, tokens_dev, logprob_dev, entropy_dev, top_ids_dev, top_logprobs_dev};
-        // a row's CTAs: enough that few rows fill the SMs (two CTAs an SM), none with less than a round of reads
-        int ctas = 1;
-        while (ctas < 8 && static_cast<long long>(rows) * ctas * 2 <= 296 && vocab >= ctas * 2 * wd::kScoreThreads * 16) ctas *= 2;
+        int n_sm = 0;
+        WD_TRY_CUDA(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, at.device));
+        wd::ScoreParams p{logits_dev, stride, rows, vocab, n_top, 1, tokens_dev, logprob_dev, entropy_dev, top_ids_dev, top_logprobs_dev};
         cudaStream_t s = static_cast<cudaStream_t>(stream);
-        return type == WD_TYPE_F32 ? wd::score_launch<float>(p, ctas, s) : type == WD_TYPE_F16 ? wd::score_launch<__half>(p, ctas, s) : wd::score_launch<__nv_bfloat16>(p, ctas, s);
+        return type == WD_TYPE_F32 ? wd::score_launch<float>(p, n_sm, s) : type == WD_TYPE_F16 ? wd::score_launch<__half>(p, n_sm, s) : wd::score_launch<__nv_bfloat16>(p, n_sm, s);
     });
 }
