@@ -77,6 +77,23 @@ def test_rows_that_make_many_candidates(vocab):
             check(got, expected(x[r:r + rows], t[r:r + rows], 32), 32, 100.0)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("vocab", [50, 5000, 140000])
+def test_masks_of_the_lowest_number(dtype, vocab):
+    """The lowest finite value as a mask: beside numbers it has no probability left, alone it is a distribution like any other."""
+    lowest = torch.finfo(TYPES[dtype][0]).min
+    x = torch.randn(4, vocab).to(TYPES[dtype][0])
+    x[0, ::2] = lowest
+    x[1] = lowest
+    x[2] = lowest
+    x[2, vocab // 3] = -float("inf")
+    x[3, :vocab - 3] = lowest
+    t = torch.tensor([1, 5, 7, vocab - 1], dtype=torch.int32)
+    got, want = score(x.cuda(), t.cuda(), 2, dtype), expected(x, t, 2)
+    assert np.abs(got[0] - want[0]).max() < 2e-5 and np.abs(got[1] - want[1]).max() < 2e-5
+    assert np.array_equal(got[2], want[2]) and np.abs(got[3] - want[3]).max() < 2e-5
+
+
 @pytest.mark.parametrize("vocab", [7, 5000, 70000])
 def test_rows_without_a_distribution_and_tokens_outside(vocab):
     x = torch.randn(6, vocab)

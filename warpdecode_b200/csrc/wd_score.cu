@@ -2,11 +2,14 @@
 //
 //   m = max x,  s = sum e^(x - m),  t = sum (x - m) e^(x - m):   log p = x - m - log s,   H = log s - t / s
 //
-// One pass over the logits. A CTA an SM walks over the rows, and a ring of bulk copies runs ahead of it, over the rows' ends too; a row is shared by
-// the CTAs of a cluster where there are few rows (they meet in the first one's shared memory, so that no workspace is needed). A thread keeps its own
-// m, s, t over rounds of 16 elements. The alternatives are collected beside: a key is (order of the value, lowest index first) in 64 bits, a candidate
-// is what is not below the CTA's bar, and the bar comes from the first round (the n_top-th of the threads' maxima, to three bits behind the leading
-// one) and rises when the list of candidates is cut to its n_top best. Behind the first rounds almost no element meets it.
+// One pass over the logits, two CTAs an SM. A thread keeps its own m, s, t over rounds of 16 elements, which it copies into a ring of its own in shared
+// memory, three rounds (F32; six of 16 bits) ahead and over the rows' ends too; it waits for no other thread between a row's first round and its end. A
+// row is shared by the CTAs of a cluster where there are few rows (they meet in the first one's shared memory, so that no workspace is needed).
+//
+// The alternatives are collected beside: a key is (order of the value, lowest index first) in 64 bits, a candidate is what is not below the CTA's bar,
+// and each warp has a list of candidates, which it cuts to its n_top best when it is full. The bar is the n_top-th of the maxima of groups of eight
+// threads (to seven bits behind the leading one; of 64 groups the 20th is met by 24 elements, not 20) after the first round, and what one warp finds
+// it to be after 2, 4, 8, ... rounds, so that few elements behind meet it, whatever their order; a warp that cuts its list raises it too.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -23,7 +26,8 @@ using wd_host::set_error;
 namespace wd {
 namespace {
 
-constexpr int kScoreThreads = 1024, kScoreTop = 32, kScoreList = 1024, kScoreSlots = 6;
+constexpr int kScoreThreads = 512, kScoreWarps = kScoreThreads / 32, kScoreTop = 32, kScoreOwn = 64, kScoreList = kScoreWarps * kScoreTop;
+constexpr int kScoreRing = 12;              // 16 bytes of a thread's ring
 typedef unsigned long long score_key;
 
 struct ScoreParams {
@@ -44,9 +48,9 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 __device__ __forceinline__ score_key key_of(float x, int i) { return static_cast<score_key>(order_of(x)) << 32 | (0xffffffffu - static_cast<uint32_t>(i)); }
 
-__device__ __forceinline__ float max_nan(float a, float b) {        // a NaN stays one
+__device__ __forceinline__ float max_nan(float a, float b, float c) {        // a NaN stays one
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 __device__ __forceinline__ float ex2s(float x) {
@@ -90,59 +94,75 @@ struct Vec<__nv_bfloat16> {
 };
 
 struct ScoreSums {
-    float m, s, t, bad;         // t in units of log 2: sum of y 2^y, y = (x - m) log2 e; bad is not 0 for a row without a distribution
+    float m, s, t, bad;         // s = sum 2^y, t = sum y 2^y, y = (x - m) log2 e; bad is not 0 for a row without a distribution
 };
-constexpr float kScoreFloor = -3.0e38f;     // a maximum over nothing
+constexpr float kScoreLog2e = 1.44269504f, kScoreFloor = -3.402823466e38f;     // a maximum over nothing, and the lowest of a number
 __device__ __forceinline__ ScoreSums both(const ScoreSums &a, const ScoreSums &b) {
     ScoreSums r;
     r.m = fmaxf(a.m, b.m);
-    const float da = (a.m - r.m) * 1.44269504f, db = (b.m - r.m) * 1.44269504f, fa = ex2s(fmaxf(da, -200.0f)), fb = ex2s(fmaxf(db, -200.0f));
+    const float da = fmaxf((a.m - r.m) * kScoreLog2e, -200.0f), db = fmaxf((b.m - r.m) * kScoreLog2e, -200.0f), fa = ex2s(da), fb = ex2s(db);
     r.s = a.s * fa + b.s * fb;
-    r.t = (fa > 0.0f ? (a.t + da * a.s) * fa : 0.0f) + (fb > 0.0f ? (b.t + db * b.s) * fb : 0.0f);
+    r.t = (a.t + da * a.s) * fa + (b.t + db * b.s) * fb;
     r.bad = a.bad + b.bad;
     return r;
 }
 
 struct ScoreShared {
-    score_key list[kScoreList], best[kScoreTop];
-    ScoreSums warp_sums[kScoreThreads / 32], sums;
-    float warp_max[kScoreThreads / 32];
+    score_key own[kScoreWarps][kScoreOwn];          // the warps' candidates
+    int own_count[kScoreWarps];
+    score_key list[kScoreList], best[kScoreTop];    // the row's, at its end
+    ScoreSums warp_sums[kScoreWarps], sums;
+    __align__(16) uint32_t reached[kScoreThreads / 8];            // the groups' maxima, in order
+    score_key others[8][kScoreTop];                 // of a cluster's first CTA: what the CTAs bring
+    ScoreSums other_sums[8];
+    int other_count[8];
     int count;
     score_key bar;
-    uint64_t full[kScoreSlots];
 };
 
-// The list is cut to its n best, in order, and the bar set to the last of them where there are n. All threads; keys are distinct.
-__device__ void score_cut(ScoreShared &sh, int n) {
-    const int tid = threadIdx.x, have = min(sh.count, kScoreList);
-    __syncthreads();
-    for (int i = tid; i < have; i += kScoreThreads) {
+// The list is cut to its n best, in order. All threads; keys are distinct. A warp ranks a key: each lane compares it with some of the others.
+__device__ __forceinline__ void score_cut(ScoreShared &sh, int n) {
+    const int tid = threadIdx.x, lane = tid & 31, have = sh.count;
+    for (int i = tid >> 5; i < have; i += kScoreWarps) {
         const score_key k = sh.list[i];
         int rank = 0;
-        for (int j = 0; j < have; ++j) rank += sh.list[j] > k;
-        if (rank < n) sh.best[rank] = k;
+        for (int j = 0; j < have; j += 32) rank += __popc(__ballot_sync(0xffffffffu, j + lane < have && sh.list[j + lane] > k));
+        if (lane == 0 && rank < n) sh.best[rank] = k;
     }
     __syncthreads();
     const int left = min(have, n);
     if (tid < left) sh.list[tid] = sh.best[tid];
-    if (tid == 0) {
-        sh.count = left;
-        if (left == n) sh.bar = max(sh.bar, sh.best[n - 1]);
-    }
+    if (tid == 0) sh.count = left;
     __syncthreads();
+}
+// A warp's candidates, `count` of them, are cut to their n best; where there are n the last of them is a bar for the row.
+__device__ __forceinline__ int score_cut_own(score_key *own, int count, int n, score_key *bar, int lane) {
+    __syncwarp();
+    const score_key a = lane < count ? own[lane] : 0, b = lane + 32 < count ? own[lane + 32] : 0;
+    int ra = 0, rb = 0;
+    for (int j = 0; j < count; ++j) {
+        const score_key k = own[j];
+        ra += k > a;
+        rb += k > b;
+    }
+    __syncwarp();
+    if (a != 0 && ra < n) own[ra] = a;
+    if (b != 0 && rb < n) own[rb] = b;
+    __syncwarp();
+    const int left = min(count, n);
+    if (lane == 0 && left == n) atomicMax(bar, own[n - 1]);
+    __syncwarp();
+    return left;
 }
 
 template <class T>
-constexpr int kSlotsOf = sizeof(T) == 4 ? 3 : kScoreSlots;        // 192 KB of a round's 16 elements a thread each
-
-template <class T>
-__global__ void __launch_bounds__(kScoreThreads, 1) score_kernel(const __grid_constant__ ScoreParams P) {
+__global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const __grid_constant__ ScoreParams P) {
     extern __shared__ __align__(128) uint8_t score_ring[];
     __shared__ ScoreShared sh;
     cg::cluster_group cluster = cg::this_cluster();
-    const int ctas = P.ctas, rank = ctas > 1 ? static_cast<int>(cluster.block_rank()) : 0, tid = threadIdx.x, n_top = P.n_top;
+    const int ctas = P.ctas, rank = ctas > 1 ? static_cast<int>(cluster.block_rank()) : 0, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_top = P.n_top;
     const int group = static_cast<int>(blockIdx.x) / ctas, groups = static_cast<int>(gridDim.x) / ctas;        // (blocks of a cluster follow one another)
-    constexpr int VN = Vec<T>::kN, PER = 16 / VN, ROUND = kScoreThreads * PER, SLOTS = kSlotsOf<T>;      // elements of 16 bytes, 16 bytes of a thread and of a round
+    constexpr int VN = Vec<T>::kN, PER = 16 / VN, ROUND = kScoreThreads * PER, SLOTS = kScoreRing / PER;       // in 16 bytes: a thread, a round
     // Where a row's reads of 16 bytes are: from the first boundary on. What lies in front and behind are single elements of the first CTA's first round.
     struct Place {
         const T *x;
@@ -158,202 +178,241 @@ __global__ void __launch_bounds__(kScoreThreads, 1) score_kernel(const __grid_co
         p.v1 = min(p.v0 + per_cta, p.n_vec);
         return p;
     };
-    // the ring: the first thread asks for rounds in the order in which they are read
-    int ask_row = group, ask_base = -1, ask_slot = 0;
+    // the ring: rounds are asked for in the order in which they are read, one group of copies each (an empty one behind the last row)
+    uint4 *ring = reinterpret_cast<uint4 *>(score_ring) + tid;
+    int ask_row = group, ask_base = 0, ask_slot = 0;
+    Place ask_at = place(group);
+    ask_base = ask_at.v0;
     auto ask = [&]() {
-        while (ask_row < P.rows) {
-            const Place p = place(ask_row);
-            if (ask_base < 0) ask_base = p.v0;
-            if (ask_base >= p.v1) {
-                ask_row += groups;
-                ask_base = -1;
-                continue;
-            }
-            const uint32_t bytes = static_cast<uint32_t>(min(ROUND, p.v1 - ask_base)) * 16u;
-            mbar_expect_tx(&sh.full[ask_slot], bytes);
-            bulk_load(score_ring + static_cast<size_t>(ask_slot) * ROUND * 16, reinterpret_cast<const uint4 *>(p.x + p.lead) + ask_base, bytes, &sh.full[ask_slot]);
+        if (ask_row < P.rows) {
+            const uint4 *xv = reinterpret_cast<const uint4 *>(ask_at.x + ask_at.lead) + ask_base + tid;
+            const uint32_t to = smem_u32(ring + ask_slot * PER * kScoreThreads);
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (ask_base + i * kScoreThreads + tid < ask_at.v1)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * kScoreThreads * 16), "l"(xv + i * kScoreThreads) : "memory");
             ask_base += ROUND;
             ask_slot = ask_slot + 1 == SLOTS ? 0 : ask_slot + 1;
-            return;
+            if (ask_base >= ask_at.v1 && (ask_row += groups) < P.rows) {
+                ask_at = place(ask_row);
+                ask_base = ask_at.v0;
+            }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (tid == 0) {
-        for (int i = 0; i < SLOTS; ++i) mbar_init(&sh.full[i], 1);
-        mbar_fence_init();
-        for (int i = 0; i < SLOTS; ++i) ask();
-    }
+#pragma unroll 1
+    for (int i = 0; i < SLOTS; ++i) ask();
     int slot = 0;
-    uint32_t par = 0;
 #pragma unroll 1
     for (int row = group; row < P.rows; row += groups) {
-        const Place at_row = place(row);
-        const T *x = at_row.x;
-        const int lead = at_row.lead, tail0 = lead + at_row.n_vec * VN, loose = lead + P.vocab - tail0, v0 = at_row.v0, v1 = at_row.v1;
+        const Place at = place(row);
+        const T *x = at.x;
+        const int lead = at.lead, tail0 = lead + at.n_vec * VN, loose = lead + P.vocab - tail0, v0 = at.v0, v1 = at.v1;
+        ScoreSums mine = {kScoreFloor, 0.0f, 0.0f, 0.0f};
         if (tid == 0) {
             sh.count = 0;
             sh.bar = 1;
         }
-        __syncthreads();
-        ScoreSums mine = {kScoreFloor, 0.0f, 0.0f, 0.0f};
-        auto add = [&](const float *v, int n, float top) {
+        if (lane == 0) sh.own_count[warp] = 0;
+        auto grow = [&](float top) {
             if (!(top < INFINITY)) mine.bad = 1.0f;
             if (top > mine.m) {
-                const float d = (mine.m - top) * 1.44269504f, f = ex2s(fmaxf(d, -200.0f));
-                mine.t = f > 0.0f ? (mine.t + d * mine.s) * f : 0.0f;
+                const float d = fmaxf((mine.m - top) * kScoreLog2e, -200.0f), f = ex2s(d);
+                mine.t = (mine.t + d * mine.s) * f;
                 mine.s *= f;
                 mine.m = top;
             }
+        };
+        auto add_clamped = [&](float x) {
+            const float y = fmaxf((x - mine.m) * kScoreLog2e, -200.0f), e = ex2s(y);
+            mine.s += e;
+            mine.t = fmaf(e, y, mine.t);
+        };
+        // 16 elements. A logit of -inf, or one far under the maximum, makes 0 times -inf of a term; then the elements are added one by one.
+        auto add = [&](const float *v, float top) {
+            grow(top);
             float s = 0.0f, t = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (i < n) {
-                    const float y = fmaxf((v[i] - mine.m) * 1.44269504f, -200.0f), e = ex2s(y);
-                    s += e;
-                    t = fmaf(e, y, t);
-                }
-            mine.s += s;
-            mine.t += t;
-        };
-        // candidates of a thread's elements; index(i) is the element's place in the row
-        auto offer = [&](const float *v, int n, float top, auto index) {
-            const score_key bar = sh.bar;
-            if (order_of(top) < static_cast<uint32_t>(bar >> 32)) return;
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (i < n && v[i] > -INFINITY) {
-                    const score_key k = key_of(v[i], index(i));
-                    if (k >= bar) {
-                        const int at = atomicAdd(&sh.count, 1);
-                        if (at < kScoreList) sh.list[at] = k;
-                    }
-                }
-        };
-        // after a round: a list that ran over is filled again above a higher bar, one that is half full is cut
-        auto settle = [&](int before, auto again) {
-            __syncthreads();
-            int count = sh.count;
-            __syncthreads();
-            while (count > kScoreList) {
-                // the n_top-th best of what found room is a bar that the round's and the older candidates can be held to
-                const score_key keep = tid < before ? sh.list[tid] : 0;        // (before is at most kScoreList / 2, a thread for each)
-                score_cut(sh, n_top);
-                if (tid == 0) sh.count = 0;
-                __syncthreads();
-                if (keep != 0 && keep >= sh.bar) sh.list[atomicAdd(&sh.count, 1)] = keep;
-                __syncthreads();
-                before = sh.count;
-                __syncthreads();
-                again();
-                __syncthreads();
-                count = sh.count;
-                __syncthreads();
+            for (int i = 0; i < 16; ++i) {
+                const float y = (v[i] - mine.m) * kScoreLog2e, e = ex2s(y);
+                s += e;
+                t = fmaf(e, y, t);
             }
-            if (count <= kScoreList / 2) return count;
-            score_cut(sh, n_top);
-            return min(count, n_top);
+            if (t == t) {
+                mine.s += s;
+                mine.t += t;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) add_clamped(v[i]);
+            }
         };
-        int before = 0;
-        const int loose_n = rank == 0 ? loose : 0;
+        // A lane's element joins its warp's candidates; false where they are full.
+        auto join = [&](float v, int index) {
+            const int at = atomicAdd(&sh.own_count[warp], 1);
+            if (at < kScoreOwn) sh.own[warp][at] = key_of(v, index);
+            return at < kScoreOwn;
+        };
+        // All lanes: the candidates are cut to their n best.
+        auto make_room = [&]() {
+            __syncwarp();
+            const int left = score_cut_own(sh.own[warp], min(sh.own_count[warp], kScoreOwn), n_top, &sh.bar, lane);
+            if (lane == 0) sh.own_count[warp] = left;
+            __syncwarp();
+        };
+        auto bar_now = [&]() {          // (-inf is no candidate)
+            const uint32_t least = static_cast<uint32_t>(*static_cast<volatile score_key *>(&sh.bar) >> 32);
+            return least ? value_of(least) : -3.402823466e38f;
+        };
+        float given = NAN;          // the given token's logit
+        if (rank == 0 && tid == 0 && P.logprob) {
+            const int token = P.tokens[row];
+            if (token >= 0 && token < P.vocab) given = Vec<T>::one(x + token);
+        }
         float lone = -INFINITY;
         int lone_at = 0;
-        if (tid < loose_n) {
+        const bool with_lone = rank == 0 && loose > 0;
+        if (with_lone && tid < loose) {
             lone_at = tid < lead ? tid : tail0 + tid - lead;
             lone = Vec<T>::one(x + lone_at);
-            add(&lone, 1, lone);
+            grow(lone);
+            add_clamped(lone);
         }
-        bool first = true;
+        __syncthreads();
+        // The bar that the published maxima allow: the n_top-th of them. One warp, and the others may publish meanwhile: whatever it reads is an element
+        // of its own for each group, and any n_top of those are reached by the least of them.
+        auto raise = [&]() {
+            const volatile uint32_t *o = sh.reached;
+            const uint32_t a = o[lane], c = o[lane + 32];
+            int ra = 0, rc = 0;
+#pragma unroll 4
+            for (int i = 0; i < 32; ++i) {
+                const uint32_t x = __shfl_sync(0xffffffffu, a, i), y = __shfl_sync(0xffffffffu, c, i);
+                ra += (x > a) + (y > a);
+                rc += (x > c) + (y > c);
+            }
+            // those that fewer than n_top are above: the least of them
+            const uint32_t least = __reduce_min_sync(0xffffffffu, min(ra < n_top ? a : 0xffffffffu, rc < n_top ? c : 0xffffffffu));
+            if (lane == 0 && least != 0u) atomicMax(&sh.bar, static_cast<score_key>(least) << 32);
+        };
 #pragma unroll 1
-        for (int base = v0; base < v1 || first; base += ROUND) {
+        for (int base = v0, round = 1; base < v1 || round == 1; base += ROUND, ++round) {
             float v[16];
-            if (base < v1) {
-                // (a copy that never lands makes its row NaN)
-                bool landed = false;
-#pragma unroll 1
-                for (unsigned i = 0; i < kSpinLimit && !landed; ++i) landed = mbar_try_wait(&sh.full[slot], par);
-                if (!landed) mine.bad = 1.0f;
-            }
-            const uint4 *from = reinterpret_cast<const uint4 *>(score_ring + static_cast<size_t>(slot) * ROUND * 16) + tid;
+            asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS - 1) : "memory");
+            const uint4 *from = ring + slot * PER * kScoreThreads;
+            slot = slot + 1 == SLOTS ? 0 : slot + 1;
 #pragma unroll
-            for (int p = 0; p < PER; ++p) {
-                if (base + p * kScoreThreads + tid < v1) {
-                    Vec<T>::get(from[p * kScoreThreads], v + p * VN);
-                } else {
+            for (int p = 0; p < PER; ++p) Vec<T>::get(from[p * kScoreThreads], v + p * VN);
+            if (base + ROUND > v1) {        // the row's last round: what lies behind was not copied
 #pragma unroll
-                    for (int i = 0; i < VN; ++i) v[p * VN + i] = -INFINITY;
-                }
-            }
-            const bool filled = base < v1;
-            if (filled && ++slot == SLOTS) {
-                slot = 0;
-                par ^= 1;
+                for (int p = 0; p < PER; ++p)
+                    if (base + p * kScoreThreads + tid >= v1) {
+#pragma unroll
+                        for (int i = 0; i < VN; ++i) v[p * VN + i] = -INFINITY;
+                    }
             }
             float top = v[0];
 #pragma unroll
-            for (int i = 1; i < 16; ++i) top = max_nan(top, v[i]);
-            if (top > -INFINITY || top != top) add(v, 16, top);
+            for (int i = 1; i < 15; i += 2) top = max_nan(top, v[i], v[i + 1]);
+            top = max_nan(top, v[15], v[15]);
+            if (top > -INFINITY || top != top) add(v, top);
             if (n_top > 0) {
-                auto index = [&](int i) { return lead + (base + (i / VN) * kScoreThreads + tid) * VN + i % VN; };
-                if (first) {
-                    // the first bar: any value that at least n_top of the threads' maxima reach, as high as 12 halvings find
-                    const float most = top == top ? fmaxf(top, lone) : lone;
-                    const uint32_t o = most > -INFINITY ? order_of(most) : 0u;
-                    uint32_t bar = 0;
-                    for (int b = 31; b >= 20; --b) {
-                        const uint32_t with = bar | 1u << b;
-                        if (__syncthreads_count(o >= with) >= n_top) bar = with;
+                unsigned late = 0;          // candidates that found no room
+                if ((round & (round - 1)) == 0) {
+                    uint32_t o = mine.s > 0.0f ? order_of(mine.m) : 0u;
+                    o = max(o, __shfl_xor_sync(0xffffffffu, o, 1));
+                    o = max(o, __shfl_xor_sync(0xffffffffu, o, 2));
+                    o = max(o, __shfl_xor_sync(0xffffffffu, o, 4));
+                    if ((lane & 7) == 0) sh.reached[tid >> 3] = o;
+                    if (round == 1) {
+                        __syncthreads();
+                        if (warp == 0) raise();
+                        __syncthreads();
+                        if (lone >= bar_now()) join(lone, lone_at);          // (fewer than 32)
+                    } else if (warp == (round >> 1) % kScoreWarps) {
+                        raise();
                     }
-                    if (tid == 0) sh.bar = max(static_cast<score_key>(1), static_cast<score_key>(bar) << 32);
-                    __syncthreads();
                 }
-                const bool with_lone = first && tid < loose_n;
-                auto round = [&]() {
-                    offer(v, 16, top, index);
-                    if (with_lone) offer(&lone, 1, lone, [&](int) { return lone_at; });
-                };
-                round();
-                before = settle(before, round);
-            } else {
-                __syncthreads();
-            }
-            if (tid == 0 && filled) ask();         // all threads have read the slot
-            first = false;
-        }
-        // the CTA's sums
+                const float bar_value = bar_now();
+                if (top >= bar_value) {         // some lane now and then (a row with a NaN has no answer)
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            const ScoreSums other = {__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.s, o), __shfl_xor_sync(0xffffffffu, mine.t, o),
-                                     __shfl_xor_sync(0xffffffffu, mine.bad, o)};
-            mine = both(mine, other);
+                    for (int i = 0; i < 16; ++i) late |= v[i] >= bar_value ? 1u << i : 0u;
+#pragma unroll 1
+                    while (late) {              // the values once more, from where they were copied to
+                        const int i = __ffs(late) - 1;
+                        const float y = Vec<T>::one(reinterpret_cast<const T *>(from + i / VN * kScoreThreads) + i % VN);
+                        if (!join(y, lead + (base + i / VN * kScoreThreads + tid) * VN + i % VN)) break;
+                        late &= late - 1;
+                    }
+                }
+                while (__any_sync(0xffffffffu, late != 0u)) {
+                    make_room();
+                    const score_key bar = *static_cast<volatile score_key *>(&sh.bar);
+                    while (late) {
+                        const int i = __ffs(late) - 1, index = lead + (base + i / VN * kScoreThreads + tid) * VN + i % VN;
+                        const float y = Vec<T>::one(reinterpret_cast<const T *>(from + i / VN * kScoreThreads) + i % VN);
+                        if (key_of(y, index) >= bar && !join(y, index)) break;
+                        late &= late - 1;
+                    }
+                }
+            }
+            ask();          // the slot has been read
         }
-        if ((tid & 31) == 0) sh.warp_sums[tid >> 5] = mine;
-        if (n_top > 0) score_cut(sh, n_top);
-        __syncthreads();
-        if (tid == 0) {
-            ScoreSums r = sh.warp_sums[0];
-            for (int w = 1; w < kScoreThreads / 32; ++w) r = both(r, sh.warp_sums[w]);
-            sh.sums = r;
+        // the CTA's sums and candidates
+        auto over_lanes = [&](ScoreSums r) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                const ScoreSums other = {__shfl_xor_sync(0xffffffffu, r.m, o), __shfl_xor_sync(0xffffffffu, r.s, o), __shfl_xor_sync(0xffffffffu, r.t, o),
+                                         __shfl_xor_sync(0xffffffffu, r.bad, o)};
+                r = both(r, other);
+            }
+            return r;
+        };
+        mine = over_lanes(mine);
+        if (lane == 0) sh.warp_sums[warp] = mine;
+        __syncthreads();        // the bar is the row's last
+        if (n_top > 0) {
+            if (sh.own_count[warp] > kScoreTop) make_room();
+            const score_key bar = sh.bar;
+            for (int i = lane; i < min(sh.own_count[warp], kScoreOwn); i += 32) {
+                const score_key k = sh.own[warp][i];
+                if (k >= bar) sh.list[atomicAdd(&sh.count, 1)] = k;
+            }
+            __syncthreads();
+            score_cut(sh, n_top);
         }
-        if (ctas > 1) cluster.sync();
-        else __syncthreads();
+        const ScoreSums nothing = {kScoreFloor, 0.0f, 0.0f, 0.0f};
+        if (tid < 32) {
+            const ScoreSums r = over_lanes(tid < kScoreWarps ? sh.warp_sums[tid] : nothing);
+            if (tid == 0) {
+                sh.sums = r;
+                if (ctas > 1) {
+                    ScoreShared *to = cluster.map_shared_rank(&sh, 0);
+                    to->other_sums[rank] = r;
+                    to->other_count[rank] = sh.count;
+                }
+            }
+        }
+        if (ctas > 1) {
+            if (tid < sh.count) cluster.map_shared_rank(&sh, 0)->others[rank][tid] = sh.list[tid];
+            cluster.sync();
+        } else {
+            __syncthreads();
+        }
         if (rank == 0) {
             ScoreSums r = sh.sums;
-            for (int c = 1; c < ctas; ++c) r = both(r, *cluster.map_shared_rank(&sh.sums, c));
-            if (n_top > 0 && ctas > 1) {
-                // at most 16 x 32 candidates of the others go behind the own ones
-                for (int i = tid; i < (ctas - 1) * n_top; i += kScoreThreads) {
-                    ScoreShared *o = cluster.map_shared_rank(&sh, 1 + i / n_top);
-                    if (i % n_top < o->count) sh.list[atomicAdd(&sh.count, 1)] = o->list[i % n_top];
+            if (ctas > 1) {
+                r = over_lanes(lane < ctas ? sh.other_sums[lane] : nothing);
+                if (n_top > 0) {
+                    if (tid >= n_top && tid < ctas * n_top && tid % n_top < sh.other_count[tid / n_top])        // (at most 8 x 32; the own ones are there)
+                        sh.list[atomicAdd(&sh.count, 1)] = sh.others[tid / n_top][tid % n_top];
+                    __syncthreads();
+                    score_cut(sh, n_top);
                 }
-                __syncthreads();
-                score_cut(sh, n_top);
             }
             const bool none = r.bad != 0.0f || !(r.s > 0.0f);
             const float log_s = logf(r.s);
             if (tid == 0 && P.entropy) P.entropy[row] = none ? NAN : fmaxf(0.0f, log_s - 0.69314718f * (r.t / r.s));
-            if (tid == 0 && P.logprob) {
-                const int token = P.tokens[row];
-                P.logprob[row] = none || token < 0 || token >= P.vocab ? NAN : (Vec<T>::one(x + token) - r.m) - log_s;
-            }
+            if (tid == 0 && P.logprob) P.logprob[row] = none ? NAN : (given - r.m) - log_s;
             if (tid < n_top) {
                 const size_t to = static_cast<size_t>(row) * n_top + tid;
                 const bool is = !none && tid < sh.count;
@@ -362,9 +421,7 @@ __global__ void __launch_bounds__(kScoreThreads, 1) score_kernel(const __grid_co
                 P.top_logprobs[to] = none ? NAN : is ? (value_of(static_cast<uint32_t>(k >> 32)) - r.m) - log_s : -INFINITY;
             }
         }
-        // the others' shared memory, and one's own, stay until they have been read
-        if (ctas > 1) cluster.sync();
-        else __syncthreads();
+        __syncthreads();        // what the next row begins with anew has been read (a cluster has no next row: its first CTA has one place for the others')
     }
 }
 
@@ -372,11 +429,13 @@ template <class T>
 int score_launch(ScoreParams p, int n_sm, cudaStream_t s) {
     // A row's CTAs: enough that few rows fill the SMs, none with less than a round.
     p.ctas = 1;
-    while (p.ctas < 8 && static_cast<long long>(p.rows) * p.ctas * 2 <= n_sm && p.vocab >= p.ctas * 2 * kScoreThreads * 16) p.ctas *= 2;
-    const int smem = kSlotsOf<T> * kScoreThreads * 16 * static_cast<int>(sizeof(T));
+    while (p.ctas < 8 && static_cast<long long>(p.rows) * p.ctas * 2 <= 2 * n_sm && p.vocab >= p.ctas * 2 * kScoreThreads * 16) p.ctas *= 2;
+    const int most = 2 * n_sm / p.ctas;         // groups of CTAs at once; a cluster has one row (p.rows * p.ctas <= 2 * n_sm)
+    constexpr int smem = kScoreThreads * kScoreRing * 16;
+    static_assert(2 * (smem + sizeof(ScoreShared) + 1024) <= 228 * 1024, "two CTAs an SM");
     WD_TRY_CUDA(cudaFuncSetAttribute(score_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(p.rows < n_sm / p.ctas ? p.rows : n_sm / p.ctas) * p.ctas);
+    cfg.gridDim = dim3(static_cast<unsigned>(p.rows < most ? p.rows : most) * p.ctas);
     cfg.blockDim = dim3(kScoreThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
