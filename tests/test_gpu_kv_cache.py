@@ -345,3 +345,43 @@ def test_calls_out_of_order_and_bad_arguments():
         wd.KvCache(1, 8, 2, 64, 8, 2, 100, device=99)
     with pytest.raises(wd.WdError, match="fit"):
         wd.KvCache(64, 8, 8, 256, 1 << 20, 2, 100, page_tokens=128)
+
+
+@pytest.mark.parametrize("geometry", GEOMETRY)
+@pytest.mark.parametrize("lengths,counts", [([128], [128]), ([130], [97]), ([400, 260, 7], [300, 1, 7]), ([513], [513]), ([1500, 700], [200, 333])])
+def test_attention_of_a_prompt(geometry, lengths, counts):
+    p = Pair(*geometry)
+    seqs = list(range(len(lengths)))
+    before = [n - c for n, c in zip(lengths, counts)]
+    if sum(before):
+        p.step(seqs, before)
+    p.step(seqs, counts)
+    p.check_attend(seqs, counts)
+    assert p.kv.status() == 0
+
+
+@pytest.mark.parametrize("geometry", [(8, 2, 64, 16, 0, "f32"), (8, 1, 128, 32, 1, "bf16"), (16, 2, 256, 64, 0, "f32"), (6, 2, 96, 128, 0, "f16")])
+@pytest.mark.parametrize("window", [1, 63, 200, 1000])
+def test_attention_of_a_prompt_in_a_window(geometry, window):
+    p = Pair(*geometry)
+    p.step([0, 1, 2], [500, 0, 30])
+    p.step([2, 0, 1], [170, 259, 600])
+    p.check_attend([2, 0, 1], [170, 259, 600], window=window)
+
+
+def test_rows_of_a_prompt_far_apart_in_size():
+    """A few rows of a tile whose scores leap (the sums are brought to a new maximum), rows of zeros, rows of 1e30 and of 1e-30."""
+    p = Pair(8, 2, 64, 16, 0, "f32")
+    k, v = p.rows(600), p.rows(600)
+    k *= torch.linspace(0.1, 30, 600)[:, None, None]
+    v[100:120] *= 1e5
+    p.step([0], [600], rows=[(k, v)] * 2)
+    q = p.rand(600, 8, 64)
+    q[5], q[200:210], q[17] = 0.0, q[200:210] * 30, q[17] * 1e-30
+    got, want, _ = p.attend([0], [600], q=q)
+    values = np.abs(p.ref[1].numbers(0)[1]).max()
+    # scores up to 30 * 30 * 8 * 5 / 8 = 4,500, in F32: 4,500 * 2^-23 of a weight, and what comes of q's terms
+    assert np.abs(got - want).max() <= (4500 * 64 * 2.0 ** -24 + 2.0 ** -18) * values
+    small = np.ones(600, bool)
+    small[200:210] = False
+    assert np.linalg.norm((got - want)[small]) <= 2e-4 * np.linalg.norm(want[small])

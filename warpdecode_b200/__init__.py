@@ -19,10 +19,10 @@ SOURCES = [os.path.join(HERE, "csrc", f) for f in
            ("wd_engine.cu", "wd_aux_kernels.cuh", "wd_moe_kernel.cuh", "wd_moe_kernel_phases.inc", "wd_moe_fast.cuh", "wd_moe_batch.cuh", "wd_dense_decoder.cuh", "wd_dense_decoder.inc", "wd_dense_token.cuh", "wd_dense_prefill.cuh", "wd_dense_prompt_tc.cuh",
             "wd_plain_moe.cuh", "wd_plain_wide.cuh", "wd_plain_moe.inc", "wd_blocks.cuh", "wd_router.cuh",
             "wd_formats.cuh", "wd_device.cuh", "wd_dense.cuh", "wd_gguf.inc",
-            "wd_grids.h", "wd_host.h", "wd_kv.cu", "wd_kv_layout.cuh", "wd_kv_kernels.cuh", "wd_kv_attend.cuh", "wd_score.cu")] + [
+            "wd_grids.h", "wd_host.h", "wd_tcgen05.cuh", "wd_kv.cu", "wd_kv_layout.cuh", "wd_kv_kernels.cuh", "wd_kv_attend.cuh", "wd_kv_prompt.cuh", "wd_score.cu")] + [
                os.path.join(ROOT, "include", "warpdecode_b200.h")]
 UNITS = {"wd_engine": [s for s in SOURCES if not os.path.basename(s).startswith(("wd_kv", "wd_score"))],        # translation units, and what they include
-         "wd_kv": [s for s in SOURCES if os.path.basename(s).startswith(("wd_kv", "wd_device", "wd_host", "warpdecode"))],
+         "wd_kv": [s for s in SOURCES if os.path.basename(s).startswith(("wd_kv", "wd_device", "wd_tcgen05", "wd_host", "warpdecode"))],
          "wd_score": [s for s in SOURCES if os.path.basename(s).startswith(("wd_score", "wd_device", "wd_host", "warpdecode"))]}
 
 TYPE_F16, TYPE_BF16 = 1, 30

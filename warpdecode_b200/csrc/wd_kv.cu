@@ -11,6 +11,7 @@
 #include "wd_host.h"
 #include "wd_kv_attend.cuh"
 #include "wd_kv_kernels.cuh"
+#include "wd_kv_prompt.cuh"
 
 using wd_host::OnDevice;
 using wd_host::set_error;
@@ -183,6 +184,9 @@ int flush(wd_kv_cache *c, cudaStream_t s) {
     return WD_OK;
 }
 
+// Rows of a sequence and kv head from which a step's attention runs on the tensor cores that work on tiles of 128.
+constexpr long long kPromptRows = 96;
+
 template <class F>
 int by_codes(const wd_kv_cache *c, F &&f) {
     return c->shape.e4m3 ? f(std::true_type{}) : f(std::false_type{});
@@ -218,6 +222,22 @@ int attend_of(wd_kv_cache *c, wd::KvAttend &p, bool few, cudaStream_t s) {
     if constexpr (D > 128) few = true;       // (the sums of 16 rows of 256 do not fit a warp's registers)
     if (p.type == wd::kRowsF32) return few ? attend_launch<D, 1, true>(c, p, s) : attend_launch<D, (D > 128 ? 1 : 2), true>(c, p, s);
     return few ? attend_launch<D, 1, false>(c, p, s) : attend_launch<D, (D > 128 ? 1 : 2), false>(c, p, s);
+}
+
+template <int D, bool SPLIT>
+int prompt_launch(wd_kv_cache *c, const wd::KvPrompt &p, cudaStream_t s) {
+    return by_codes(c, [&](auto e4m3) {
+        auto kernel = wd::kv_prompt_kernel<D, SPLIT, decltype(e4m3)::value>;
+        constexpr int smem = wd::PromptAttPlan<D, SPLIT>::kSmem;
+        WD_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        kernel<<<c->n_sm, wd::kPromptThreads, smem, s>>>(p);
+        WD_TRY_CUDA(cudaGetLastError());
+        return WD_OK;
+    });
+}
+template <int D>
+int prompt_of(wd_kv_cache *c, const wd::KvPrompt &p, cudaStream_t s) {
+    return p.type == wd::kRowsF32 ? prompt_launch<D, true>(c, p, s) : prompt_launch<D, false>(c, p, s);
 }
 
 }  // namespace
@@ -423,8 +443,24 @@ int wd_kv_attend(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, in
         p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
         p.window = window;
         p.s = c->shape;
-        const bool few = static_cast<long long>(c->max_rows) * (c->cfg.n_heads / c->cfg.n_kv_heads) <= 8;
+        const long long group = static_cast<long long>(c->max_rows) * (c->cfg.n_heads / c->cfg.n_kv_heads);
         cudaStream_t s = static_cast<cudaStream_t>(stream);
+        if (group >= kPromptRows) {
+            wd::KvPrompt r;
+            r.pool = p.pool, r.scales = p.scales, r.book = p.book, r.table = p.table, r.q = p.q, r.out = p.out;
+            r.q_stride = p.q_stride, r.out_stride = p.out_stride, r.status = p.status, r.scale_log2 = p.scale_log2;
+            r.type = p.type, r.window = p.window, r.s = p.s;
+            const size_t size = rows_size(p.type);
+            r.vec = (reinterpret_cast<uintptr_t>(q_dev) | reinterpret_cast<uintptr_t>(out_dev)) % 16 == 0 && p.q_stride * size % 16 == 0 && p.out_stride * size % 16 == 0;
+            switch (c->cfg.head_dim) {
+                case 32: return prompt_of<32>(c, r, s);
+                case 64: return prompt_of<64>(c, r, s);
+                case 96: return prompt_of<96>(c, r, s);
+                case 128: return prompt_of<128>(c, r, s);
+                default: return prompt_of<256>(c, r, s);
+            }
+        }
+        const bool few = group <= 8;
         switch (c->cfg.head_dim) {
             case 32: return attend_of<32>(c, p, few, s);
             case 64: return attend_of<64>(c, p, few, s);

@@ -1,0 +1,466 @@
+// Attention over the 8-bit cache for many rows (a prompt's chunk), on the fifth-generation tensor cores. The arithmetic is that of the kernel for few
+// rows (wd_kv_attend.cuh): q = 2^e (hi + lo) in F16, codes exact in F16, P = 2^(x + log2 sv - m) in F16 (hi + lo for F32 rows), the denominator takes
+// P / sv in F32; lo is left out for rows of 16 bits.
+//
+// An item is 128 TILES rows of one kv head of a sequence (the G query heads of a token are neighbouring rows) against the tokens that they see, KT = 128
+// at a time (64 where F32 rows of 256 leave no room). Scores, then weights in their place, and sums are in tensor memory:
+//
+//   warps 0 .. 3, 4 .. 7   a row tile each, a thread a row: scores -> weights; the sums are brought to a new maximum only when it has grown by 2^8
+//                          (the weights stay below 256, which F16 holds as exactly), then the answer at the item's end
+//   warps 8 .. 11          codes -> F16 operands in shared memory, K-major without swizzle; the tokens of a sub-block are taken in the order in which a
+//                          value's bytes have them, for keys and values alike
+//   warp 12                issues the products: P V of a tile, then Q K of its next tokens, the two row tiles in turn
+//
+// Items are dealt out heaviest first, back and forth over the CTAs (the last rows of a sequence see the most).
+#pragma once
+
+#include "wd_kv_attend.cuh"
+#include "wd_tcgen05.cuh"
+
+namespace wd {
+
+constexpr int kPromptThreads = 512;
+// Registers a thread: two warpgroups that work on scores take what the two others give back (128 at launch).
+constexpr int kPromptRegsMore = 168, kPromptRegsLess = 88;
+static_assert(2 * (kPromptRegsMore + kPromptRegsLess) <= 4 * 128, "more than the block was launched with: the increase would wait for ever");
+
+struct KvPrompt {
+    const uint8_t *pool;        // of the layer
+    const float *scales;        // of the layer
+    const int *book;
+    const int *table;
+    const void *q;
+    void *out;
+    long long q_stride, out_stride;
+    unsigned *status;
+    float scale_log2;
+    int type, window, vec;      // vec: rows of q and out lie on boundaries of 16 bytes
+    KvShape s;
+};
+
+template <int D, bool SPLIT>
+struct PromptAttPlan {
+    static constexpr int kTiles = D <= 128 ? 2 : 1, kKt = D == 256 && SPLIT ? 64 : 128, kRows = 128 * kTiles;
+    static constexpr int kQ = 128 * D * 2, kQTile = kQ * (SPLIT ? 2 : 1);               // bytes: a tile's hi (or lo), both
+    static constexpr int kKStep = kKt * 16, kK = D / 8 * kKStep;                        // eight elements of the head of all tokens, all of them
+    static constexpr int kVStep = D * 16 + 64, kV = kKt / 8 * kVStep;                   // eight tokens of all elements (and 64 bytes, which spread the stores over the banks)
+    static constexpr int kStages = kTiles * kQTile + 2 * (kK + kV) <= 216 * 1024 ? 2 : 1;
+    static constexpr int kSmem = kTiles * kQTile + kStages * (kK + kV) + (kAttMaxSeqs + 4) * 4 + 1024;
+    static constexpr int kColO = 128 * kTiles;                                          // tensor memory: scores of each tile, then sums
+    static constexpr uint32_t kIdescS = 1u << 4 | (kKt >> 3) << 17 | (128 >> 4) << 24, kIdescO = 1u << 4 | (D >> 3) << 17 | (128 >> 4) << 24;
+    static_assert(kColO + kTiles * D <= 512 && kSmem <= 226 * 1024, "plan of the memories");
+};
+
+struct PromptItem {
+    int seq, row0, count, length, head, item_row, rows, lo, hi;         // rows: of the sequence and head; lo .. hi - 1: tiles of KT tokens
+};
+
+template <int D, bool SPLIT, bool E4M3>
+__global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __grid_constant__ KvPrompt P) {
+    using A = PromptAttPlan<D, SPLIT>;
+    constexpr int KT = A::kKt, T = A::kTiles, ST = A::kStages, CW = D % 64 == 0 ? 64 : 32, SUBS = KT / 16;
+    extern __shared__ __align__(1024) uint8_t psm[];
+    __shared__ __align__(8) uint64_t q_full, k_full[ST], k_free[ST], v_full[ST], v_free[ST], s_full[T], p_full[T], o_done[T];
+    __shared__ __align__(16) float4 scales[4][SUBS];
+    __shared__ uint32_t tmem_base;
+    uint8_t *qs = psm, *ks = psm + T * A::kQTile, *vs = ks + ST * A::kK;
+    int *prefix = reinterpret_cast<int *>(vs + ST * A::kV);
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const int n_seq = P.book[0], g_heads = P.s.heads / P.s.kv_heads, H = P.s.kv_heads;
+    const int *entries = P.book + kKvHead;
+    if (warp == 0) {
+        if (lane == 0) {
+            mbar_init(&q_full, 128 * T);
+            for (int i = 0; i < ST; ++i) {
+                mbar_init(&k_full[i], 128);
+                mbar_init(&v_full[i], 128);
+                mbar_init(&k_free[i], 1);
+                mbar_init(&v_free[i], 1);
+            }
+            for (int i = 0; i < T; ++i) {
+                mbar_init(&s_full[i], 2);         // the products' completion, and the thread that issued them
+                mbar_init(&p_full[i], 128);
+                mbar_init(&o_done[i], 1);
+            }
+            mbar_fence_init();
+        }
+        int sum = 0;
+        for (int i0 = 0; i0 < n_seq; i0 += 32) {
+            const int i = i0 + lane;
+            int inc = 0;
+            if (i < n_seq) inc = static_cast<int>((static_cast<long long>(entries[i * kKvStepWords + 2]) * g_heads + A::kRows - 1) / A::kRows);
+            const int v = inc;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += y;
+            }
+            if (i < n_seq) prefix[i] = sum + inc - v;
+            sum += __shfl_sync(0xffffffffu, inc, 31);
+        }
+        if (lane == 0) prefix[n_seq] = sum;
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_base)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tm = tmem_base;
+    const long long n_items = static_cast<long long>(prefix[n_seq]) * H;
+
+    // item number `turn` of this CTA; false behind the last
+    auto item_of = [&](int turn, PromptItem &it) {
+        const long long at = static_cast<long long>(turn) * gridDim.x + (turn & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        if (at >= n_items) return false;
+        int lo = 0, hi = n_seq - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (static_cast<long long>(prefix[mid]) * H <= at) lo = mid;
+            else hi = mid - 1;
+        }
+        const int *e = entries + lo * kKvStepWords;
+        it.seq = e[0], it.row0 = e[1], it.count = e[2], it.length = e[3];
+        const int in = static_cast<int>(at - static_cast<long long>(prefix[lo]) * H), blocks = prefix[lo + 1] - prefix[lo];
+        it.head = in % H;
+        it.item_row = (blocks - 1 - in / H) * A::kRows;
+        it.rows = it.count * g_heads;
+        const int start = it.length - it.count, pos0 = start + it.item_row / g_heads, pos1 = start + min(it.item_row + A::kRows - 1, it.rows - 1) / g_heads;
+        it.lo = P.window ? max(0, pos0 - P.window + 1) / KT : 0;
+        it.hi = pos1 / KT + 1;
+        return true;
+    };
+
+    PromptItem it;
+    if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptRegsLess));
+        if (warp == 12 && lane == 0) {
+            int k = 0, v = 0, items = 0;            // tiles of keys and of values that products have been issued for, items
+            int n_p[2] = {0, 0};
+            auto score = [&](int x) {               // of key tile k
+                const uint32_t d = tm + x * 128;
+                const uint32_t q0 = smem_u32(qs + x * A::kQTile), k0 = smem_u32(ks + (k % ST) * A::kK);
+#pragma unroll 4
+                for (int i = 0; i < D / 16; ++i)
+                    tc_mma_f16(d, tc_smem_desc(q0 + i * 4096, 2048), tc_smem_desc(k0 + i * 2 * A::kKStep, A::kKStep), A::kIdescS, i > 0);
+                if constexpr (SPLIT) {
+#pragma unroll 4
+                    for (int i = 0; i < D / 16; ++i)
+                        tc_mma_f16(d, tc_smem_desc(q0 + A::kQ + i * 4096, 2048), tc_smem_desc(k0 + i * 2 * A::kKStep, A::kKStep), A::kIdescS, 1);
+                }
+                tc_commit(&s_full[x]);
+                mbar_arrive(&s_full[x]);        // what this thread saw of the keys' warps, for those who read the scales
+            };
+            auto weigh = [&](int x, bool add) {     // with value tile v
+                const uint32_t d = tm + A::kColO + x * D, p = tm + x * 128, v0 = smem_u32(vs + (v % ST) * A::kV);
+#pragma unroll 4
+                for (int i = 0; i < KT / 16; ++i) {
+                    const uint64_t desc = tc_smem_desc(v0 + i * 2 * A::kVStep, A::kVStep);
+                    tc_mma_f16_t(d, p + i / 2 * 32 + i % 2 * 8, desc, A::kIdescO, add || i > 0);
+                    if constexpr (SPLIT) tc_mma_f16_t(d, p + i / 2 * 32 + i % 2 * 8 + 16, desc, A::kIdescO, 1);
+                }
+                tc_commit(&o_done[x]);
+                ++n_p[x];
+            };
+            for (int turn = 0; item_of(turn, it); ++turn, ++items) {
+                const int n = it.hi - it.lo;
+                att_wait(&q_full, items & 1, P.status);
+                att_wait(&k_full[k % ST], k / ST & 1, P.status);
+                tc_fence_after();
+                for (int x = 0; x < T; ++x) {
+                    if (n_p[x] > 0) att_wait(&o_done[x], (n_p[x] - 1) & 1, P.status);       // the last item's weights lie where these scores go
+                    score(x);
+                }
+                tc_commit(&k_free[k % ST]);
+                ++k;
+                for (int j = 0; j < n; ++j) {
+                    att_wait(&v_full[v % ST], v / ST & 1, P.status);
+                    if (j + 1 < n) att_wait(&k_full[k % ST], k / ST & 1, P.status);
+                    for (int x = 0; x < T; ++x) {
+                        att_wait(&p_full[x], n_p[x] & 1, P.status);
+                        tc_fence_after();
+                        weigh(x, j > 0);
+                        if (x == T - 1) tc_commit(&v_free[v % ST]);
+                        if (j + 1 < n) {
+                            att_wait(&o_done[x], (n_p[x] - 1) & 1, P.status);
+                            score(x);
+                            if (x == T - 1) tc_commit(&k_free[k % ST]);
+                        }
+                    }
+                    ++v;
+                    if (j + 1 < n) ++k;
+                }
+            }
+            for (int x = 0; x < T; ++x)
+                if (n_p[x] > 0) tc_drain(&o_done[x], (n_p[x] - 1) & 1);
+        }
+    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptRegsLess));
+        const int ct = tid - 256, cw = warp - 8, shift = P.s.page_shift;
+        int n = 0;              // tiles so far
+        for (int turn = 0; item_of(turn, it); ++turn) {
+            const int *table = P.table + static_cast<size_t>(it.seq) * P.s.max_pages;
+            const int last_sub = (it.length - 1) >> 4;
+            const uint8_t *head = P.pool + it.head * kv_head_bytes(P.s);
+            // lane l: page of sub-block l of a tile, where the sub-block is in the page, and the scales (behind the last sub-block: the last one)
+            int page = 0, in_page = 0;
+            float2 sc = make_float2(0.0f, 0.0f);
+            auto look_up = [&](int tile) {
+                const int sub = min(tile * SUBS + (lane & (SUBS - 1)), last_sub);
+                page = table[sub >> (shift - 4)];
+                in_page = sub & ((1 << (shift - 4)) - 1);
+                if (cw == 0) sc = *reinterpret_cast<const float2 *>(P.scales + (static_cast<size_t>(page) * H + it.head) * 2);
+            };
+            look_up(it.lo);
+            for (int tile = it.lo; tile < it.hi; ++tile, ++n) {
+                const size_t at = static_cast<size_t>(page) * kv_page_bytes(P.s) + static_cast<size_t>(in_page) * (16 * D);
+                const float vsc = sc.y > 0.0f ? sc.y : kKvLeastScale;
+                const float4 mine = make_float4(sc.x, log2f(vsc), 1.0f / vsc, 0.0f);
+                const int st = n % ST;
+                const uint32_t par = (static_cast<uint32_t>(n / ST) & 1u) ^ 1u;
+                // keys: unit u is 16 elements of token u % KT
+                constexpr int KU = KT * D / 16 / 128, KB = KU < 8 ? KU : 8;
+                const int row = ct % KT, sub = row >> 4, place = row & 15, token = (place >> 2) * 2 + (place & 1) + ((place & 2) << 2);
+                const uint8_t *kp = head + __shfl_sync(0xffffffffu, at, sub) + token * CW;
+                auto key_at = [&](int i) {
+                    const int k16 = (i * 128 + ct) / KT * 16;
+                    return reinterpret_cast<const uint4 *>(kp + k16 / CW * (16 * CW) + k16 % CW);
+                };
+                uint4 raw[KB];
+#pragma unroll
+                for (int i = 0; i < KB; ++i) raw[i] = __ldg(key_at(i));
+                att_wait(&k_free[st], par, P.status);
+#pragma unroll
+                for (int b = 0; b < KU; b += KB) {
+                    if (b > 0) {
+#pragma unroll
+                        for (int i = 0; i < KB; ++i) raw[i] = __ldg(key_at(b + i));
+                    }
+#pragma unroll
+                    for (int i = 0; i < KB; ++i) {
+                        const int k16 = ((b + i) * 128 + ct) / KT;
+                        uint4 *to = reinterpret_cast<uint4 *>(ks + st * A::kK + k16 * 2 * A::kKStep + row * 16);
+                        uint4 lo, hi;
+                        kv_halves<E4M3>(raw[i].x, lo.x, lo.y);
+                        kv_halves<E4M3>(raw[i].y, lo.z, lo.w);
+                        kv_halves<E4M3>(raw[i].z, hi.x, hi.y);
+                        kv_halves<E4M3>(raw[i].w, hi.z, hi.w);
+                        to[0] = lo;
+                        to[A::kKStep / 16] = hi;
+                    }
+                }
+                if (cw == 0 && lane < SUBS) scales[n & 3][lane] = mine;
+                fence_proxy_async();
+                mbar_arrive(&k_full[st]);
+                // values: a warp takes 512 bytes (16 tokens of 32 elements) at a time
+                constexpr int VU = SUBS * (D / 32) / 4, VB = VU < 8 ? VU : 8;
+                auto value_at = [&](int i) {
+                    const int u = i * 4 + cw, s = u / (D / 32), blk = u % (D / 32);
+                    return reinterpret_cast<const uint4 *>(head + __shfl_sync(0xffffffffu, at, s) + kv_half_bytes(P.s) + blk * 512 + lane * 16);
+                };
+                uint4 val[VB];
+#pragma unroll
+                for (int i = 0; i < VB; ++i) val[i] = __ldg(value_at(i));
+                if (tile + 1 < it.hi) look_up(tile + 1);
+                att_wait(&v_free[st], par, P.status);
+                const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+                for (int b = 0; b < VU; b += VB) {
+                    if (b > 0) {
+#pragma unroll
+                        for (int i = 0; i < VB; ++i) val[i] = __ldg(value_at(b + i));
+                    }
+#pragma unroll
+                    for (int i = 0; i < VB; ++i) {
+                        const int u = (b + i) * 4 + cw, s = u / (D / 32), blk = u % (D / 32);
+                        uint8_t *to = vs + st * A::kV + (2 * s + (t >> 1)) * A::kVStep + (blk * 32 + g) * 16 + (t & 1) * 8;
+                        const uint32_t w[4] = {val[i].x, val[i].y, val[i].z, val[i].w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint2 h;
+                            kv_halves<E4M3>(w[j], h.x, h.y);
+                            *reinterpret_cast<uint2 *>(to + j * 128) = h;
+                        }
+                    }
+                }
+                fence_proxy_async();
+                mbar_arrive(&v_full[st]);
+            }
+        }
+    } else if (warp < 4 * T) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromptRegsMore));
+        const int x = warp >> 2, r = tid & 127;
+        const uint32_t lanes = tm + (static_cast<uint32_t>((warp & 3) * 32) << 16), sc = lanes + x * 128, oc = lanes + A::kColO + x * D;
+        int n_s = 0, n_o = 0, n = 0;
+        for (int turn = 0; item_of(turn, it); ++turn) {
+            const int row = it.item_row + x * 128 + r, last = it.rows - 1, start = it.length - it.count;
+            const int pos = start + min(row, last) / g_heads;
+            const int warp_row = it.item_row + x * 128 + (warp & 3) * 32, pos_lo = start + min(warp_row, last) / g_heads, pos_hi = start + min(warp_row + 31, last) / g_heads;
+            const bool is = row <= last;
+            const size_t elem = (static_cast<size_t>(it.head) * g_heads + row % g_heads) * D;
+            const size_t src = static_cast<size_t>(it.row0 + row / g_heads) * P.q_stride + elem;
+            // q: the row's largest magnitude, then its F16 terms; element k of row r lies at (k / 8) 2048 + r 16
+            auto load16 = [&](int k, float *y) {
+                if (!is) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) y[i] = 0.0f;
+                } else if (P.type == kRowsF32) {
+                    row_load16(static_cast<const float *>(P.q) + src + k, P.vec != 0, y);
+                } else if (P.type == kRowsF16) {
+                    row_load16(static_cast<const __half *>(P.q) + src + k, P.vec != 0, y);
+                } else {
+                    row_load16(static_cast<const __nv_bfloat16 *>(P.q) + src + k, P.vec != 0, y);
+                }
+            };
+            float top = 0.0f;
+#pragma unroll 1
+            for (int k = 0; k < D; k += 16) {
+                float y[16];
+                load16(k, y);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(y[i]));
+            }
+            const int e = top > 0.0f ? max(-100, min(128, static_cast<int>(__float_as_uint(top) >> 23) - 126)) : 0, e1 = e / 2, e2 = e - e1;
+            const float mul = P.scale_log2 * __uint_as_float((127 + e1) << 23) * __uint_as_float((127 + e2) << 23);
+            const float down = __uint_as_float((127 - e1) << 23), down2 = __uint_as_float((127 - e2) << 23);
+            uint8_t *to = qs + x * A::kQTile + r * 16;
+#pragma unroll 1
+            for (int k = 0; k < D; k += 16) {
+                float y[16];
+                load16(k, y);
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float a = y[2 * i] * down * down2, b = y[2 * i + 1] * down * down2;
+                    hi[i] = half_pair(a, b);
+                    if constexpr (SPLIT) lo[i] = half_rest(a, b, hi[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    *reinterpret_cast<uint4 *>(to + (k / 8 + i) * 2048) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
+                    if constexpr (SPLIT) *reinterpret_cast<uint4 *>(to + A::kQ + (k / 8 + i) * 2048) = make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+                }
+            }
+            fence_proxy_async();
+            mbar_arrive(&q_full);
+            float m = kAttFloor, l = 0.0f;
+#pragma unroll 1
+            for (int tile = it.lo; tile < it.hi; ++tile, ++n) {
+                att_wait(&s_full[x], n_s++ & 1, P.status);
+                tc_fence_after();
+                const int first = tile * KT;
+                const bool edge = first + KT - 1 > pos_lo || (P.window && first <= pos_hi - P.window);
+                // column 16 s + p of the scores is token 2 (p / 4) + (p & 1) + 8 ((p & 3) / 2) of sub-block s
+                auto mask = [&](uint32_t (&v)[32], int c) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int p = i & 15, token = first + c * 32 + (i & 16) + (p >> 2) * 2 + (p & 1) + ((p & 2) << 2);
+                        if (token > pos || (P.window && token <= pos - P.window)) v[i] = 0xff800000u;
+                    }
+                };
+                float most = kAttFloor;
+#pragma unroll
+                for (int c = 0; c < KT / 32; ++c) {
+                    uint32_t v[32];
+                    tc_ld(sc + c * 32, v);
+                    tc_wait_ld(v);
+                    if (edge) mask(v, c);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float4 s4 = scales[n & 3][2 * c + h];
+                        float t = __uint_as_float(v[16 * h]);
+#pragma unroll
+                        for (int i = 1; i < 16; ++i) t = fmaxf(t, __uint_as_float(v[16 * h + i]));
+                        most = fmaxf(most, fmaf(t, fmaxf(mul * s4.x, 1e-37f), s4.y));
+                    }
+                }
+                if (tile == it.lo) {
+                    m = most;
+                } else if (__any_sync(0xffffffffu, most > m + 8.0f)) {
+                    const float now = fmaxf(m, most), f = ex2(m - now);
+                    m = now;
+                    l *= f;
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t v[32];
+                        tc_ld(oc + c * 32, v);
+                        tc_wait_ld(v);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                        tc_st(oc + c * 32, v);
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < KT / 32; ++c) {
+                    uint32_t v[32];
+                    tc_ld(sc + c * 32, v);
+                    tc_wait_ld(v);
+                    if (edge) mask(v, c);
+                    uint32_t hi[16], lo[16];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float4 s4 = scales[n & 3][2 * c + h];
+                        const float mk = fmaxf(mul * s4.x, 1e-37f), off = s4.y - m;
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float a = ex2(fmaf(__uint_as_float(v[16 * h + 2 * i]), mk, off)), b = ex2(fmaf(__uint_as_float(v[16 * h + 2 * i + 1]), mk, off));
+                            sum += a + b;
+                            hi[8 * h + i] = half_pair(a, b);
+                            if constexpr (SPLIT) lo[8 * h + i] = half_rest(a, b, hi[8 * h + i]);
+                        }
+                        l = fmaf(sum, s4.z, l);
+                    }
+                    tc_st(sc + c * 32, hi);
+                    if constexpr (SPLIT) tc_st(sc + c * 32 + 16, lo);
+                }
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(&p_full[x]);
+                ++n_o;
+            }
+            att_wait(&o_done[x], (n_o - 1) & 1, P.status);
+            tc_fence_after();
+            const float inv = 1.0f / l;
+            const size_t dst = static_cast<size_t>(it.row0 + row / g_heads) * P.out_stride + elem;
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+                uint32_t v[16];
+                tc_ld(oc + c * 16, v);
+                tc_wait_ld(v);
+                if (is) {
+                    float y[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) y[i] = __uint_as_float(v[i]) * inv;
+                    auto put = [&](auto *o) {
+                        using R = std::remove_pointer_t<decltype(o)>;
+                        __align__(16) R z[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) z[i] = row_number<R>(y[i]);
+                        if (P.vec) {
+#pragma unroll
+                            for (int i = 0; i < static_cast<int>(sizeof(z)) / 16; ++i) reinterpret_cast<uint4 *>(o)[i] = reinterpret_cast<const uint4 *>(z)[i];
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = z[i];
+                        }
+                    };
+                    if (P.type == kRowsF32) put(static_cast<float *>(P.out) + dst + c * 16);
+                    else if (P.type == kRowsF16) put(static_cast<__half *>(P.out) + dst + c * 16);
+                    else put(static_cast<__nv_bfloat16 *>(P.out) + dst + c * 16);
+                }
+                __syncwarp();
+            }
+            tc_fence_before();      // the sums have been read: the next item's may be written once its weights are there
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromptRegsMore));
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm) : "memory");
+}
+
+}  // namespace wd
