@@ -9,7 +9,8 @@
 //                          (the weights stay below 256, which F16 holds as exactly), then the answer at the item's end
 //   warps 8 .. 11          codes -> F16 operands in shared memory, K-major without swizzle; the tokens of a sub-block are taken in the order in which a
 //                          value's bytes have them, for keys and values alike
-//   warp 12                issues the products: P V of a tile, then Q K of its next tokens, the two row tiles in turn
+//   warp 12                issues the products, the two row tiles in turn: Q K of the next tokens, P V of these (a warp for each tile is slower:
+//                          249 -> 196 us with one, 209 with two)
 //
 // Items are dealt out heaviest first, back and forth over the CTAs (the last rows of a sequence see the most).
 #pragma once
@@ -21,7 +22,7 @@ namespace wd {
 
 constexpr int kPromptThreads = 512;
 // Registers a thread: two warpgroups that work on scores take what the two others give back (128 at launch).
-constexpr int kPromptRegsMore = 168, kPromptRegsLess = 88;
+constexpr int kPromptRegsMore = 176, kPromptRegsLess = 80;
 static_assert(2 * (kPromptRegsMore + kPromptRegsLess) <= 4 * 128, "more than the block was launched with: the increase would wait for ever");
 
 struct KvPrompt {
@@ -46,10 +47,19 @@ struct PromptAttPlan {
     static constexpr int kVStep = D * 16 + 64, kV = kKt / 8 * kVStep;                   // eight tokens of all elements (and 64 bytes, which spread the stores over the banks)
     static constexpr int kStages = kTiles * kQTile + 2 * (kK + kV) <= 216 * 1024 ? 2 : 1;
     static constexpr int kSmem = kTiles * kQTile + kStages * (kK + kV) + (kAttMaxSeqs + 4) * 4 + 1024;
-    static constexpr int kColO = 128 * kTiles;                                          // tensor memory: scores of each tile, then sums
+    // Tensor memory: scores of each tile, then sums, then weights where there is room for them beside the scores. (Then the next scores are made while
+    // a tile's weights still are.)
+    static constexpr int kColO = 128 * kTiles, kColP = kColO + kTiles * D, kWidthP = kKt / 2 * (SPLIT ? 2 : 1);
+    static constexpr bool kApart = kColP + kTiles * kWidthP <= 512;
     static constexpr uint32_t kIdescS = 1u << 4 | (kKt >> 3) << 17 | (128 >> 4) << 24, kIdescO = 1u << 4 | (D >> 3) << 17 | (128 >> 4) << 24;
     static_assert(kColO + kTiles * D <= 512 && kSmem <= 226 * 1024, "plan of the memories");
 };
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 
 struct PromptItem {
     int seq, row0, count, length, head, item_row, rows, lo, hi;         // rows: of the sequence and head; lo .. hi - 1: tiles of KT tokens
@@ -59,8 +69,9 @@ template <int D, bool SPLIT, bool E4M3>
 __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __grid_constant__ KvPrompt P) {
     using A = PromptAttPlan<D, SPLIT>;
     constexpr int KT = A::kKt, T = A::kTiles, ST = A::kStages, CW = D % 64 == 0 ? 64 : 32, SUBS = KT / 16;
+    constexpr int kPartP = A::kApart && !SPLIT ? 16 : 32;           // columns of the weights of 32 tokens
     extern __shared__ __align__(1024) uint8_t psm[];
-    __shared__ __align__(8) uint64_t q_full, k_full[ST], k_free[ST], v_full[ST], v_free[ST], s_full[T], p_full[T], o_done[T];
+    __shared__ __align__(8) uint64_t q_full[T], k_full[ST], k_free[ST], v_full[ST], v_free[ST], s_full[T], s_free[T], p_full[T], o_done[T];
     __shared__ __align__(16) float4 scales[4][SUBS];
     __shared__ uint32_t tmem_base;
     uint8_t *qs = psm, *ks = psm + T * A::kQTile, *vs = ks + ST * A::kK;
@@ -70,7 +81,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
     const int *entries = P.book + kKvHead;
     if (warp == 0) {
         if (lane == 0) {
-            mbar_init(&q_full, 128 * T);
             for (int i = 0; i < ST; ++i) {
                 mbar_init(&k_full[i], 128);
                 mbar_init(&v_full[i], 128);
@@ -79,6 +89,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
             }
             for (int i = 0; i < T; ++i) {
                 mbar_init(&s_full[i], 2);         // the products' completion, and the thread that issued them
+                mbar_init(&q_full[i], 128);
+                mbar_init(&s_free[i], 128);
                 mbar_init(&p_full[i], 128);
                 mbar_init(&o_done[i], 1);
             }
@@ -137,7 +149,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptRegsLess));
         if (warp == 12 && lane == 0) {
             int k = 0, v = 0, items = 0;            // tiles of keys and of values that products have been issued for, items
-            int n_p[2] = {0, 0};
+            int n_p[2] = {0, 0}, n_f[2] = {0, 0};
             auto score = [&](int x) {               // of key tile k
                 const uint32_t d = tm + x * 128;
                 const uint32_t q0 = smem_u32(qs + x * A::kQTile), k0 = smem_u32(ks + (k % ST) * A::kK);
@@ -153,37 +165,50 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
                 mbar_arrive(&s_full[x]);        // what this thread saw of the keys' warps, for those who read the scales
             };
             auto weigh = [&](int x, bool add) {     // with value tile v
-                const uint32_t d = tm + A::kColO + x * D, p = tm + x * 128, v0 = smem_u32(vs + (v % ST) * A::kV);
+                const uint32_t d = tm + A::kColO + x * D, p = tm + (A::kApart ? A::kColP + x * A::kWidthP : x * 128), v0 = smem_u32(vs + (v % ST) * A::kV);
 #pragma unroll 4
                 for (int i = 0; i < KT / 16; ++i) {
                     const uint64_t desc = tc_smem_desc(v0 + i * 2 * A::kVStep, A::kVStep);
-                    tc_mma_f16_t(d, p + i / 2 * 32 + i % 2 * 8, desc, A::kIdescO, add || i > 0);
-                    if constexpr (SPLIT) tc_mma_f16_t(d, p + i / 2 * 32 + i % 2 * 8 + 16, desc, A::kIdescO, 1);
+                    tc_mma_f16_t(d, p + i / 2 * kPartP + i % 2 * 8, desc, A::kIdescO, add || i > 0);
+                    if constexpr (SPLIT) tc_mma_f16_t(d, p + i / 2 * kPartP + i % 2 * 8 + 16, desc, A::kIdescO, 1);
                 }
                 tc_commit(&o_done[x]);
                 ++n_p[x];
             };
             for (int turn = 0; item_of(turn, it); ++turn, ++items) {
                 const int n = it.hi - it.lo;
-                att_wait(&q_full, items & 1, P.status);
                 att_wait(&k_full[k % ST], k / ST & 1, P.status);
-                tc_fence_after();
                 for (int x = 0; x < T; ++x) {
-                    if (n_p[x] > 0) att_wait(&o_done[x], (n_p[x] - 1) & 1, P.status);       // the last item's weights lie where these scores go
+                    att_wait(&q_full[x], items & 1, P.status);
+                    // the last item's scores have been read, or its weights, which lie where these scores go
+                    if (A::kApart && n_p[x] > 0) att_wait(&s_free[x], n_f[x]++ & 1, P.status);
+                    if (!A::kApart && n_p[x] > 0) att_wait(&o_done[x], (n_p[x] - 1) & 1, P.status);
+                    tc_fence_after();
                     score(x);
                 }
                 tc_commit(&k_free[k % ST]);
                 ++k;
                 for (int j = 0; j < n; ++j) {
-                    att_wait(&v_full[v % ST], v / ST & 1, P.status);
                     if (j + 1 < n) att_wait(&k_full[k % ST], k / ST & 1, P.status);
+                    if constexpr (A::kApart) {
+                        if (j + 1 < n) {
+                            for (int x = 0; x < T; ++x) {
+                                att_wait(&s_free[x], n_f[x]++ & 1, P.status);
+                                tc_fence_after();
+                                score(x);
+                            }
+                            tc_commit(&k_free[k % ST]);
+                        }
+                    }
+                    att_wait(&v_full[v % ST], v / ST & 1, P.status);
                     for (int x = 0; x < T; ++x) {
                         att_wait(&p_full[x], n_p[x] & 1, P.status);
                         tc_fence_after();
                         weigh(x, j > 0);
                         if (x == T - 1) tc_commit(&v_free[v % ST]);
-                        if (j + 1 < n) {
+                        if (!A::kApart && j + 1 < n) {
                             att_wait(&o_done[x], (n_p[x] - 1) & 1, P.status);
+                            tc_fence_after();
                             score(x);
                             if (x == T - 1) tc_commit(&k_free[k % ST]);
                         }
@@ -227,9 +252,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
                     const int k16 = (i * 128 + ct) / KT * 16;
                     return reinterpret_cast<const uint4 *>(kp + k16 / CW * (16 * CW) + k16 % CW);
                 };
-                uint4 raw[KB];
+                // values: a warp takes 512 bytes (16 tokens of 32 elements) at a time
+                constexpr int VU = SUBS * (D / 32) / 4, VB = VU < 8 ? VU : 8;
+                constexpr bool kBoth = KU <= 4 && VU <= 4;         // both asked for at once, where the registers hold them
+                auto value_at = [&](int i) {
+                    const int u = i * 4 + cw, s = u / (D / 32), blk = u % (D / 32);
+                    return reinterpret_cast<const uint4 *>(head + __shfl_sync(0xffffffffu, at, s) + kv_half_bytes(P.s) + blk * 512 + lane * 16);
+                };
+                uint4 raw[KB], val[VB];
 #pragma unroll
                 for (int i = 0; i < KB; ++i) raw[i] = __ldg(key_at(i));
+                if constexpr (kBoth) {
+#pragma unroll
+                    for (int i = 0; i < VB; ++i) val[i] = __ldg(value_at(i));
+                }
                 att_wait(&k_free[st], par, P.status);
 #pragma unroll
                 for (int b = 0; b < KU; b += KB) {
@@ -253,15 +289,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
                 if (cw == 0 && lane < SUBS) scales[n & 3][lane] = mine;
                 fence_proxy_async();
                 mbar_arrive(&k_full[st]);
-                // values: a warp takes 512 bytes (16 tokens of 32 elements) at a time
-                constexpr int VU = SUBS * (D / 32) / 4, VB = VU < 8 ? VU : 8;
-                auto value_at = [&](int i) {
-                    const int u = i * 4 + cw, s = u / (D / 32), blk = u % (D / 32);
-                    return reinterpret_cast<const uint4 *>(head + __shfl_sync(0xffffffffu, at, s) + kv_half_bytes(P.s) + blk * 512 + lane * 16);
-                };
-                uint4 val[VB];
+                if constexpr (!kBoth) {
 #pragma unroll
-                for (int i = 0; i < VB; ++i) val[i] = __ldg(value_at(i));
+                    for (int i = 0; i < VB; ++i) val[i] = __ldg(value_at(i));
+                }
                 if (tile + 1 < it.hi) look_up(tile + 1);
                 att_wait(&v_free[st], par, P.status);
                 const int g = lane >> 2, t = lane & 3;
@@ -291,7 +322,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
     } else if (warp < 4 * T) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromptRegsMore));
         const int x = warp >> 2, r = tid & 127;
-        const uint32_t lanes = tm + (static_cast<uint32_t>((warp & 3) * 32) << 16), sc = lanes + x * 128, oc = lanes + A::kColO + x * D;
+        const uint32_t lanes = tm + (static_cast<uint32_t>((warp & 3) * 32) << 16), sc = lanes + x * 128, oc = lanes + A::kColO + x * D, pc = A::kApart ? lanes + A::kColP + x * A::kWidthP : sc;
         int n_s = 0, n_o = 0, n = 0;
         for (int turn = 0; item_of(turn, it); ++turn) {
             const int row = it.item_row + x * 128 + r, last = it.rows - 1, start = it.length - it.count;
@@ -343,7 +374,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
                 }
             }
             fence_proxy_async();
-            mbar_arrive(&q_full);
+            mbar_arrive(&q_full[x]);
             float m = kAttFloor, l = 0.0f;
 #pragma unroll 1
             for (int tile = it.lo; tile < it.hi; ++tile, ++n) {
@@ -351,29 +382,39 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
                 tc_fence_after();
                 const int first = tile * KT;
                 const bool edge = first + KT - 1 > pos_lo || (P.window && first <= pos_hi - P.window);
-                // column 16 s + p of the scores is token 2 (p / 4) + (p & 1) + 8 ((p & 3) / 2) of sub-block s
-                auto mask = [&](uint32_t (&v)[32], int c) {
+                uint32_t v[KT / 32][32];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int p = i & 15, token = first + c * 32 + (i & 16) + (p >> 2) * 2 + (p & 1) + ((p & 2) << 2);
-                        if (token > pos || (P.window && token <= pos - P.window)) v[i] = 0xff800000u;
-                    }
-                };
+                for (int c = 0; c < KT / 32; ++c) tc_ld(sc + c * 32, v[c]);
+#pragma unroll
+                for (int c = 0; c < KT / 32; ++c) tc_wait_ld(v[c]);
+                if constexpr (A::kApart) {
+                    tc_fence_before();
+                    mbar_arrive(&s_free[x]);
+                }
+                // column 16 s + p of the scores is token 2 (p / 4) + (p & 1) + 8 ((p & 3) / 2) of sub-block s
+                if (edge) {
+#pragma unroll
+                    for (int c = 0; c < KT / 32; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const int p = i & 15, token = first + c * 32 + (i & 16) + (p >> 2) * 2 + (p & 1) + ((p & 2) << 2);
+                            if (token > pos || (P.window && token <= pos - P.window)) v[c][i] = 0xff800000u;
+                        }
+                }
                 float most = kAttFloor;
 #pragma unroll
-                for (int c = 0; c < KT / 32; ++c) {
-                    uint32_t v[32];
-                    tc_ld(sc + c * 32, v);
-                    tc_wait_ld(v);
-                    if (edge) mask(v, c);
+                for (int b = 0; b < SUBS; ++b) {
+                    const float4 s4 = scales[n & 3][b];
+                    auto at = [&](int i) { return __uint_as_float(v[b / 2][b % 2 * 16 + i]); };
+                    float t = max3(at(0), at(1), at(2));
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float4 s4 = scales[n & 3][2 * c + h];
-                        float t = __uint_as_float(v[16 * h]);
-#pragma unroll
-                        for (int i = 1; i < 16; ++i) t = fmaxf(t, __uint_as_float(v[16 * h + i]));
-                        most = fmaxf(most, fmaf(t, fmaxf(mul * s4.x, 1e-37f), s4.y));
-                    }
+                    for (int i = 3; i < 15; i += 2) t = max3(t, at(i), at(i + 1));
+                    t = fmaxf(t, at(15));
+                    most = fmaxf(most, fmaf(t, fmaxf(mul * s4.x, 1e-37f), s4.y));
+                }
+                if constexpr (A::kApart) {          // the sums, and the place of the weights, are free
+                    if (n_o > 0) att_wait(&o_done[x], (n_o - 1) & 1, P.status);
+                    tc_fence_after();
                 }
                 if (tile == it.lo) {
                     m = most;
@@ -382,38 +423,39 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
                     m = now;
                     l *= f;
 #pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t v[32];
-                        tc_ld(oc + c * 32, v);
-                        tc_wait_ld(v);
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t u[16];
+                        tc_ld(oc + c * 16, u);
+                        tc_wait_ld(u);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                        tc_st(oc + c * 32, v);
+                        for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * f);
+                        tc_st(oc + c * 16, u);
                     }
                 }
 #pragma unroll
                 for (int c = 0; c < KT / 32; ++c) {
-                    uint32_t v[32];
-                    tc_ld(sc + c * 32, v);
-                    tc_wait_ld(v);
-                    if (edge) mask(v, c);
                     uint32_t hi[16], lo[16];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const float4 s4 = scales[n & 3][2 * c + h];
                         const float mk = fmaxf(mul * s4.x, 1e-37f), off = s4.y - m;
-                        float sum = 0.0f;
+                        const f32x2 mk2 = pack2(mk, mk), off2 = pack2(off, off);
+                        f32x2 sum = pack2(0.0f, 0.0f);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            const float a = ex2(fmaf(__uint_as_float(v[16 * h + 2 * i]), mk, off)), b = ex2(fmaf(__uint_as_float(v[16 * h + 2 * i + 1]), mk, off));
-                            sum += a + b;
+                            float a, b;
+                            unpack2(fma2(pack2(__uint_as_float(v[c][16 * h + 2 * i]), __uint_as_float(v[c][16 * h + 2 * i + 1])), mk2, off2), a, b);
+                            a = ex2(a), b = ex2(b);
+                            sum = add2(sum, pack2(a, b));
                             hi[8 * h + i] = half_pair(a, b);
                             if constexpr (SPLIT) lo[8 * h + i] = half_rest(a, b, hi[8 * h + i]);
                         }
-                        l = fmaf(sum, s4.z, l);
+                        float a, b;
+                        unpack2(sum, a, b);
+                        l = fmaf(a + b, s4.z, l);
                     }
-                    tc_st(sc + c * 32, hi);
-                    if constexpr (SPLIT) tc_st(sc + c * 32 + 16, lo);
+                    tc_st(pc + c * kPartP, hi);
+                    if constexpr (SPLIT) tc_st(pc + c * kPartP + 16, lo);
                 }
                 tc_wait_st();
                 tc_fence_before();
