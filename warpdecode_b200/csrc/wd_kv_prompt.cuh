@@ -50,7 +50,7 @@ struct PromptAttPlan {
     // Tensor memory: scores of each tile, then sums, then weights where there is room for them beside the scores. (Then the next scores are made while
     // a tile's weights still are.)
     static constexpr int kColO = 128 * kTiles, kColP = kColO + kTiles * D, kWidthP = kKt / 2 * (SPLIT ? 2 : 1);
-    static constexpr bool kApart = kColP + kTiles * kWidthP <= 512;
+    static constexpr bool kApart = kColP + kTiles * kWidthP <= 512 && kStages >= kTiles;         // (the second tile's first scores come behind the first's second)
     static constexpr uint32_t kIdescS = 1u << 4 | (kKt >> 3) << 17 | (128 >> 4) << 24, kIdescO = 1u << 4 | (D >> 3) << 17 | (128 >> 4) << 24;
     static_assert(kColO + kTiles * D <= 512 && kSmem <= 226 * 1024, "plan of the memories");
 };
@@ -147,74 +147,102 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
     PromptItem it;
     if (warp >= 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptRegsLess));
-        if (warp == 12 && lane == 0) {
+        if (warp == 12) {
             int k = 0, v = 0, items = 0;            // tiles of keys and of values that products have been issued for, items
             int n_p[2] = {0, 0}, n_f[2] = {0, 0};
-            auto score = [&](int x) {               // of key tile k
+            auto score = [&](int x, int i0) {       // of key tile k + i0
                 const uint32_t d = tm + x * 128;
-                const uint32_t q0 = smem_u32(qs + x * A::kQTile), k0 = smem_u32(ks + (k % ST) * A::kK);
-#pragma unroll 4
+                const uint32_t q0 = smem_u32(qs + x * A::kQTile), k0 = smem_u32(ks + ((k + i0) % ST) * A::kK);
+#pragma unroll
                 for (int i = 0; i < D / 16; ++i)
                     tc_mma_f16(d, tc_smem_desc(q0 + i * 4096, 2048), tc_smem_desc(k0 + i * 2 * A::kKStep, A::kKStep), A::kIdescS, i > 0);
                 if constexpr (SPLIT) {
-#pragma unroll 4
+#pragma unroll
                     for (int i = 0; i < D / 16; ++i)
                         tc_mma_f16(d, tc_smem_desc(q0 + A::kQ + i * 4096, 2048), tc_smem_desc(k0 + i * 2 * A::kKStep, A::kKStep), A::kIdescS, 1);
                 }
-                tc_commit(&s_full[x]);
-                mbar_arrive(&s_full[x]);        // what this thread saw of the keys' warps, for those who read the scales
+                tc_commit_warp(&s_full[x]);
+                if (lane == 0) mbar_arrive(&s_full[x]);         // what this thread saw of the keys' warps, for those who read the scales
             };
             auto weigh = [&](int x, bool add) {     // with value tile v
                 const uint32_t d = tm + A::kColO + x * D, p = tm + (A::kApart ? A::kColP + x * A::kWidthP : x * 128), v0 = smem_u32(vs + (v % ST) * A::kV);
-#pragma unroll 4
+#pragma unroll
                 for (int i = 0; i < KT / 16; ++i) {
                     const uint64_t desc = tc_smem_desc(v0 + i * 2 * A::kVStep, A::kVStep);
                     tc_mma_f16_t(d, p + i / 2 * kPartP + i % 2 * 8, desc, A::kIdescO, add || i > 0);
                     if constexpr (SPLIT) tc_mma_f16_t(d, p + i / 2 * kPartP + i % 2 * 8 + 16, desc, A::kIdescO, 1);
                 }
-                tc_commit(&o_done[x]);
+                tc_commit_warp(&o_done[x]);
                 ++n_p[x];
+            };
+            auto keys = [&](int i) { att_wait(&k_full[(k + i) % ST], (k + i) / ST & 1, P.status); };
+            // the item's first scores of a tile: the last item's have been read, or its weights, which lie where these scores go
+            auto begin = [&](int x) {
+                att_wait(&q_full[x], items & 1, P.status);
+                if (A::kApart && n_p[x] > 0) att_wait(&s_free[x], n_f[x]++ & 1, P.status);
+                if (!A::kApart && n_p[x] > 0) att_wait(&o_done[x], (n_p[x] - 1) & 1, P.status);
+                tc_fence_after();
+                score(x, 0);
+            };
+            auto weights = [&](int x, int j) {
+                att_wait(&p_full[x], n_p[x] & 1, P.status);
+                tc_fence_after();
+                weigh(x, j > 0);
             };
             for (int turn = 0; item_of(turn, it); ++turn, ++items) {
                 const int n = it.hi - it.lo;
-                att_wait(&k_full[k % ST], k / ST & 1, P.status);
-                for (int x = 0; x < T; ++x) {
-                    att_wait(&q_full[x], items & 1, P.status);
-                    // the last item's scores have been read, or its weights, which lie where these scores go
-                    if (A::kApart && n_p[x] > 0) att_wait(&s_free[x], n_f[x]++ & 1, P.status);
-                    if (!A::kApart && n_p[x] > 0) att_wait(&o_done[x], (n_p[x] - 1) & 1, P.status);
-                    tc_fence_after();
-                    score(x);
-                }
-                tc_commit(&k_free[k % ST]);
-                ++k;
-                for (int j = 0; j < n; ++j) {
-                    if (j + 1 < n) att_wait(&k_full[k % ST], k / ST & 1, P.status);
-                    if constexpr (A::kApart) {
+                keys(0);
+                if constexpr (A::kApart && T == 2) {
+                    // The second tile begins when the first has its weights, and stays that much behind: one makes exponentials while the other reads
+                    // scores and looks for their maximum.
+                    begin(0);
+                    for (int j = 0; j < n; ++j, ++k, ++v) {
                         if (j + 1 < n) {
+                            keys(1);
+                            att_wait(&s_free[0], n_f[0]++ & 1, P.status);
+                            tc_fence_after();
+                            score(0, 1);
+                        }
+                        att_wait(&v_full[v % ST], v / ST & 1, P.status);
+                        weights(0, j);
+                        if (j == 0) {
+                            begin(1);
+                            tc_commit_warp(&k_free[k % ST]);
+                        }
+                        if (j + 1 < n) {
+                            att_wait(&s_free[1], n_f[1]++ & 1, P.status);
+                            tc_fence_after();
+                            score(1, 1);
+                            tc_commit_warp(&k_free[(k + 1) % ST]);
+                        }
+                        weights(1, j);
+                        tc_commit_warp(&v_free[v % ST]);
+                    }
+                } else {
+                    for (int x = 0; x < T; ++x) begin(x);
+                    tc_commit_warp(&k_free[k % ST]);
+                    for (int j = 0; j < n; ++j, ++k, ++v) {
+                        if (j + 1 < n) keys(1);
+                        if (A::kApart && j + 1 < n) {
                             for (int x = 0; x < T; ++x) {
                                 att_wait(&s_free[x], n_f[x]++ & 1, P.status);
                                 tc_fence_after();
-                                score(x);
+                                score(x, 1);
                             }
-                            tc_commit(&k_free[k % ST]);
+                            tc_commit_warp(&k_free[(k + 1) % ST]);
+                        }
+                        att_wait(&v_full[v % ST], v / ST & 1, P.status);
+                        for (int x = 0; x < T; ++x) {
+                            weights(x, j);
+                            if (x == T - 1) tc_commit_warp(&v_free[v % ST]);
+                            if (!A::kApart && j + 1 < n) {
+                                att_wait(&o_done[x], (n_p[x] - 1) & 1, P.status);
+                                tc_fence_after();
+                                score(x, 1);
+                                if (x == T - 1) tc_commit_warp(&k_free[(k + 1) % ST]);
+                            }
                         }
                     }
-                    att_wait(&v_full[v % ST], v / ST & 1, P.status);
-                    for (int x = 0; x < T; ++x) {
-                        att_wait(&p_full[x], n_p[x] & 1, P.status);
-                        tc_fence_after();
-                        weigh(x, j > 0);
-                        if (x == T - 1) tc_commit(&v_free[v % ST]);
-                        if (!A::kApart && j + 1 < n) {
-                            att_wait(&o_done[x], (n_p[x] - 1) & 1, P.status);
-                            tc_fence_after();
-                            score(x);
-                            if (x == T - 1) tc_commit(&k_free[k % ST]);
-                        }
-                    }
-                    ++v;
-                    if (j + 1 < n) ++k;
                 }
             }
             for (int x = 0; x < T; ++x)
@@ -432,30 +460,40 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
                         tc_st(oc + c * 16, u);
                     }
                 }
+                // exponents of all columns, then the exponentials (scales read between the stores of weights would wait for them)
+#pragma unroll
+                for (int b = 0; b < SUBS; ++b) {
+                    const float4 s4 = scales[n & 3][b];
+                    const float mk = fmaxf(mul * s4.x, 1e-37f), off = s4.y - m;
+                    const f32x2 mk2 = pack2(mk, mk), off2 = pack2(off, off);
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        uint32_t *u = &v[b / 2][b % 2 * 16 + i];
+                        float a, c;
+                        unpack2(fma2(pack2(__uint_as_float(u[0]), __uint_as_float(u[1])), mk2, off2), a, c);
+                        u[0] = __float_as_uint(a), u[1] = __float_as_uint(c);
+                    }
+                }
+                uint32_t hi[KT / 32][16], lo[SPLIT ? KT / 32 : 1][16];
+#pragma unroll
+                for (int b = 0; b < SUBS; ++b) {
+                    f32x2 s0 = pack2(0.0f, 0.0f), s1 = s0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float a = ex2(__uint_as_float(v[b / 2][b % 2 * 16 + 2 * i])), c = ex2(__uint_as_float(v[b / 2][b % 2 * 16 + 2 * i + 1]));
+                        if (i & 1) s1 = add2(s1, pack2(a, c));
+                        else s0 = add2(s0, pack2(a, c));
+                        hi[b / 2][b % 2 * 8 + i] = half_pair(a, c);
+                        if constexpr (SPLIT) lo[b / 2][b % 2 * 8 + i] = half_rest(a, c, hi[b / 2][b % 2 * 8 + i]);
+                    }
+                    float a, c;
+                    unpack2(add2(s0, s1), a, c);
+                    l = fmaf(a + c, scales[n & 3][b].z, l);
+                }
 #pragma unroll
                 for (int c = 0; c < KT / 32; ++c) {
-                    uint32_t hi[16], lo[16];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float4 s4 = scales[n & 3][2 * c + h];
-                        const float mk = fmaxf(mul * s4.x, 1e-37f), off = s4.y - m;
-                        const f32x2 mk2 = pack2(mk, mk), off2 = pack2(off, off);
-                        f32x2 sum = pack2(0.0f, 0.0f);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            float a, b;
-                            unpack2(fma2(pack2(__uint_as_float(v[c][16 * h + 2 * i]), __uint_as_float(v[c][16 * h + 2 * i + 1])), mk2, off2), a, b);
-                            a = ex2(a), b = ex2(b);
-                            sum = add2(sum, pack2(a, b));
-                            hi[8 * h + i] = half_pair(a, b);
-                            if constexpr (SPLIT) lo[8 * h + i] = half_rest(a, b, hi[8 * h + i]);
-                        }
-                        float a, b;
-                        unpack2(sum, a, b);
-                        l = fmaf(a + b, s4.z, l);
-                    }
-                    tc_st(pc + c * kPartP, hi);
-                    if constexpr (SPLIT) tc_st(pc + c * kPartP + 16, lo);
+                    tc_st(pc + c * kPartP, hi[c]);
+                    if constexpr (SPLIT) tc_st(pc + c * kPartP + 16, lo[c]);
                 }
                 tc_wait_st();
                 tc_fence_before();

@@ -66,13 +66,23 @@ __device__ __forceinline__ void tc_mma_s8(uint32_t d, uint32_t a, uint64_t b, ui
     asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::i8 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(0u)
                  : "memory");
 }
-// D[128][N] (f32, tensor memory) (+)= A[128][16] * B[N][16] of f16, A in shared memory or in tensor memory (two elements a column); by one thread
+// D[128][N] (f32, tensor memory) (+)= A[128][16] * B[N][16] of f16, A in shared memory or in tensor memory (two elements a column). By a whole warp with
+// the same arguments in every lane, of which one issues it: so the descriptors stay in uniform registers. (From one lane's branch a product took 100 cycles
+// to issue.)
 __device__ __forceinline__ void tc_mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add)
+    asm volatile("{\n .reg .pred p, e;\n .reg .b32 r;\n elect.sync r|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+                 " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add)
                  : "memory");
 }
 __device__ __forceinline__ void tc_mma_f16_t(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add)
+    asm volatile("{\n .reg .pred p, e;\n .reg .b32 r;\n elect.sync r|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+                 " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add)
+                 : "memory");
+}
+// as tc_commit, by a whole warp
+__device__ __forceinline__ void tc_commit_warp(uint64_t *bar) {
+    asm volatile("{\n .reg .pred e;\n .reg .b32 r;\n elect.sync r|e, 0xffffffff;\n"
+                 " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar))
                  : "memory");
 }
 __device__ __forceinline__ void tc_commit(uint64_t *bar) {      // the barrier takes an arrival when the MMAs issued so far are done
