@@ -442,6 +442,8 @@ int wd_kv_attend(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, in
         p.status = c->d_status;
         p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
         p.window = window;
+        p.max_seqs = c->cfg.max_seqs;
+        p.vec = reinterpret_cast<uintptr_t>(q_dev) % 16 == 0 && p.q_stride * rows_size(p.type) % 16 == 0;
         p.s = c->shape;
         const long long group = static_cast<long long>(c->max_rows) * (c->cfg.n_heads / c->cfg.n_kv_heads);
         cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -18,11 +18,13 @@
 // hold by the last CTA to arrive, always in the workers' order.
 #pragma once
 
+#include <type_traits>
+
 #include "wd_kv_layout.cuh"
 
 namespace wd {
 
-constexpr int kAttWorkers = 8, kAttThreads = 512, kAttMaxSeqs = 1024, kAttMaxRows = 16, kAttMaxSlots = 8;
+constexpr int kAttWorkers = 8, kAttThreads = 512, kAttMaxSeqs = 1024, kAttMaxRows = 16, kAttMaxSlots = 8, kAttEntries = 64;
 // Registers a thread: the warps that compute take what those that copy give back (128 at launch).
 constexpr int kAttRegsMore = 192, kAttRegsLess = 64;
 static_assert(256 * kAttRegsMore + 256 * kAttRegsLess <= kAttThreads * 128, "more than the block was launched with: the increase would wait for ever");
@@ -36,12 +38,12 @@ struct KvAttend {
     const void *q;
     void *out;
     long long q_stride, out_stride;
-    float *part;                // [workers][2][kAttMaxRows][D + 4]: sums, then maximum and denominator
+    float *part;                // [workers][kAttMaxRows][D + 4]: sums, then maximum and denominator
     float *cta_part;            // [CTAs][2][kAttMaxRows][D + 4]
     unsigned *arrived;          // [CTAs]
     unsigned *status;
     float scale_log2;
-    int type, window, workers, slots;
+    int type, window, workers, slots, max_seqs, vec;          // vec: rows of q lie on boundaries of 16 bytes
     KvShape s;
 };
 
@@ -114,12 +116,15 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
     __shared__ __align__(8) uint64_t full[kAttWorkers][kAttMaxSlots], empty[kAttWorkers][kAttMaxSlots];
     __shared__ long long part_item[kAttWorkers * 2][2];          // first and last number of the item that a worker's first or last part belongs to; -1: none
     __shared__ int4 part_rows[kAttWorkers * 2];                 // row0, head, item_row, rows
-    __shared__ int run_first[kAttWorkers * 2], run_last[kAttWorkers * 2], n_runs, last_one[2];
+    __shared__ const float *part_at[kAttWorkers * 2];           // where it is
+    __shared__ int part_place[kAttWorkers * 2];                 // places that have a part, in order; runs of them belong to one item
+    __shared__ int run_first[kAttWorkers * 2], run_last[kAttWorkers * 2], n_runs, last_one[2], of_step[3];
+    __shared__ int4 step[kAttEntries];                          // the first entries of the step
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), worker = warp & 7;
     uint8_t *ring = att_sm + worker * P.slots * A::kSlot;
     uint8_t *qs = att_sm + P.workers * (P.slots * A::kSlot + 0) + worker * A::q_bytes(N8, SPLIT);
     long long *prefix = reinterpret_cast<long long *>(att_sm + P.workers * (P.slots * A::kSlot + A::q_bytes(N8, SPLIT)));
-    const int n_seq = P.book[0], g_heads = P.s.heads / P.s.kv_heads;
+    const int g_heads = P.s.heads / P.s.kv_heads;
     const int *entries = P.book + kKvHead;
     if (tid < kAttWorkers * kAttMaxSlots) {
         mbar_init(&full[tid / kAttMaxSlots][tid % kAttMaxSlots], 1);
@@ -127,16 +132,35 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
         mbar_fence_init();
     }
     if (tid < kAttWorkers * 2) part_item[tid][0] = -1;
-    // numbers of one head in front of each sequence, without what an item costs beside its tiles: items in the upper half of a word
+    // Numbers of one head in front of each sequence. An item counts a few tiles more than it has, for what it costs to begin and end one; nothing where
+    // each worker has a part of one item anyway.
+    const int all_workers = static_cast<int>(gridDim.x) * P.workers, me = static_cast<int>(blockIdx.x) * P.workers + worker;
     if (warp == 0) {
+        int4 e0 = lane < P.max_seqs ? *reinterpret_cast<const int4 *>(entries + lane * kKvStepWords) : make_int4(0, 0, 0, 0);      // asked for beside their number
+        const int n = P.book[0];
+        if (lane < kAttEntries) step[lane] = e0;
+        auto entry = [&](int i) { return i < 32 ? e0 : *reinterpret_cast<const int4 *>(entries + i * kKvStepWords); };
+        auto items_of = [&](const int4 &e) { return (static_cast<long long>(e.z) * g_heads + ROWS - 1) / ROWS; };
+        long long tiles = 0;
+        int most = 0;
+        for (int i = lane; i < n; i += 32) {
+            const int4 e = entry(i);
+            const int per = att_tiles(e.w, e.z, ROWS, g_heads, P.window);
+            tiles += items_of(e) * per;
+            most = max(most, per);
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+        const int more = tiles * P.s.kv_heads >= 2ll * all_workers ? 2 : 0;
         long long sum = 0;
-        for (int i0 = 0; i0 < n_seq; i0 += 32) {
+        for (int i0 = 0; i0 < n; i0 += 32) {
             const int i = i0 + lane;
             long long v = 0;
-            if (i < n_seq) {
-                const int *e = entries + i * kKvStepWords;
-                const long long items = (static_cast<long long>(e[2]) * g_heads + ROWS - 1) / ROWS;
-                v = items * att_tiles(e[3], e[2], ROWS, g_heads, P.window);
+            if (i < n) {
+                const int4 e = entry(i);
+                if (i >= 32 && i < kAttEntries) step[i] = e;
+                v = items_of(e) * (att_tiles(e.w, e.z, ROWS, g_heads, P.window) + more);
             }
             long long inc = v;
 #pragma unroll
@@ -144,40 +168,25 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
                 const long long y = __shfl_up_sync(0xffffffffu, inc, o);
                 if (lane >= o) inc += y;
             }
-            if (i < n_seq) prefix[i] = sum + inc - v;
+            if (i < n) prefix[i] = sum + inc - v;
             sum += __shfl_sync(0xffffffffu, inc, 31);
         }
-        if (lane == 0) prefix[n_seq] = sum;
+        if (lane == 0) {
+            prefix[n] = sum;
+            of_step[0] = n;
+            of_step[1] = more;
+            of_step[2] = most <= 6 ? most : 1;
+        }
     }
     __syncthreads();
-    const int all_workers = static_cast<int>(gridDim.x) * P.workers, me = static_cast<int>(blockIdx.x) * P.workers + worker;
-    // what an item costs beside its tiles, in tiles: next to nothing where each worker has one part of one item anyway
-    const long long tiles = prefix[n_seq] * P.s.kv_heads;
-    const int extra = tiles >= 2ll * all_workers ? 2 : 0;
-    if (extra > 0) {
-        __syncthreads();
-        if (warp == 0) {
-            long long sum = 0;
-            for (int i0 = 0; i0 < n_seq; i0 += 32) {
-                const int i = i0 + lane;
-                long long v = i < n_seq ? (static_cast<long long>(entries[i * kKvStepWords + 2]) * g_heads + ROWS - 1) / ROWS * extra : 0, inc = v;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const long long y = __shfl_up_sync(0xffffffffu, inc, o);
-                    if (lane >= o) inc += y;
-                }
-                if (i < n_seq) prefix[i] += sum + inc - v;
-                sum += __shfl_sync(0xffffffffu, inc, 31);
-            }
-            if (lane == 0) prefix[n_seq] += sum;
-        }
-        __syncthreads();
-    }
+    const int n_seq = of_step[0], extra = of_step[1];
     const long long total = prefix[n_seq] * P.s.kv_heads;
     if (total == 0) return;
-    const long long chunk = (total + all_workers - 1) / all_workers, cta_chunk = chunk * P.workers;
+    // To put parts together costs as much as six tiles do: items of up to six stay whole where there are not enough of them for all workers.
+    const long long even = (total + all_workers - 1) / all_workers, chunk = max(even, static_cast<long long>(of_step[2])), cta_chunk = chunk * P.workers;
     if (blockIdx.x * cta_chunk >= total) return;
     const long long begin = worker < P.workers ? min(me * chunk, total) : total, end = min(begin + chunk, total);
+    const bool small = total < (1ll << 31);             // numbers that 32 bits hold are divided in 32 bits
 
     auto segment = [&](long long at) {
         AttSegment s;
@@ -187,12 +196,13 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
             if (prefix[mid] * P.s.kv_heads <= at) lo = mid;
             else hi = mid - 1;
         }
-        const int *e = entries + lo * kKvStepWords;
-        s.seq = e[0], s.row0 = e[1], s.count = e[2], s.length = e[3];
+        const int4 e = lo < kAttEntries ? step[lo] : *reinterpret_cast<const int4 *>(entries + lo * kKvStepWords);
+        s.seq = e.x, s.row0 = e.y, s.count = e.z, s.length = e.w;
         const int per_item = att_tiles(s.length, s.count, ROWS, g_heads, P.window) + extra;
         const long long per_head = prefix[lo + 1] - prefix[lo], base = prefix[lo] * P.s.kv_heads, in = at - base;
-        s.head = static_cast<int>(in / per_head);
-        const int group = static_cast<int>((in - s.head * per_head) / per_item);
+        auto over = [&](long long a, long long b) { return small ? static_cast<int>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : static_cast<int>(a / b); };
+        s.head = over(in, per_head);
+        const int group = over(in - s.head * per_head, per_item);
         s.item0 = base + s.head * per_head + static_cast<long long>(group) * per_item;
         s.item1 = s.item0 + per_item;
         s.item_row = group * ROWS;
@@ -279,43 +289,60 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
         const AttSegment s = segment(at);
         const bool first_part = at == begin;
         at = s.next;
-        // q -> fragments: [8 rows][D / CW][half of LB][lane][8 elements], hi, then lo
+        // q -> fragments: [8 rows][D / CW][half of LB][lane][8 elements], hi, then lo. A lane brings a quarter of row lane / 4.
         float mul[N8][2];
         __syncwarp();
 #pragma unroll
         for (int n = 0; n < N8; ++n) {
+            const int r = 8 * n + g, row = s.item_row + r;
+            const size_t src = static_cast<size_t>(s.row0 + row / g_heads) * P.q_stride + (static_cast<size_t>(s.head) * g_heads + row % g_heads) * D + t * (D / 4);
+            float x[D / 4];
+            // (the type is asked for once: asked for at each element, every load would be waited for by itself)
+            auto load = [&](const auto *q) {
+                using R = std::remove_const_t<std::remove_pointer_t<decltype(q)>>;
+                constexpr int N = 16 / sizeof(R);
+                if (P.vec) {
+                    uint4 u[D / 4 / N];
 #pragma unroll
-            for (int rb = 0; rb < 8; rb += 4) {
-                float x[4][D / 32];
+                    for (int i = 0; i < D / 4 / N; ++i) u[i] = reinterpret_cast<const uint4 *>(q + src)[i];
+#pragma unroll
+                    for (int i = 0; i < D / 4; ++i) x[i] = static_cast<float>(reinterpret_cast<const R *>(&u[i / N])[i % N]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < D / 4; ++i) x[i] = static_cast<float>(q[src + i]);
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
+            if (r < s.rows) {
+                if (P.type == kRowsF32) load(static_cast<const float *>(P.q));
+                else if (P.type == kRowsF16) load(static_cast<const __half *>(P.q));
+                else load(static_cast<const __nv_bfloat16 *>(P.q));
+            }
+            __syncwarp();
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = top > 0.0f ? max(-100, min(128, static_cast<int>(__float_as_uint(top) >> 23) - 126)) : 0, e1 = e / 2, e2 = e - e1;
+            const float up = __uint_as_float((127 + e1) << 23), up2 = __uint_as_float((127 + e2) << 23), down = __uint_as_float((127 - e1) << 23),
+                        down2 = __uint_as_float((127 - e2) << 23), mine = P.scale_log2 * up * up2;
+            mul[n][0] = __shfl_sync(0xffffffffu, mine, 8 * t);
+            mul[n][1] = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
+#pragma unroll
+            for (int i = 0; i < D / 4; i += 8) {
+                const int d = t * (D / 4) + i, kk = d % CW;
+                uint4 *to = reinterpret_cast<uint4 *>(qs) + ((n * (D / CW) + d / CW) * NH + kk % LB / 8) * 32 + g * 4 + kk / LB;
+                uint32_t hi[4], lo[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int r = 8 * n + rb + j, row = s.item_row + r;
-                    const size_t src = static_cast<size_t>(s.row0 + row / g_heads) * P.q_stride + (static_cast<size_t>(s.head) * g_heads + row % g_heads) * D;
-#pragma unroll
-                    for (int i = 0; i < D / 32; ++i) x[j][i] = r < s.rows ? row_load(P.q, P.type, src + i * 32 + lane) : 0.0f;
+                    const float a = x[i + 2 * j] * down * down2, b = x[i + 2 * j + 1] * down * down2;
+                    hi[j] = half_pair(a, b);
+                    if (SPLIT) lo[j] = half_rest(a, b, hi[j]);
                 }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int gr = rb + j;
-                    float top = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < D / 32; ++i) top = fmaxf(top, fabsf(x[j][i]));
-#pragma unroll
-                    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    const int e = top > 0.0f ? max(-100, min(128, static_cast<int>(__float_as_uint(top) >> 23) - 126)) : 0, e1 = e / 2, e2 = e - e1;
-                    const float up = __uint_as_float((127 + e1) << 23), up2 = __uint_as_float((127 + e2) << 23), down = __uint_as_float((127 - e1) << 23),
-                                down2 = __uint_as_float((127 - e2) << 23);
-                    if ((gr >> 1) == t) mul[n][gr & 1] = P.scale_log2 * up * up2;
-#pragma unroll
-                    for (int i = 0; i < D / 32; ++i) {
-                        const int d = i * 32 + lane, kk = d % CW, el = kk % LB;
-                        const float v = x[j][i] * down * down2;
-                        const __half hi = __float2half_rn(v);
-                        __half *to = reinterpret_cast<__half *>(qs) + (((n * (D / CW) + d / CW) * NH + el / 8) * 32 + gr * 4 + kk / LB) * 8 + el % 8;
-                        *to = hi;
-                        if (SPLIT) to[ROWS * D] = __float2half_rn(v - __half2float(hi));
-                    }
-                }
+                to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                if (SPLIT) to[ROWS * D / 8] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
         }
         __syncwarp();
@@ -354,24 +381,28 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
                         qh[n][h] = qp[((n * (D / CW) + c) * NH + h) * 32];
                         if constexpr (SPLIT) ql[n][h] = qp[((n * (D / CW) + c) * NH + h) * 32 + ROWS * D / 8];
                     }
+                // (the four sub-blocks in turn at each step: products in a row on the same sums would wait for one another)
+                uint32_t w0[4][LB / 4], w1[4][LB / 4];
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    uint32_t w0[LB / 4], w1[LB / 4];
                     const uint8_t *p = kp + b * 16 * D + c * 16 * CW;
                     if constexpr (LB == 16) {
                         const uint4 u = *reinterpret_cast<const uint4 *>(p), v = *reinterpret_cast<const uint4 *>(p + 8 * CW);
-                        w0[0] = u.x, w0[1] = u.y, w0[2] = u.z, w0[3] = u.w;
-                        w1[0] = v.x, w1[1] = v.y, w1[2] = v.z, w1[3] = v.w;
+                        w0[b][0] = u.x, w0[b][1] = u.y, w0[b][2] = u.z, w0[b][3] = u.w;
+                        w1[b][0] = v.x, w1[b][1] = v.y, w1[b][2] = v.z, w1[b][3] = v.w;
                     } else {
                         const uint2 u = *reinterpret_cast<const uint2 *>(p), v = *reinterpret_cast<const uint2 *>(p + 8 * CW);
-                        w0[0] = u.x, w0[1] = u.y;
-                        w1[0] = v.x, w1[1] = v.y;
+                        w0[b][0] = u.x, w0[b][1] = u.y;
+                        w1[b][0] = v.x, w1[b][1] = v.y;
                     }
+                }
 #pragma unroll
-                    for (int w = 0; w < LB / 4; ++w) {
+                for (int w = 0; w < LB / 4; ++w)
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
                         uint32_t a0, a1, a2, a3;
-                        kv_halves<E4M3>(w0[w], a0, a2);
-                        kv_halves<E4M3>(w1[w], a1, a3);
+                        kv_halves<E4M3>(w0[b][w], a0, a2);
+                        kv_halves<E4M3>(w1[b][w], a1, a3);
 #pragma unroll
                         for (int n = 0; n < N8; ++n) {
                             const uint4 q = qh[n][w >> 1];
@@ -382,7 +413,6 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
                             }
                         }
                     }
-                }
             }
             float4 sc[4];
 #pragma unroll
@@ -449,9 +479,9 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
             att_wait(&fu[slot], par, P.status);
             const uint4 *vp = reinterpret_cast<const uint4 *>(ring + slot * A::kSlot) + lane;
 #pragma unroll
-            for (int k = 0; k < D / 32; ++k)
+            for (int b = 0; b < 4; ++b)
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
+                for (int k = 0; k < D / 32; ++k) {
                     const uint4 v = vp[b * D + k * 32];
                     uint32_t a0, a1, a2, a3;
                     kv_halves<E4M3>(v.x, a0, a2);
@@ -473,7 +503,9 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
         }
         // ---- the item's end, or this worker's part of it
         const int place = worker * 2 + (first_part ? 0 : 1);
-        float *part = P.part + (static_cast<size_t>(me) * 2 + (first_part ? 0 : 1)) * kAttMaxRows * PITCH;
+        // the worker's last part: its ring is free, and holds it
+        const bool here = at >= end;
+        float *part = here ? reinterpret_cast<float *>(ring) : P.part + static_cast<size_t>(me) * kAttMaxRows * PITCH;
 #pragma unroll
         for (int n = 0; n < N8; ++n)
 #pragma unroll
@@ -495,35 +527,37 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
                 } else {
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
-                        __stcg(part + r * PITCH + 16 * k + g, o[n][k][i]);
-                        __stcg(part + r * PITCH + 16 * k + 8 + g, o[n][k][2 + i]);
+                        part[r * PITCH + 16 * k + g] = o[n][k][i];
+                        part[r * PITCH + 16 * k + 8 + g] = o[n][k][2 + i];
                     }
-                    if (g == 0) __stcg(reinterpret_cast<float2 *>(part + r * PITCH + D), make_float2(m[n][i], den));
+                    if (g == 0) *reinterpret_cast<float2 *>(part + r * PITCH + D) = make_float2(m[n][i], den);
                 }
             }
         if (!s.whole && lane == 0) {
             part_item[place][0] = s.item0;
             part_item[place][1] = s.item1;
             part_rows[place] = make_int4(s.row0, s.head, s.item_row, s.rows);
+            part_at[place] = part;
         }
     }
 
     // ---- parts of the CTA's workers: runs of places that belong to one item
     __threadfence_block();
     att_bar();
-    if (tid == 0) {
-        int runs = 0;
-        for (int p = 0; p < kAttWorkers * 2; ++p) {
-            if (part_item[p][0] < 0) continue;
-            if (runs > 0 && part_item[run_last[runs - 1]][0] == part_item[p][0]) {
-                run_last[runs - 1] = p;
-            } else {
-                run_first[runs] = run_last[runs] = p;
-                ++runs;
-            }
+    if (warp == 0) {
+        const long long item = lane < kAttWorkers * 2 ? part_item[lane][0] : -1;
+        const unsigned there = __ballot_sync(0xffffffffu, item >= 0), in_front = there & ((1u << lane) - 1u);
+        const long long before = __shfl_sync(0xffffffffu, item, in_front ? 31 - __clz(in_front) : lane);
+        const unsigned starts = __ballot_sync(0xffffffffu, item >= 0 && (in_front == 0u || before != item));
+        const unsigned behind = there & ~((2u << lane) - 1u);
+        const int run = __popc(starts & ((2u << lane) - 1u)) - 1, rank = __popc(in_front);
+        if (item >= 0) part_place[rank] = lane;
+        if (starts >> lane & 1u) run_first[run] = rank;
+        if (item >= 0 && (behind == 0u || (starts >> (__ffs(behind) - 1) & 1u))) run_last[run] = rank;
+        if (lane == 0) {
+            n_runs = __popc(starts);
+            last_one[0] = last_one[1] = -1;
         }
-        n_runs = runs;
-        last_one[0] = last_one[1] = -1;
     }
     att_bar();
     const int runs = n_runs;
@@ -539,42 +573,63 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
         row_store(P.out, P.type, to + 2, sum.z * inv);
         row_store(P.out, P.type, to + 3, sum.w * inv);
     };
-    auto join = [&](float &top, float &den, float4 &sum, const float *p, int c) {
-        const float4 y = __ldcg(reinterpret_cast<const float4 *>(p + c));
-        const float2 z = __ldcg(reinterpret_cast<const float2 *>(p + D));
-        const float both = fmaxf(top, z.x), fa = ex2(top - both), fb = ex2(z.x - both);
-        top = both;
-        den = den * fa + z.y * fb;
-        sum.x = sum.x * fa + y.x * fb, sum.y = sum.y * fa + y.y * fb, sum.z = sum.z * fa + y.z * fb, sum.w = sum.w * fa + y.w * fb;
+    // parts of an item, four at a time: all of their loads are on their way before the first is needed
+    struct Joined {
+        float top, den;
+        float4 sum;
     };
+    auto join = [&](int n, int c, auto row_of, auto get4, auto get2) {        // row_of(i): the row of part i
+        Joined j = {kAttFloor, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+#pragma unroll 1
+        for (int i0 = 0; i0 < n; i0 += 4) {
+            float4 y[4];
+            float2 z[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float *p = row_of(min(i0 + k, n - 1));
+                y[k] = get4(reinterpret_cast<const float4 *>(p + c));
+                z[k] = get2(reinterpret_cast<const float2 *>(p + D));
+                if (i0 + k >= n) z[k] = make_float2(kAttFloor, 0.0f), y[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float both = fmaxf(j.top, z[k].x), fa = ex2(j.top - both), fb = ex2(z[k].x - both);
+                j.top = both;
+                j.den = j.den * fa + z[k].y * fb;
+                j.sum.x = j.sum.x * fa + y[k].x * fb, j.sum.y = j.sum.y * fa + y[k].y * fb, j.sum.z = j.sum.z * fa + y[k].z * fb, j.sum.w = j.sum.w * fa + y[k].w * fb;
+            }
+        }
+        return j;
+    };
+    auto cta_of = [&](long long at) { return small ? static_cast<int>(static_cast<uint32_t>(at) / static_cast<uint32_t>(cta_chunk)) : static_cast<int>(at / cta_chunk); };
     bool crosses = false;
     for (int i = tid; i < runs * ROWS * V; i += kAttWorkers * 32) {
-        const int run = i / (ROWS * V), r = i / V % ROWS, c = i % V * 4, p0 = run_first[run], p1 = run_last[run];
+        const int run = i / (ROWS * V), r = i / V % ROWS, c = i % V * 4, q0 = run_first[run], q1 = run_last[run], p0 = part_place[q0];
         const int4 rw = part_rows[p0];
         if (r >= rw.w) continue;
-        float top = kAttFloor, den = 0.0f;
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int p = p0; p <= p1; ++p)
-            if (part_item[p][0] == part_item[p0][0])
-                join(top, den, sum, P.part + (static_cast<size_t>(blockIdx.x) * P.workers * 2 + p) * kAttMaxRows * PITCH + r * PITCH, c);
+        // (volatile: what other warps of the CTA have written)
+        const Joined j = join(q1 - q0 + 1, c, [&](int k) { return part_at[part_place[q0 + k]] + r * PITCH; },
+                              [](const float4 *p) { const volatile float *v = reinterpret_cast<const volatile float *>(p); return make_float4(v[0], v[1], v[2], v[3]); },
+                              [](const float2 *p) { const volatile float *v = reinterpret_cast<const volatile float *>(p); return make_float2(v[0], v[1]); });
         if (part_item[p0][0] >= cta0 && part_item[p0][1] <= cta1) {
-            put(rw, r, c, sum, den);
+            put(rw, r, c, j.sum, j.den);
         } else {
             float *to = P.cta_part + (static_cast<size_t>(blockIdx.x) * 2 + (part_item[p0][0] <= cta0 ? 0 : 1)) * kAttMaxRows * PITCH + r * PITCH;
-            __stcg(reinterpret_cast<float4 *>(to + c), sum);
-            if (c == 0) __stcg(reinterpret_cast<float2 *>(to + D), make_float2(top, den));
+            __stcg(reinterpret_cast<float4 *>(to + c), j.sum);
+            if (c == 0) __stcg(reinterpret_cast<float2 *>(to + D), make_float2(j.top, j.den));
         }
     }
     // ---- and of the CTAs: the first or the last run may be shared with others
-    const bool shared0 = !(part_item[run_first[0]][0] >= cta0 && part_item[run_first[0]][1] <= cta1);
-    const bool shared1 = runs > 1 && !(part_item[run_first[runs - 1]][0] >= cta0 && part_item[run_first[runs - 1]][1] <= cta1);
+    auto item_of_run = [&](int run) { return part_place[run_first[run]]; };
+    const bool shared0 = !(part_item[item_of_run(0)][0] >= cta0 && part_item[item_of_run(0)][1] <= cta1);
+    const bool shared1 = runs > 1 && !(part_item[item_of_run(runs - 1)][0] >= cta0 && part_item[item_of_run(runs - 1)][1] <= cta1);
     crosses = shared0 || shared1;
     if (!crosses) return;
     __threadfence();
     att_bar();
     if (tid < 2 && (tid == 0 ? shared0 : shared1)) {
         const int run = tid == 0 ? 0 : runs - 1;
-        const int c0 = static_cast<int>(part_item[run_first[run]][0] / cta_chunk), c1 = static_cast<int>((part_item[run_first[run]][1] - 1) / cta_chunk);
+        const int c0 = cta_of(part_item[item_of_run(run)][0]), c1 = cta_of(part_item[item_of_run(run)][1] - 1);
         const unsigned before = atomicAdd(P.arrived + c0, 1u);
         if (before == static_cast<unsigned>(c1 - c0)) {
             P.arrived[c0] = 0u;
@@ -586,18 +641,17 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
     for (int w = 0; w < 2; ++w) {
         const int run = last_one[w];
         if (run < 0) continue;
-        const int p0 = run_first[run];
+        const int p0 = item_of_run(run);
         const long long item0 = part_item[p0][0], item1 = part_item[p0][1];
-        const int c0 = static_cast<int>(item0 / cta_chunk), c1 = static_cast<int>((item1 - 1) / cta_chunk);
+        const int c0 = cta_of(item0), c1 = cta_of(item1 - 1);
         const int4 rw = part_rows[p0];
         for (int i = tid; i < rw.w * V; i += kAttWorkers * 32) {
             const int r = i / V, c = i % V * 4;
-            float top = kAttFloor, den = 0.0f;
-            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-            for (int u = c0; u <= c1; ++u)
-                join(top, den, sum, P.cta_part + (static_cast<size_t>(u) * 2 + (item0 <= u * cta_chunk ? 0 : 1)) * kAttMaxRows * PITCH + r * PITCH, c);
-            put(rw, r, c, sum, den);
+            const Joined j = join(c1 - c0 + 1, c, [&](int k) {
+                const int u = c0 + k;
+                return static_cast<const float *>(P.cta_part + (static_cast<size_t>(u) * 2 + (item0 <= u * cta_chunk ? 0 : 1)) * kAttMaxRows * PITCH + r * PITCH);
+            }, [](const float4 *p) { return __ldcg(p); }, [](const float2 *p) { return __ldcg(p); });
+            put(rw, r, c, j.sum, j.den);
         }
     }
 }
