@@ -202,7 +202,7 @@ int by_rows_and_codes(const wd_kv_cache *c, int rows, F &&f) {
 template <int D, int N8, bool SPLIT>
 int attend_launch(wd_kv_cache *c, wd::KvAttend &p, cudaStream_t s) {
     using A = wd::AttendPlan<D>;
-    constexpr int kMost = 227 * 1024 - 3072;        // what a block may have, less what the kernel declares itself
+    constexpr int kMost = 227 * 1024 - 8192;        // what a block may have, less what the kernel declares itself
     static_assert(A::fixed_bytes(4, N8, SPLIT) + 4 * 2 * A::kSlot <= kMost, "four workers with two slots fit");
     // keys of one tile and values of the one before should be on their way while a worker computes
     for (p.workers = 8; p.workers > 4; p.workers /= 2)
@@ -212,7 +212,7 @@ int attend_launch(wd_kv_cache *c, wd::KvAttend &p, cudaStream_t s) {
     return by_codes(c, [&](auto e4m3) {
         auto kernel = wd::kv_attend_kernel<D, N8, SPLIT, decltype(e4m3)::value>;
         WD_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        kernel<<<c->n_sm, wd::kAttThreads, smem, s>>>(p);
+        kernel<<<std::min(c->n_sm, wd::kAttMaxCtas), wd::kAttThreads, smem, s>>>(p);
         WD_TRY_CUDA(cudaGetLastError());
         return WD_OK;
     });

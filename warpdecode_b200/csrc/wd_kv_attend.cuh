@@ -24,7 +24,7 @@
 
 namespace wd {
 
-constexpr int kAttWorkers = 8, kAttThreads = 512, kAttMaxSeqs = 1024, kAttMaxRows = 16, kAttMaxSlots = 8, kAttEntries = 64;
+constexpr int kAttWorkers = 8, kAttThreads = 512, kAttMaxSeqs = 1024, kAttMaxRows = 16, kAttMaxSlots = 8, kAttEntries = 64, kAttMaxCtas = 256;
 // Registers a thread: the warps that compute take what those that copy give back (128 at launch).
 constexpr int kAttRegsMore = 192, kAttRegsLess = 64;
 static_assert(256 * kAttRegsMore + 256 * kAttRegsLess <= kAttThreads * 128, "more than the block was launched with: the increase would wait for ever");
@@ -118,7 +118,11 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
     __shared__ int4 part_rows[kAttWorkers * 2];                 // row0, head, item_row, rows
     __shared__ const float *part_at[kAttWorkers * 2];           // where it is
     __shared__ int part_place[kAttWorkers * 2];                 // places that have a part, in order; runs of them belong to one item
-    __shared__ int run_first[kAttWorkers * 2], run_last[kAttWorkers * 2], n_runs, last_one[2], of_step[3];
+    __shared__ int run_first[kAttWorkers * 2], run_last[kAttWorkers * 2], n_runs, n_parts, n_shared, last_one[2], of_step[3];
+    __shared__ int2 job[kAttWorkers * 2];                       // to put together: first and number in job_from
+    __shared__ int4 job_rows[kAttWorkers * 2];
+    __shared__ float *job_to[kAttWorkers * 2];                  // null: the answer
+    __shared__ const float *job_from[2 * kAttMaxCtas];
     __shared__ int4 step[kAttEntries];                          // the first entries of the step
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), worker = warp & 7;
     uint8_t *ring = att_sm + worker * P.slots * A::kSlot;
@@ -140,21 +144,28 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
         const int n = P.book[0];
         if (lane < kAttEntries) step[lane] = e0;
         auto entry = [&](int i) { return i < 32 ? e0 : *reinterpret_cast<const int4 *>(entries + i * kKvStepWords); };
+        if (n == 1) e0 = make_int4(__shfl_sync(0xffffffffu, e0.x, 0), __shfl_sync(0xffffffffu, e0.y, 0), __shfl_sync(0xffffffffu, e0.z, 0), __shfl_sync(0xffffffffu, e0.w, 0));
         auto items_of = [&](const int4 &e) { return (static_cast<long long>(e.z) * g_heads + ROWS - 1) / ROWS; };
         long long tiles = 0;
         int most = 0;
-        for (int i = lane; i < n; i += 32) {
+        for (int i = n == 1 ? 0 : lane; i < n; i += 32) {
             const int4 e = entry(i);
             const int per = att_tiles(e.w, e.z, ROWS, g_heads, P.window);
             tiles += items_of(e) * per;
             most = max(most, per);
         }
-        most = __reduce_max_sync(0xffffffffu, most);
+        if (n > 1) {
+            most = __reduce_max_sync(0xffffffffu, most);
 #pragma unroll
-        for (int o = 16; o; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+            for (int o = 16; o; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+        }
         const int more = tiles * P.s.kv_heads >= 2ll * all_workers ? 2 : 0;
         long long sum = 0;
-        for (int i0 = 0; i0 < n; i0 += 32) {
+        if (n == 1) {               // (the usual step of a single user)
+            if (lane == 0) prefix[0] = 0;
+            sum = tiles + items_of(e0) * more;
+        }
+        for (int i0 = n == 1 ? 1 : 0; i0 < n; i0 += 32) {
             const int i = i0 + lane;
             long long v = 0;
             if (i < n) {
@@ -556,6 +567,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
         if (item >= 0 && (behind == 0u || (starts >> (__ffs(behind) - 1) & 1u))) run_last[run] = rank;
         if (lane == 0) {
             n_runs = __popc(starts);
+            n_parts = __popc(there);
+            n_shared = 0;
             last_one[0] = last_one[1] = -1;
         }
     }
@@ -564,95 +577,103 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
     if (runs == 0) return;
     const long long cta0 = blockIdx.x * cta_chunk, cta1 = min(cta0 + cta_chunk, total);
     constexpr int V = D / 4;
-    auto put = [&](const int4 &rw, int r, int c, const float4 &sum, float den) {
-        const int row = rw.z + r;
-        const size_t to = static_cast<size_t>(rw.x + row / g_heads) * P.out_stride + (static_cast<size_t>(rw.y) * g_heads + row % g_heads) * D + c;
-        const float inv = 1.0f / den;
-        row_store(P.out, P.type, to, sum.x * inv);
-        row_store(P.out, P.type, to + 1, sum.y * inv);
-        row_store(P.out, P.type, to + 2, sum.z * inv);
-        row_store(P.out, P.type, to + 3, sum.w * inv);
-    };
-    // parts of an item, four at a time: all of their loads are on their way before the first is needed
-    struct Joined {
-        float top, den;
-        float4 sum;
-    };
-    auto join = [&](int n, int c, auto row_of, auto get4, auto get2) {        // row_of(i): the row of part i
-        Joined j = {kAttFloor, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
-#pragma unroll 1
-        for (int i0 = 0; i0 < n; i0 += 4) {
-            float4 y[4];
-            float2 z[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float *p = row_of(min(i0 + k, n - 1));
-                y[k] = get4(reinterpret_cast<const float4 *>(p + c));
-                z[k] = get2(reinterpret_cast<const float2 *>(p + D));
-                if (i0 + k >= n) z[k] = make_float2(kAttFloor, 0.0f), y[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float both = fmaxf(j.top, z[k].x), fa = ex2(j.top - both), fb = ex2(z[k].x - both);
-                j.top = both;
-                j.den = j.den * fa + z[k].y * fb;
-                j.sum.x = j.sum.x * fa + y[k].x * fb, j.sum.y = j.sum.y * fa + y[k].y * fb, j.sum.z = j.sum.z * fa + y[k].z * fb, j.sum.w = j.sum.w * fa + y[k].w * fb;
-            }
-        }
-        return j;
-    };
     auto cta_of = [&](long long at) { return small ? static_cast<int>(static_cast<uint32_t>(at) / static_cast<uint32_t>(cta_chunk)) : static_cast<int>(at / cta_chunk); };
-    bool crosses = false;
-    for (int i = tid; i < runs * ROWS * V; i += kAttWorkers * 32) {
-        const int run = i / (ROWS * V), r = i / V % ROWS, c = i % V * 4, q0 = run_first[run], q1 = run_last[run], p0 = part_place[q0];
-        const int4 rw = part_rows[p0];
-        if (r >= rw.w) continue;
-        // (volatile: what other warps of the CTA have written)
-        const Joined j = join(q1 - q0 + 1, c, [&](int k) { return part_at[part_place[q0 + k]] + r * PITCH; },
-                              [](const float4 *p) { const volatile float *v = reinterpret_cast<const volatile float *>(p); return make_float4(v[0], v[1], v[2], v[3]); },
-                              [](const float2 *p) { const volatile float *v = reinterpret_cast<const volatile float *>(p); return make_float2(v[0], v[1]); });
-        if (part_item[p0][0] >= cta0 && part_item[p0][1] <= cta1) {
-            put(rw, r, c, j.sum, j.den);
-        } else {
-            float *to = P.cta_part + (static_cast<size_t>(blockIdx.x) * 2 + (part_item[p0][0] <= cta0 ? 0 : 1)) * kAttMaxRows * PITCH + r * PITCH;
-            __stcg(reinterpret_cast<float4 *>(to + c), j.sum);
-            if (c == 0) __stcg(reinterpret_cast<float2 *>(to + D), make_float2(j.top, j.den));
-        }
-    }
-    // ---- and of the CTAs: the first or the last run may be shared with others
-    auto item_of_run = [&](int run) { return part_place[run_first[run]]; };
-    const bool shared0 = !(part_item[item_of_run(0)][0] >= cta0 && part_item[item_of_run(0)][1] <= cta1);
-    const bool shared1 = runs > 1 && !(part_item[item_of_run(runs - 1)][0] >= cta0 && part_item[item_of_run(runs - 1)][1] <= cta1);
-    crosses = shared0 || shared1;
-    if (!crosses) return;
-    __threadfence();
-    att_bar();
-    if (tid < 2 && (tid == 0 ? shared0 : shared1)) {
-        const int run = tid == 0 ? 0 : runs - 1;
-        const int c0 = cta_of(part_item[item_of_run(run)][0]), c1 = cta_of(part_item[item_of_run(run)][1] - 1);
-        const unsigned before = atomicAdd(P.arrived + c0, 1u);
-        if (before == static_cast<unsigned>(c1 - c0)) {
-            P.arrived[c0] = 0u;
-            last_one[tid] = run;
-        }
-        __threadfence();
-    }
-    att_bar();
-    for (int w = 0; w < 2; ++w) {
-        const int run = last_one[w];
-        if (run < 0) continue;
-        const int p0 = item_of_run(run);
+    // the CTA's parts of its runs: answers, or a part of the first or the last run, which others may hold parts of too
+    if (tid < runs) {
+        const int p0 = part_place[run_first[tid]];
         const long long item0 = part_item[p0][0], item1 = part_item[p0][1];
-        const int c0 = cta_of(item0), c1 = cta_of(item1 - 1);
-        const int4 rw = part_rows[p0];
-        for (int i = tid; i < rw.w * V; i += kAttWorkers * 32) {
-            const int r = i / V, c = i % V * 4;
-            const Joined j = join(c1 - c0 + 1, c, [&](int k) {
-                const int u = c0 + k;
-                return static_cast<const float *>(P.cta_part + (static_cast<size_t>(u) * 2 + (item0 <= u * cta_chunk ? 0 : 1)) * kAttMaxRows * PITCH + r * PITCH);
-            }, [](const float4 *p) { return __ldcg(p); }, [](const float2 *p) { return __ldcg(p); });
-            put(rw, r, c, j.sum, j.den);
+        const bool ours = item0 >= cta0 && item1 <= cta1;
+        job[tid] = make_int2(run_first[tid], run_last[tid] - run_first[tid] + 1);
+        job_rows[tid] = part_rows[p0];
+        job_to[tid] = ours ? nullptr : P.cta_part + (static_cast<size_t>(blockIdx.x) * 2 + (item0 <= cta0 ? 0 : 1)) * kAttMaxRows * PITCH;
+        if (!ours) atomicAdd_block(&n_shared, 1);
+    }
+    if (tid < n_parts) job_from[tid] = part_at[part_place[tid]];
+    att_bar();
+    // Parts are put together twice: the workers' of a CTA, then the CTAs' of an item, by the last of them to arrive. One loop serves both: code that an SM
+    // has not run yet costs far more than what it does (two copies: 13 us for the second one).
+    int jobs = runs;
+#pragma unroll 1
+    for (int turn = 0;; ++turn) {
+#pragma unroll 1
+        for (int i = tid; i < jobs * ROWS * V; i += kAttWorkers * 32) {
+            const int j = i / (ROWS * V), r = i / V % ROWS, c = i % V * 4, n = job[j].y;
+            const int4 rw = job_rows[j];
+            if (r >= rw.w) continue;
+            const float *const *from = job_from + job[j].x;
+            float top = kAttFloor, den = 0.0f;
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+            for (int k0 = 0; k0 < n; k0 += 4) {
+                float4 y[4];
+                float2 z[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {           // (volatile: what other warps, or CTAs, have written)
+                    const float *p = from[min(k0 + k, n - 1)] + r * PITCH;
+                    asm volatile("ld.volatile.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(y[k].x), "=f"(y[k].y), "=f"(y[k].z), "=f"(y[k].w) : "l"(p + c));
+                    asm volatile("ld.volatile.v2.f32 {%0, %1}, [%2];" : "=f"(z[k].x), "=f"(z[k].y) : "l"(p + D));
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (k0 + k >= n) break;
+                    const float both = fmaxf(top, z[k].x), fa = ex2(top - both), fb = ex2(z[k].x - both);
+                    top = both;
+                    den = den * fa + z[k].y * fb;
+                    sum.x = sum.x * fa + y[k].x * fb, sum.y = sum.y * fa + y[k].y * fb, sum.z = sum.z * fa + y[k].z * fb, sum.w = sum.w * fa + y[k].w * fb;
+                }
+            }
+            if (float *to = job_to[j]) {
+                __stcg(reinterpret_cast<float4 *>(to + r * PITCH + c), sum);
+                if (c == 0) __stcg(reinterpret_cast<float2 *>(to + r * PITCH + D), make_float2(top, den));
+            } else {
+                const int row = rw.z + r;
+                const size_t to0 = static_cast<size_t>(rw.x + row / g_heads) * P.out_stride + (static_cast<size_t>(rw.y) * g_heads + row % g_heads) * D + c;
+                const float inv = 1.0f / den;
+#pragma unroll 1
+                for (int k = 0; k < 4; ++k) {
+                    row_store(P.out, P.type, to0 + k, sum.x * inv);
+                    sum.x = sum.y, sum.y = sum.z, sum.z = sum.w;
+                }
+            }
         }
+        if (turn > 0 || n_shared == 0) return;
+        __threadfence();
+        att_bar();
+        if (tid < 2) {
+            const int run = tid == 0 ? 0 : runs - 1;
+            if (job_to[run] && (tid == 0 || runs > 1)) {
+                const int p0 = part_place[run_first[run]];
+                const int c0 = cta_of(part_item[p0][0]), c1 = cta_of(part_item[p0][1] - 1);
+                const unsigned before = atomicAdd(P.arrived + c0, 1u);
+                if (before == static_cast<unsigned>(c1 - c0)) {
+                    P.arrived[c0] = 0u;
+                    last_one[tid] = run;
+                }
+                __threadfence();
+            }
+        }
+        att_bar();
+        // the jobs of the second turn: one for each run that this CTA was the last to bring its part of
+        jobs = 0;
+        int at = 0;
+        for (int w = 0; w < 2; ++w) {
+            const int run = last_one[w];
+            if (run < 0) continue;
+            const int p0 = part_place[run_first[run]];
+            const long long item0 = part_item[p0][0];
+            const int c0 = cta_of(item0), n = cta_of(part_item[p0][1] - 1) - c0 + 1;
+            for (int k = tid; k < n; k += kAttWorkers * 32)
+                job_from[at + k] = P.cta_part + (static_cast<size_t>(c0 + k) * 2 + (item0 <= (c0 + k) * cta_chunk ? 0 : 1)) * kAttMaxRows * PITCH;
+            if (tid == 0) {
+                job[jobs] = make_int2(at, n);
+                job_rows[jobs] = part_rows[p0];
+                job_to[jobs] = nullptr;
+            }
+            ++jobs;
+            at += n;
+        }
+        if (jobs == 0) return;
+        att_bar();
     }
 }
 
