@@ -424,6 +424,8 @@ int wd_kv_free(wd_kv_cache *c, int n, const int *seqs, void *stream);
 int wd_kv_length(const wd_kv_cache *c, int seq);
 int wd_kv_free_pages(const wd_kv_cache *c);
 int wd_kv_pages(const wd_kv_cache *c, int seq, int *pages, int cap);
+/* Name of the kernels that the last wd_kv_attend ran on: one for few rows or one for prompts, whichever is expected to be through first. */
+const char *wd_kv_kernel_name(const wd_kv_cache *c);
 /* Waits for the device, returns its status word and clears it: 0, or 32 where a NaN or an infinity was appended. */
 int wd_kv_status(wd_kv_cache *c, int *status);
 

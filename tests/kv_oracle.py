@@ -81,12 +81,15 @@ class Cache:
             new.append(g)
         self.pages[seq], self.length[seq] = new, end
 
-    def attend(self, seq, q, scale, window):
-        """q [count][q heads][dim] of the sequence's last tokens."""
+    def attend(self, seq, q, scale, window, rows=None):
+        """q [count][q heads][dim] of the sequence's last tokens, or of some of them: `rows` of the last count ones."""
         k, v = self.numbers(seq)
         n, m, g = self.length[seq], q.shape[0], q.shape[1] // self.heads
+        pos = np.arange(n - m, n)
+        if rows is not None:
+            pos, q = pos[rows], q[rows]
         out = np.zeros(q.shape)
-        pos = np.arange(n - m, n)[:, None]
+        pos = pos[:, None]
         j = np.arange(n)[None]
         seen = (j <= pos) & ((j > pos - window) if window else True)
         for h in range(q.shape[1]):

@@ -385,3 +385,62 @@ def test_rows_of_a_prompt_far_apart_in_size():
     small = np.ones(600, bool)
     small[200:210] = False
     assert np.linalg.norm((got - want)[small]) <= 2e-4 * np.linalg.norm(want[small])
+
+
+@pytest.mark.parametrize("geometry", GEOMETRY + [(16, 2, 128, 64, 1, "f16"), (8, 8, 64, 32, 0, "bf16"), (32, 4, 32, 16, 1, "bf16"), (12, 2, 256, 32, 1, "bf16")])
+@pytest.mark.parametrize("before,count,window", [(0, 4000, 0), (700, 4031, 0), (300, 3500, 1500), (5000, 900, 0), (20, 6001, 100)])
+def test_prompts_that_the_tensor_cores_take(geometry, before, count, window):
+    """Chunks that are large enough for the kernel for prompts, whole items and items cut into runs; some of the rows are looked at."""
+    p = Pair(*geometry, n_pages=900, max_context=7000, layers=1)
+    if before:
+        p.step([1], [before])
+    p.step([1, 0], [count, 3])
+    q = p.rand(count + 3, p.heads, p.dim, size=1.5)
+    qd = q.cuda()
+    out = torch.full_like(qd, 3.0)
+    p.kv.attend(0, qd.data_ptr(), out.data_ptr(), TYPES[p.dtype][1], window=window)
+    if count > 3000 and not window:
+        assert p.kv.kernel_name().startswith("kv_prompt_kernel")
+    torch.cuda.synchronize()
+    rows = np.unique(np.concatenate([[0, 1, 127, 128, 255, 256, count // 2, count - 2, count - 1], np.random.default_rng(1).integers(0, count, 60)]))
+    got = out.double().cpu().numpy()
+    values = max(np.abs(p.ref[0].numbers(i)[1]).max() for i in (0, 1))
+    tol = p.tolerance(q, [1], layer=0)
+    want = p.ref[0].attend(1, q[:count].double().numpy(), p.dim ** -0.5, window, rows=rows)
+    assert np.abs(got[rows] - want).max() <= tol * values
+    assert np.linalg.norm(got[rows] - want) <= 4 * (HALF_STEP[p.dtype] + 2.0 ** -19) * np.linalg.norm(want)
+    want = p.ref[0].attend(0, q[count:].double().numpy(), p.dim ** -0.5, window)
+    assert np.abs(got[count:] - want).max() <= tol * values
+    again = torch.empty_like(out)
+    p.kv.attend(0, qd.data_ptr(), again.data_ptr(), TYPES[p.dtype][1], window=window)
+    torch.cuda.synchronize()
+    assert torch.equal(out, again) and p.kv.status() == 0
+
+
+@pytest.mark.parametrize("chunk,name", [(6000, "kv_prompt_kernel"), (4000, "kv_prompt_kernel, kv_prompt_join_kernel")])       # 94 items; 63, in two runs each
+def test_a_prompt_kernel_in_a_graph_serves_other_steps(chunk, name):
+    """Captured at a long chunk, replayed at shorter ones, at a step of many sequences, and at one without rows."""
+    p = Pair(4, 1, 64, 32, 0, "bf16", n_pages=900, max_context=9000, layers=1)
+    p.step([0], [chunk])
+    q = p.rand(6000, 4, 64).cuda()
+    out = torch.full_like(q, 3.0)
+    s = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        p.kv.attend(0, q.data_ptr(), out.data_ptr(), wd.TYPE_BF16, stream=s.cuda_stream)
+    assert p.kv.kernel_name() == name
+    for seqs, counts in (([0], [100]), ([1, 2, 3, 0], [700, 1, 64, 1]), ([4, 5, 6, 7, 1, 2], [900, 800, 300, 200, 100, 600]), ([2], [0]), ([3], [1])):
+        p.step(seqs, counts)
+        torch.cuda.synchronize()
+        out.fill_(3.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            g.replay()
+        s.synchronize()
+        got, at = out.double().cpu().numpy(), 0
+        for seq, n in zip(seqs, counts):
+            if n:
+                want = p.ref[0].attend(seq, q[at:at + n].double().cpu().numpy(), 0.125, 0)
+                assert np.linalg.norm(got[at:at + n] - want) <= 4 * 2.0 ** -8 * np.linalg.norm(want)
+            at += n
+        assert (got[at:] == 3.0).all()

@@ -185,6 +185,8 @@ def lib():
         L.wd_kv_free_pages.argtypes = [vp]
         L.wd_kv_pages.argtypes = [vp, i, vp, i]
         L.wd_kv_status.argtypes = [vp, C.POINTER(i)]
+        L.wd_kv_kernel_name.argtypes = [vp]
+        L.wd_kv_kernel_name.restype = C.c_char_p
         L.wd_token_logprobs.argtypes = [vp, i, i, i, i64, vp, vp, vp, i, vp, vp, vp]
         L.wd_gguf_open.argtypes = [C.c_char_p, C.POINTER(vp)]
         L.wd_gguf_close.argtypes = [vp]
@@ -681,6 +683,10 @@ class KvCache:
         a = np.zeros(n, np.int32)
         lib().wd_kv_pages(self.h, seq, _ptr(a), n)
         return a
+
+    def kernel_name(self):
+        """Name of the kernels that the last attend ran on."""
+        return lib().wd_kv_kernel_name(self.h).decode()
 
     def status(self):
         """Waits for the device; 0, or 32 where a NaN or an infinity was appended since the last call."""

@@ -44,6 +44,7 @@ struct wd_kv_cache {
     int *d_book = nullptr, *d_index = nullptr;
     unsigned *d_arrived = nullptr, *d_status = nullptr;
     size_t pool_layer = 0, scales_layer = 0;
+    const char *last_kernel = "";           // of wd_kv_attend
     bool broken = false;                    // a launch failed half-way: mirror and device may differ
 
     bool host_only() const { return cfg.device < 0; }
@@ -184,9 +185,6 @@ int flush(wd_kv_cache *c, cudaStream_t s) {
     return WD_OK;
 }
 
-// Rows of a sequence and kv head from which a step's attention runs on the tensor cores that work on tiles of 128.
-constexpr long long kPromptRows = 96;
-
 template <class F>
 int by_codes(const wd_kv_cache *c, F &&f) {
     return c->shape.e4m3 ? f(std::true_type{}) : f(std::false_type{});
@@ -224,6 +222,41 @@ int attend_of(wd_kv_cache *c, wd::KvAttend &p, bool few, cudaStream_t s) {
     return few ? attend_launch<D, 1, false>(c, p, s) : attend_launch<D, (D > 128 ? 1 : 2), false>(c, p, s);
 }
 
+// Which of the two attention kernels a step takes: the one that is expected to be through first, by what each was measured to take (us):
+//   for few rows   c_f for 64 tokens of a head by 16 rows (8 of heads of 256) and worker: heads of 64 1.8, of 128 in F32 4.2, of 256 1.8
+//   for prompts    3 more, and c_p for 128 tokens by 256 rows (128 of heads of 256) and CTA: heads of 64 1.8, of 128 in F32 3.3, of 256 4.5;
+//                  8 more where items are cut into runs
+// (64 rows a head of 64, 1,000 tokens: 15 against 23 us; 512 rows, 8,000 tokens: 63 against 39.)
+struct Choice {
+    bool prompt, split;
+};
+Choice choose(const wd_kv_cache *c, bool f32, int window) {
+    const int g = c->cfg.n_heads / c->cfg.n_kv_heads, d = c->cfg.head_dim, h = c->cfg.n_kv_heads;
+    const int few_rows = d > 128 ? 8 : 16, item_rows = d > 128 ? 128 : 256;
+    double few = 0.0, tiles = 0.0;
+    long long items = 0;
+    int most = 0;
+    for (int i = 0; i < c->book[0]; ++i) {
+        const int *e = c->book.data() + wd::kKvHead + static_cast<size_t>(i) * wd::kKvStepWords;
+        const long long rows = static_cast<long long>(e[2]) * g;
+        if (rows == 0) continue;
+        const int seen = window ? std::min(e[3], window + item_rows / g) : e[3], n = (seen + 127) / 128;
+        const long long blocks = (rows + item_rows - 1) / item_rows;
+        few += static_cast<double>((rows + few_rows - 1) / few_rows) * h * ((seen + 63) / 64);
+        tiles += static_cast<double>(blocks) * h * n;
+        items += blocks * h;
+        most = std::max(most, n);
+    }
+    Choice r;
+    const int runs = wd::prompt_runs(c->n_sm, items, most);
+    r.split = runs > 1;
+    const double c_f = d / 36.0 * (f32 ? 1.2 : 1.0) * (d > 128 ? 0.25 : 1.0), c_p = (1.0 + d / 80.0) * (f32 ? 1.3 : 1.0);
+    const double of_few = c_f * few / (c->n_sm * (d > 128 ? 4.0 : 8.0));
+    const double of_prompt = 3.0 + (r.split ? 8.0 + c_p * most / runs : c_p * std::max<double>(most, tiles / c->n_sm));
+    r.prompt = of_prompt < of_few;
+    return r;
+}
+
 template <int D, bool SPLIT>
 int prompt_launch(wd_kv_cache *c, const wd::KvPrompt &p, cudaStream_t s) {
     return by_codes(c, [&](auto e4m3) {
@@ -231,6 +264,7 @@ int prompt_launch(wd_kv_cache *c, const wd::KvPrompt &p, cudaStream_t s) {
         constexpr int smem = wd::PromptAttPlan<D, SPLIT>::kSmem;
         WD_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         kernel<<<c->n_sm, wd::kPromptThreads, smem, s>>>(p);
+        if (p.split) wd::kv_prompt_join_kernel<D><<<2 * c->n_sm, 256, 0, s>>>(p);
         WD_TRY_CUDA(cudaGetLastError());
         return WD_OK;
     });
@@ -381,14 +415,14 @@ int wd_kv_append(wd_kv_cache *c, int layer, const void *k_dev, const void *v_dev
         wd::KvAppend p;
         int rows_of = 0;
         if (int rc = rows_type(type, &rows_of)) return rc;
+        if (c->book[0] == 0) return set_error(WD_E_STATE, "key/value cache: no step has begun");
+        if (c->items == 0) return WD_OK;        // (no rows: nothing is asked of their address)
         const size_t size = rows_size(rows_of);
         p.stride[0] = k_stride;
         p.stride[1] = v_stride;
         const long long width = static_cast<long long>(c->cfg.n_kv_heads) * c->cfg.head_dim;
         if (int rc = check_rows(k_dev, size, &p.stride[0], width, "k")) return rc;
         if (int rc = check_rows(v_dev, size, &p.stride[1], width, "v")) return rc;
-        if (c->book[0] == 0) return set_error(WD_E_STATE, "key/value cache: no step has begun");
-        if (c->items == 0) return WD_OK;
         OnDevice on(c->cfg.device);
         p.pool = c->d_pool + layer * c->pool_layer;
         p.scales = c->d_scales + layer * c->scales_layer;
@@ -422,13 +456,13 @@ int wd_kv_attend(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, in
         if (window < 0) return set_error(WD_E_INVALID, "key/value cache: a window is 0 (none) or at least 1");
         wd::KvAttend p;
         if (int rc = rows_type(type, &p.type)) return rc;
+        if (c->book[0] == 0) return set_error(WD_E_STATE, "key/value cache: no step has begun");
+        if (c->rows == 0) return WD_OK;
         p.q_stride = q_stride;
         p.out_stride = out_stride;
         const long long width = static_cast<long long>(c->cfg.n_heads) * c->cfg.head_dim;
         if (int rc = check_rows(q_dev, rows_size(p.type), &p.q_stride, width, "q")) return rc;
         if (int rc = check_rows(out_dev, rows_size(p.type), &p.out_stride, width, "out")) return rc;
-        if (c->book[0] == 0) return set_error(WD_E_STATE, "key/value cache: no step has begun");
-        if (c->rows == 0) return WD_OK;
         OnDevice on(c->cfg.device);
         p.pool = c->d_pool + layer * c->pool_layer;
         p.scales = c->d_scales + layer * c->scales_layer;
@@ -447,11 +481,14 @@ int wd_kv_attend(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, in
         p.s = c->shape;
         const long long group = static_cast<long long>(c->max_rows) * (c->cfg.n_heads / c->cfg.n_kv_heads);
         cudaStream_t s = static_cast<cudaStream_t>(stream);
-        if (group >= kPromptRows) {
+        const Choice by = choose(c, p.type == wd::kRowsF32, window);
+        c->last_kernel = by.prompt ? by.split ? "kv_prompt_kernel, kv_prompt_join_kernel" : "kv_prompt_kernel" : "kv_attend_kernel";
+        if (by.prompt) {
             wd::KvPrompt r;
             r.pool = p.pool, r.scales = p.scales, r.book = p.book, r.table = p.table, r.q = p.q, r.out = p.out;
             r.q_stride = p.q_stride, r.out_stride = p.out_stride, r.status = p.status, r.scale_log2 = p.scale_log2;
-            r.type = p.type, r.window = p.window, r.s = p.s;
+            r.type = p.type, r.window = p.window, r.s = p.s, r.part = c->d_part, r.ctas = c->n_sm;
+            r.split = by.split;         // (the kernels count the items of the step that is current when they run)
             const size_t size = rows_size(p.type);
             r.vec = (reinterpret_cast<uintptr_t>(q_dev) | reinterpret_cast<uintptr_t>(out_dev)) % 16 == 0 && p.q_stride * size % 16 == 0 && p.out_stride * size % 16 == 0;
             switch (c->cfg.head_dim) {
@@ -688,6 +725,7 @@ int wd_kv_pages(const wd_kv_cache *c, int seq, int *pages, int cap) {
     std::copy_n(p.begin(), std::min<size_t>(p.size(), cap), pages);
     return static_cast<int>(p.size());
 }
+const char *wd_kv_kernel_name(const wd_kv_cache *c) { return c ? c->last_kernel : ""; }
 int wd_kv_status(wd_kv_cache *c, int *status) {
     return wd_host::guarded([&]() -> int {
         if (int rc = check_device(c)) return rc;

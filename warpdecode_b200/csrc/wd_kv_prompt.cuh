@@ -12,7 +12,8 @@
 //   warp 12                issues the products, the two row tiles in turn: Q K of the next tokens, P V of these (a warp for each tile is slower:
 //                          249 -> 196 us with one, 209 with two)
 //
-// Items are dealt out heaviest first, back and forth over the CTAs (the last rows of a sequence see the most).
+// Items are dealt out heaviest first, back and forth over the CTAs (the last rows of a sequence see the most). Where there are not half as many as CTAs
+// each is cut into as many runs of its tokens as fill them, and a second kernel puts the runs' sums together.
 #pragma once
 
 #include "wd_kv_attend.cuh"
@@ -34,8 +35,9 @@ struct KvPrompt {
     void *out;
     long long q_stride, out_stride;
     unsigned *status;
+    float *part;                // [CTAs][rows of an item][D + 4]: sums, then maximum and denominator
     float scale_log2;
-    int type, window, vec;      // vec: rows of q and out lie on boundaries of 16 bytes
+    int type, window, vec, split, ctas;         // vec: rows of q and out lie on boundaries of 16 bytes; split: items may be cut into runs
     KvShape s;
 };
 
@@ -62,8 +64,63 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 struct PromptItem {
-    int seq, row0, count, length, head, item_row, rows, lo, hi;         // rows: of the sequence and head; lo .. hi - 1: tiles of KT tokens
+    int seq, row0, count, length, head, item_row, rows, lo, hi, at;         // rows: of the sequence and head; lo .. hi - 1: tiles of KT tokens; at: place of a part
 };
+
+// Items of one head in front of each sequence, and behind their number the most tiles of 128 tokens that one sees; by one warp.
+__device__ __forceinline__ void prompt_prefix(const KvPrompt &P, int rows, int *prefix, int lane) {
+    const int n_seq = P.book[0], g_heads = P.s.heads / P.s.kv_heads;
+    const int *entries = P.book + kKvHead;
+    int sum = 0, most = 0;
+    for (int i0 = 0; i0 < n_seq; i0 += 32) {
+        const int i = i0 + lane;
+        int inc = 0;
+        if (i < n_seq) {
+            const int4 e = *reinterpret_cast<const int4 *>(entries + i * kKvStepWords);
+            inc = static_cast<int>((static_cast<long long>(e.z) * g_heads + rows - 1) / rows);
+            most = max(most, (P.window ? min(e.w, min(P.window, e.w) + rows / g_heads) : e.w) + 127 >> 7);
+        }
+        const int v = inc;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += y;
+        }
+        if (i < n_seq) prefix[i] = sum + inc - v;
+        sum += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) {
+        prefix[n_seq] = sum;
+        prefix[n_seq + 1] = most;
+    }
+}
+// Runs that each of n items, of `most` tiles the longest, is cut into: parts and the second kernel cost what four tiles do, so that items of less than
+// seven stay whole. (8 items of 63 tiles: 112 -> 27 us; of 8: 28 -> 23; 64 of 4, in two: 19 -> 33, left alone.)
+__host__ __device__ inline int prompt_runs(int ctas, long long n, int most) {
+    if (n < 1 || 2 * n > ctas || most < 7) return 1;
+    const int fit = static_cast<int>(ctas / n), few = most / 3;
+    return fit < few ? fit : few;
+}
+// item number n: where its rows are
+__device__ __forceinline__ PromptItem prompt_item(const KvPrompt &P, const int *prefix, int n_seq, long long n, int rows) {
+    PromptItem it;
+    const int H = P.s.kv_heads;
+    int lo = 0, hi = n_seq - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (static_cast<long long>(prefix[mid]) * H <= n) lo = mid;
+        else hi = mid - 1;
+    }
+    const int4 e = *reinterpret_cast<const int4 *>(P.book + kKvHead + lo * kKvStepWords);
+    it.seq = e.x, it.row0 = e.y, it.count = e.z, it.length = e.w;
+    const int in = static_cast<int>(n - static_cast<long long>(prefix[lo]) * H), blocks = prefix[lo + 1] - prefix[lo];
+    it.head = in % H;
+    it.item_row = (blocks - 1 - in / H) * rows;
+    it.rows = it.count * (P.s.heads / H);
+    it.at = 0;
+    return it;
+}
 
 template <int D, bool SPLIT, bool E4M3>
 __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __grid_constant__ KvPrompt P) {
@@ -78,7 +135,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
     int *prefix = reinterpret_cast<int *>(vs + ST * A::kV);
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int n_seq = P.book[0], g_heads = P.s.heads / P.s.kv_heads, H = P.s.kv_heads;
-    const int *entries = P.book + kKvHead;
     if (warp == 0) {
         if (lane == 0) {
             for (int i = 0; i < ST; ++i) {
@@ -96,21 +152,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
             }
             mbar_fence_init();
         }
-        int sum = 0;
-        for (int i0 = 0; i0 < n_seq; i0 += 32) {
-            const int i = i0 + lane;
-            int inc = 0;
-            if (i < n_seq) inc = static_cast<int>((static_cast<long long>(entries[i * kKvStepWords + 2]) * g_heads + A::kRows - 1) / A::kRows);
-            const int v = inc;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += y;
-            }
-            if (i < n_seq) prefix[i] = sum + inc - v;
-            sum += __shfl_sync(0xffffffffu, inc, 31);
-        }
-        if (lane == 0) prefix[n_seq] = sum;
+        prompt_prefix(P, A::kRows, prefix, lane);
     }
     if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_base)) : "memory");
@@ -122,25 +164,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
     const uint32_t tm = tmem_base;
     const long long n_items = static_cast<long long>(prefix[n_seq]) * H;
 
-    // item number `turn` of this CTA; false behind the last
+    const int runs = P.split ? prompt_runs(P.ctas, n_items, prefix[n_seq + 1]) : 1;
+    // item number `turn` of this CTA, or its run of one; false behind the last
     auto item_of = [&](int turn, PromptItem &it) {
         const long long at = static_cast<long long>(turn) * gridDim.x + (turn & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-        if (at >= n_items) return false;
-        int lo = 0, hi = n_seq - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (static_cast<long long>(prefix[mid]) * H <= at) lo = mid;
-            else hi = mid - 1;
-        }
-        const int *e = entries + lo * kKvStepWords;
-        it.seq = e[0], it.row0 = e[1], it.count = e[2], it.length = e[3];
-        const int in = static_cast<int>(at - static_cast<long long>(prefix[lo]) * H), blocks = prefix[lo + 1] - prefix[lo];
-        it.head = in % H;
-        it.item_row = (blocks - 1 - in / H) * A::kRows;
-        it.rows = it.count * g_heads;
+        if (at >= n_items * runs) return false;
+        it = prompt_item(P, prefix, n_seq, runs > 1 ? at / runs : at, A::kRows);
         const int start = it.length - it.count, pos0 = start + it.item_row / g_heads, pos1 = start + min(it.item_row + A::kRows - 1, it.rows - 1) / g_heads;
         it.lo = P.window ? max(0, pos0 - P.window + 1) / KT : 0;
         it.hi = pos1 / KT + 1;
+        if (runs > 1) {
+            const int run = static_cast<int>(at % runs), n = it.hi - it.lo, lo = it.lo;
+            it.lo = lo + static_cast<int>(static_cast<long long>(n) * run / runs);
+            it.hi = lo + static_cast<int>(static_cast<long long>(n) * (run + 1) / runs);
+            it.at = static_cast<int>(at);
+        }
         return true;
     };
 
@@ -191,6 +229,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
             };
             for (int turn = 0; item_of(turn, it); ++turn, ++items) {
                 const int n = it.hi - it.lo;
+                if (n == 0) break;              // (a run of a short item; there is no other item then)
                 keys(0);
                 if constexpr (A::kApart && T == 2) {
                     // The second tile begins when the first has its weights, and stays that much behind: one makes exponentials while the other reads
@@ -265,7 +304,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
                 in_page = sub & ((1 << (shift - 4)) - 1);
                 if (cw == 0) sc = *reinterpret_cast<const float2 *>(P.scales + (static_cast<size_t>(page) * H + it.head) * 2);
             };
-            look_up(it.lo);
+            if (it.lo < it.hi) look_up(it.lo);
             for (int tile = it.lo; tile < it.hi; ++tile, ++n) {
                 const size_t at = static_cast<size_t>(page) * kv_page_bytes(P.s) + static_cast<size_t>(in_page) * (16 * D);
                 const float vsc = sc.y > 0.0f ? sc.y : kKvLeastScale;
@@ -402,7 +441,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
                 }
             }
             fence_proxy_async();
-            mbar_arrive(&q_full[x]);
+            if (it.lo < it.hi) mbar_arrive(&q_full[x]);
             float m = kAttFloor, l = 0.0f;
 #pragma unroll 1
             for (int tile = it.lo; tile < it.hi; ++tile, ++n) {
@@ -500,8 +539,25 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
                 mbar_arrive(&p_full[x]);
                 ++n_o;
             }
-            att_wait(&o_done[x], (n_o - 1) & 1, P.status);
+            if (it.lo < it.hi) att_wait(&o_done[x], (n_o - 1) & 1, P.status);
             tc_fence_after();
+            if (runs > 1) {         // for the kernel behind
+                float *part = P.part + (static_cast<size_t>(it.at) * A::kRows + x * 128 + r) * (D + 4);
+#pragma unroll 1
+                for (int c = 0; c < D / 16; ++c) {
+                    uint32_t v[16];
+                    tc_ld(oc + c * 16, v);
+                    tc_wait_ld(v);
+                    if (is && it.lo < it.hi) {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4)
+                            *reinterpret_cast<uint4 *>(part + c * 16 + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                    }
+                    __syncwarp();
+                }
+                if (is) *reinterpret_cast<float2 *>(part + D) = make_float2(m, l);         // (of an empty run nothing else is read)
+                continue;
+            }
             const float inv = 1.0f / l;
             const size_t dst = static_cast<size_t>(it.row0 + row / g_heads) * P.out_stride + elem;
 #pragma unroll 1
@@ -541,6 +597,48 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
     __syncthreads();
     tc_fence_after();
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm) : "memory");
+}
+
+// The runs' sums of each row of the items: a warp has a row.
+template <int D>
+__global__ void __launch_bounds__(256) kv_prompt_join_kernel(const __grid_constant__ KvPrompt P) {
+    constexpr int ROWS = D <= 128 ? 256 : 128;
+    __shared__ int prefix[kAttMaxSeqs + 2];
+    const int tid = threadIdx.x, lane = tid & 31, n_seq = P.book[0], g_heads = P.s.heads / P.s.kv_heads;
+    if (tid < 32) prompt_prefix(P, ROWS, prefix, lane);
+    __syncthreads();
+    const long long n_items = static_cast<long long>(prefix[n_seq]) * P.s.kv_heads;
+    const int runs = P.split ? prompt_runs(P.ctas, n_items, prefix[n_seq + 1]) : 1;
+    if (runs == 1) return;
+    for (long long u = static_cast<long long>(blockIdx.x) * 8 + (tid >> 5); u < n_items * ROWS; u += static_cast<long long>(gridDim.x) * 8) {
+        const long long n = u / ROWS;
+        const int r = static_cast<int>(u % ROWS);
+        const PromptItem it = prompt_item(P, prefix, n_seq, n, ROWS);
+        const int row = it.item_row + r;
+        if (row >= it.rows) continue;
+        const float *part = P.part + (static_cast<size_t>(n) * runs * ROWS + r) * (D + 4);
+        // the maximum, the denominator and each run's factor: a lane has every 32nd run's
+        float top = kAttFloor;
+        for (int k = lane; k < runs; k += 32) top = fmaxf(top, part[static_cast<size_t>(k) * ROWS * (D + 4) + D]);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float sum[D / 32], den = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) sum[i] = 0.0f;
+#pragma unroll 4
+        for (int k = 0; k < runs; ++k) {
+            const float *p = part + static_cast<size_t>(k) * ROWS * (D + 4);
+            const float2 z = *reinterpret_cast<const float2 *>(p + D);
+            const float f = z.y > 0.0f ? ex2(z.x - top) : 0.0f;
+            den = fmaf(z.y, f, den);
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) sum[i] = f > 0.0f ? fmaf(p[i * 32 + lane], f, sum[i]) : sum[i];
+        }
+        const float inv = 1.0f / den;
+        const size_t to = static_cast<size_t>(it.row0 + row / g_heads) * P.out_stride + (static_cast<size_t>(it.head) * g_heads + row % g_heads) * D + lane;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) row_store(P.out, P.type, to + i * 32, sum[i] * inv);
+    }
 }
 
 }  // namespace wd
