@@ -560,7 +560,7 @@ int wd_kv_read(wd_kv_cache *c, int layer, int n, const int *seqs, const int *fir
                 row += counts[i];
             }
             if (p.n == 0) continue;
-            const dim3 grid(static_cast<unsigned>(items), static_cast<unsigned>(layers));
+            const dim3 grid(static_cast<unsigned>(items), static_cast<unsigned>(layers), 2);
             const int rc = by_rows_and_codes(c, rows_of, [&](auto t, auto e4m3) {
                 wd::kv_read_kernel<decltype(t), decltype(e4m3)::value><<<grid, wd::kReadThreads, 0, s>>>(p);
                 WD_TRY_CUDA(cudaGetLastError());
@@ -688,14 +688,20 @@ int wd_kv_keep(wd_kv_cache *c, int seq, int first, int n, const int *index, void
             p.pages = pages;
             p.s = c->shape;
             const size_t smem = static_cast<size_t>(c->cfg.page_tokens) * c->cfg.head_dim;
-            const int per = std::max(1, 65535 / c->cfg.n_kv_heads);
-            for (int l = 0; l < c->cfg.n_layers; l += per) {
-                const dim3 grid(fresh ? pages : 1, static_cast<unsigned>(std::min(per, c->cfg.n_layers - l) * c->cfg.n_kv_heads), 2);
-                wd::KvKeep pl = p;
-                pl.pool += l * c->pool_layer;
-                pl.scales += l * c->scales_layer;
-                if (c->shape.e4m3) wd::kv_keep_kernel<true><<<grid, wd::kKeepThreads, smem, s>>>(pl);
-                else wd::kv_keep_kernel<false><<<grid, wd::kKeepThreads, smem, s>>>(pl);
+            if (fresh) {
+                const dim3 grid(pages, c->cfg.n_layers, (c->cfg.n_kv_heads + wd::kKeepHeads - 1) / wd::kKeepHeads);
+                if (c->shape.e4m3) wd::kv_keep_new_kernel<true><<<grid, wd::kKeepThreads, 0, s>>>(p);
+                else wd::kv_keep_new_kernel<false><<<grid, wd::kKeepThreads, 0, s>>>(p);
+            } else {
+                const int per = std::max(1, 65535 / c->cfg.n_kv_heads);         // (the second index of a grid ends at 65,535)
+                for (int l = 0; l < c->cfg.n_layers; l += per) {
+                    const dim3 grid(1, static_cast<unsigned>(std::min(per, c->cfg.n_layers - l) * c->cfg.n_kv_heads), 2);
+                    wd::KvKeep pl = p;
+                    pl.pool += l * c->pool_layer;
+                    pl.scales += l * c->scales_layer;
+                    if (c->shape.e4m3) wd::kv_keep_kernel<true><<<grid, wd::kKeepThreads, smem, s>>>(pl);
+                    else wd::kv_keep_kernel<false><<<grid, wd::kKeepThreads, smem, s>>>(pl);
+                }
             }
             WD_TRY_CUDA(cudaGetLastError());
             c->broken = false;

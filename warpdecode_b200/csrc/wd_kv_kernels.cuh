@@ -42,7 +42,7 @@ struct KvAppend {
 };
 
 template <class T, bool E4M3, int THREADS>
-__global__ void __launch_bounds__(THREADS) kv_append_kernel(const __grid_constant__ KvAppend P) {
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 5 : 8) kv_append_kernel(const __grid_constant__ KvAppend P) {
     extern __shared__ __align__(16) uint8_t app_sm[];           // values: the codes of the sub-blocks that the rows touch
     __shared__ float part[THREADS / 32];
     __shared__ int bad_any;
@@ -97,12 +97,15 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(const __grid_constan
                 const int sub = i / D, v = i - sub * D, cw = kv_cw(D), token = (v * 16 % (16 * cw)) / cw;      // (of keys)
                 if (kv == 0 && sub * kKvSub + token >= a) continue;        // another thread may have written its new codes already
                 uint4 *p = reinterpret_cast<uint4 *>(base + sub * kv_sub_bytes(D)) + v;
-                uint4 x = *p;
-                uint8_t *c = reinterpret_cast<uint8_t *>(&x);
+                const uint4 x = *p;
+                uint4 y = make_uint4(kv_recode4<E4M3>(x.x, s0, s1, ratio), kv_recode4<E4M3>(x.y, s0, s1, ratio), kv_recode4<E4M3>(x.z, s0, s1, ratio), kv_recode4<E4M3>(x.w, s0, s1, ratio));
+                if (kv) {               // tokens from a on are written behind
+                    uint32_t mask = 0;
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (sub * kKvSub + (kv ? kv_v_token(v, j) : token) < a) c[j] = static_cast<uint8_t>(kv_recode<E4M3>(c[j], s0, s1, ratio));
-                *p = x;
+                    for (int j = 0; j < 4; ++j) mask |= sub * kKvSub + kv_v_token(v, j) < a ? 0xffu << (8 * j) : 0u;
+                    y = make_uint4((y.x & mask) | (x.x & ~mask), (y.y & mask) | (x.y & ~mask), (y.z & mask) | (x.z & ~mask), (y.w & mask) | (x.w & ~mask));
+                }
+                *p = y;
             }
         }
         const int sub0 = a / kKvSub;
@@ -110,10 +113,8 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(const __grid_constan
             const int t = i / per, k = (i - t * per) * 16, token = a + t;
             float y[16];
             row_load16(rows + t * stride + k, vec, y);
-            uint4 x;
-            uint8_t *c = reinterpret_cast<uint8_t *>(&x);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) c[j] = static_cast<uint8_t>(kv_code<E4M3>(y[j], s1, r));
+            const uint4 x = kv_encode16<E4M3>(y, s1, r);
+            const uint8_t *c = reinterpret_cast<const uint8_t *>(&x);
             if (kv == 0) {
                 *reinterpret_cast<uint4 *>(base + (token / kKvSub) * kv_sub_bytes(D) + kv_k_offset(D, token % kKvSub, k)) = x;
             } else {
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(const __grid_constan
 
 // ---- read -----------------------------------------------------------------------------------------------------------------
 // Tokens first .. first + count - 1 of sequences as numbers, rows one after the other: [layer][row][kv head][D]. A block takes a sub-block of
-// 16 tokens of a layer, all heads, keys and values; a warp 512 bytes, which are 16 tokens of 32 elements of a value's head (turned in shared
+// 16 tokens of a layer, all heads, keys (blockIdx.z = 0) or values; a warp 512 bytes, which are 16 tokens of 32 elements of a value's head (turned in shared
 // memory, so that rows are written in pieces of 64 bytes and more).
 struct KvReadEntry {
     int seq, first, count, row0, item0;         // items: sub-blocks that the range touches
@@ -185,42 +186,55 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const __grid_cons
     T *ko = static_cast<T *>(P.out[0]), *vo = static_cast<T *>(P.out[1]);
     const size_t row0 = static_cast<size_t>(e.row0 + t0 - e.first);        // of token 0, which may lie in front of the rows
     const int per_head = D / 32, units = P.s.kv_heads * per_head, cw = kv_cw(D);         // a unit is 512 bytes
-    constexpr int N = 16 / sizeof(T);
-#pragma unroll 2
-    for (int u = warp; u < 2 * units; u += kReadThreads / 32) {
-        const int kv = u >= units, in = u - kv * units, h = in / per_head, blk = in - h * per_head;
-        if ((kv ? vo : ko) == nullptr) continue;
-        const uint4 x = *reinterpret_cast<const uint4 *>(base + h * head_bytes + kv * half + blk * 512 + lane * 16);
-        const uint8_t *c = reinterpret_cast<const uint8_t *>(&x);
-        const float s = scales[h * 2 + kv];
-        if (kv == 0) {
-            const int at = blk * 512 + lane * 16, token = at % (16 * cw) / cw, k = at / (16 * cw) * cw + at % cw;
-            if (token < a || token >= b) continue;
-            T *to = ko + layer * P.out_layer + (row0 + token) * pitch + static_cast<size_t>(h) * D + k;
-            __align__(16) T y[16];
+    constexpr int N = 16 / sizeof(T), BATCH = 4, WARPS = kReadThreads / 32;
+    const int kv = blockIdx.z;
+    if ((kv ? vo : ko) == nullptr) return;
+#pragma unroll 1
+    for (int u0 = warp; u0 < units; u0 += BATCH * WARPS) {
+        uint4 x[BATCH];
+        float s[BATCH];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) y[j] = row_number<T>(__fmul_rn(kv_value<E4M3>(c[j]), s));
-            if (P.vec) {
+        for (int i = 0; i < BATCH; ++i) {           // all on their way before the first is needed
+            const int u = min(u0 + i * WARPS, units - 1), h = u / per_head, blk = u - h * per_head;
+            x[i] = *reinterpret_cast<const uint4 *>(base + h * head_bytes + kv * half + blk * 512 + lane * 16);
+            s[i] = scales[h * 2 + kv];
+        }
 #pragma unroll
-                for (int j = 0; j < 16; j += N) *reinterpret_cast<uint4 *>(to + j) = *reinterpret_cast<const uint4 *>(y + j);
-            } else {
+        for (int i = 0; i < BATCH; ++i) {
+            const int u = u0 + i * WARPS, h = u / per_head, blk = u - h * per_head;
+            if (u >= units) break;
+            float v[16];
+            kv_values4<E4M3>(x[i].x, v), kv_values4<E4M3>(x[i].y, v + 4), kv_values4<E4M3>(x[i].z, v + 8), kv_values4<E4M3>(x[i].w, v + 12);
+            if (kv == 0) {
+                const int at = blk * 512 + lane * 16, token = at % (16 * cw) / cw, k = at / (16 * cw) * cw + at % cw;
+                if (token >= a && token < b) {
+                    T *to = ko + layer * P.out_layer + (row0 + token) * pitch + static_cast<size_t>(h) * D + k;
+                    __align__(16) T y[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) to[j] = y[j];
-            }
-        } else {
-            __syncwarp();
+                    for (int j = 0; j < 16; ++j) y[j] = row_number<T>(__fmul_rn(v[j], s[i]));
+                    if (P.vec) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) turned[warp][kv_v_token(lane, j)][kv_v_element(lane, j)] = row_number<T>(__fmul_rn(kv_value<E4M3>(c[j]), s));
-            __syncwarp();
-            T *to = vo + layer * P.out_layer + row0 * pitch + static_cast<size_t>(h) * D + blk * 32;
-            if (P.vec) {
+                        for (int j = 0; j < 16; j += N) *reinterpret_cast<uint4 *>(to + j) = *reinterpret_cast<const uint4 *>(y + j);
+                    } else {
 #pragma unroll
-                for (int i = lane; i < kKvSub * 32 / N; i += 32) {
-                    const int token = i / (32 / N), d = i % (32 / N) * N;
-                    if (token >= a && token < b) *reinterpret_cast<uint4 *>(to + token * pitch + d) = *reinterpret_cast<const uint4 *>(&turned[warp][token][d]);
+                        for (int j = 0; j < 16; ++j) to[j] = y[j];
+                    }
                 }
             } else {
-                for (int token = a; token < b; ++token) to[token * pitch + lane] = turned[warp][token][lane];
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) turned[warp][kv_v_token(lane, j)][kv_v_element(lane, j)] = row_number<T>(__fmul_rn(v[j], s[i]));
+                __syncwarp();
+                T *to = vo + layer * P.out_layer + row0 * pitch + static_cast<size_t>(h) * D + blk * 32;
+                if (P.vec) {
+#pragma unroll
+                    for (int j = lane; j < kKvSub * 32 / N; j += 32) {
+                        const int token = j / (32 / N), d = j % (32 / N) * N;
+                        if (token >= a && token < b) *reinterpret_cast<uint4 *>(to + token * pitch + d) = *reinterpret_cast<const uint4 *>(&turned[warp][token][d]);
+                    }
+                } else {
+                    for (int token = a; token < b; ++token) to[token * pitch + lane] = turned[warp][token][lane];
+                }
             }
         }
     }
@@ -251,9 +265,8 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(const __grid_constant__ Kv
 
 // ---- keep -----------------------------------------------------------------------------------------------------------------
 // Of a sequence's tokens from `first` on those of `index` stay and move together. A block builds one page, one head, keys or values of one layer:
-// its tokens come from pages behind it (or itself), its scale is the largest of theirs, codes of smaller ones are rounded anew. Pages that are built
-// into new pages are independent of one another (gridDim.x = pages); where there are none to be had, a block walks over the pages in their order,
-// reading all of a page's tokens before it writes (gridDim.x = 1).
+// its tokens come from pages behind it (or itself), its scale is the largest of theirs, codes of smaller ones are rounded anew. Where there are no free
+// pages to be had, a block walks over the pages in their order, reading all of a page's tokens before it writes.
 struct KvKeep {
     uint8_t *pool;
     float *scales;
@@ -265,6 +278,14 @@ struct KvKeep {
     KvShape s;
 };
 constexpr int kKeepThreads = 256;
+// byte shift8 / 8 of each word as the bytes of one, and the bytes of z as byte q of each word
+__device__ __forceinline__ uint32_t kv_byte_of_each(const uint4 &y, int shift8) {
+    return __byte_perm(__byte_perm(y.x >> shift8, y.y >> shift8, 0x0040), __byte_perm(y.z >> shift8, y.w >> shift8, 0x0040), 0x5410);
+}
+__device__ __forceinline__ void kv_byte_to_each(uint4 &x, uint32_t z, int q) {
+    const uint32_t shift = 8 * q;
+    x.x |= (z & 0xffu) << shift, x.y |= (z >> 8 & 0xffu) << shift, x.z |= (z >> 16 & 0xffu) << shift, x.w |= (z >> 24) << shift;
+}
 
 template <bool E4M3>
 __global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(const __grid_constant__ KvKeep P) {
@@ -279,7 +300,7 @@ __global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(const __grid_cons
     const size_t page_bytes = kv_page_bytes(P.s);
     const int page_scales = P.s.kv_heads * 2;
 #pragma unroll 1
-    for (int i = blockIdx.x; i < P.pages; i += gridDim.x) {
+    for (int i = 0; i < P.pages; ++i) {
         const int p0 = (P.page0 + i) << shift;
         if (tid < tokens) {
             const int pos = p0 + tid;
@@ -303,7 +324,6 @@ __global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(const __grid_cons
         for (int j = tid; j < used * D; j += kKeepThreads) {         // 16 bytes each
             const int sub = j / D, v = j - sub * D;
             uint4 x = make_uint4(0, 0, 0, 0);
-            uint8_t *c = reinterpret_cast<uint8_t *>(&x);
             if (kv == 0) {
                 const int cw = kv_cw(D), at = v * 16, t = sub * kKvSub + at % (16 * cw) / cw, src = source[t];
                 if (src >= 0) {
@@ -312,8 +332,7 @@ __global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(const __grid_cons
                     const float s0 = from_scale[t];
                     if (s0 != s1) {
                         const float ratio = __fdiv_rn(s0, s1);
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) c[k] = static_cast<uint8_t>(kv_recode<E4M3>(c[k], s0, s1, ratio));
+                        x = make_uint4(kv_recode4<E4M3>(x.x, s0, s1, ratio), kv_recode4<E4M3>(x.y, s0, s1, ratio), kv_recode4<E4M3>(x.z, s0, s1, ratio), kv_recode4<E4M3>(x.w, s0, s1, ratio));
                     }
                 }
             } else {
@@ -326,16 +345,10 @@ __global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(const __grid_cons
                     const uint8_t *p = pool + from_page[t] + (o / kKvSub) * kv_sub_bytes(D) + kv_v_offset(o % kKvSub, kv_v_element(v, 0));
                     const uint4 y = *reinterpret_cast<const uint4 *>(reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(15));
                     const int shift8 = 8 * static_cast<int>(reinterpret_cast<uintptr_t>(p) & 3);
-                    int z[4] = {static_cast<int>(y.x >> shift8 & 0xff), static_cast<int>(y.y >> shift8 & 0xff), static_cast<int>(y.z >> shift8 & 0xff),
-                                static_cast<int>(y.w >> shift8 & 0xff)};
+                    uint32_t z = kv_byte_of_each(y, shift8);
                     const float s0 = from_scale[t];
-                    if (s0 != s1) {
-                        const float ratio = __fdiv_rn(s0, s1);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) z[k] = kv_recode<E4M3>(z[k], s0, s1, ratio);
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) c[4 * k + q] = static_cast<uint8_t>(z[k]);
+                    if (s0 != s1) z = kv_recode4<E4M3>(z, s0, s1, __fdiv_rn(s0, s1));
+                    kv_byte_to_each(x, z, q);
                 }
             }
             reinterpret_cast<uint4 *>(keep_sm)[j] = x;
@@ -349,6 +362,87 @@ __global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(const __grid_cons
         if (tid == 0) scales[static_cast<size_t>(page) * page_scales] = s1;
         __syncthreads();
     }
+}
+
+// The same into new pages, which need no order: a block builds a page of a layer for up to eight heads, keys and values, and writes what it gathers. (With a
+// block for each head, the chain of index, table and scale in front of the first code was most of its time: 3,301 of 5,900 tokens in 16 layers of 8 heads
+// of 64, 92 us.)
+constexpr int kKeepHeads = 8;
+template <bool E4M3>
+__global__ void __launch_bounds__(kKeepThreads) kv_keep_new_kernel(const __grid_constant__ KvKeep P) {
+    __shared__ int source[128];                               // position of each token, -1 behind the last
+    __shared__ size_t from_page[128];
+    __shared__ float from_scale[2 * kKeepHeads][128], top[2 * kKeepHeads];
+    const int i = blockIdx.x, layer = blockIdx.y, h0 = blockIdx.z * kKeepHeads, hk_n = 2 * min(kKeepHeads, P.s.kv_heads - h0), D = P.s.head_dim, tid = threadIdx.x;
+    const int lane = tid & 31, shift = P.s.page_shift, tokens = 1 << shift, mask = tokens - 1, page_scales = P.s.kv_heads * 2;
+    uint8_t *pool = P.pool + layer * P.pool_layer + h0 * kv_head_bytes(P.s);
+    float *scales = P.scales + layer * P.scales_layer + h0 * 2;
+    const size_t page_bytes = kv_page_bytes(P.s), half = kv_half_bytes(P.s);
+    const int p0 = (P.page0 + i) << shift;
+    if (tid < tokens) {
+        const int pos = p0 + tid, src = pos < P.first ? pos : pos < P.first + P.kept ? P.first + P.index[pos - P.first] : -1;
+        source[tid] = src;
+        from_page[tid] = src < 0 ? 0 : static_cast<size_t>(P.table[src >> shift]);
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int u = tid; u < tokens * hk_n; u += kKeepThreads) {
+        const int t = u & mask, hk = u >> shift;
+        from_scale[hk][t] = source[t] < 0 ? 0.0f : scales[from_page[t] * page_scales + hk];
+    }
+    __syncthreads();
+    for (int hk = tid >> 5; hk < hk_n; hk += kKeepThreads / 32) {
+        float m = 0.0f;
+        for (int t = lane; t < tokens; t += 32) m = fmaxf(m, from_scale[hk][t]);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (lane == 0) top[hk] = m;
+    }
+    __syncthreads();
+    const size_t page = static_cast<size_t>(P.to[i]);
+    const int used = (min(P.first + P.kept - p0, tokens) + kKvSub - 1) / kKvSub, vecs = used * D, cw = kv_cw(D);
+#pragma unroll 1
+    for (int hk = 0; hk < hk_n; ++hk) {
+        const int kv = hk & 1;
+        uint8_t *mine = pool + (hk >> 1) * kv_head_bytes(P.s) + kv * half;
+        const float s1 = top[hk];
+#pragma unroll 2
+        for (int j = tid; j < vecs; j += kKeepThreads) {
+            const int sub = j / D, v = j - sub * D;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (kv == 0) {
+                const int at = v * 16, t = sub * kKvSub + at % (16 * cw) / cw, src = source[t];
+                if (src >= 0) {
+                    const int o = src & mask;
+                    x = *reinterpret_cast<const uint4 *>(mine + from_page[t] * page_bytes + (o / kKvSub) * kv_sub_bytes(D) + (o % kKvSub) * cw + at / (16 * cw) * (16 * cw) + at % cw);
+                    const float s0 = from_scale[hk][t];
+                    if (s0 != s1) {
+                        const float ratio = __fdiv_rn(s0, s1);
+                        x = make_uint4(kv_recode4<E4M3>(x.x, s0, s1, ratio), kv_recode4<E4M3>(x.y, s0, s1, ratio), kv_recode4<E4M3>(x.z, s0, s1, ratio), kv_recode4<E4M3>(x.w, s0, s1, ratio));
+                    }
+                }
+            } else {
+                uint4 y[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int t = sub * kKvSub + kv_v_token(v, q), o = max(source[t], 0) & mask;
+                    const uint8_t *p = mine + from_page[t] * page_bytes + (o / kKvSub) * kv_sub_bytes(D) + kv_v_offset(o % kKvSub, kv_v_element(v, 0));
+                    y[q] = *reinterpret_cast<const uint4 *>(reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(15));
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int t = sub * kKvSub + kv_v_token(v, q), src = source[t], o = max(src, 0) & mask;
+                    const int shift8 = 8 * (kv_v_offset(o % kKvSub, kv_v_element(v, 0)) & 3);
+                    uint32_t z = src < 0 ? 0u : kv_byte_of_each(y[q], shift8);
+                    const float s0 = from_scale[hk][t];
+                    if (src >= 0 && s0 != s1) z = kv_recode4<E4M3>(z, s0, s1, __fdiv_rn(s0, s1));
+                    kv_byte_to_each(x, z, q);
+                }
+            }
+            *reinterpret_cast<uint4 *>(mine + page * page_bytes + sub * kv_sub_bytes(D) + v * 16) = x;
+        }
+    }
+    if (tid < hk_n) scales[page * page_scales + tid] = top[tid];
 }
 
 }  // namespace wd

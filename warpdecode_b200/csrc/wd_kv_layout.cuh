@@ -100,29 +100,6 @@ __device__ __forceinline__ int kv_code_exact(double n, float s) {
     if (E4M3) return e4m3_of(q);
     return max(-127, min(127, __double2int_rn(q))) + 128;
 }
-// x finite or not (an infinity becomes the largest code, a NaN zero); r = 1 / s. The product x r is off by at most 2^-22 of itself, so that only
-// quotients that near to a middle are worked out in 64 bits.
-template <bool E4M3>
-__device__ __forceinline__ int kv_code(float x, float s, float r) {
-    const float q = x * r;
-    if (E4M3) {
-        const uint32_t b = __float_as_uint(q) & 0x7fffffffu;
-        const uint32_t off = (b & 0xfffffu) - 0x80000u + 16u;
-        if (off <= 32u || (b < 0x3c800000u && b > 0x3a000000u) || b > 0x43e00000u) {     // a middle; between 2^-11 and 2^-6 (codes without leading bit); over 448
-            if (!(fabsf(x) <= 3.402823466e38f)) return x != x ? 0 : x > 0.0f ? 0x7e : 0xfe;
-            return kv_code_exact<true>(static_cast<double>(x), s);
-        }
-        uint16_t c;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(0.0f), "f"(q));
-        return c & 0xff;
-    }
-    const float k = rintf(q);
-    if (fabsf(fabsf(q - k) - 0.5f) < 1e-4f || !(fabsf(q) <= 127.0f)) {
-        if (!(fabsf(x) <= 3.402823466e38f)) return x != x ? 128 : x > 0.0f ? 255 : 1;
-        return kv_code_exact<false>(static_cast<double>(x), s);
-    }
-    return static_cast<int>(k) + 128;
-}
 template <bool E4M3>
 __device__ __forceinline__ float kv_value(int byte) {
     if (E4M3) {
@@ -132,20 +109,81 @@ __device__ __forceinline__ float kv_value(int byte) {
     }
     return static_cast<float>(byte - 128);
 }
-// a code under scale s0 as a code under s1 >= s0 (> 0), ratio = s0 / s1: the product with it is off by 2^-22, as in kv_code
+// Four codes' values, and four quotients' codes. A quotient made as x * (1 / s), or as value * (s0 / s1), is off by at most 2^-22 of itself: `unsure` says that
+// one of them is that near to a middle between codes (or is no number, or beyond the largest code), and then the codes are worked out by kv_code_exact.
+// (int8: 2^23 + byte and 1.5 2^23 + quotient instead of conversions, which have a quarter of the rate.)
 template <bool E4M3>
-__device__ __forceinline__ int kv_recode(int byte, float s0, float s1, float ratio) {
-    const float v = kv_value<E4M3>(byte), q = v * ratio;
+__device__ __forceinline__ void kv_values4(uint32_t w, float *v) {
     if (E4M3) {
-        const uint32_t b = __float_as_uint(q) & 0x7fffffffu, off = (b & 0xfffffu) - 0x80000u + 16u;
-        if (off <= 32u || (b < 0x3c800000u && b > 0x3a000000u)) return kv_code_exact<true>(static_cast<double>(v) * static_cast<double>(s0), s1);
-        uint16_t c;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(0.0f), "f"(q));
-        return c & 0xff;
+        uint32_t lo, hi;
+        asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(w));
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&lo)), b = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+        v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + i)) - 8388736.0f;
     }
-    const float k = rintf(q);
-    if (fabsf(fabsf(q - k) - 0.5f) < 1e-4f) return kv_code_exact<false>(static_cast<double>(v) * static_cast<double>(s0), s1);
-    return static_cast<int>(k) + 128;
+}
+template <bool E4M3>
+__device__ __forceinline__ uint32_t kv_codes4(const float *q, bool &unsure) {
+    if (E4M3) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t b = __float_as_uint(q[i]) & 0x7fffffffu;
+            // a middle; between 2^-11 and 2^-6 (codes without leading bit); over 448, or no number
+            unsure |= (b & 0xfffffu) - 0x7fff0u <= 32u || b - 0x3a000000u < 0x2800000u || b > 0x43e00000u;
+        }
+        uint32_t r;
+        asm("{\n .reg .b16 a, b;\n cvt.rn.satfinite.e4m3x2.f32 a, %2, %1;\n cvt.rn.satfinite.e4m3x2.f32 b, %4, %3;\n mov.b32 %0, {a, b};\n}" : "=r"(r) : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]));
+        return r;
+    }
+    float t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        t[i] = q[i] + 12583040.0f;
+        unsure |= !(fabsf(q[i] - (t[i] - 12583040.0f)) <= 0.4999f);
+    }
+    return __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040), __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
+}
+// the code of any x under s: an infinity becomes the largest code, a NaN zero
+template <bool E4M3>
+__device__ __forceinline__ int kv_code_any(float x, float s) {
+    if (!(fabsf(x) <= 3.402823466e38f)) return x != x ? (E4M3 ? 0 : 128) : E4M3 ? (x > 0.0f ? 0x7e : 0xfe) : (x > 0.0f ? 255 : 1);
+    return s > 0.0f ? kv_code_exact<E4M3>(static_cast<double>(x), s) : E4M3 ? 0 : 128;
+}
+// 16 numbers -> codes under s, r = 1 / s (0 where s is: then every number is 0, or none)
+template <bool E4M3>
+__device__ __forceinline__ uint4 kv_encode16(const float *x, float s, float r) {
+    uint32_t w[4];
+    bool unsure = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float q[4] = {x[4 * i] * r, x[4 * i + 1] * r, x[4 * i + 2] * r, x[4 * i + 3] * r};
+        w[i] = kv_codes4<E4M3>(q, unsure);
+    }
+    if (unsure) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t c = static_cast<uint32_t>(kv_code_any<E4M3>(x[i], s)) << (8 * (i & 3));
+            w[i / 4] = (w[i / 4] & ~(0xffu << (8 * (i & 3)))) | c;
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// four codes under scale s0 as codes under s1 >= s0 (> 0), ratio = s0 / s1
+template <bool E4M3>
+__device__ __forceinline__ uint32_t kv_recode4(uint32_t w, float s0, float s1, float ratio) {
+    float v[4];
+    kv_values4<E4M3>(w, v);
+    const float q[4] = {v[0] * ratio, v[1] * ratio, v[2] * ratio, v[3] * ratio};
+    bool unsure = false;
+    uint32_t r = kv_codes4<E4M3>(q, unsure);
+    if (unsure) {
+        r = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r |= static_cast<uint32_t>(kv_code_exact<E4M3>(static_cast<double>(v[i]) * static_cast<double>(s0), s1)) << (8 * i);
+    }
+    return r;
 }
 // four codes -> their values as f16 pairs (exact: both code sets are subsets of f16)
 template <bool E4M3>
