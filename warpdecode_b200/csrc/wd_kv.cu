@@ -560,7 +560,7 @@ int wd_kv_read(wd_kv_cache *c, int layer, int n, const int *seqs, const int *fir
                 row += counts[i];
             }
             if (p.n == 0) continue;
-            const dim3 grid(static_cast<unsigned>(items), static_cast<unsigned>(layers), 2);
+            const dim3 grid(static_cast<unsigned>(items), static_cast<unsigned>(layers));
             const int rc = by_rows_and_codes(c, rows_of, [&](auto t, auto e4m3) {
                 wd::kv_read_kernel<decltype(t), decltype(e4m3)::value><<<grid, wd::kReadThreads, 0, s>>>(p);
                 WD_TRY_CUDA(cudaGetLastError());

@@ -42,7 +42,7 @@ struct KvAppend {
 };
 
 template <class T, bool E4M3, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 5 : 8) kv_append_kernel(const __grid_constant__ KvAppend P) {
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 16) kv_append_kernel(const __grid_constant__ KvAppend P) {
     extern __shared__ __align__(16) uint8_t app_sm[];           // values: the codes of the sub-blocks that the rows touch
     __shared__ float part[THREADS / 32];
     __shared__ int bad_any;
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 5 : 8) kv_append_ker
 
 // ---- read -----------------------------------------------------------------------------------------------------------------
 // Tokens first .. first + count - 1 of sequences as numbers, rows one after the other: [layer][row][kv head][D]. A block takes a sub-block of
-// 16 tokens of a layer, all heads, keys (blockIdx.z = 0) or values; a warp 512 bytes, which are 16 tokens of 32 elements of a value's head (turned in shared
+// 16 tokens of a layer, all heads, keys and values; a warp 512 bytes, which are 16 tokens of 32 elements of a value's head (turned in shared
 // memory, so that rows are written in pieces of 64 bytes and more).
 struct KvReadEntry {
     int seq, first, count, row0, item0;         // items: sub-blocks that the range touches
@@ -186,55 +186,59 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const __grid_cons
     T *ko = static_cast<T *>(P.out[0]), *vo = static_cast<T *>(P.out[1]);
     const size_t row0 = static_cast<size_t>(e.row0 + t0 - e.first);        // of token 0, which may lie in front of the rows
     const int per_head = D / 32, units = P.s.kv_heads * per_head, cw = kv_cw(D);         // a unit is 512 bytes
-    constexpr int N = 16 / sizeof(T), BATCH = 4, WARPS = kReadThreads / 32;
-    const int kv = blockIdx.z;
-    if ((kv ? vo : ko) == nullptr) return;
-#pragma unroll 1
-    for (int u0 = warp; u0 < units; u0 += BATCH * WARPS) {
-        uint4 x[BATCH];
-        float s[BATCH];
+    constexpr int N = 16 / sizeof(T);
+#pragma unroll 2
+    for (int u = warp; u < 2 * units; u += kReadThreads / 32) {
+        const int kv = u >= units, in = u - kv * units, h = in / per_head, blk = in - h * per_head;
+        if ((kv ? vo : ko) == nullptr) continue;
+        const uint4 x = *reinterpret_cast<const uint4 *>(base + h * head_bytes + kv * half + blk * 512 + lane * 16);
+        const float s = scales[h * 2 + kv];
+        float v[16];
+        kv_values4<E4M3>(x.x, v), kv_values4<E4M3>(x.y, v + 4), kv_values4<E4M3>(x.z, v + 8), kv_values4<E4M3>(x.w, v + 12);
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {           // all on their way before the first is needed
-            const int u = min(u0 + i * WARPS, units - 1), h = u / per_head, blk = u - h * per_head;
-            x[i] = *reinterpret_cast<const uint4 *>(base + h * head_bytes + kv * half + blk * 512 + lane * 16);
-            s[i] = scales[h * 2 + kv];
-        }
+        for (int j = 0; j < 16; ++j) v[j] = __fmul_rn(v[j], s);
+        if (kv == 0) {
+            const int at = blk * 512 + lane * 16, token = at % (16 * cw) / cw, k = at / (16 * cw) * cw + at % cw;
+            if (token >= a && token < b) {
+                T *to = ko + layer * P.out_layer + (row0 + token) * pitch + static_cast<size_t>(h) * D + k;
+                __align__(16) T y[16];
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-            const int u = u0 + i * WARPS, h = u / per_head, blk = u - h * per_head;
-            if (u >= units) break;
-            float v[16];
-            kv_values4<E4M3>(x[i].x, v), kv_values4<E4M3>(x[i].y, v + 4), kv_values4<E4M3>(x[i].z, v + 8), kv_values4<E4M3>(x[i].w, v + 12);
-            if (kv == 0) {
-                const int at = blk * 512 + lane * 16, token = at % (16 * cw) / cw, k = at / (16 * cw) * cw + at % cw;
-                if (token >= a && token < b) {
-                    T *to = ko + layer * P.out_layer + (row0 + token) * pitch + static_cast<size_t>(h) * D + k;
-                    __align__(16) T y[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) y[j] = row_number<T>(__fmul_rn(v[j], s[i]));
-                    if (P.vec) {
-#pragma unroll
-                        for (int j = 0; j < 16; j += N) *reinterpret_cast<uint4 *>(to + j) = *reinterpret_cast<const uint4 *>(y + j);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) to[j] = y[j];
-                    }
-                }
-            } else {
-                __syncwarp();
-#pragma unroll
-                for (int j = 0; j < 16; ++j) turned[warp][kv_v_token(lane, j)][kv_v_element(lane, j)] = row_number<T>(__fmul_rn(v[j], s[i]));
-                __syncwarp();
-                T *to = vo + layer * P.out_layer + row0 * pitch + static_cast<size_t>(h) * D + blk * 32;
+                for (int j = 0; j < 16; j += 2) row_pair(y + j, v[j], v[j + 1]);
                 if (P.vec) {
 #pragma unroll
-                    for (int j = lane; j < kKvSub * 32 / N; j += 32) {
-                        const int token = j / (32 / N), d = j % (32 / N) * N;
-                        if (token >= a && token < b) *reinterpret_cast<uint4 *>(to + token * pitch + d) = *reinterpret_cast<const uint4 *>(&turned[warp][token][d]);
-                    }
+                    for (int j = 0; j < 16; j += N) *reinterpret_cast<uint4 *>(to + j) = *reinterpret_cast<const uint4 *>(y + j);
                 } else {
-                    for (int token = a; token < b; ++token) to[token * pitch + lane] = turned[warp][token][lane];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) to[j] = y[j];
                 }
+            }
+        } else {
+            __syncwarp();
+            if constexpr (sizeof(T) == 2) {
+                // word i: element 8 i + g of tokens 2 t, 2 t + 1 and 8 more; turned, a lane has elements 8 i + 2 t and the next of tokens g and g + 8
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    __align__(4) T pair[4];
+                    row_pair(pair, v[4 * i], v[4 * i + 1]);
+                    row_pair(pair + 2, v[4 * i + 2], v[4 * i + 3]);
+                    const uint32_t *w = reinterpret_cast<const uint32_t *>(pair);
+                    *reinterpret_cast<uint32_t *>(&turned[warp][lane >> 2][8 * i + 2 * (lane & 3)]) = transposed(w[0]);
+                    *reinterpret_cast<uint32_t *>(&turned[warp][(lane >> 2) + 8][8 * i + 2 * (lane & 3)]) = transposed(w[1]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) turned[warp][kv_v_token(lane, j)][kv_v_element(lane, j)] = row_number<T>(v[j]);
+            }
+            __syncwarp();
+            T *to = vo + layer * P.out_layer + row0 * pitch + static_cast<size_t>(h) * D + blk * 32;
+            if (P.vec) {
+#pragma unroll
+                for (int i = lane; i < kKvSub * 32 / N; i += 32) {
+                    const int token = i / (32 / N), d = i % (32 / N) * N;
+                    if (token >= a && token < b) *reinterpret_cast<uint4 *>(to + token * pitch + d) = *reinterpret_cast<const uint4 *>(&turned[warp][token][d]);
+                }
+            } else {
+                for (int token = a; token < b; ++token) to[token * pitch + lane] = turned[warp][token][lane];
             }
         }
     }
@@ -401,45 +405,50 @@ __global__ void __launch_bounds__(kKeepThreads) kv_keep_new_kernel(const __grid_
     __syncthreads();
     const size_t page = static_cast<size_t>(P.to[i]);
     const int used = (min(P.first + P.kept - p0, tokens) + kKvSub - 1) / kKvSub, vecs = used * D, cw = kv_cw(D);
+    // 16 bytes of each head: where they come from and go to is the same for all of them
+    const size_t head_bytes = kv_head_bytes(P.s);
 #pragma unroll 1
-    for (int hk = 0; hk < hk_n; ++hk) {
-        const int kv = hk & 1;
-        uint8_t *mine = pool + (hk >> 1) * kv_head_bytes(P.s) + kv * half;
-        const float s1 = top[hk];
-#pragma unroll 2
-        for (int j = tid; j < vecs; j += kKeepThreads) {
-            const int sub = j / D, v = j - sub * D;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (kv == 0) {
-                const int at = v * 16, t = sub * kKvSub + at % (16 * cw) / cw, src = source[t];
-                if (src >= 0) {
-                    const int o = src & mask;
-                    x = *reinterpret_cast<const uint4 *>(mine + from_page[t] * page_bytes + (o / kKvSub) * kv_sub_bytes(D) + (o % kKvSub) * cw + at / (16 * cw) * (16 * cw) + at % cw);
-                    const float s0 = from_scale[hk][t];
-                    if (s0 != s1) {
-                        const float ratio = __fdiv_rn(s0, s1);
-                        x = make_uint4(kv_recode4<E4M3>(x.x, s0, s1, ratio), kv_recode4<E4M3>(x.y, s0, s1, ratio), kv_recode4<E4M3>(x.z, s0, s1, ratio), kv_recode4<E4M3>(x.w, s0, s1, ratio));
-                    }
+    for (int j = tid; j < vecs; j += kKeepThreads) {
+        const int sub = j / D, v = j - sub * D;
+        uint8_t *to = pool + page * page_bytes + sub * kv_sub_bytes(D) + v * 16;
+        {
+            const int at = v * 16, t = sub * kKvSub + at % (16 * cw) / cw, src = source[t], o = max(src, 0) & mask;
+            const uint8_t *from = pool + from_page[t] * page_bytes + (o / kKvSub) * kv_sub_bytes(D) + (o % kKvSub) * cw + at / (16 * cw) * (16 * cw) + at % cw;
+#pragma unroll 4
+            for (int hk = 0; hk < hk_n; hk += 2) {
+                uint4 x = *reinterpret_cast<const uint4 *>(from + (hk >> 1) * head_bytes);
+                const float s0 = from_scale[hk][t], s1 = top[hk];
+                if (s0 != s1 && s0 > 0.0f) {        // (a scale of 0: codes of 0 under any scale)
+                    const float ratio = __fdiv_rn(s0, s1);
+                    x = make_uint4(kv_recode4<E4M3>(x.x, s0, s1, ratio), kv_recode4<E4M3>(x.y, s0, s1, ratio), kv_recode4<E4M3>(x.z, s0, s1, ratio), kv_recode4<E4M3>(x.w, s0, s1, ratio));
                 }
-            } else {
-                uint4 y[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int t = sub * kKvSub + kv_v_token(v, q), o = max(source[t], 0) & mask;
-                    const uint8_t *p = mine + from_page[t] * page_bytes + (o / kKvSub) * kv_sub_bytes(D) + kv_v_offset(o % kKvSub, kv_v_element(v, 0));
-                    y[q] = *reinterpret_cast<const uint4 *>(reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(15));
-                }
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int t = sub * kKvSub + kv_v_token(v, q), src = source[t], o = max(src, 0) & mask;
-                    const int shift8 = 8 * (kv_v_offset(o % kKvSub, kv_v_element(v, 0)) & 3);
-                    uint32_t z = src < 0 ? 0u : kv_byte_of_each(y[q], shift8);
-                    const float s0 = from_scale[hk][t];
-                    if (src >= 0 && s0 != s1) z = kv_recode4<E4M3>(z, s0, s1, __fdiv_rn(s0, s1));
-                    kv_byte_to_each(x, z, q);
-                }
+                *reinterpret_cast<uint4 *>(to + (hk >> 1) * head_bytes) = x;           // (behind the last token: codes of some other one)
             }
-            *reinterpret_cast<uint4 *>(mine + page * page_bytes + sub * kv_sub_bytes(D) + v * 16) = x;
+        }
+        int t[4], shift8[4];
+        const uint8_t *from[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            t[q] = sub * kKvSub + kv_v_token(v, q);
+            const int o = max(source[t[q]], 0) & mask;
+            const uint8_t *p = pool + from_page[t[q]] * page_bytes + half + (o / kKvSub) * kv_sub_bytes(D) + kv_v_offset(o % kKvSub, kv_v_element(v, 0));
+            from[q] = reinterpret_cast<const uint8_t *>(reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(15));
+            shift8[q] = 8 * static_cast<int>(reinterpret_cast<uintptr_t>(p) & 3);
+        }
+#pragma unroll 2
+        for (int hk = 1; hk < hk_n; hk += 2) {
+            uint4 y[4], x = make_uint4(0, 0, 0, 0);
+            const float s1 = top[hk];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) y[q] = *reinterpret_cast<const uint4 *>(from[q] + (hk >> 1) * head_bytes);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                uint32_t z = kv_byte_of_each(y[q], shift8[q]);
+                const float s0 = from_scale[hk][t[q]];
+                if (s0 != s1 && s0 > 0.0f) z = kv_recode4<E4M3>(z, s0, s1, __fdiv_rn(s0, s1));
+                kv_byte_to_each(x, z, q);
+            }
+            *reinterpret_cast<uint4 *>(to + half + (hk >> 1) * head_bytes) = x;
         }
     }
     if (tid < hk_n) scales[page * page_scales + tid] = top[tid];

@@ -82,6 +82,15 @@ template <>
 __device__ __forceinline__ __half row_number<__half>(float v) { return __float2half_rn(v); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 row_number<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ void row_pair(float *to, float a, float b) { to[0] = a, to[1] = b; }
+__device__ __forceinline__ void row_pair(__half *to, float a, float b) { *reinterpret_cast<__half2 *>(to) = __floats2half2_rn(a, b); }
+__device__ __forceinline__ void row_pair(__nv_bfloat16 *to, float a, float b) { *reinterpret_cast<__nv_bfloat162 *>(to) = __floats2bfloat162_rn(a, b); }
+// 8 x 8 matrix of 16-bit elements, a row's pairs in four lanes, turned
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 
 // ---- codes --------------------------------------------------------------------------------------------------------------
 // The code of the quotient n / s, to the nearest, ties to even, and exactly so: a quotient that F32 rounds onto the middle between two codes is
@@ -125,13 +134,13 @@ __device__ __forceinline__ void kv_values4(uint32_t w, float *v) {
     }
 }
 template <bool E4M3>
-__device__ __forceinline__ uint32_t kv_codes4(const float *q, bool &unsure) {
+__device__ __forceinline__ uint32_t kv_codes4(const float *q, uint32_t &unsure) {
     if (E4M3) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t b = __float_as_uint(q[i]) & 0x7fffffffu;
             // a middle; between 2^-11 and 2^-6 (codes without leading bit); over 448, or no number
-            unsure |= (b & 0xfffffu) - 0x7fff0u <= 32u || b - 0x3a000000u < 0x2800000u || b > 0x43e00000u;
+            unsure |= (b & 0xfffffu) - 0x7fff0u <= 32u || b - 0x3a000000u < 0x2800000u || b > 0x43e00000u ? 1u << i : 0u;
         }
         uint32_t r;
         asm("{\n .reg .b16 a, b;\n cvt.rn.satfinite.e4m3x2.f32 a, %2, %1;\n cvt.rn.satfinite.e4m3x2.f32 b, %4, %3;\n mov.b32 %0, {a, b};\n}" : "=r"(r) : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]));
@@ -141,7 +150,7 @@ __device__ __forceinline__ uint32_t kv_codes4(const float *q, bool &unsure) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         t[i] = q[i] + 12583040.0f;
-        unsure |= !(fabsf(q[i] - (t[i] - 12583040.0f)) <= 0.4999f);
+        unsure |= !(fabsf(q[i] - (t[i] - 12583040.0f)) <= 0.4999f) ? 1u << i : 0u;
     }
     return __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040), __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
 }
@@ -154,16 +163,18 @@ __device__ __forceinline__ int kv_code_any(float x, float s) {
 // 16 numbers -> codes under s, r = 1 / s (0 where s is: then every number is 0, or none)
 template <bool E4M3>
 __device__ __forceinline__ uint4 kv_encode16(const float *x, float s, float r) {
-    uint32_t w[4];
-    bool unsure = false;
+    uint32_t w[4], unsure = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float q[4] = {x[4 * i] * r, x[4 * i + 1] * r, x[4 * i + 2] * r, x[4 * i + 3] * r};
-        w[i] = kv_codes4<E4M3>(q, unsure);
+        uint32_t some = 0;
+        w[i] = kv_codes4<E4M3>(q, some);
+        unsure |= some << (4 * i);
     }
     if (unsure) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
+            if (!(unsure >> i & 1u)) continue;
             const uint32_t c = static_cast<uint32_t>(kv_code_any<E4M3>(x[i], s)) << (8 * (i & 3));
             w[i / 4] = (w[i / 4] & ~(0xffu << (8 * (i & 3)))) | c;
         }
@@ -176,12 +187,12 @@ __device__ __forceinline__ uint32_t kv_recode4(uint32_t w, float s0, float s1, f
     float v[4];
     kv_values4<E4M3>(w, v);
     const float q[4] = {v[0] * ratio, v[1] * ratio, v[2] * ratio, v[3] * ratio};
-    bool unsure = false;
-    uint32_t r = kv_codes4<E4M3>(q, unsure);
+    uint32_t unsure = 0, r = kv_codes4<E4M3>(q, unsure);
     if (unsure) {
-        r = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r |= static_cast<uint32_t>(kv_code_exact<E4M3>(static_cast<double>(v[i]) * static_cast<double>(s0), s1)) << (8 * i);
+        for (int i = 0; i < 4; ++i)
+            if (unsure >> i & 1u)
+                r = (r & ~(0xffu << (8 * i))) | static_cast<uint32_t>(kv_code_exact<E4M3>(static_cast<double>(v[i]) * static_cast<double>(s0), s1)) << (8 * i);
     }
     return r;
 }
