@@ -52,6 +52,19 @@ def test_a_step_takes_all_of_its_pages_or_none():
     kv.begin([], [])
 
 
+def test_lists_are_whole_numbers_of_32_bits():
+    kv = cache()
+    kv.begin(np.array([0, 1], np.int64), np.array([3, 2], np.uint8))
+    for bad in (np.array([2 ** 32]), np.array([0.5]), np.array([[0]])):
+        with pytest.raises(ValueError):
+            kv.begin(bad, bad)
+    with pytest.raises((TypeError, OverflowError)):
+        kv.begin([0], [2 ** 31])
+    with pytest.raises(TypeError):
+        kv.free([0.5])
+    assert kv.length(0) == 3 and kv.length(1) == 2
+
+
 def test_fork_shares_and_copies_when_written():
     kv = cache()
     kv.begin([0], [20])

@@ -604,8 +604,8 @@ def _ints(values):
     """(what holds the whole numbers as int32, their address, how many)"""
     if isinstance(values, np.ndarray):
         a = np.ascontiguousarray(values, np.int32)
-        if a.ndim != 1:
-            raise ValueError("a list of whole numbers is wanted")
+        if values.ndim != 1 or values.dtype.kind not in "iu" or (values.dtype != np.int32 and not np.array_equal(a, values)):
+            raise ValueError("a list of whole numbers of 32 bits is wanted")
         return a, a.ctypes.data, a.size
     a = array("i", values)
     at, n = a.buffer_info()

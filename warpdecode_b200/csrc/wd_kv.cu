@@ -372,8 +372,10 @@ int wd_kv_begin(wd_kv_cache *c, int n, const int *seqs, const int *counts, void 
         if (need > static_cast<long long>(c->free_pages.size()))
             return set_error(WD_E_NOMEM, "key/value cache: " + std::to_string(need) + " pages wanted, " + std::to_string(c->free_pages.size()) + " free");
         if (int rc = check_not_captured(c, s)) return rc;
-        c->changed.reserve(static_cast<size_t>(n) * 5 + need + 8);
+        // (no memory is asked for between the first change and the last)
+        c->changed.reserve(c->changed.size() + static_cast<size_t>(n) * 5 + need + 8);
         c->copies.reserve(n);
+        for (int i = 0; i < n; ++i) c->seqs[seqs[i]].pages.reserve(c->pages_for(c->seqs[seqs[i]].length + counts[i]));
         c->rows = c->max_rows = c->items = 0;
         for (int i = 0; i < n; ++i) {
             Sequence &q = c->seqs[seqs[i]];
@@ -585,6 +587,8 @@ int wd_kv_fork(wd_kv_cache *c, int src, int n, const int *dsts, void *stream) {
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         if (int rc = check_not_captured(c, s)) return rc;
         const Sequence &from = c->seqs[src];
+        c->changed.reserve(c->changed.size() + from.pages.size() * n);
+        for (int i = 0; i < n; ++i) c->seqs[dsts[i]].pages.reserve(from.pages.size());
         for (int i = 0; i < n; ++i) {
             c->seqs[dsts[i]] = from;
             for (size_t j = 0; j < from.pages.size(); ++j) {
@@ -649,6 +653,9 @@ int wd_kv_keep(wd_kv_cache *c, int seq, int first, int n, const int *index, void
         if (!fresh && shared > static_cast<int>(c->free_pages.size()))
             return set_error(WD_E_NOMEM, "key/value cache: " + std::to_string(shared) + " pages wanted, " + std::to_string(c->free_pages.size()) + " free");
         std::vector<int> words(index + still, index + n), to(pages);
+        words.reserve(words.size() + pages);
+        c->changed.reserve(c->changed.size() + pages + 3);
+        c->free_pages.reserve(c->free_pages.size() + q.pages.size());
         for (int &w : words) w -= still;
         for (int i = 0; i < pages; ++i) to[i] = fresh || c->holders[q.pages[page0 + i]] > 1 ? c->take_page() : q.pages[page0 + i];
         OnDevice on(c->host_only() ? 0 : c->cfg.device);
