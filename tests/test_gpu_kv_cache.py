@@ -444,3 +444,83 @@ def test_a_prompt_kernel_in_a_graph_serves_other_steps(chunk, name):
                 assert np.linalg.norm(got[at:at + n] - want) <= 4 * 2.0 ** -8 * np.linalg.norm(want)
             at += n
         assert (got[at:] == 3.0).all()
+
+
+@pytest.mark.parametrize("counts", [[1, 2], [700, 300]])        # the kernel for few rows, and the one for prompts
+def test_a_window_beyond_every_context_is_none(counts):
+    p = Pair(8, 2, 64, 16, 0, "f16")
+    p.step([0, 1], counts)
+    q = p.rand(sum(counts), 8, 64, size=1.5)
+    seen = []
+    for window in (0, 2 ** 31 - 1, 2 ** 31 - 64, 6000):
+        p.check_attend([0, 1], counts, window=window, q=q)
+        seen.append(p.attend([0, 1], counts, window=window, q=q)[0])
+    assert all(np.array_equal(seen[0], x) for x in seen[1:])
+
+
+def test_a_scale_that_no_number_holds():
+    kv = wd.KvCache(1, 8, 2, 64, 8, 2, 100)
+    x = torch.zeros(1, 8, 64, device="cuda")
+    kv.begin([0], [1])
+    with pytest.raises(wd.WdError, match="scale"):
+        kv.attend(0, x.data_ptr(), x.data_ptr(), scale=3.0e38)
+
+
+def test_a_step_without_rows_is_not_captured():
+    """A graph of it would hold nothing, and its replays would leave the steps that follow undone."""
+    kv = wd.KvCache(1, 8, 2, 64, 8, 2, 100)
+    x = torch.zeros(1, 8, 64, device="cuda")
+    s = torch.cuda.Stream()
+    kv.begin([0], [0], s.cuda_stream)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        x.add_(0.0)
+        with pytest.raises(wd.WdError, match="captured"):
+            kv.append(0, x.data_ptr(), x.data_ptr(), stream=s.cuda_stream)
+        with pytest.raises(wd.WdError, match="captured"):
+            kv.attend(0, x.data_ptr(), x.data_ptr(), stream=s.cuda_stream)
+    kv.append(0, x.data_ptr(), x.data_ptr(), stream=s.cuda_stream)
+
+
+@pytest.mark.parametrize("page", [16, 128])
+def test_a_captured_step_of_a_token_serves_one_of_many(page):
+    """More pages, items and rows than the captured launch was made for."""
+    p = Pair(8, 2, 64, page, 0, "f32", layers=1)
+    k, v, q = (torch.zeros(300, h, 64, device="cuda") for h in (2, 2, 8))
+    out = torch.zeros_like(q)
+    s = torch.cuda.Stream()
+    p.kv.begin([0], [1], s.cuda_stream)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        p.kv.append(0, k.data_ptr(), v.data_ptr(), stream=s.cuda_stream)
+        p.kv.attend(0, q.data_ptr(), out.data_ptr(), stream=s.cuda_stream)
+    p.kv.free([0], s.cuda_stream)
+    p.kv.begin([0, 1], [133, 167], s.cuda_stream)
+    rows = [p.rand(300, h, 64) for h in (2, 2, 8)]
+    with torch.cuda.stream(s):
+        for to, x in zip((k, v, q), rows):
+            to.copy_(x)
+        g.replay()
+    s.synchronize()
+    for seq, at, n in ((0, 0, 133), (1, 133, 167)):
+        p.ref[0].append(seq, rows[0][at:at + n].double().numpy(), rows[1][at:at + n].double().numpy())
+        want = p.ref[0].attend(seq, rows[2][at:at + n].double().numpy(), 0.125, 0)
+        values = np.abs(p.ref[0].numbers(seq)[1]).max()
+        assert np.abs(out[at:at + n].double().cpu().numpy() - want).max() <= p.tolerance(rows[2], [seq], layer=0) * values
+    p.check_numbers([0, 1])
+
+
+def test_a_refused_call_leaves_nothing_behind():
+    """An error of the runtime that one call has returned is not found by the next one's look at its launches."""
+    kv = wd.KvCache(1, 8, 2, 64, 8, 2, 100)
+    x = torch.ones(1, 8, 64, device="cuda")
+    for _ in range(2):
+        with pytest.raises(wd.WdError, match="device"):
+            wd.KvCache(1, 8, 2, 64, 8, 2, 100, device=99)
+        kv.begin([0], [1])
+        with pytest.raises(wd.WdError, match="device"):
+            wd.KvCache(1, 8, 2, 64, 8, 2, 100, device=99)
+        kv.append(0, x.data_ptr(), x.data_ptr())
+    kv.attend(0, x.data_ptr(), x.data_ptr())
+    torch.cuda.synchronize()
+    assert torch.equal(x, torch.ones_like(x))

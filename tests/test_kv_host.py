@@ -52,6 +52,21 @@ def test_a_step_takes_all_of_its_pages_or_none():
     kv.begin([], [])
 
 
+@pytest.mark.parametrize("kw", [dict(n_pages=2 ** 31 - 1, n_layers=4096), dict(n_pages=2 ** 31 - 1, n_layers=4096, n_heads=4096, n_kv_heads=4096, head_dim=256, page_tokens=128)])
+def test_pages_that_no_memory_holds(kw):
+    with pytest.raises(wd.WdError, match="4 TiB"):
+        cache(**kw)
+
+
+def test_rows_of_heads_are_counted_in_32_bits():
+    kv = cache(n_heads=4096, n_kv_heads=1, n_pages=2 ** 16, max_context=2 ** 22)
+    with pytest.raises(wd.WdError, match="too many rows"):
+        kv.begin([0], [2 ** 18])
+    assert kv.length(0) == 0 and kv.free_pages() == 2 ** 16
+    kv.begin([0], [2 ** 18 - 1])
+    assert kv.length(0) == 2 ** 18 - 1
+
+
 def test_lists_are_whole_numbers_of_32_bits():
     kv = cache()
     kv.begin(np.array([0, 1], np.int64), np.array([3, 2], np.uint8))
@@ -163,7 +178,7 @@ def test_calls_on_the_device_are_refused_without_one():
 
 
 @pytest.mark.parametrize("bad", [dict(rows=-1), dict(vocab=0), dict(n_top=33), dict(n_top=-1), dict(type=wd.TYPE_Q8_0), dict(logits_ptr=None),
-                                 dict(tokens_ptr=None), dict(n_top=2), dict(logits_ptr=1026), dict(stride=99), dict(logprob_ptr=None)])
+                                 dict(tokens_ptr=None), dict(n_top=2), dict(rows=2 ** 30 + 1), dict(vocab=2 ** 30 + 1), dict(logits_ptr=1026), dict(stride=99), dict(logprob_ptr=None)])
 def test_scores_refuse(bad):
     a = dict(logits_ptr=1024, rows=2, vocab=100, tokens_ptr=1024, logprob_ptr=1024, entropy_ptr=None)
     a.update(bad)

@@ -25,6 +25,7 @@ public:
     explicit OnDevice(int device) {
         if (cudaGetDevice(&before_) != cudaSuccess) before_ = device;
         if (before_ != device) ok_ = cudaSetDevice(device) == cudaSuccess, changed_ = ok_;
+        if (!ok_) cudaGetLastError();       // (the caller says so; a later launch is not to be blamed for it)
     }
     ~OnDevice() {
         if (changed_) cudaSetDevice(before_);

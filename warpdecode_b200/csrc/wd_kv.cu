@@ -113,19 +113,21 @@ int check_rows(const void *p, size_t size, long long *stride, long long least, c
 int check_not_captured(const wd_kv_cache *c, cudaStream_t s) {
     if (c->broken) return set_error(WD_E_STATE, "key/value cache: an earlier call failed on the device");
     if (c->host_only()) return WD_OK;
+    cudaGetLastError();         // what an earlier call failed with was said then
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
     const cudaError_t ce = cudaStreamIsCapturing(s, &st);
     if (ce != cudaSuccess) {
         cudaGetLastError();
         return set_error(WD_E_STATE, std::string("key/value cache: ") + cudaGetErrorString(ce));
     }
-    if (st != cudaStreamCaptureStatusNone) return set_error(WD_E_STATE, "key/value cache: sequences cannot be changed while a graph is captured");
+    if (st != cudaStreamCaptureStatusNone) return set_error(WD_E_STATE, "key/value cache: sequences cannot be changed, nor a step without rows taken, while a graph is captured");
     return WD_OK;
 }
 int check_device(const wd_kv_cache *c) {
     if (!c) return set_error(WD_E_INVALID, "key/value cache: null handle");
     if (c->host_only()) return set_error(WD_E_STATE, "key/value cache: created without a device");
     if (c->broken) return set_error(WD_E_STATE, "key/value cache: an earlier call failed on the device");
+    cudaGetLastError();
     return WD_OK;
 }
 
@@ -142,7 +144,6 @@ template <int N>
 void send_words(wd_kv_cache *c, size_t from, cudaStream_t s) {
     wd::KvWords<N> w;
     w.n = static_cast<int>(std::min<size_t>(N, c->changed.size() - from));
-    w.pad = 0;
     for (int i = 0; i < w.n; ++i) {
         const int at = c->changed[from + i];
         w.w[i] = make_int2(at, c->book[at]);
@@ -301,6 +302,8 @@ int wd_kv_create(const wd_kv_config *cfg, wd_kv_cache **out) {
         k->table_at = wd::kKvHead + c.max_seqs * wd::kKvStepWords;
         const size_t words = k->table_at + static_cast<size_t>(c.max_seqs) * k->shape.max_pages;
         if (words > INT_MAX / 2) return set_error(WD_E_INVALID, "key/value cache: max_seqs times max_context is too large for one table");
+        // (more than any device has, and more than 64 bits count; where there is less, the device says so)
+        if (static_cast<double>(wd::kv_page_bytes(k->shape)) * c.n_pages * c.n_layers > 0x1p42) return set_error(WD_E_NOMEM, "key/value cache: more than 4 TiB of pages do not fit");
         k->book.assign(words, 0);
         k->dirty.assign(words, 0);
         k->seqs.resize(c.max_seqs);
@@ -368,7 +371,7 @@ int wd_kv_begin(wd_kv_cache *c, int n, const int *seqs, const int *counts, void 
                 if (at->second > 1) --at->second, ++need;
             }
         }
-        if (rows > INT_MAX / 2) return set_error(WD_E_INVALID, "key/value cache: too many rows in a step");
+        if (rows * c->cfg.n_heads > INT_MAX / 2) return set_error(WD_E_INVALID, "key/value cache: too many rows in a step");        // (kernels count rows of heads in 32 bits)
         if (need > static_cast<long long>(c->free_pages.size()))
             return set_error(WD_E_NOMEM, "key/value cache: " + std::to_string(need) + " pages wanted, " + std::to_string(c->free_pages.size()) + " free");
         if (int rc = check_not_captured(c, s)) return rc;
@@ -418,7 +421,8 @@ int wd_kv_append(wd_kv_cache *c, int layer, const void *k_dev, const void *v_dev
         int rows_of = 0;
         if (int rc = rows_type(type, &rows_of)) return rc;
         if (c->book[0] == 0) return set_error(WD_E_STATE, "key/value cache: no step has begun");
-        if (c->items == 0) return WD_OK;        // (no rows: nothing is asked of their address)
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        if (c->items == 0) return check_not_captured(c, s);         // (no rows: nothing is asked of their address, and a graph would hold nothing)
         const size_t size = rows_size(rows_of);
         p.stride[0] = k_stride;
         p.stride[1] = v_stride;
@@ -437,7 +441,6 @@ int wd_kv_append(wd_kv_cache *c, int layer, const void *k_dev, const void *v_dev
         for (int i = 0; i < 2; ++i) p.vec[i] = reinterpret_cast<uintptr_t>(p.rows[i]) % 16 == 0 && p.stride[i] * size % 16 == 0;
         const dim3 grid(static_cast<unsigned>(c->items), c->cfg.n_kv_heads, 2);
         const size_t smem = static_cast<size_t>(c->cfg.page_tokens) * c->cfg.head_dim;
-        cudaStream_t s = static_cast<cudaStream_t>(stream);
         // few tokens a page: a warp reads them at once, and more threads would only meet at the barriers
         const bool small = static_cast<long long>(std::min(c->max_rows, c->cfg.page_tokens)) * c->cfg.head_dim <= 2048;
         return by_rows_and_codes(c, rows_of, [&](auto t, auto e4m3) {
@@ -454,12 +457,14 @@ int wd_kv_attend(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, in
     return wd_host::guarded([&]() -> int {
         if (int rc = check_device(c)) return rc;
         if (layer < 0 || layer >= c->cfg.n_layers) return set_error(WD_E_INVALID, "key/value cache: layer out of range");
-        if (!(scale > 0.0f) || !std::isfinite(scale)) return set_error(WD_E_INVALID, "key/value cache: the scale of the scores must be positive and finite");
+        if (!(scale > 0.0f && scale * 1.4426950408889634 <= 3.4028234663852886e38)) return set_error(WD_E_INVALID, "key/value cache: the scale of the scores must be positive and finite");
         if (window < 0) return set_error(WD_E_INVALID, "key/value cache: a window is 0 (none) or at least 1");
         wd::KvAttend p;
         if (int rc = rows_type(type, &p.type)) return rc;
         if (c->book[0] == 0) return set_error(WD_E_STATE, "key/value cache: no step has begun");
-        if (c->rows == 0) return WD_OK;
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        if (c->rows == 0) return check_not_captured(c, s);
+        if (window >= c->cfg.max_context) window = 0;
         p.q_stride = q_stride;
         p.out_stride = out_stride;
         const long long width = static_cast<long long>(c->cfg.n_heads) * c->cfg.head_dim;
@@ -482,7 +487,6 @@ int wd_kv_attend(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, in
         p.vec = reinterpret_cast<uintptr_t>(q_dev) % 16 == 0 && p.q_stride * rows_size(p.type) % 16 == 0;
         p.s = c->shape;
         const long long group = static_cast<long long>(c->max_rows) * (c->cfg.n_heads / c->cfg.n_kv_heads);
-        cudaStream_t s = static_cast<cudaStream_t>(stream);
         const Choice by = choose(c, p.type == wd::kRowsF32, window);
         c->last_kernel = by.prompt ? by.split ? "kv_prompt_kernel, kv_prompt_join_kernel" : "kv_prompt_kernel" : "kv_attend_kernel";
         if (by.prompt) {

@@ -16,6 +16,10 @@
 // the sequences' lengths. A worker has a warp beside it that brings its keys and values into a ring of its own by bulk copies. Nothing is waited for
 // between workers until all of a CTA's are done; then the parts of items that several of them hold are put together, and those that several CTAs
 // hold by the last CTA to arrive, always in the workers' order.
+//
+// Bound: memory for long work. 131,089 tokens of 8 heads of 128: 58 us, 4.6 TB/s of codes (the copy rate's floor is 42); 64 sequences of 90 to 8,000
+// tokens, 8 heads of 64: 46 us, 3.9 TB/s (28): the rest is the way to the first tile and the joining of parts. Short work is a chain of latencies: 131
+// tokens, 4 heads of 64: 10 us, most of them the launch, entry -> table -> page -> tile, and code that an SM fetches for the first time.
 #pragma once
 
 #include <type_traits>
@@ -121,7 +125,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
     __shared__ int4 step[kAttEntries];                          // the first entries of the step
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), worker = warp & 7;
     uint8_t *ring = att_sm + worker * P.slots * A::kSlot;
-    uint8_t *qs = att_sm + P.workers * (P.slots * A::kSlot + 0) + worker * A::q_bytes(N8, SPLIT);
+    uint8_t *qs = att_sm + P.workers * P.slots * A::kSlot + worker * A::q_bytes(N8, SPLIT);
     long long *prefix = reinterpret_cast<long long *>(att_sm + P.workers * (P.slots * A::kSlot + A::q_bytes(N8, SPLIT)));
     const int g_heads = P.s.heads / P.s.kv_heads;
     const int *entries = P.book + kKvHead;
@@ -274,6 +278,10 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
                 }
             }
         }
+        // No copy outlives the block, not where a worker's wait ran out either: the last fill of each slot (of this turn of the ring, or of the one before;
+        // of none where the ring was never full, and that wait is over at once).
+#pragma unroll 1
+        for (int i = 0; i < P.slots; ++i) att_wait(&fu[i], i < slot ? par ^ 1 : par, P.status);
         return;
     }
 

@@ -8,7 +8,7 @@ namespace wd {
 // ---- words of the book, by value: ordered by the stream, and no staging buffer that a later call could overwrite -----------------
 template <int N>
 struct KvWords {
-    int n, pad;
+    int n;
     int2 w[N];          // offset, value
 };
 template <int N>
@@ -29,6 +29,8 @@ __global__ void __launch_bounds__(256) kv_run_kernel(const __grid_constant__ KvR
 // A block takes the step's tokens that lie in one page, one kv head, keys (blockIdx.z = 0) or values. Two passes over its rows: the largest
 // magnitude, from which the scale follows, then the codes (the rows come from the caches the second time). A page that held tokens before keeps its
 // scale unless the new ones need a larger one; then the codes that are there are rounded anew. Values are turned in shared memory.
+// Bound: instruction issue for a prompt (8,191 tokens of 8 heads of 128, written and read back: 52 us, 1.9 TB/s over both), the chain entry -> table ->
+// scale -> rows for one token of each of 64 sequences (with the step's begin and the reading back 18.5 us).
 struct KvAppend {
     uint8_t *pool;              // of the layer
     float *scales;              // of the layer
@@ -148,7 +150,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 16) kv_append_ke
 // ---- read -----------------------------------------------------------------------------------------------------------------
 // Tokens first .. first + count - 1 of sequences as numbers, rows one after the other: [layer][row][kv head][D]. A block takes a sub-block of
 // 16 tokens of a layer, all heads, keys and values; a warp 512 bytes, which are 16 tokens of 32 elements of a value's head (turned in shared
-// memory, so that rows are written in pieces of 64 bytes and more).
+// memory, so that rows are written in pieces of 64 bytes and more). Bound: instruction issue (70 % of the slots).
 struct KvReadEntry {
     int seq, first, count, row0, item0;         // items: sub-blocks that the range touches
 };
@@ -270,7 +272,7 @@ __global__ void __launch_bounds__(256) kv_copy_kernel(const __grid_constant__ Kv
 // ---- keep -----------------------------------------------------------------------------------------------------------------
 // Of a sequence's tokens from `first` on those of `index` stay and move together. A block builds one page, one head, keys or values of one layer:
 // its tokens come from pages behind it (or itself), its scale is the largest of theirs, codes of smaller ones are rounded anew. Where there are no free
-// pages to be had, a block walks over the pages in their order, reading all of a page's tokens before it writes.
+// pages to be had, a block walks over the pages in their order, reading all of a page's tokens before it writes (the order is the bound).
 struct KvKeep {
     uint8_t *pool;
     float *scales;
@@ -370,7 +372,8 @@ __global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(const __grid_cons
 
 // The same into new pages, which need no order: a block builds a page of a layer for up to eight heads, keys and values, and writes what it gathers. (With a
 // block for each head, the chain of index, table and scale in front of the first code was most of its time: 3,301 of 5,900 tokens in 16 layers of 8 heads
-// of 64, 92 us.)
+// of 64, 92 us; so 73, and 20 less since the tokens' places are worked out once for all heads. Bound: instruction issue, 62 % of the slots then; its 110 MB
+// would take 17 us.)
 constexpr int kKeepHeads = 8;
 template <bool E4M3>
 __global__ void __launch_bounds__(kKeepThreads) kv_keep_new_kernel(const __grid_constant__ KvKeep P) {

@@ -46,11 +46,6 @@ __host__ __device__ inline int kv_v_element(int v, int j) { return (v >> 5) * 32
 
 // ---- numbers of the rows ------------------------------------------------------------------------------------------------
 enum { kRowsF32 = 0, kRowsF16 = 1, kRowsBF16 = 2 };
-__device__ __forceinline__ float row_load(const void *p, int type, size_t i) {
-    if (type == kRowsF32) return static_cast<const float *>(p)[i];
-    if (type == kRowsF16) return __half2float(static_cast<const __half *>(p)[i]);
-    return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
-}
 __device__ __forceinline__ void row_store(void *p, int type, size_t i, float v) {
     if (type == kRowsF32) static_cast<float *>(p)[i] = v;
     else if (type == kRowsF16) static_cast<__half *>(p)[i] = __float2half_rn(v);
@@ -108,15 +103,6 @@ __device__ __forceinline__ int kv_code_exact(double n, float s) {
     const double q = n / static_cast<double>(s);
     if (E4M3) return e4m3_of(q);
     return max(-127, min(127, __double2int_rn(q))) + 128;
-}
-template <bool E4M3>
-__device__ __forceinline__ float kv_value(int byte) {
-    if (E4M3) {
-        uint32_t h2;
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(byte)));
-        return __half2float(__ushort_as_half(static_cast<unsigned short>(h2 & 0xffff)));
-    }
-    return static_cast<float>(byte - 128);
 }
 // Four codes' values, and four quotients' codes. A quotient made as x * (1 / s), or as value * (s0 / s1), is off by at most 2^-22 of itself: `unsure` says that
 // one of them is that near to a middle between codes (or is no number, or beyond the largest code), and then the codes are worked out by kv_code_exact.

