@@ -524,3 +524,24 @@ def test_a_refused_call_leaves_nothing_behind():
     kv.attend(0, x.data_ptr(), x.data_ptr())
     torch.cuda.synchronize()
     assert torch.equal(x, torch.ones_like(x))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("counts", [[1, 3], [400, 300]])        # the kernel for few rows, and the one for prompts
+def test_queries_that_are_not_numbers_stay_by_themselves(dtype, counts):
+    p = Pair(8, 2, 64, 16, 0, dtype)
+    p.step([0, 1], [200, 40])
+    p.step([0, 1], counts)
+    q = p.rand(sum(counts), 8, 64)
+    clean = p.attend([0, 1], counts, q=q)[0]
+    values = max(np.abs(p.ref[1].numbers(i)[1]).max() for i in (0, 1))
+    tol = 2 * p.tolerance(q, [0, 1]) * values           # both are that near to the real answer (a row may take another's reason to be scaled anew)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        x = q.clone()
+        x[0, 3, 5] = bad
+        x[-1, 0, 63] = bad
+        got = p.attend([0, 1], counts, q=x)[0]
+        hit = np.zeros(got.shape[:2], bool)
+        hit[0, 3] = hit[-1, 0] = True
+        assert np.abs(got[~hit] - clean[~hit]).max() <= tol
+        assert np.isnan(got[hit]).all()
