@@ -208,6 +208,8 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const __grid_co
     int slot = 0;
 #pragma unroll 1
     for (int row = group; row < P.rows; row += groups) {
+        // Another CTA's shared memory is there from that CTA's start on: all of a cluster say here that they run, and wait for it in front of the exchange.
+        if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
         const Place at = place(row);
         const T *x = at.x;
         const int lead = at.lead, tail0 = lead + at.n_vec * VN, loose = lead + P.vocab - tail0, v0 = at.v0, v1 = at.v1;
@@ -384,6 +386,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) score_kernel(const __grid_co
             score_cut(sh, n_top);
         }
         const ScoreSums nothing = {kScoreFloor, 0.0f, 0.0f, 0.0f};
+        if (ctas > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
         if (tid < 32) {
             const ScoreSums r = over_lanes(tid < kScoreWarps ? sh.warp_sums[tid] : nothing);
             if (tid == 0) {
