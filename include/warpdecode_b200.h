@@ -369,7 +369,7 @@ int wd_head_argmax_q8_0(void *packed_dev, int rows, int cols, const float *x_dev
  *   number = code * scale;   scale = max(largest finite magnitude / (127 or 448), 2^-100), 0 where every number is 0.
  * Tokens that come into a page that holds some already keep its scale s unless they need a larger one, s'; then the codes c that are
  * there become round(c s / s'). All roundings of codes are exact: the nearest code of the real quotient, ties to even. An infinity
- * becomes the largest code, a NaN zero, and either raises bit 32 of the status.
+ * becomes the largest code (0 in a page and head without a finite number other than 0), a NaN zero, and either raises bit 32 of the status.
  *
  * Which sequence holds which pages is kept on the host (calls fail there, with nothing changed) and sent to the device in the
  * stream's order: calls of one cache are made from one host thread at a time and on one stream, or on streams that the caller orders.

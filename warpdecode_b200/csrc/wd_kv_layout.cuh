@@ -140,11 +140,12 @@ __device__ __forceinline__ uint32_t kv_codes4(const float *q, uint32_t &unsure) 
     }
     return __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040), __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
 }
-// the code of any x under s: an infinity becomes the largest code, a NaN zero
+// the code of any x under s: an infinity becomes the largest code, a NaN zero; under a scale of 0 every code is zero (what reads the page counts on it)
 template <bool E4M3>
 __device__ __forceinline__ int kv_code_any(float x, float s) {
-    if (!(fabsf(x) <= 3.402823466e38f)) return x != x ? (E4M3 ? 0 : 128) : E4M3 ? (x > 0.0f ? 0x7e : 0xfe) : (x > 0.0f ? 255 : 1);
-    return s > 0.0f ? kv_code_exact<E4M3>(static_cast<double>(x), s) : E4M3 ? 0 : 128;
+    if (s == 0.0f || x != x) return E4M3 ? 0 : 128;
+    if (fabsf(x) > 3.402823466e38f) return E4M3 ? (x > 0.0f ? 0x7e : 0xfe) : (x > 0.0f ? 255 : 1);
+    return kv_code_exact<E4M3>(static_cast<double>(x), s);
 }
 // 16 numbers -> codes under s, r = 1 / s (0 where s is: then every number is 0, or none)
 template <bool E4M3>
