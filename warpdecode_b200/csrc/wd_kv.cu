@@ -45,6 +45,7 @@ struct wd_kv_cache {
     unsigned *d_arrived = nullptr, *d_status = nullptr;
     size_t pool_layer = 0, scales_layer = 0;
     const char *last_kernel = "";           // of wd_kv_attend
+    bool graphs = false;                    // an append or an attend has been captured: replays look for the step in the device's book
     bool broken = false;                    // a launch failed half-way: mirror and device may differ
 
     bool host_only() const { return cfg.device < 0; }
@@ -137,6 +138,20 @@ int later(wd_kv_cache *c) {
         for (int at : c->changed) c->dirty[at] = 0;
         c->changed.clear();
     }
+    return WD_OK;
+}
+int flush(wd_kv_cache *c, cudaStream_t s);
+// The end of a step waits likewise, unless replays of captured calls may come before: they are not to find it any more.
+int step_ended(wd_kv_cache *c, cudaStream_t s) {
+    if (!c->graphs) return later(c);
+    OnDevice on(c->cfg.device);
+    return flush(c, s);
+}
+// Whether the call becomes part of a graph; then the cache's steps end on the device too.
+int note_capture(wd_kv_cache *c, cudaStream_t s) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    WD_TRY_CUDA(cudaStreamIsCapturing(s, &st));
+    if (st != cudaStreamCaptureStatusNone) c->graphs = true;
     return WD_OK;
 }
 
@@ -430,6 +445,7 @@ int wd_kv_append(wd_kv_cache *c, int layer, const void *k_dev, const void *v_dev
         if (int rc = check_rows(k_dev, size, &p.stride[0], width, "k")) return rc;
         if (int rc = check_rows(v_dev, size, &p.stride[1], width, "v")) return rc;
         OnDevice on(c->cfg.device);
+        if (int rc = note_capture(c, s)) return rc;
         p.pool = c->d_pool + layer * c->pool_layer;
         p.scales = c->d_scales + layer * c->scales_layer;
         p.book = c->d_book;
@@ -471,6 +487,7 @@ int wd_kv_attend(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, in
         if (int rc = check_rows(q_dev, rows_size(p.type), &p.q_stride, width, "q")) return rc;
         if (int rc = check_rows(out_dev, rows_size(p.type), &p.out_stride, width, "out")) return rc;
         OnDevice on(c->cfg.device);
+        if (int rc = note_capture(c, s)) return rc;
         p.pool = c->d_pool + layer * c->pool_layer;
         p.scales = c->d_scales + layer * c->scales_layer;
         p.book = c->d_book;
@@ -611,9 +628,10 @@ int wd_kv_truncate(wd_kv_cache *c, int seq, int length, void *stream) {
         if (length < 0 || length > c->seqs[seq].length) return set_error(WD_E_INVALID, "key/value cache: a sequence can be cut to 0 up to its length");
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         if (int rc = check_not_captured(c, s)) return rc;
+        c->changed.reserve(c->changed.size() + 3);
         c->cut(c->seqs[seq], length);
         c->end_step();
-        return later(c);
+        return step_ended(c, s);
     });
 }
 
@@ -624,9 +642,10 @@ int wd_kv_free(wd_kv_cache *c, int n, const int *seqs, void *stream) {
             if (int rc = check_seq(c, seqs[i])) return rc;
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         if (int rc = check_not_captured(c, s)) return rc;
+        c->changed.reserve(c->changed.size() + 3);
         for (int i = 0; i < n; ++i) c->cut(c->seqs[seqs[i]], 0);
         c->end_step();
-        return later(c);
+        return step_ended(c, s);
     });
 }
 
@@ -645,9 +664,10 @@ int wd_kv_keep(wd_kv_cache *c, int seq, int first, int n, const int *index, void
         while (still < n && index[still] == still) ++still;
         const int from = first + still, kept = n - still, end = first + n;
         if (kept == 0) {
+            c->changed.reserve(c->changed.size() + 3);
             c->cut(q, end);
             c->end_step();
-            return later(c);
+            return step_ended(c, s);
         }
         const int page0 = from / c->page_tokens(), pages = c->pages_for(end) - page0;
         // Into new pages, all at once, where there are enough of them; else in place, page by page, but never into a page that others hold.
