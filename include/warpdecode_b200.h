@@ -406,7 +406,8 @@ int wd_kv_begin(wd_kv_cache *c, int n, const int *seqs, const int *counts, void 
 /* Keys and values of the step's rows into a layer. The same rows again leave the cache as it is. */
 int wd_kv_append(wd_kv_cache *c, int layer, const void *k_dev, const void *v_dev, int type, int64_t k_stride, int64_t v_stride, void *stream);
 /* out = softmax(scale q k) v of the step's rows, each against the tokens up to its own (which must have been appended), or the last
- * `window` of them (0 = all). Row i of a sequence's n rows is the token n - 1 - i before its last. out may be q. */
+ * `window` of them (0 = all). Row i of a sequence's n rows is the token n - 1 - i before its last. out may be q, with the same stride; they
+ * do not overlap otherwise. */
 int wd_kv_attend(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, int type, float scale, int window, int64_t q_stride,
                  int64_t out_stride, void *stream);
 /* Tokens firsts[i] .. firsts[i] + counts[i] - 1 of the sequences as numbers, one behind the other: [rows][n_kv_heads][head_dim], for

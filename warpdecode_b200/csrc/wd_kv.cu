@@ -486,6 +486,7 @@ int wd_kv_attend(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, in
         const long long width = static_cast<long long>(c->cfg.n_heads) * c->cfg.head_dim;
         if (int rc = check_rows(q_dev, rows_size(p.type), &p.q_stride, width, "q")) return rc;
         if (int rc = check_rows(out_dev, rows_size(p.type), &p.out_stride, width, "out")) return rc;
+        if (q_dev == out_dev && p.q_stride != p.out_stride) return set_error(WD_E_INVALID, "key/value cache: out over q needs q's stride");
         OnDevice on(c->cfg.device);
         if (int rc = note_capture(c, s)) return rc;
         p.pool = c->d_pool + layer * c->pool_layer;
