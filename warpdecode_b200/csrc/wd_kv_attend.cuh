@@ -64,6 +64,11 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {        // on sums of 0
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -446,7 +451,6 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
                         }
             }
             uint32_t ph[N8][4][2], pl[SPLIT ? N8 : 1][4][2];
-            bool grown = false;
             float f[N8][2];
 #pragma unroll
             for (int n = 0; n < N8; ++n) {
@@ -464,7 +468,6 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                     const float now = fmaxf(m[n][i], top);
                     f[n][i] = ex2(m[n][i] - now);
-                    grown |= now != m[n][i];
                     m[n][i] = now;
                     float sum = 0.0f;
 #pragma unroll
@@ -485,35 +488,40 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
                         if constexpr (SPLIT) pl[n][b][h] = transposed(half_rest(x[n][b][2 * h], x[n][b][2 * h + 1], hi));
                     }
             }
-            if (__any_sync(0xffffffffu, grown)) {
-#pragma unroll
-                for (int n = 0; n < N8; ++n)
-#pragma unroll
-                    for (int i = 0; i < D / 16; ++i) o[n][i][0] *= f[n][0], o[n][i][1] *= f[n][1], o[n][i][2] *= f[n][0], o[n][i][3] *= f[n][1];
-            }
             att_wait(&fu[slot], par, P.status);
             const uint4 *vp = reinterpret_cast<const uint4 *>(ring + slot * A::kSlot) + lane;
+            // A tile's sums are made apart and added in F32: a tensor core cuts its sums off, low by 6e-9 of themselves for each token that they hold.
+            constexpr int KB = D / 32 < 2 ? 1 : D / 32 % 2 ? 3 : 2;          // 32 elements each; at once, for products that do not wait for one another
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
+            for (int k0 = 0; k0 < D / 32; k0 += KB) {
+                float y[KB][N8][2][4];
 #pragma unroll
-                for (int k = 0; k < D / 32; ++k) {
-                    const uint4 v = vp[b * D + k * 32];
-                    uint32_t a0, a1, a2, a3;
-                    kv_halves<E4M3>(v.x, a0, a2);
-                    kv_halves<E4M3>(v.y, a1, a3);
+                for (int b = 0; b < 4; ++b)
 #pragma unroll
-                    for (int n = 0; n < N8; ++n) {
-                        mma_f16(o[n][2 * k], a0, a1, a2, a3, ph[n][b][0], ph[n][b][1]);
-                        if constexpr (SPLIT) mma_f16(o[n][2 * k], a0, a1, a2, a3, pl[n][b][0], pl[n][b][1]);
+                    for (int k = 0; k < KB; ++k) {
+                        const uint4 v = vp[b * D + (k0 + k) * 32];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            uint32_t a0, a1, a2, a3;
+                            kv_halves<E4M3>(j ? v.z : v.x, a0, a2);
+                            kv_halves<E4M3>(j ? v.w : v.y, a1, a3);
+#pragma unroll
+                            for (int n = 0; n < N8; ++n) {
+                                if (b == 0) mma_f16_first(y[k][n][j], a0, a1, a2, a3, ph[n][b][0], ph[n][b][1]);
+                                else mma_f16(y[k][n][j], a0, a1, a2, a3, ph[n][b][0], ph[n][b][1]);
+                                if constexpr (SPLIT) mma_f16(y[k][n][j], a0, a1, a2, a3, pl[n][b][0], pl[n][b][1]);
+                            }
+                        }
                     }
-                    kv_halves<E4M3>(v.z, a0, a2);
-                    kv_halves<E4M3>(v.w, a1, a3);
 #pragma unroll
-                    for (int n = 0; n < N8; ++n) {
-                        mma_f16(o[n][2 * k + 1], a0, a1, a2, a3, ph[n][b][0], ph[n][b][1]);
-                        if constexpr (SPLIT) mma_f16(o[n][2 * k + 1], a0, a1, a2, a3, pl[n][b][0], pl[n][b][1]);
-                    }
-                }
+                for (int k = 0; k < KB; ++k)
+#pragma unroll
+                    for (int n = 0; n < N8; ++n)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) o[n][2 * (k0 + k) + j][c] = fmaf(o[n][2 * (k0 + k) + j][c], f[n][c & 1], y[k][n][j][c]);
+            }
             pass_on();
         }
         // ---- the item's end, or this worker's part of it

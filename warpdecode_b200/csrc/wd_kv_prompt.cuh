@@ -39,7 +39,7 @@ struct KvPrompt {
     void *out;
     long long q_stride, out_stride;
     unsigned *status;
-    float *part;                // [CTAs][rows of an item][D + 4]: sums, then maximum and denominator
+    float *part;                // [CTAs]: sums [row tile][D / 4][128 rows][4], then [rows] of maximum and denominator; until an item's end the sums of its chains
     float scale_log2;
     int type, window, vec, split, ctas;         // vec: rows of q and out lie on boundaries of 16 bytes; split: items may be cut into runs
     KvShape s;
@@ -57,6 +57,9 @@ struct PromptAttPlan {
     // a tile's weights still are.)
     static constexpr int kColO = 128 * kTiles, kColP = kColO + kTiles * D, kWidthP = kKt / 2 * (SPLIT ? 2 : 1);
     static constexpr bool kApart = kColP + kTiles * kWidthP <= 512 && kStages >= kTiles;         // (the second tile's first scores come behind the first's second)
+    // Tiles after which sums are brought to memory and begun anew: a tensor core cuts its sums off, so that those of values of one sign come out low, by 3.3e-9
+    // of themselves for each token and term (F32 rows, 100,000 tokens in one sum: 6.6e-4). So F32 rows add 2,048 tokens at a time, others 8,192.
+    static constexpr int kChain = (SPLIT ? 2048 : 8192) / kKt;
     static constexpr uint32_t kIdescS = 1u << 4 | (kKt >> 3) << 17 | (128 >> 4) << 24, kIdescO = 1u << 4 | (D >> 3) << 17 | (128 >> 4) << 24;
     static_assert(kColO + kTiles * D <= 512 && kSmem <= 226 * 1024, "plan of the memories");
 };
@@ -65,6 +68,16 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
+}
+
+// Where a CTA's (or a run's) part has the four sums from column c on of a row, and its maximum and denominator: a warp's rows lie side by side.
+template <int D, int ROWS>
+__device__ __forceinline__ float *prompt_part(float *parts, int at, int row, int c) {
+    return parts + static_cast<size_t>(at) * ROWS * (D + 4) + ((row >> 7) * (D / 4) + c / 4) * 512 + (row & 127) * 4;
+}
+template <int D, int ROWS>
+__device__ __forceinline__ float2 *prompt_part_end(float *parts, int at, int row) {
+    return reinterpret_cast<float2 *>(parts + static_cast<size_t>(at) * ROWS * (D + 4) + ROWS * D + row * 2);
 }
 
 struct PromptItem {
@@ -229,7 +242,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
             auto weights = [&](int x, int j) {
                 att_wait(&p_full[x], n_p[x] & 1, P.status);
                 tc_fence_after();
-                weigh(x, j > 0);
+                weigh(x, j % A::kChain != 0);
             };
             for (int turn = 0; item_of(turn, it); ++turn, ++items) {
                 const int n = it.hi - it.lo;
@@ -448,118 +461,173 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
             if (it.lo < it.hi) mbar_arrive(&q_full[x]);
             float m = kAttFloor, l = 0.0f;
 #pragma unroll 1
-            for (int tile = it.lo; tile < it.hi; ++tile, ++n) {
-                att_wait(&s_full[x], n_s++ & 1, P.status);
-                tc_fence_after();
-                const int first = tile * KT;
-                const bool edge = first + KT - 1 > pos_lo || (P.window && first <= pos_hi - P.window);
-                uint32_t v[KT / 32][32];
-#pragma unroll
-                for (int c = 0; c < KT / 32; ++c) tc_ld(sc + c * 32, v[c]);
-#pragma unroll
-                for (int c = 0; c < KT / 32; ++c) tc_wait_ld(v[c]);
-                if constexpr (A::kApart) {
-                    tc_fence_before();
-                    mbar_arrive(&s_free[x]);
-                }
-                // column 16 s + p of the scores is token 2 (p / 4) + (p & 1) + 8 ((p & 3) / 2) of sub-block s
-                if (edge) {
-#pragma unroll
-                    for (int c = 0; c < KT / 32; ++c)
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int p = i & 15, token = first + c * 32 + (i & 16) + (p >> 2) * 2 + (p & 1) + ((p & 2) << 2);
-                            if (token > pos || (P.window && token <= pos - P.window)) v[c][i] = 0xff800000u;
-                        }
-                }
-                float most = kAttFloor;
-#pragma unroll
-                for (int b = 0; b < SUBS; ++b) {
-                    const float4 s4 = scales[n & 3][b];
-                    auto at = [&](int i) { return __uint_as_float(v[b / 2][b % 2 * 16 + i]); };
-                    float t = max3(at(0), at(1), at(2));
-#pragma unroll
-                    for (int i = 3; i < 15; i += 2) t = max3(t, at(i), at(i + 1));
-                    t = fmaxf(t, at(15));
-                    most = fmaxf(most, fmaf(t, fmaxf(mul * s4.x, 1e-37f), s4.y));
-                }
-                if constexpr (A::kApart) {          // the sums, and the place of the weights, are free
-                    if (n_o > 0) att_wait(&o_done[x], (n_o - 1) & 1, P.status);
-                    tc_fence_after();
-                }
-                if (tile == it.lo) {
-                    m = most;
-                } else if (__any_sync(0xffffffffu, most > m + 8.0f)) {
-                    const float now = fmaxf(m, most), f = ex2(m - now);
-                    m = now;
-                    l *= f;
+            for (int tile = it.lo; tile < it.hi;) {
+                const int chain_end = min(tile + A::kChain, it.hi);
 #pragma unroll 1
-                    for (int c = 0; c < D / 16; ++c) {
-                        uint32_t u[16];
-                        tc_ld(oc + c * 16, u);
-                        tc_wait_ld(u);
+                for (; tile < chain_end; ++tile, ++n) {
+                    att_wait(&s_full[x], n_s++ & 1, P.status);
+                    tc_fence_after();
+                    const int first = tile * KT;
+                    const bool edge = first + KT - 1 > pos_lo || (P.window && first <= pos_hi - P.window);
+                    uint32_t v[KT / 32][32];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * f);
-                        tc_st(oc + c * 16, u);
+                    for (int c = 0; c < KT / 32; ++c) tc_ld(sc + c * 32, v[c]);
+#pragma unroll
+                    for (int c = 0; c < KT / 32; ++c) tc_wait_ld(v[c]);
+                    if constexpr (A::kApart) {
+                        tc_fence_before();
+                        mbar_arrive(&s_free[x]);
                     }
-                }
-                // exponents of all columns, then the exponentials (scales read between the stores of weights would wait for them)
+                    // column 16 s + p of the scores is token 2 (p / 4) + (p & 1) + 8 ((p & 3) / 2) of sub-block s
+                    if (edge) {
 #pragma unroll
-                for (int b = 0; b < SUBS; ++b) {
-                    const float4 s4 = scales[n & 3][b];
-                    const float mk = fmaxf(mul * s4.x, 1e-37f), off = s4.y - m;
-                    const f32x2 mk2 = pack2(mk, mk), off2 = pack2(off, off);
+                        for (int c = 0; c < KT / 32; ++c)
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        uint32_t *u = &v[b / 2][b % 2 * 16 + i];
+                            for (int i = 0; i < 32; ++i) {
+                                const int p = i & 15, token = first + c * 32 + (i & 16) + (p >> 2) * 2 + (p & 1) + ((p & 2) << 2);
+                                if (token > pos || (P.window && token <= pos - P.window)) v[c][i] = 0xff800000u;
+                            }
+                    }
+                    float most = kAttFloor;
+#pragma unroll
+                    for (int b = 0; b < SUBS; ++b) {
+                        const float4 s4 = scales[n & 3][b];
+                        auto at = [&](int i) { return __uint_as_float(v[b / 2][b % 2 * 16 + i]); };
+                        float t = max3(at(0), at(1), at(2));
+#pragma unroll
+                        for (int i = 3; i < 15; i += 2) t = max3(t, at(i), at(i + 1));
+                        t = fmaxf(t, at(15));
+                        most = fmaxf(most, fmaf(t, fmaxf(mul * s4.x, 1e-37f), s4.y));
+                    }
+                    if constexpr (A::kApart) {          // the sums, and the place of the weights, are free
+                        if (n_o > 0) att_wait(&o_done[x], (n_o - 1) & 1, P.status);
+                        tc_fence_after();
+                    }
+                    if (tile == it.lo) {
+                        m = most;
+                    } else if (__any_sync(0xffffffffu, most > m + 8.0f)) {
+                        const float now = fmaxf(m, most), f = ex2(m - now);
+                        m = now;
+                        l *= f;
+#pragma unroll 1
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t u[16];
+                            tc_ld(oc + c * 16, u);
+                            tc_wait_ld(u);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * f);
+                            tc_st(oc + c * 16, u);
+                        }
+                    }
+                    // exponents of all columns, then the exponentials (scales read between the stores of weights would wait for them)
+#pragma unroll
+                    for (int b = 0; b < SUBS; ++b) {
+                        const float4 s4 = scales[n & 3][b];
+                        const float mk = fmaxf(mul * s4.x, 1e-37f), off = s4.y - m;
+                        const f32x2 mk2 = pack2(mk, mk), off2 = pack2(off, off);
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            uint32_t *u = &v[b / 2][b % 2 * 16 + i];
+                            float a, c;
+                            unpack2(fma2(pack2(__uint_as_float(u[0]), __uint_as_float(u[1])), mk2, off2), a, c);
+                            u[0] = __float_as_uint(a), u[1] = __float_as_uint(c);
+                        }
+                    }
+                    uint32_t hi[KT / 32][16], lo[SPLIT ? KT / 32 : 1][16];
+#pragma unroll
+                    for (int b = 0; b < SUBS; ++b) {
+                        f32x2 s0 = pack2(0.0f, 0.0f), s1 = s0;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float a = ex2(__uint_as_float(v[b / 2][b % 2 * 16 + 2 * i])), c = ex2(__uint_as_float(v[b / 2][b % 2 * 16 + 2 * i + 1]));
+                            if (i & 1) s1 = add2(s1, pack2(a, c));
+                            else s0 = add2(s0, pack2(a, c));
+                            hi[b / 2][b % 2 * 8 + i] = half_pair(a, c);
+                            if constexpr (SPLIT) lo[b / 2][b % 2 * 8 + i] = half_rest(a, c, hi[b / 2][b % 2 * 8 + i]);
+                        }
                         float a, c;
-                        unpack2(fma2(pack2(__uint_as_float(u[0]), __uint_as_float(u[1])), mk2, off2), a, c);
-                        u[0] = __float_as_uint(a), u[1] = __float_as_uint(c);
+                        unpack2(add2(s0, s1), a, c);
+                        l = fmaf(a + c, scales[n & 3][b].z, l);
                     }
-                }
-                uint32_t hi[KT / 32][16], lo[SPLIT ? KT / 32 : 1][16];
 #pragma unroll
-                for (int b = 0; b < SUBS; ++b) {
-                    f32x2 s0 = pack2(0.0f, 0.0f), s1 = s0;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float a = ex2(__uint_as_float(v[b / 2][b % 2 * 16 + 2 * i])), c = ex2(__uint_as_float(v[b / 2][b % 2 * 16 + 2 * i + 1]));
-                        if (i & 1) s1 = add2(s1, pack2(a, c));
-                        else s0 = add2(s0, pack2(a, c));
-                        hi[b / 2][b % 2 * 8 + i] = half_pair(a, c);
-                        if constexpr (SPLIT) lo[b / 2][b % 2 * 8 + i] = half_rest(a, c, hi[b / 2][b % 2 * 8 + i]);
+                    for (int c = 0; c < KT / 32; ++c) {
+                        tc_st(pc + c * kPartP, hi[c]);
+                        if constexpr (SPLIT) tc_st(pc + c * kPartP + 16, lo[c]);
                     }
-                    float a, c;
-                    unpack2(add2(s0, s1), a, c);
-                    l = fmaf(a + c, scales[n & 3][b].z, l);
+                    tc_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(&p_full[x]);
+                    ++n_o;
                 }
+                // a chain's end: its sums are added to those of the chains in front of it
+                if (tile < it.hi) {
+                    int of = x * 128 + r;
+                    asm volatile("" : "+r"(of));          // (addresses are made here, not held through the tiles)
+                    const int place = runs > 1 ? it.at : blockIdx.x;
+                    const bool more = tile - it.lo > A::kChain;
+                    float *held_m = &prompt_part_end<D, A::kRows>(P.part, place, of)->x;
+                    const float f = more ? ex2(*held_m - m) : 0.0f;         // (m does not go down)
+                    *held_m = m;
+                    float4 h[8];
+                    auto ask = [&](int c) {
 #pragma unroll
-                for (int c = 0; c < KT / 32; ++c) {
-                    tc_st(pc + c * kPartP, hi[c]);
-                    if constexpr (SPLIT) tc_st(pc + c * kPartP + 16, lo[c]);
+                        for (int i = 0; i < 8; ++i) h[i] = more ? *reinterpret_cast<const float4 *>(prompt_part<D, A::kRows>(P.part, place, of, c + 4 * i)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    };
+                    ask(0);
+                    att_wait(&o_done[x], (n_o - 1) & 1, P.status);
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t u[32];
+                        tc_ld(oc + c, u);
+                        tc_wait_ld(u);
+                        float4 y[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            y[i] = make_float4(fmaf(h[i].x, f, __uint_as_float(u[4 * i])), fmaf(h[i].y, f, __uint_as_float(u[4 * i + 1])),
+                                               fmaf(h[i].z, f, __uint_as_float(u[4 * i + 2])), fmaf(h[i].w, f, __uint_as_float(u[4 * i + 3])));
+                        if (c + 32 < D) ask(c + 32);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) *reinterpret_cast<float4 *>(prompt_part<D, A::kRows>(P.part, place, of, c + 4 * i)) = y[i];
+                    }
+                    tc_fence_before();
                 }
-                tc_wait_st();
-                tc_fence_before();
-                mbar_arrive(&p_full[x]);
-                ++n_o;
             }
             if (it.lo < it.hi) att_wait(&o_done[x], (n_o - 1) & 1, P.status);
             tc_fence_after();
+            const bool held = it.hi - it.lo > A::kChain;
+            int of = x * 128 + r;
+            asm volatile("" : "+r"(of));
+            const int place = runs > 1 ? it.at : blockIdx.x;
+            const float f_held = held ? ex2(prompt_part_end<D, A::kRows>(P.part, place, of)->x - m) : 0.0f;
+            // 16 columns of the sums
+            auto sums = [&](int c, uint32_t (&v)[16]) {
+                tc_ld(oc + c * 16, v);
+                tc_wait_ld(v);
+                if (held) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 h = *reinterpret_cast<const float4 *>(prompt_part<D, A::kRows>(P.part, place, of, c * 16 + i));
+                        v[i] = __float_as_uint(fmaf(h.x, f_held, __uint_as_float(v[i])));
+                        v[i + 1] = __float_as_uint(fmaf(h.y, f_held, __uint_as_float(v[i + 1])));
+                        v[i + 2] = __float_as_uint(fmaf(h.z, f_held, __uint_as_float(v[i + 2])));
+                        v[i + 3] = __float_as_uint(fmaf(h.w, f_held, __uint_as_float(v[i + 3])));
+                    }
+                }
+            };
             if (runs > 1) {         // for the kernel behind
-                float *part = P.part + (static_cast<size_t>(it.at) * A::kRows + x * 128 + r) * (D + 4);
 #pragma unroll 1
                 for (int c = 0; c < D / 16; ++c) {
                     uint32_t v[16];
-                    tc_ld(oc + c * 16, v);
-                    tc_wait_ld(v);
+                    sums(c, v);
                     if (is && it.lo < it.hi) {
 #pragma unroll
                         for (int i = 0; i < 16; i += 4)
-                            *reinterpret_cast<uint4 *>(part + c * 16 + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                            *reinterpret_cast<uint4 *>(prompt_part<D, A::kRows>(P.part, place, of, c * 16 + i)) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                     }
                     __syncwarp();
                 }
-                if (is) *reinterpret_cast<float2 *>(part + D) = make_float2(m, l);         // (of an empty run nothing else is read)
+                if (is) *prompt_part_end<D, A::kRows>(P.part, place, of) = make_float2(m, l);         // (of an empty run nothing else is read)
                 continue;
             }
             const float inv = 1.0f / l;
@@ -567,8 +635,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
                 uint32_t v[16];
-                tc_ld(oc + c * 16, v);
-                tc_wait_ld(v);
+                sums(c, v);
                 if (is) {
                     float y[16];
 #pragma unroll
@@ -603,45 +670,43 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm) : "memory");
 }
 
-// The runs' sums of each row of the items: a warp has a row.
+// The runs' sums of each row of the items: a thread has four elements of a row, a warp 32 rows.
 template <int D>
 __global__ void __launch_bounds__(256) kv_prompt_join_kernel(const __grid_constant__ KvPrompt P) {
-    constexpr int ROWS = D <= 128 ? 256 : 128;
+    constexpr int ROWS = D <= 128 ? 256 : 128, UNITS = ROWS * (D / 4);
     __shared__ int prefix[kAttMaxSeqs + 2];
-    const int tid = threadIdx.x, lane = tid & 31, n_seq = P.book[0], g_heads = P.s.heads / P.s.kv_heads;
-    if (tid < 32) prompt_prefix(P, ROWS, prefix, lane);
+    const int tid = threadIdx.x, n_seq = P.book[0], g_heads = P.s.heads / P.s.kv_heads;
+    if (tid < 32) prompt_prefix(P, ROWS, prefix, tid);
     __syncthreads();
     const long long n_items = static_cast<long long>(prefix[n_seq]) * P.s.kv_heads;
     const int runs = P.split ? prompt_runs(P.ctas, n_items, prefix[n_seq + 1]) : 1;
     if (runs == 1) return;
-    for (long long u = static_cast<long long>(blockIdx.x) * 8 + (tid >> 5); u < n_items * ROWS; u += static_cast<long long>(gridDim.x) * 8) {
-        const long long n = u / ROWS;
-        const int r = static_cast<int>(u % ROWS);
+    for (long long u = static_cast<long long>(blockIdx.x) * 256 + tid; u < n_items * UNITS; u += static_cast<long long>(gridDim.x) * 256) {
+        const long long n = u / UNITS;
+        const int in = static_cast<int>(u % UNITS), r = in % ROWS, c = in / ROWS * 4;
         const PromptItem it = prompt_item(P, prefix, n_seq, n, ROWS);
         const int row = it.item_row + r;
         if (row >= it.rows) continue;
-        const float *part = P.part + (static_cast<size_t>(n) * runs * ROWS + r) * (D + 4);
-        // the maximum, the denominator and each run's factor: a lane has every 32nd run's
-        float top = kAttFloor;
-        for (int k = lane; k < runs; k += 32) top = fmaxf(top, part[static_cast<size_t>(k) * ROWS * (D + 4) + D]);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        float sum[D / 32], den = 0.0f;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) sum[i] = 0.0f;
+        const int at = static_cast<int>(n) * runs;
+        float top = kAttFloor, den = 0.0f;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int k = 0; k < runs; ++k) top = fmaxf(top, prompt_part_end<D, ROWS>(P.part, at + k, r)->x);
 #pragma unroll 4
         for (int k = 0; k < runs; ++k) {
-            const float *p = part + static_cast<size_t>(k) * ROWS * (D + 4);
-            const float2 z = *reinterpret_cast<const float2 *>(p + D);
-            const float f = z.y > 0.0f ? ex2(z.x - top) : 0.0f;
+            const float2 z = *prompt_part_end<D, ROWS>(P.part, at + k, r);
+            const float4 y = *reinterpret_cast<const float4 *>(prompt_part<D, ROWS>(P.part, at + k, r, c));
+            const float f = z.y != 0.0f ? ex2(z.x - top) : 0.0f;        // (an empty run has no sums)
+            if (f == 0.0f) continue;
             den = fmaf(z.y, f, den);
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) sum[i] = f > 0.0f ? fmaf(p[i * 32 + lane], f, sum[i]) : sum[i];
+            sum.x = fmaf(y.x, f, sum.x), sum.y = fmaf(y.y, f, sum.y), sum.z = fmaf(y.z, f, sum.z), sum.w = fmaf(y.w, f, sum.w);
         }
         const float inv = 1.0f / den;
-        const size_t to = static_cast<size_t>(it.row0 + row / g_heads) * P.out_stride + (static_cast<size_t>(it.head) * g_heads + row % g_heads) * D + lane;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) row_store(P.out, P.type, to + i * 32, sum[i] * inv);
+        const size_t to = static_cast<size_t>(it.row0 + row / g_heads) * P.out_stride + (static_cast<size_t>(it.head) * g_heads + row % g_heads) * D + c;
+        row_store(P.out, P.type, to, sum.x * inv);
+        row_store(P.out, P.type, to + 1, sum.y * inv);
+        row_store(P.out, P.type, to + 2, sum.z * inv);
+        row_store(P.out, P.type, to + 3, sum.w * inv);
     }
 }
 
