@@ -1,0 +1,62 @@
+"""Attention over the 8-bit cache where the weights, or the sizes of values and scores, lie far apart."""
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_kv_cache import HALF_STEP, TYPES, Pair
+
+pytestmark = pytest.mark.gpu
+FEW, PROMPT, RUNS = "kv_attend_kernel", "kv_prompt_kernel", "kv_prompt_kernel, kv_prompt_join_kernel"
+
+
+def heavy_first(dtype, tokens, rows, nats, dim, alike):
+    """One kv head, `rows` last tokens. The first token's score is `nats` above the others', which differ by 0.2 (alike: not at all); its values are 0."""
+    p = Pair(4, 1, dim, 64, 0, dtype, n_pages=tokens // 64 + 2, max_seqs=1, max_context=tokens + 64, layers=1, seed=nats)
+    size = 8.0
+    q = torch.zeros(rows, 4, dim)
+    q[..., 0] = size
+    k = torch.zeros(tokens, 1, dim)
+    k[..., 0] = 0.0 if alike else (torch.rand(tokens, 1, generator=p.gen) - 0.5) * 0.2 / size
+    k[..., 1] = 1.0                     # (the pages' scale)
+    k[0, 0, 0] = nats / size
+    v = torch.full((tokens, 1, dim), 1.0) if alike else torch.randn(tokens, 1, dim, generator=p.gen) + 1.0
+    v[0] = 0.0
+    t = TYPES[dtype][0]
+    return p, q.to(t), k.to(t), v.to(t)
+
+
+def run(p, q, k, v, kernel):
+    n, m = k.shape[0], q.shape[0]
+    if n > m:
+        p.step([0], [n - m], rows=[(k[:n - m], v[:n - m])])
+    p.step([0], [m], rows=[(k[n - m:], v[n - m:])])
+    qd = q.cuda()
+    out = torch.full_like(qd, 3.0)
+    p.kv.attend(0, qd.data_ptr(), out.data_ptr(), TYPES[p.dtype][1], scale=1.0)
+    torch.cuda.synchronize()
+    assert p.kv.kernel_name() == kernel and p.kv.status() == 0
+    rows = np.unique(np.linspace(0, m - 1, 5).astype(int))
+    want = p.ref[0].attend(0, q.double().numpy(), 1.0, 0, rows=rows)
+    return out.double().cpu().numpy()[rows], want
+
+
+SHORT = [(4097, 1, FEW), (4097, 900, RUNS), (4900, 4800, PROMPT)]
+LONG = [(131073, 1, FEW), (131073, 400, RUNS)]
+
+
+@pytest.mark.parametrize("dtype,tokens,rows,kernel,nats,dim,alike",
+                         [(t, *s, n, d, a) for t in TYPES for s in SHORT for n in (10, 14, 18) for d in (64, 256) for a in (False, True)] +
+                         [(t, *s, n, 64, a) for t in ("f32", "bf16") for s in LONG for n in (12, 18) for a in (False, True)])
+def test_a_long_tail_behind_a_heavy_token(dtype, tokens, rows, kernel, nats, dim, alike):
+    """The first token has nearly all of the weight, and values of 0: the answer is the tail's alone, and is held to the tail's size.
+
+    Weights are F16 terms below a maximum of at least 2^13 (16 bits: 2^9): one is off by half a step of its own (2^-11; of two terms 2^-22), and by 2^-25 where
+    F16 ends, which is 2^-38 (2^-34) e^(nats + 0.2) of the tail's least weight. Scores (F32) are below 2^5, off by 2^-19 of e each, exponentials by 2^-21; all
+    of it once more for the denominator; then the answer's own rounding. A tensor core cuts each of the products that it adds where the sum ends, by up to 2^-23
+    of a sum that holds 2,048 tokens of two terms at most (16 bits: 8,192 of one), and half of its last value on average: 2,048 2^-23 (4,096 2^-23)."""
+    p, q, k, v = heavy_first(dtype, tokens, rows, nats, dim, alike)
+    got, want = run(p, q, k, v, kernel)
+    own = 2.0 ** -22 if dtype == "f32" else 2.0 ** -11
+    end = 2.0 ** (-38 if dtype == "f32" else -34) * np.exp(nats + 0.2)
+    tol = 2 * (own + 2.0 ** -19 + 2.0 ** -21) + end + (2048 if dtype == "f32" else 4096) * 2.0 ** -23 + HALF_STEP[dtype]
+    assert np.linalg.norm(got - want) <= tol * np.linalg.norm(want)

@@ -15,9 +15,10 @@ FEW, PROMPT, RUNS = "kv_attend_kernel", "kv_prompt_kernel", "kv_prompt_kernel, k
 @pytest.mark.parametrize("kernel,seqs,kv_heads,tokens,rows", [(FEW, 64, 4, 20000, 1), (FEW, 1, 4, 300, 1), (PROMPT, 1, 1, 30000, 4800), (RUNS, 1, 1, 131072, 300), (PROMPT, 3, 2, 1800, 1700)])
 @pytest.mark.parametrize("spread", [0.0, 0.4])
 def test_values_alike(dtype, dim, kernel, seqs, kv_heads, tokens, rows, spread):
-    """A sum on tensor cores may be cut off by 2^-23 of itself at each 16 tokens and term. The kernel for few rows adds 64 tokens at a time (2 4 2^-23), the one for
-    prompts 2,048 (F32; half of 2 128 2^-23, as sums grow evenly) or 8,192 (16 bits, half of 512 2^-23). Pieces are added in F32: 30 at most, 2^-24 each;
-    the denominator likewise; the weights' terms are off by 2^-22 (two), or 2^-11 each way, and the answer by its own rounding."""
+    """A tensor core cuts the products that it adds where the sum ends; over random weights that comes to 2^-23 of the sum for 16 tokens and a term at most. The
+    kernel for few rows adds 64 tokens at a time (2 4 2^-23), the one for prompts 2,048 (F32; half of 2 128 2^-23, as sums grow evenly) or 8,192 (16 bits, half
+    of 512 2^-23). Pieces are added in F32: 30 at most, 2^-24 each; the denominator likewise; the weights' terms are off by 2^-22 (two), or 2^-11 each way, and
+    the answer by its own rounding. Weights that are all alike are powers of two here, and their sums exact."""
     t, code = TYPES[dtype]
     heads = kv_heads * (4 if rows > 1 else 1)
     kv = wd.KvCache(1, heads, kv_heads, dim, seqs * (tokens // 128 + 1), seqs, tokens, page_tokens=128)

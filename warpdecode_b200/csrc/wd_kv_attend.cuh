@@ -3,9 +3,14 @@
 //   out[r] = sum_j p_j cv_j sv_j / sum_j p_j,   p_j = 2^(x_j - m),   x_j = (q[r] . ck_j) (2^e scale log2(e) sk_j)
 //
 // q is brought to F16 row by row: q = 2^e (hi + lo) with |hi| <= 1, lo = 0 unless the rows are F32; codes are exact in F16; sums are F32.
-// The scales of the values go into the exponent: m is the running maximum of x_j + log2(sv_j), P_j = 2^(x_j + log2 sv_j - m) <= 1 is what meets the
-// codes (F16, hi + lo for F32 rows), and the denominator takes P_j / sv_j in F32. A page whose values are small loses nothing beside one whose values
-// are large unless its part of the sum is small.
+// The scales of the values go into the exponent: m is the running maximum of x_j + log2(sv_j), P_j = 2^(15 + x_j + log2 sv_j - m) <= 2^15 is what meets
+// the codes (F16, hi + lo for F32 rows), and the denominator takes 2^-15 P_j / sv_j in F32. A page whose values are small loses nothing beside one whose
+// values are large unless its part of the sum is small.
+//
+// The 2^15 (it divides out) puts the largest weight at the upper end of F16's range, so that the many small weights behind a heavy token are not lost at
+// the lower one: a weight is off by half a step of its terms (2^-11 of itself; 2^-22 of two), and by 2^-40 of the row's largest, where F16 ends. So
+// n tokens' answer is off by n 2^-40 of the values' size at most. (With the largest weight at 1 it was n 2^-25: the sum of 131,072 tokens that have
+// 10 % of the weight behind one that has the rest was off by 2e-2 of itself.)
 //
 // Products: keys and values are the A operands (16 tokens, or 16 elements of the head), 8 rows of q the B operand, so that a group of up to 8 query
 // heads wastes nothing and the codes are expanded once for all of a warp's rows. The weights come out of the first product with tokens along the
@@ -33,6 +38,7 @@ constexpr int kAttWorkers = 8, kAttThreads = 512, kAttMaxSeqs = 1024, kAttMaxRow
 constexpr int kAttRegsMore = 192, kAttRegsLess = 64;
 static_assert(256 * kAttRegsMore + 256 * kAttRegsLess <= kAttThreads * 128, "more than the block was launched with: the increase would wait for ever");
 constexpr float kAttFloor = -1.0e30f;       // a maximum over nothing
+constexpr float kAttTop = 15.0f, kAttUnit = 1.0f / (1 << 15);        // the largest weight's exponent, and what a weight of 1 is of it
 
 struct KvAttend {
     const uint8_t *pool;        // of the layer
@@ -54,7 +60,7 @@ struct KvAttend {
 template <int D>
 struct AttendPlan {
     static constexpr int kCw = D % 64 == 0 ? 64 : 32;
-    static constexpr int kSlot = 64 * D + 64;           // keys or values of a tile; behind the keys 4 x {key scale, log2 of the value scale, 1 / value scale}
+    static constexpr int kSlot = 64 * D + 64;           // keys or values of a tile; behind the keys 4 x {key scale, log2 of the value scale, 2^-15 / value scale}
     __host__ __device__ static constexpr int q_bytes(int n8, bool split) { return n8 * 8 * D * 2 * (split ? 2 : 1); }
     __host__ __device__ static constexpr int fixed_bytes(int workers, int n8, bool split) { return workers * q_bytes(n8, split) + (kAttMaxSeqs + 2) * 8; }
 };
@@ -260,7 +266,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
             for (int t0 = s.lo; t0 < s.hi; t0 += 8) {
                 const uint8_t *now = src;
                 const float v = sc.y > 0.0f ? sc.y : kKvLeastScale;         // 0: nothing but zeros
-                const float4 mine = make_float4(sc.x, log2f(v), 1.0f / v, 0.0f);
+                const float4 mine = make_float4(sc.x, log2f(v), kAttUnit / v, 0.0f);
                 if (t0 + 8 < s.hi) look_up(t0 + 8);
 #pragma unroll 1
                 for (int j = 0; j < 8 && t0 + j < s.hi; ++j) {
@@ -472,7 +478,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
                     float sum = 0.0f;
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
-                        const float c = fmaxf(mul[n][i] * sc[b].x, 1e-37f), off = sc[b].y - now;
+                        const float c = fmaxf(mul[n][i] * sc[b].x, 1e-37f), off = sc[b].y - (now - kAttTop);
                         x[n][b][i] = ex2(fmaf(x[n][b][i], c, off));
                         x[n][b][2 + i] = ex2(fmaf(x[n][b][2 + i], c, off));
                         sum = fmaf(x[n][b][i] + x[n][b][2 + i], sc[b].z, sum);
@@ -540,7 +546,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
                 const int r = 8 * n + 2 * t + i, row = s.item_row + r;
                 if (r >= s.rows) continue;
                 if (s.whole) {
-                    const float inv = 1.0f / den;
+                    const float inv = kAttUnit / den;
                     const size_t to = static_cast<size_t>(s.row0 + row / g_heads) * P.out_stride + (static_cast<size_t>(s.head) * g_heads + row % g_heads) * D + g;
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
@@ -640,7 +646,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
             } else {
                 const int row = rw.z + r;
                 const size_t to0 = static_cast<size_t>(rw.x + row / g_heads) * P.out_stride + (static_cast<size_t>(rw.y) * g_heads + row % g_heads) * D + c;
-                const float inv = 1.0f / den;
+                const float inv = kAttUnit / den;
 #pragma unroll 1
                 for (int k = 0; k < 4; ++k) {
                     row_store(P.out, P.type, to0 + k, sum.x * inv);

@@ -1,12 +1,12 @@
 // Attention over the 8-bit cache for many rows (a prompt's chunk), on the fifth-generation tensor cores. The arithmetic is that of the kernel for few
-// rows (wd_kv_attend.cuh): q = 2^e (hi + lo) in F16, codes exact in F16, P = 2^(x + log2 sv - m) in F16 (hi + lo for F32 rows), the denominator takes
-// P / sv in F32; lo is left out for rows of 16 bits.
+// rows (wd_kv_attend.cuh): q = 2^e (hi + lo) in F16, codes exact in F16, P = 2^(13 + x + log2 sv - m) in F16 (hi + lo for F32 rows), the denominator takes
+// 2^-13 P / sv in F32; for rows of 16 bits lo is left out, and the 13 are 9.
 //
 // An item is 128 TILES rows of one kv head of a sequence (the G query heads of a token are neighbouring rows) against the tokens that they see, KT = 128
 // at a time (64 where F32 rows of 256 leave no room). Scores, then weights in their place, and sums are in tensor memory:
 //
-//   warps 0 .. 3, 4 .. 7   a row tile each, a thread a row: scores -> weights; the sums are brought to a new maximum only when it has grown by 2^8
-//                          (the weights stay below 256, which F16 holds as exactly), then the answer at the item's end
+//   warps 0 .. 3, 4 .. 7   a row tile each, a thread a row: scores -> weights; the sums are brought to a new maximum only when it has grown by 2^2
+//                          (16 bits: 2^6; weights stay below 2^15), then the answer at the item's end
 //   warps 8 .. 11          codes -> F16 operands in shared memory, K-major without swizzle; the tokens of a sub-block are taken in the order in which a
 //                          value's bytes have them, for keys and values alike
 //   warp 12                issues the products, the two row tiles in turn: Q K of the next tokens, P V of these (a warp for each tile is slower:
@@ -60,6 +60,9 @@ struct PromptAttPlan {
     // Tiles after which sums are brought to memory and begun anew: a tensor core cuts its sums off, so that those of values of one sign come out low, by 3.3e-9
     // of themselves for each token and term (F32 rows, 100,000 tokens in one sum: 6.6e-4). So F32 rows add 2,048 tokens at a time, others 8,192.
     static constexpr int kChain = (SPLIT ? 2048 : 8192) / kKt;
+    // The largest weight's exponent, as kAttTop, when the sums were brought to its maximum, and what it may grow by before they are again: the less, the more of
+    // F16's range is there for small weights, and the more often sums are brought (4,000 rows of 64 behind 1,011 tokens: by 2^8 188 us, 2^6 192, 2^4 193).
+    static constexpr float kTop = SPLIT ? 13.0f : 9.0f, kGrowth = 15.0f - kTop, kUnit = SPLIT ? 1.0f / 8192 : 1.0f / 512;
     static constexpr uint32_t kIdescS = 1u << 4 | (kKt >> 3) << 17 | (128 >> 4) << 24, kIdescO = 1u << 4 | (D >> 3) << 17 | (128 >> 4) << 24;
     static_assert(kColO + kTiles * D <= 512 && kSmem <= 226 * 1024, "plan of the memories");
 };
@@ -325,7 +328,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
             for (int tile = it.lo; tile < it.hi; ++tile, ++n) {
                 const size_t at = static_cast<size_t>(page) * kv_page_bytes(P.s) + static_cast<size_t>(in_page) * (16 * D);
                 const float vsc = sc.y > 0.0f ? sc.y : kKvLeastScale;
-                const float4 mine = make_float4(sc.x, log2f(vsc), 1.0f / vsc, 0.0f);
+                const float4 mine = make_float4(sc.x, log2f(vsc), A::kUnit / vsc, 0.0f);
                 const int st = n % ST;
                 const uint32_t par = (static_cast<uint32_t>(n / ST) & 1u) ^ 1u;
                 // keys: unit u is 16 elements of token u % KT
@@ -505,7 +508,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
                     }
                     if (tile == it.lo) {
                         m = most;
-                    } else if (__any_sync(0xffffffffu, most > m + 8.0f)) {
+                    } else if (__any_sync(0xffffffffu, most > m + A::kGrowth)) {
                         const float now = fmaxf(m, most), f = ex2(m - now);
                         m = now;
                         l *= f;
@@ -519,11 +522,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
                             tc_st(oc + c * 16, u);
                         }
                     }
+                    const float base = m - A::kTop;
                     // exponents of all columns, then the exponentials (scales read between the stores of weights would wait for them)
 #pragma unroll
                     for (int b = 0; b < SUBS; ++b) {
                         const float4 s4 = scales[n & 3][b];
-                        const float mk = fmaxf(mul * s4.x, 1e-37f), off = s4.y - m;
+                        const float mk = fmaxf(mul * s4.x, 1e-37f), off = s4.y - base;
                         const f32x2 mk2 = pack2(mk, mk), off2 = pack2(off, off);
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
@@ -630,7 +634,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
                 if (is) *prompt_part_end<D, A::kRows>(P.part, place, of) = make_float2(m, l);         // (of an empty run nothing else is read)
                 continue;
             }
-            const float inv = 1.0f / l;
+            const float inv = A::kUnit / l;
             const size_t dst = static_cast<size_t>(it.row0 + row / g_heads) * P.out_stride + elem;
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
@@ -701,7 +705,7 @@ __global__ void __launch_bounds__(256) kv_prompt_join_kernel(const __grid_consta
             den = fmaf(z.y, f, den);
             sum.x = fmaf(y.x, f, sum.x), sum.y = fmaf(y.y, f, sum.y), sum.z = fmaf(y.z, f, sum.z), sum.w = fmaf(y.w, f, sum.w);
         }
-        const float inv = 1.0f / den;
+        const float inv = (P.type == kRowsF32 ? PromptAttPlan<D, true>::kUnit : PromptAttPlan<D, false>::kUnit) / den;
         const size_t to = static_cast<size_t>(it.row0 + row / g_heads) * P.out_stride + (static_cast<size_t>(it.head) * g_heads + row % g_heads) * D + c;
         row_store(P.out, P.type, to, sum.x * inv);
         row_store(P.out, P.type, to + 1, sum.y * inv);
