@@ -7,6 +7,7 @@ from test_gpu_kv_cache import HALF_STEP, TYPES, Pair
 
 pytestmark = pytest.mark.gpu
 FEW, PROMPT, RUNS = "kv_attend_kernel", "kv_prompt_kernel", "kv_prompt_kernel, kv_prompt_join_kernel"
+KERNELS = [(FEW, 4, 2), (RUNS, 8, 1000), (PROMPT, 16, 1200)]         # heads over two, and last rows, that run on each
 
 
 def heavy_first(dtype, tokens, rows, nats, dim, alike):
@@ -60,3 +61,54 @@ def test_a_long_tail_behind_a_heavy_token(dtype, tokens, rows, kernel, nats, dim
     end = 2.0 ** (-38 if dtype == "f32" else -34) * np.exp(nats + 0.2)
     tol = 2 * (own + 2.0 ** -19 + 2.0 ** -21) + end + (2048 if dtype == "f32" else 4096) * 2.0 ** -23 + HALF_STEP[dtype]
     assert np.linalg.norm(got - want) <= tol * np.linalg.norm(want)
+
+
+# sums of 2,400 tokens, 150 times 16 of two terms: 2 150 2^-24, and weights off by 2^-21
+TOL = 2.0 ** -15
+SPREADS = [(1e12, 0.0), (0.0, 1e12), (1e20, 1e-20), (1e-20, 1e20), (1e26, 0.0), (1e34, 1.0), (1.0, 1e34), (1e-25, 0.0), (1e37, 1e37), (0.0, 0.0)]
+
+
+@pytest.mark.parametrize("kernel,heads,count", KERNELS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("first,second", SPREADS)
+def test_pages_whose_values_are_far_apart_weigh_alike(first, second, dim, kernel, heads, count):
+    """Scores are all alike, values of one stretch of pages are `first`, of another `second` in size, turn about: each token has its share of the weight."""
+    n = 1200 + count
+    p = Pair(heads, 2, dim, 16, 0, "f32", n_pages=400, layers=1)
+    k, v = torch.zeros(n, 2, dim), p.rand(n, 2, dim).abs() + 0.5
+    stretch = torch.arange(n) // 400 % 2 == 0
+    v = torch.where(stretch[:, None, None], v * first, v * second)
+    got, want = run(p, torch.zeros(count, heads, dim), k, v, kernel)
+    assert np.isfinite(got).all()
+    assert np.linalg.norm(got - want) <= TOL * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("kernel,heads,count", KERNELS)
+@pytest.mark.parametrize("size", [1.0, 1e12, 1e-20])
+def test_small_values_that_have_the_weight(size, kernel, heads, count):
+    """Large values whose scores are 120 below: what remains of them (1e-42 of the answer) is added to the small ones' sum, which does not lose by it."""
+    n = 1200 + count
+    p = Pair(heads, 2, 64, 16, 0, "f32", n_pages=400, layers=1)
+    k, v = torch.zeros(n, 2, 64), (p.rand(n, 2, 64).abs() + 0.5) * size
+    k[:, :, 0] = k[:, :, 1] = 1.0
+    k[400:608, :, 0] = -1.0
+    v[400:608] *= 1e10
+    q = torch.zeros(count, heads, 64)
+    q[..., 0] = 60.0
+    got, want = run(p, q, k, v, kernel)
+    assert np.linalg.norm(got - want) <= TOL * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("kernel,heads,count", KERNELS)
+@pytest.mark.parametrize("was", [1e30, 1e-24])
+def test_values_of_another_size_that_are_gone(was, kernel, heads, count):
+    """What a cache has held before, in pages that are in use again, changes nothing."""
+    n = 1200 + count
+    p = Pair(heads, 2, 64, 16, 0, "f32", n_pages=400, layers=1)
+    k, v = p.rand(n, 2, 64), p.rand(n, 2, 64)
+    p.step([0], [3000], rows=[(p.rand(3000, 2, 64), p.rand(3000, 2, 64) * was)])
+    p.kv.free([0])
+    p.ref[0].truncate(0, 0)
+    got, want = run(p, p.rand(count, heads, 64) * 0.125, k, v, kernel)
+    # scores of at most 5 5 64 / 8, off by 2^-22 of that; norms over values of either sign, whose sums are a part of them
+    assert np.linalg.norm(got - want) <= 2.0 ** -13 * np.linalg.norm(want)

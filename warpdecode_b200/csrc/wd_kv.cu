@@ -43,6 +43,7 @@ struct wd_kv_cache {
     float *d_scales = nullptr, *d_part = nullptr, *d_cta_part = nullptr;
     int *d_book = nullptr, *d_index = nullptr;
     unsigned *d_arrived = nullptr, *d_status = nullptr;
+    int2 *d_reach = nullptr;
     size_t pool_layer = 0, scales_layer = 0;
     const char *last_kernel = "";           // of wd_kv_attend
     bool graphs = false;                    // an append or an attend has been captured: replays look for the step in the device's book
@@ -345,7 +346,8 @@ int wd_kv_create(const wd_kv_config *cfg, wd_kv_cache **out) {
         if (alloc(&k->d_pool, k->pool_layer * c.n_layers) != cudaSuccess || alloc(&k->d_scales, k->scales_layer * c.n_layers * 4) != cudaSuccess ||
             alloc(&k->d_part, part * wd::kAttWorkers) != cudaSuccess || alloc(&k->d_cta_part, part) != cudaSuccess || alloc(&k->d_book, words * 4) != cudaSuccess ||
             alloc(&k->d_index, (static_cast<size_t>(c.max_context) + k->shape.max_pages) * 4) != cudaSuccess ||
-            alloc(&k->d_arrived, static_cast<size_t>(k->n_sm) * 4) != cudaSuccess || alloc(&k->d_status, 16) != cudaSuccess)
+            alloc(&k->d_arrived, static_cast<size_t>(k->n_sm) * 4) != cudaSuccess || alloc(&k->d_status, 16) != cudaSuccess ||
+            alloc(&k->d_reach, static_cast<size_t>(c.n_layers) * c.n_kv_heads * sizeof(int2)) != cudaSuccess)
             return set_error(WD_E_NOMEM, "key/value cache: " + std::to_string((k->pool_layer * c.n_layers) >> 20) + " MiB of pages do not fit");
         WD_TRY_CUDA(cudaStreamSynchronize(cudaStreamLegacy));
         *out = k.release();
@@ -358,7 +360,7 @@ void wd_kv_destroy(wd_kv_cache *c) {
     if (!c->host_only()) {
         OnDevice on(c->cfg.device);
         for (void *p : {static_cast<void *>(c->d_pool), static_cast<void *>(c->d_scales), static_cast<void *>(c->d_part), static_cast<void *>(c->d_cta_part), static_cast<void *>(c->d_book),
-                        static_cast<void *>(c->d_index), static_cast<void *>(c->d_arrived), static_cast<void *>(c->d_status)})
+                        static_cast<void *>(c->d_index), static_cast<void *>(c->d_arrived), static_cast<void *>(c->d_status), static_cast<void *>(c->d_reach)})
             if (p) cudaFree(p);
     }
     delete c;
@@ -448,6 +450,7 @@ int wd_kv_append(wd_kv_cache *c, int layer, const void *k_dev, const void *v_dev
         if (int rc = note_capture(c, s)) return rc;
         p.pool = c->d_pool + layer * c->pool_layer;
         p.scales = c->d_scales + layer * c->scales_layer;
+        p.reach = c->d_reach + static_cast<size_t>(layer) * c->cfg.n_kv_heads;
         p.book = c->d_book;
         p.table = c->d_book + c->table_at;
         p.rows[0] = k_dev;
@@ -509,7 +512,7 @@ int wd_kv_attend(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, in
         c->last_kernel = by.prompt ? by.split ? "kv_prompt_kernel, kv_prompt_join_kernel" : "kv_prompt_kernel" : "kv_attend_kernel";
         if (by.prompt) {
             wd::KvPrompt r;
-            r.pool = p.pool, r.scales = p.scales, r.book = p.book, r.table = p.table, r.q = p.q, r.out = p.out;
+            r.pool = p.pool, r.scales = p.scales, r.reach = c->d_reach + static_cast<size_t>(layer) * c->cfg.n_kv_heads, r.book = p.book, r.table = p.table, r.q = p.q, r.out = p.out;
             r.q_stride = p.q_stride, r.out_stride = p.out_stride, r.status = p.status, r.scale_log2 = p.scale_log2;
             r.type = p.type, r.window = p.window, r.s = p.s, r.part = c->d_part, r.ctas = c->n_sm;
             r.split = by.split;         // (the kernels count the items of the step that is current when they run)

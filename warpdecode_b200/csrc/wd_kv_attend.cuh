@@ -3,13 +3,14 @@
 //   out[r] = sum_j p_j cv_j sv_j / sum_j p_j,   p_j = 2^(x_j - m),   x_j = (q[r] . ck_j) (2^e scale log2(e) sk_j)
 //
 // q is brought to F16 row by row: q = 2^e (hi + lo) with |hi| <= 1, lo = 0 unless the rows are F32; codes are exact in F16; sums are F32.
-// The scales of the values go into the exponent: m is the running maximum of x_j + log2(sv_j), P_j = 2^(15 + x_j + log2 sv_j - m) <= 2^15 is what meets
-// the codes (F16, hi + lo for F32 rows), and the denominator takes 2^-15 P_j / sv_j in F32. A page whose values are small loses nothing beside one whose
-// values are large unless its part of the sum is small.
+// Weights: m is the running maximum of x_j + log2(sv_j). E_j = 2^(7 + x_j - m) makes the denominator, P_j = E_j (2^6 sv_j) <= 2^13 meets the codes (F16,
+// hi + lo for F32 rows); the answer is 2^-6 sum P_j cv_j / sum E_j. So a page whose values are small loses nothing beside one whose values are large
+// unless its part of the sum is small, and its tokens' weights are counted whatever their values. Within F32: E_j is at least 2^-79 for the token
+// with the largest weight where scales are below 2^86 (2^-114 at the largest F32 has), and at most 2^107.
 //
-// The 2^15 (it divides out) puts the largest weight at the upper end of F16's range, so that the many small weights behind a heavy token are not lost at
-// the lower one: a weight is off by half a step of its terms (2^-11 of itself; 2^-22 of two), and by 2^-40 of the row's largest, where F16 ends. So
-// n tokens' answer is off by n 2^-40 of the values' size at most. (With the largest weight at 1 it was n 2^-25: the sum of 131,072 tokens that have
+// The 2^13 (it divides out) puts the largest weight near the upper end of F16's range, so that the many small weights behind a heavy token are not lost at
+// the lower one: a weight is off by half a step of its terms (2^-11 of itself; 2^-22 of two), and by 2^-38 of the row's largest, where F16 ends. So
+// n tokens' answer is off by n 2^-38 of the values' size at most. (With the largest weight at 1 it was n 2^-25: the sum of 131,072 tokens that have
 // 10 % of the weight behind one that has the rest was off by 2e-2 of itself.)
 //
 // Products: keys and values are the A operands (16 tokens, or 16 elements of the head), 8 rows of q the B operand, so that a group of up to 8 query
@@ -38,7 +39,8 @@ constexpr int kAttWorkers = 8, kAttThreads = 512, kAttMaxSeqs = 1024, kAttMaxRow
 constexpr int kAttRegsMore = 192, kAttRegsLess = 64;
 static_assert(256 * kAttRegsMore + 256 * kAttRegsLess <= kAttThreads * 128, "more than the block was launched with: the increase would wait for ever");
 constexpr float kAttFloor = -1.0e30f;       // a maximum over nothing
-constexpr float kAttTop = 15.0f, kAttUnit = 1.0f / (1 << 15);        // the largest weight's exponent, and what a weight of 1 is of it
+constexpr int kAttTop = 13, kAttScale = 6;              // exponents: of the largest P_j, of what a value scale is multiplied by (F32's largest scale is below 2^122)
+constexpr float kAttUnit = 1.0f / (1 << kAttScale);
 
 struct KvAttend {
     const uint8_t *pool;        // of the layer
@@ -60,7 +62,7 @@ struct KvAttend {
 template <int D>
 struct AttendPlan {
     static constexpr int kCw = D % 64 == 0 ? 64 : 32;
-    static constexpr int kSlot = 64 * D + 64;           // keys or values of a tile; behind the keys 4 x {key scale, log2 of the value scale, 2^-15 / value scale}
+    static constexpr int kSlot = 64 * D + 64;           // keys or values of a tile; behind the keys 4 x {key scale, log2 of the value scale, 2^6 times the value scale}
     __host__ __device__ static constexpr int q_bytes(int n8, bool split) { return n8 * 8 * D * 2 * (split ? 2 : 1); }
     __host__ __device__ static constexpr int fixed_bytes(int workers, int n8, bool split) { return workers * q_bytes(n8, split) + (kAttMaxSeqs + 2) * 8; }
 };
@@ -265,8 +267,8 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
 #pragma unroll 1
             for (int t0 = s.lo; t0 < s.hi; t0 += 8) {
                 const uint8_t *now = src;
-                const float v = sc.y > 0.0f ? sc.y : kKvLeastScale;         // 0: nothing but zeros
-                const float4 mine = make_float4(sc.x, log2f(v), kAttUnit / v, 0.0f);
+                // (of a scale of 0, nothing but zeros, the logarithm of the least one: it costs no other weight its place)
+                const float4 mine = make_float4(sc.x, log2f(fmaxf(sc.y, kKvLeastScale)), static_cast<float>(1 << kAttScale) * sc.y, 0.0f);
                 if (t0 + 8 < s.hi) look_up(t0 + 8);
 #pragma unroll 1
                 for (int j = 0; j < 8 && t0 + j < s.hi; ++j) {
@@ -473,17 +475,18 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                     const float now = fmaxf(m[n][i], top);
-                    f[n][i] = ex2(m[n][i] - now);
+                    const float half_way = ex2(0.5f * (m[n][i] - now)), off = static_cast<float>(kAttTop - kAttScale) - now;
+                    f[n][i] = half_way * half_way;
                     m[n][i] = now;
-                    float sum = 0.0f;
+                    float sum = l[n][i] * half_way * half_way;         // (what is nothing beside the sums now may be something in the denominator)
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
-                        const float c = fmaxf(mul[n][i] * sc[b].x, 1e-37f), off = sc[b].y - (now - kAttTop);
-                        x[n][b][i] = ex2(fmaf(x[n][b][i], c, off));
-                        x[n][b][2 + i] = ex2(fmaf(x[n][b][2 + i], c, off));
-                        sum = fmaf(x[n][b][i] + x[n][b][2 + i], sc[b].z, sum);
+                        const float c = fmaxf(mul[n][i] * sc[b].x, 1e-37f), e0 = ex2(fmaf(x[n][b][i], c, off)), e1 = ex2(fmaf(x[n][b][2 + i], c, off));
+                        sum += e0 + e1;
+                        x[n][b][i] = e0 * sc[b].z;
+                        x[n][b][2 + i] = e1 * sc[b].z;
                     }
-                    l[n][i] = fmaf(l[n][i], f[n][i], sum);
+                    l[n][i] = sum;
                 }
 #pragma unroll
                 for (int b = 0; b < 4; ++b)
@@ -634,9 +637,9 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     if (k0 + k >= n) break;
-                    const float both = fmaxf(top, z[k].x), fa = ex2(top - both), fb = ex2(z[k].x - both);
+                    const float both = fmaxf(top, z[k].x), ha = ex2(0.5f * (top - both)), hb = ex2(0.5f * (z[k].x - both)), fa = ha * ha, fb = hb * hb;
                     top = both;
-                    den = den * fa + z[k].y * fb;
+                    den = den * ha * ha + z[k].y * hb * hb;
                     sum.x = sum.x * fa + y[k].x * fb, sum.y = sum.y * fa + y[k].y * fb, sum.z = sum.z * fa + y[k].z * fb, sum.w = sum.w * fa + y[k].w * fb;
                 }
             }

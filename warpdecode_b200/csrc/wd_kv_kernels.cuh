@@ -34,6 +34,7 @@ __global__ void __launch_bounds__(256) kv_run_kernel(const __grid_constant__ KvR
 struct KvAppend {
     uint8_t *pool;              // of the layer
     float *scales;              // of the layer
+    int2 *reach;                // of the layer
     const int *book;
     const int *table;
     const void *rows[2];
@@ -65,6 +66,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 16) kv_append_ke
         uint8_t *base = P.pool + static_cast<size_t>(page) * kv_page_bytes(P.s) + h * kv_head_bytes(P.s) + kv * kv_half_bytes(P.s);
         float *scale = P.scales + (static_cast<size_t>(page) * P.s.kv_heads + h) * 2 + kv;
         const float s0 = a > 0 ? *scale : 0.0f;
+        const int2 reach = tid == 0 && kv ? P.reach[h] : make_int2(0, 0);        // (as it was, or newer)
         const int per = D / 16, groups = (b - a) * per;
         // the largest finite magnitude
         float top = 0.0f;
@@ -142,7 +144,14 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 16) kv_append_ke
                 }
             }
         }
-        if (tid == 0) *scale = s1;
+        if (tid == 0) {
+            *scale = s1;
+            const int at_1 = static_cast<int>(__float_as_uint(s1) >> 23) - 127;
+            if (kv && s1 > 0.0f && (at_1 + 1024 > reach.x || 1024 - at_1 > reach.y)) {
+                atomicMax(&P.reach[h].x, at_1 + 1024);
+                atomicMax(&P.reach[h].y, 1024 - at_1);
+            }
+        }
         __syncthreads();
     }
 }

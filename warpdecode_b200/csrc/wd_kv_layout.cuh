@@ -2,6 +2,7 @@
 //
 // pool    [layer][page][kv head][K: page_tokens D bytes | V: page_tokens D bytes]
 // scales  [layer][page][kv head][2]  (F32; keys, values)
+// reach   [layer][kv head]           how large and how small value scales have been since the cache began: largest exponent + 1024, 1024 - least exponent; 0: none
 // book    int32 words: the step's header and entries, then the page table [max_seqs][max_pages]
 //
 // K and V are sub-blocks of 16 tokens, 16 D bytes each, laid out as the A operands of a matrix instruction of 16 x 8 x 16 want them: a lane
@@ -23,6 +24,13 @@ constexpr int kKvSub = 16;              // tokens of a sub-block
 constexpr int kKvStepWords = 8;         // words of a step's entry: sequence, first row, rows, length with the step's tokens, first page item
 constexpr int kKvHead = 8;              // words in front of the entries: sequences, rows, page items
 constexpr float kKvLeastScale = 7.888609052210118e-31f;     // 2^-100: keeps 1 / scale and sums of it far inside F32
+
+// whether value scales may be so far apart that a weight times the one is nothing in F32 where that times the other is of size 1; and what may stand for a
+// scale of 0 (nothing but zeros) among them: far below the largest, so that it costs no weight its place, and no farther apart than the others
+__device__ __forceinline__ bool kv_far_apart(int2 reach) { return reach.x && (reach.x - 1024) - (1024 - reach.y) > 90; }
+__device__ __forceinline__ float kv_zero_scale(int2 reach) {
+    return __uint_as_float(static_cast<uint32_t>((reach.x ? max(reach.x - 1024, -40) : -40) - 60 + 127) << 23);
+}
 
 enum : unsigned { kKvNonFinite = 32u };     // status bit: a NaN or an infinity was appended
 

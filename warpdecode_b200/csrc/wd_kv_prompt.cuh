@@ -1,6 +1,7 @@
 // Attention over the 8-bit cache for many rows (a prompt's chunk), on the fifth-generation tensor cores. The arithmetic is that of the kernel for few
-// rows (wd_kv_attend.cuh): q = 2^e (hi + lo) in F16, codes exact in F16, P = 2^(13 + x + log2 sv - m) in F16 (hi + lo for F32 rows), the denominator takes
-// 2^-13 P / sv in F32; for rows of 16 bits lo is left out, and the 13 are 9.
+// rows (wd_kv_attend.cuh), with E = 2^(7 + x - m) and P = E 2^6 sv in F16 (hi + lo for F32 rows; for rows of 16 bits lo is left out, and the 7 are 3). A
+// multiplication each is dear here (184 -> 204 us): where the value scales of a head have never been more than 2^90 apart, P is made at once as
+// 2^(13 + x + log2 sv - m), and the denominator takes P 2^-6 / sv, which is E. (Farther apart P may be nothing where E is not.)
 //
 // An item is 128 TILES rows of one kv head of a sequence (the G query heads of a token are neighbouring rows) against the tokens that they see, KT = 128
 // at a time (64 where F32 rows of 256 leave no room). Scores, then weights in their place, and sums are in tensor memory:
@@ -35,6 +36,7 @@ struct KvPrompt {
     const float *scales;        // of the layer
     const int *book;
     const int *table;
+    const int2 *reach;          // of the layer, [kv heads]
     const void *q;
     void *out;
     long long q_stride, out_stride;
@@ -62,7 +64,7 @@ struct PromptAttPlan {
     static constexpr int kChain = (SPLIT ? 2048 : 8192) / kKt;
     // The largest weight's exponent, as kAttTop, when the sums were brought to its maximum, and what it may grow by before they are again: the less, the more of
     // F16's range is there for small weights, and the more often sums are brought (4,000 rows of 64 behind 1,011 tokens: by 2^8 188 us, 2^6 192, 2^4 193).
-    static constexpr float kTop = SPLIT ? 13.0f : 9.0f, kGrowth = 15.0f - kTop, kUnit = SPLIT ? 1.0f / 8192 : 1.0f / 512;
+    static constexpr float kTop = SPLIT ? 13.0f : 9.0f, kGrowth = 15.0f - kTop;
     static constexpr uint32_t kIdescS = 1u << 4 | (kKt >> 3) << 17 | (128 >> 4) << 24, kIdescO = 1u << 4 | (D >> 3) << 17 | (128 >> 4) << 24;
     static_assert(kColO + kTiles * D <= 512 && kSmem <= 226 * 1024, "plan of the memories");
 };
@@ -315,6 +317,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
             const int *table = P.table + static_cast<size_t>(it.seq) * P.s.max_pages;
             const int last_sub = (it.length - 1) >> 4;
             const uint8_t *head = P.pool + it.head * kv_head_bytes(P.s);
+            const float zero = kv_zero_scale(P.reach[it.head]);        // what stands for a scale of 0
             // lane l: page of sub-block l of a tile, where the sub-block is in the page, and the scales (behind the last sub-block: the last one)
             int page = 0, in_page = 0;
             float2 sc = make_float2(0.0f, 0.0f);
@@ -327,8 +330,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
             if (it.lo < it.hi) look_up(it.lo);
             for (int tile = it.lo; tile < it.hi; ++tile, ++n) {
                 const size_t at = static_cast<size_t>(page) * kv_page_bytes(P.s) + static_cast<size_t>(in_page) * (16 * D);
-                const float vsc = sc.y > 0.0f ? sc.y : kKvLeastScale;
-                const float4 mine = make_float4(sc.x, log2f(vsc), A::kUnit / vsc, 0.0f);
+                const float vsc = sc.y > 0.0f ? sc.y : zero, up = static_cast<float>(1 << kAttScale);
+                const float4 mine = make_float4(sc.x, log2f(vsc), 1.0f / (up * vsc), up * sc.y);
                 const int st = n % ST;
                 const uint32_t par = (static_cast<uint32_t>(n / ST) & 1u) ^ 1u;
                 // keys: unit u is 16 elements of token u % KT
@@ -463,140 +466,196 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
             fence_proxy_async();
             if (it.lo < it.hi) mbar_arrive(&q_full[x]);
             float m = kAttFloor, l = 0.0f;
+            // the row's maximum is now `most` or what it was; brought to it where it has grown enough
+            auto follow = [&](int tile, float most) {
+                if (tile == it.lo) {
+                    m = most;
+                } else if (__any_sync(0xffffffffu, most > m + A::kGrowth)) {
+                    const float now = fmaxf(m, most), half_way = ex2(0.5f * (m - now)), f = half_way * half_way;        // (see the kernel for few rows)
+                    m = now;
+                    l = l * half_way * half_way;
 #pragma unroll 1
-            for (int tile = it.lo; tile < it.hi;) {
-                const int chain_end = min(tile + A::kChain, it.hi);
-#pragma unroll 1
-                for (; tile < chain_end; ++tile, ++n) {
-                    att_wait(&s_full[x], n_s++ & 1, P.status);
-                    tc_fence_after();
-                    const int first = tile * KT;
-                    const bool edge = first + KT - 1 > pos_lo || (P.window && first <= pos_hi - P.window);
-                    uint32_t v[KT / 32][32];
-#pragma unroll
-                    for (int c = 0; c < KT / 32; ++c) tc_ld(sc + c * 32, v[c]);
-#pragma unroll
-                    for (int c = 0; c < KT / 32; ++c) tc_wait_ld(v[c]);
-                    if constexpr (A::kApart) {
-                        tc_fence_before();
-                        mbar_arrive(&s_free[x]);
-                    }
-                    // column 16 s + p of the scores is token 2 (p / 4) + (p & 1) + 8 ((p & 3) / 2) of sub-block s
-                    if (edge) {
-#pragma unroll
-                        for (int c = 0; c < KT / 32; ++c)
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                const int p = i & 15, token = first + c * 32 + (i & 16) + (p >> 2) * 2 + (p & 1) + ((p & 2) << 2);
-                                if (token > pos || (P.window && token <= pos - P.window)) v[c][i] = 0xff800000u;
-                            }
-                    }
-                    float most = kAttFloor;
-#pragma unroll
-                    for (int b = 0; b < SUBS; ++b) {
-                        const float4 s4 = scales[n & 3][b];
-                        auto at = [&](int i) { return __uint_as_float(v[b / 2][b % 2 * 16 + i]); };
-                        float t = max3(at(0), at(1), at(2));
-#pragma unroll
-                        for (int i = 3; i < 15; i += 2) t = max3(t, at(i), at(i + 1));
-                        t = fmaxf(t, at(15));
-                        most = fmaxf(most, fmaf(t, fmaxf(mul * s4.x, 1e-37f), s4.y));
-                    }
-                    if constexpr (A::kApart) {          // the sums, and the place of the weights, are free
-                        if (n_o > 0) att_wait(&o_done[x], (n_o - 1) & 1, P.status);
-                        tc_fence_after();
-                    }
-                    if (tile == it.lo) {
-                        m = most;
-                    } else if (__any_sync(0xffffffffu, most > m + A::kGrowth)) {
-                        const float now = fmaxf(m, most), f = ex2(m - now);
-                        m = now;
-                        l *= f;
-#pragma unroll 1
-                        for (int c = 0; c < D / 16; ++c) {
-                            uint32_t u[16];
-                            tc_ld(oc + c * 16, u);
-                            tc_wait_ld(u);
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * f);
-                            tc_st(oc + c * 16, u);
-                        }
-                    }
-                    const float base = m - A::kTop;
-                    // exponents of all columns, then the exponentials (scales read between the stores of weights would wait for them)
-#pragma unroll
-                    for (int b = 0; b < SUBS; ++b) {
-                        const float4 s4 = scales[n & 3][b];
-                        const float mk = fmaxf(mul * s4.x, 1e-37f), off = s4.y - base;
-                        const f32x2 mk2 = pack2(mk, mk), off2 = pack2(off, off);
-#pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            uint32_t *u = &v[b / 2][b % 2 * 16 + i];
-                            float a, c;
-                            unpack2(fma2(pack2(__uint_as_float(u[0]), __uint_as_float(u[1])), mk2, off2), a, c);
-                            u[0] = __float_as_uint(a), u[1] = __float_as_uint(c);
-                        }
-                    }
-                    uint32_t hi[KT / 32][16], lo[SPLIT ? KT / 32 : 1][16];
-#pragma unroll
-                    for (int b = 0; b < SUBS; ++b) {
-                        f32x2 s0 = pack2(0.0f, 0.0f), s1 = s0;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float a = ex2(__uint_as_float(v[b / 2][b % 2 * 16 + 2 * i])), c = ex2(__uint_as_float(v[b / 2][b % 2 * 16 + 2 * i + 1]));
-                            if (i & 1) s1 = add2(s1, pack2(a, c));
-                            else s0 = add2(s0, pack2(a, c));
-                            hi[b / 2][b % 2 * 8 + i] = half_pair(a, c);
-                            if constexpr (SPLIT) lo[b / 2][b % 2 * 8 + i] = half_rest(a, c, hi[b / 2][b % 2 * 8 + i]);
-                        }
-                        float a, c;
-                        unpack2(add2(s0, s1), a, c);
-                        l = fmaf(a + c, scales[n & 3][b].z, l);
-                    }
-#pragma unroll
-                    for (int c = 0; c < KT / 32; ++c) {
-                        tc_st(pc + c * kPartP, hi[c]);
-                        if constexpr (SPLIT) tc_st(pc + c * kPartP + 16, lo[c]);
-                    }
-                    tc_wait_st();
-                    tc_fence_before();
-                    mbar_arrive(&p_full[x]);
-                    ++n_o;
-                }
-                // a chain's end: its sums are added to those of the chains in front of it
-                if (tile < it.hi) {
-                    int of = x * 128 + r;
-                    asm volatile("" : "+r"(of));          // (addresses are made here, not held through the tiles)
-                    const int place = runs > 1 ? it.at : blockIdx.x;
-                    const bool more = tile - it.lo > A::kChain;
-                    float *held_m = &prompt_part_end<D, A::kRows>(P.part, place, of)->x;
-                    const float f = more ? ex2(*held_m - m) : 0.0f;         // (m does not go down)
-                    *held_m = m;
-                    float4 h[8];
-                    auto ask = [&](int c) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) h[i] = more ? *reinterpret_cast<const float4 *>(prompt_part<D, A::kRows>(P.part, place, of, c + 4 * i)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    };
-                    ask(0);
-                    att_wait(&o_done[x], (n_o - 1) & 1, P.status);
-                    tc_fence_after();
-#pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t u[32];
-                        tc_ld(oc + c, u);
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t u[16];
+                        tc_ld(oc + c * 16, u);
                         tc_wait_ld(u);
-                        float4 y[8];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            y[i] = make_float4(fmaf(h[i].x, f, __uint_as_float(u[4 * i])), fmaf(h[i].y, f, __uint_as_float(u[4 * i + 1])),
-                                               fmaf(h[i].z, f, __uint_as_float(u[4 * i + 2])), fmaf(h[i].w, f, __uint_as_float(u[4 * i + 3])));
-                        if (c + 32 < D) ask(c + 32);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) *reinterpret_cast<float4 *>(prompt_part<D, A::kRows>(P.part, place, of, c + 4 * i)) = y[i];
+                        for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * f);
+                        tc_st(oc + c * 16, u);
                     }
-                    tc_fence_before();
                 }
-            }
+            };
+            auto tiles = [&](auto apart) {
+                constexpr bool kFar = decltype(apart)::value;
+#pragma unroll 1
+                for (int tile = it.lo; tile < it.hi;) {
+                    const int chain_end = min(tile + A::kChain, it.hi);
+#pragma unroll 1
+                    for (; tile < chain_end; ++tile, ++n) {
+                        att_wait(&s_full[x], n_s++ & 1, P.status);
+                        tc_fence_after();
+                        const int first = tile * KT;
+                        const bool edge = first + KT - 1 > pos_lo || (P.window && first <= pos_hi - P.window);
+                        if constexpr (kFar) {           // (rare: little code, few registers, the scores read twice)
+                            float most = kAttFloor;
+                            uint32_t u[32], hi[16], lo[16];
+                            auto scores = [&](int c) {          // of the 32 tokens from 32 c on
+                                tc_ld(sc + c * 32, u);
+                                tc_wait_ld(u);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) {
+                                    const int p = i & 15, token = first + c * 32 + (i & 16) + (p >> 2) * 2 + (p & 1) + ((p & 2) << 2);
+                                    if (token > pos || (P.window && token <= pos - P.window)) u[i] = 0xff800000u;
+                                }
+                            };
+#pragma unroll 1
+                            for (int c = 0; c < KT / 32; ++c) {
+                                scores(c);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) {
+                                    const float4 s4 = scales[n & 3][2 * c + i / 16];
+                                    most = fmaxf(most, fmaf(__uint_as_float(u[i]), fmaxf(mul * s4.x, 1e-37f), s4.y));
+                                }
+                            }
+                            if constexpr (A::kApart) {
+                                if (n_o > 0) att_wait(&o_done[x], (n_o - 1) & 1, P.status);
+                                tc_fence_after();
+                            }
+                            follow(tile, most);
+                            const float off = (A::kTop - static_cast<float>(kAttScale)) - m;
+#pragma unroll 1
+                            for (int c = 0; c < KT / 32; ++c) {
+                                scores(c);
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) {
+                                    const float4 s4 = scales[n & 3][2 * c + i / 8];
+                                    const float mk = fmaxf(mul * s4.x, 1e-37f), a = ex2(fmaf(__uint_as_float(u[2 * i]), mk, off)), b = ex2(fmaf(__uint_as_float(u[2 * i + 1]), mk, off));
+                                    l += a + b;
+                                    hi[i] = half_pair(a * s4.w, b * s4.w);
+                                    if constexpr (SPLIT) lo[i] = half_rest(a * s4.w, b * s4.w, hi[i]);
+                                }
+                                tc_st(pc + c * kPartP, hi);
+                                if constexpr (SPLIT) tc_st(pc + c * kPartP + 16, lo);
+                            }
+                            if constexpr (A::kApart) {
+                                tc_fence_before();
+                                mbar_arrive(&s_free[x]);
+                            }
+                        } else {
+                            uint32_t v[KT / 32][32];
+#pragma unroll
+                            for (int c = 0; c < KT / 32; ++c) tc_ld(sc + c * 32, v[c]);
+#pragma unroll
+                            for (int c = 0; c < KT / 32; ++c) tc_wait_ld(v[c]);
+                            if constexpr (A::kApart) {
+                                tc_fence_before();
+                                mbar_arrive(&s_free[x]);
+                            }
+                            // column 16 s + p of the scores is token 2 (p / 4) + (p & 1) + 8 ((p & 3) / 2) of sub-block s
+                            if (edge) {
+#pragma unroll
+                                for (int c = 0; c < KT / 32; ++c)
+#pragma unroll
+                                    for (int i = 0; i < 32; ++i) {
+                                        const int p = i & 15, token = first + c * 32 + (i & 16) + (p >> 2) * 2 + (p & 1) + ((p & 2) << 2);
+                                        if (token > pos || (P.window && token <= pos - P.window)) v[c][i] = 0xff800000u;
+                                    }
+                            }
+                            float most = kAttFloor;
+#pragma unroll
+                            for (int b = 0; b < SUBS; ++b) {
+                                const float4 s4 = scales[n & 3][b];
+                                auto at = [&](int i) { return __uint_as_float(v[b / 2][b % 2 * 16 + i]); };
+                                float t = max3(at(0), at(1), at(2));
+#pragma unroll
+                                for (int i = 3; i < 15; i += 2) t = max3(t, at(i), at(i + 1));
+                                t = fmaxf(t, at(15));
+                                most = fmaxf(most, fmaf(t, fmaxf(mul * s4.x, 1e-37f), s4.y));
+                            }
+                            if constexpr (A::kApart) {          // the sums, and the place of the weights, are free
+                                if (n_o > 0) att_wait(&o_done[x], (n_o - 1) & 1, P.status);
+                                tc_fence_after();
+                            }
+                            follow(tile, most);
+                            const float base = m - A::kTop;
+                            // exponents of all columns, then the exponentials (scales read between the stores of weights would wait for them)
+#pragma unroll
+                            for (int b = 0; b < SUBS; ++b) {
+                                const float4 s4 = scales[n & 3][b];
+                                const float mk = fmaxf(mul * s4.x, 1e-37f), off = s4.y - base;
+                                const f32x2 mk2 = pack2(mk, mk), off2 = pack2(off, off);
+#pragma unroll
+                                for (int i = 0; i < 16; i += 2) {
+                                    uint32_t *u = &v[b / 2][b % 2 * 16 + i];
+                                    float a, c;
+                                    unpack2(fma2(pack2(__uint_as_float(u[0]), __uint_as_float(u[1])), mk2, off2), a, c);
+                                    u[0] = __float_as_uint(a), u[1] = __float_as_uint(c);
+                                }
+                            }
+                            uint32_t hi[KT / 32][16], lo[SPLIT ? KT / 32 : 1][16];
+#pragma unroll
+                            for (int b = 0; b < SUBS; ++b) {
+                                f32x2 s0 = pack2(0.0f, 0.0f), s1 = s0;
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) {
+                                    const float a = ex2(__uint_as_float(v[b / 2][b % 2 * 16 + 2 * i])), c = ex2(__uint_as_float(v[b / 2][b % 2 * 16 + 2 * i + 1]));
+                                    if (i & 1) s1 = add2(s1, pack2(a, c));
+                                    else s0 = add2(s0, pack2(a, c));
+                                    hi[b / 2][b % 2 * 8 + i] = half_pair(a, c);
+                                    if constexpr (SPLIT) lo[b / 2][b % 2 * 8 + i] = half_rest(a, c, hi[b / 2][b % 2 * 8 + i]);
+                                }
+                                float a, c;
+                                unpack2(add2(s0, s1), a, c);
+                                l = fmaf(a + c, scales[n & 3][b].z, l);
+                            }
+#pragma unroll
+                            for (int c = 0; c < KT / 32; ++c) {
+                                tc_st(pc + c * kPartP, hi[c]);
+                                if constexpr (SPLIT) tc_st(pc + c * kPartP + 16, lo[c]);
+                            }
+                        }
+                        tc_wait_st();
+                        tc_fence_before();
+                        mbar_arrive(&p_full[x]);
+                        ++n_o;
+                    }
+                    // a chain's end: its sums are added to those of the chains in front of it
+                    if (tile < it.hi) {
+                        int of = x * 128 + r;
+                        asm volatile("" : "+r"(of));          // (addresses are made here, not held through the tiles)
+                        const int place = runs > 1 ? it.at : blockIdx.x;
+                        const bool more = tile - it.lo > A::kChain;
+                        float *held_m = &prompt_part_end<D, A::kRows>(P.part, place, of)->x;
+                        const float f = more ? ex2(*held_m - m) : 0.0f;         // (m does not go down)
+                        *held_m = m;
+                        float4 h[8];
+                        auto ask = [&](int c) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) h[i] = more ? *reinterpret_cast<const float4 *>(prompt_part<D, A::kRows>(P.part, place, of, c + 4 * i)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        };
+                        ask(0);
+                        att_wait(&o_done[x], (n_o - 1) & 1, P.status);
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t u[32];
+                            tc_ld(oc + c, u);
+                            tc_wait_ld(u);
+                            float4 y[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                y[i] = make_float4(fmaf(h[i].x, f, __uint_as_float(u[4 * i])), fmaf(h[i].y, f, __uint_as_float(u[4 * i + 1])),
+                                                   fmaf(h[i].z, f, __uint_as_float(u[4 * i + 2])), fmaf(h[i].w, f, __uint_as_float(u[4 * i + 3])));
+                            if (c + 32 < D) ask(c + 32);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) *reinterpret_cast<float4 *>(prompt_part<D, A::kRows>(P.part, place, of, c + 4 * i)) = y[i];
+                        }
+                        tc_fence_before();
+                    }
+                }
+            };
+            if (kv_far_apart(P.reach[it.head])) tiles(std::true_type{});
+            else tiles(std::false_type{});
             if (it.lo < it.hi) att_wait(&o_done[x], (n_o - 1) & 1, P.status);
             tc_fence_after();
             const bool held = it.hi - it.lo > A::kChain;
@@ -634,7 +693,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
                 if (is) *prompt_part_end<D, A::kRows>(P.part, place, of) = make_float2(m, l);         // (of an empty run nothing else is read)
                 continue;
             }
-            const float inv = A::kUnit / l;
+            const float inv = kAttUnit / l;
             const size_t dst = static_cast<size_t>(it.row0 + row / g_heads) * P.out_stride + elem;
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
@@ -700,12 +759,12 @@ __global__ void __launch_bounds__(256) kv_prompt_join_kernel(const __grid_consta
         for (int k = 0; k < runs; ++k) {
             const float2 z = *prompt_part_end<D, ROWS>(P.part, at + k, r);
             const float4 y = *reinterpret_cast<const float4 *>(prompt_part<D, ROWS>(P.part, at + k, r, c));
-            const float f = z.y != 0.0f ? ex2(z.x - top) : 0.0f;        // (an empty run has no sums)
-            if (f == 0.0f) continue;
-            den = fmaf(z.y, f, den);
+            if (z.y == 0.0f) continue;          // (an empty run has no sums)
+            const float half_way = ex2(0.5f * (z.x - top)), f = half_way * half_way;
+            den += z.y * half_way * half_way;
             sum.x = fmaf(y.x, f, sum.x), sum.y = fmaf(y.y, f, sum.y), sum.z = fmaf(y.z, f, sum.z), sum.w = fmaf(y.w, f, sum.w);
         }
-        const float inv = (P.type == kRowsF32 ? PromptAttPlan<D, true>::kUnit : PromptAttPlan<D, false>::kUnit) / den;
+        const float inv = kAttUnit / den;
         const size_t to = static_cast<size_t>(it.row0 + row / g_heads) * P.out_stride + (static_cast<size_t>(it.head) * g_heads + row % g_heads) * D + c;
         row_store(P.out, P.type, to, sum.x * inv);
         row_store(P.out, P.type, to + 1, sum.y * inv);
