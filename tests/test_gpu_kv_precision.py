@@ -112,3 +112,19 @@ def test_values_of_another_size_that_are_gone(was, kernel, heads, count):
     got, want = run(p, p.rand(count, heads, 64) * 0.125, k, v, kernel)
     # scores of at most 5 5 64 / 8, off by 2^-22 of that; norms over values of either sign, whose sums are a part of them
     assert np.linalg.norm(got - want) <= 2.0 ** -13 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("kernel,heads,count", KERNELS)
+def test_queries_whose_elements_are_far_apart(dtype, kernel, heads, count):
+    """One element of the queries is 3e6 times the others, and meets keys of 0: scores are the others' alone (about 2.5 in size), and exact but for F32 sums.
+
+    Elements are off by 2^-40 of the largest: 64 30000 2^-40 30 4 / 8 of a score, 2^-14; weights by 2^-11 each way for rows of 16 bits; sums as above."""
+    n = 1200 + count
+    p = Pair(heads, 2, 64, 32, 0, dtype, n_pages=400, layers=1)
+    q, k, v = p.rand(count, heads, 64) * 0.01, p.rand(n, 2, 64) * 30, p.rand(n, 2, 64)
+    q[..., 7], k[..., 7] = 30000.0, 0.0
+    t = TYPES[dtype][0]
+    got, want = run(p, q.to(t), k.to(t), v.to(t), kernel)
+    values = np.abs(v.double().numpy()).max()
+    assert np.abs(got - want).max() <= (2.0 ** -12 + (0.0 if dtype == "f32" else 2.0 ** -10) + 2.0 ** -14 + HALF_STEP[dtype]) * values

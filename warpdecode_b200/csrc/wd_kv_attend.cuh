@@ -2,7 +2,8 @@
 //
 //   out[r] = sum_j p_j cv_j sv_j / sum_j p_j,   p_j = 2^(x_j - m),   x_j = (q[r] . ck_j) (2^e scale log2(e) sk_j)
 //
-// q is brought to F16 row by row: q = 2^e (hi + lo) with |hi| <= 1, lo = 0 unless the rows are F32; codes are exact in F16; sums are F32.
+// q is brought to F16 row by row: q = 2^e (hi + lo) with |hi| <= 2^15, lo = 0 unless the rows are F32; codes are exact in F16; sums are F32. (2^15 for the
+// row's largest element, so that one that is far smaller is not rounded away at F16's lower end: elements are off by 2^-40 of the largest at most.)
 // Weights: m is the running maximum of x_j + log2(sv_j). E_j = 2^(7 + x_j - m) makes the denominator, P_j = E_j (2^6 sv_j) <= 2^13 meets the codes (F16,
 // hi + lo for F32 rows); the answer is 2^-6 sum P_j cv_j / sum E_j. So a page whose values are small loses nothing beside one whose values are large
 // unless its part of the sum is small, and its tokens' weights are counted whatever their values. Within F32: E_j is at least 2^-79 for the token
@@ -353,7 +354,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
             for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int e = top > 0.0f ? max(-100, min(128, static_cast<int>(__float_as_uint(top) >> 23) - 126)) : 0, e1 = e / 2, e2 = e - e1;
+            const int e = top > 0.0f ? max(-100, min(128, static_cast<int>(__float_as_uint(top) >> 23) - 126)) - 15 : 0, e1 = e / 2, e2 = e - e1;
             const float up = __uint_as_float((127 + e1) << 23), up2 = __uint_as_float((127 + e2) << 23), down = __uint_as_float((127 - e1) << 23),
                         down2 = __uint_as_float((127 - e2) << 23), mine = P.scale_log2 * up * up2;
             mul[n][0] = __shfl_sync(0xffffffffu, mine, 8 * t);

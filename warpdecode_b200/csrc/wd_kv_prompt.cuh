@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(y[i]));
             }
-            const int e = top > 0.0f ? max(-100, min(128, static_cast<int>(__float_as_uint(top) >> 23) - 126)) : 0, e1 = e / 2, e2 = e - e1;
+            const int e = top > 0.0f ? max(-100, min(128, static_cast<int>(__float_as_uint(top) >> 23) - 126)) - 15 : 0, e1 = e / 2, e2 = e - e1;
             const float mul = P.scale_log2 * __uint_as_float((127 + e1) << 23) * __uint_as_float((127 + e2) << 23);
             const float down = __uint_as_float((127 - e1) << 23), down2 = __uint_as_float((127 - e2) << 23);
             uint8_t *to = qs + x * A::kQTile + r * 16;
