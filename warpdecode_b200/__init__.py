@@ -612,6 +612,19 @@ def _ints(values):
     return a, at, n
 
 
+def _fit(*numbers):
+    """Numbers of 32 bits (ctypes would cut what is beyond off)."""
+    for n in numbers:
+        if not -0x80000000 <= n <= 0x7fffffff:
+            raise ValueError("a whole number of 32 bits is wanted, not %r" % (n,))
+
+
+def _fit64(*numbers):
+    for n in numbers:
+        if not -(1 << 63) <= n < 1 << 63:
+            raise ValueError("a whole number of 64 bits is wanted, not %r" % (n,))
+
+
 class KvCache:
     """Keys and values in 8 bits, in pages that sequences share, and attention over them (wd_kv_*). device=-1: the host's part alone.
 
@@ -619,8 +632,9 @@ class KvCache:
     of F32, F16 or BF16; a stride is in elements, 0 = rows lie one behind the other."""
 
     def __init__(self, n_layers, n_heads, n_kv_heads, head_dim, n_pages, max_seqs, max_context, page_tokens=64, codes=KV_INT8, device=0):
-        self.cfg = KvConfig(n_layers, n_heads, n_kv_heads, head_dim, page_tokens, n_pages, max_seqs, max_context, codes, device)
         self.h = C.c_void_p()
+        _fit(n_layers, n_heads, n_kv_heads, head_dim, page_tokens, n_pages, max_seqs, max_context, codes, device)
+        self.cfg = KvConfig(n_layers, n_heads, n_kv_heads, head_dim, page_tokens, n_pages, max_seqs, max_context, codes, device)
         _check(lib().wd_kv_create(C.byref(self.cfg), C.byref(self.h)))
 
     def begin(self, seqs, counts, stream=None):
@@ -632,18 +646,25 @@ class KvCache:
         _check(lib().wd_kv_begin(self.h, n, s_at, c_at, stream))
 
     def append(self, layer, k_ptr, v_ptr, type=TYPE_F32, k_stride=0, v_stride=0, stream=None):
+        if (layer | type) >> 31 or (k_stride | v_stride) >> 63:        # (no more than this on the way of every call)
+            _fit(layer, type)
+            _fit64(k_stride, v_stride)
         rc = lib().wd_kv_append(self.h, layer, k_ptr, v_ptr, type, k_stride, v_stride, stream)
         if rc:
             _check(rc)
 
     def attend(self, layer, q_ptr, out_ptr, type=TYPE_F32, scale=None, window=0, q_stride=0, out_stride=0, stream=None):
         """out = softmax(scale q k) v of the step's rows (scale: 1 / sqrt(head_dim) by default)."""
+        if (layer | type | window) >> 31 or (q_stride | out_stride) >> 63:
+            _fit(layer, type, window)
+            _fit64(q_stride, out_stride)
         rc = lib().wd_kv_attend(self.h, layer, q_ptr, out_ptr, type, self.cfg.head_dim ** -0.5 if scale is None else scale, window, q_stride, out_stride, stream)
         if rc:
             _check(rc)
 
     def read(self, layer, seqs, firsts, counts, k_ptr, v_ptr, type=TYPE_F32, stream=None):
         """Tokens of sequences as numbers; layer -1: of every layer, one behind the other."""
+        _fit(layer, type)
         s, s_at, n = _ints(seqs)
         f, f_at, nf = _ints(firsts)
         c, c_at, nc = _ints(counts)
@@ -652,15 +673,18 @@ class KvCache:
         _check(lib().wd_kv_read(self.h, layer, n, s_at, f_at, c_at, k_ptr, v_ptr, type, stream))
 
     def fork(self, src, dsts, stream=None):
+        _fit(src)
         d, at, n = _ints(dsts)
         _check(lib().wd_kv_fork(self.h, src, n, at, stream))
 
     def keep(self, seq, first, index, stream=None):
         """Of the tokens from `first` on those at `index` (relative to it, going up) stay and move together."""
+        _fit(seq, first)
         x, at, n = _ints(index)
         _check(lib().wd_kv_keep(self.h, seq, first, n, at, stream))
 
     def truncate(self, seq, length, stream=None):
+        _fit(seq, length)
         _check(lib().wd_kv_truncate(self.h, seq, length, stream))
 
     def free(self, seqs, stream=None):
@@ -668,6 +692,7 @@ class KvCache:
         _check(lib().wd_kv_free(self.h, n, at, stream))
 
     def length(self, seq):
+        _fit(seq)
         n = lib().wd_kv_length(self.h, seq)
         _check(0 if n >= 0 else n)
         return n
@@ -678,6 +703,7 @@ class KvCache:
         return n
 
     def pages(self, seq):
+        _fit(seq)
         n = lib().wd_kv_pages(self.h, seq, None, 0)
         _check(0 if n >= 0 else n)
         a = np.zeros(n, np.int32)
@@ -709,6 +735,8 @@ class KvCache:
 def token_logprobs(logits_ptr, rows, vocab, tokens_ptr=None, logprob_ptr=None, entropy_ptr=None, n_top=0, top_ids_ptr=None, top_logprobs_ptr=None,
                    type=TYPE_F32, stride=0, stream=None):
     """Log probabilities of given tokens, the entropy and the likeliest alternatives of rows of logits, on device buffers (wd_token_logprobs)."""
+    _fit(rows, vocab, n_top, type)
+    _fit64(stride)
     rc = lib().wd_token_logprobs(logits_ptr, type, rows, vocab, stride, tokens_ptr, logprob_ptr, entropy_ptr, n_top, top_ids_ptr, top_logprobs_ptr, stream)
     if rc:
         _check(rc)
