@@ -6,6 +6,7 @@ no CPU fallback: loading fails loudly when the library is missing, and every cal
 library's own error text.
 """
 import ctypes as C
+import fcntl
 import os
 import subprocess
 from array import array
@@ -35,34 +36,47 @@ NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", 
 
 
 def build(force=False, verbose=False):
-    """Compile csrc/ into libwarpdecode_b200.so with nvcc (cross-compiles without a GPU)."""
-    if not force and os.path.exists(LIB_PATH):
-        newest = max(os.path.getmtime(s) for s in SOURCES)
-        if os.path.getmtime(LIB_PATH) >= newest:
-            return LIB_PATH
-    nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+    """Compile csrc/ into libwarpdecode_b200.so with nvcc (cross-compiles without a GPU). Several processes may call it: one builds, the others wait for it."""
+    def fresh():
+        return os.path.exists(LIB_PATH) and os.path.getmtime(LIB_PATH) >= max(os.path.getmtime(s) for s in SOURCES)
+
+    if not force and fresh():
+        return LIB_PATH
     objects = os.path.join(HERE, "build")
     os.makedirs(objects, exist_ok=True)
-    jobs, out = [], ""
+    with open(os.path.join(objects, "lock"), "w") as lock:
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        if force or not fresh():
+            _build(objects, force, verbose)
+    return LIB_PATH
+
+
+def _build(objects, force, verbose):
+    nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+    jobs, out, failed = [], "", False
     for unit, files in UNITS.items():           # side by side; a unit is compiled again when one of its files is newer
         obj = os.path.join(objects, unit + ".o")
         if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(f) for f in files):
             continue
-        cmd = [nvcc] + [f for f in NVCC_FLAGS if f != "-shared"] + (["-Xptxas", "-v"] if verbose else []) + ["-c", "-o", obj, os.path.join(HERE, "csrc", unit + ".cu")]
+        cmd = [nvcc] + [f for f in NVCC_FLAGS if f != "-shared"] + (["-Xptxas", "-v"] if verbose else []) + ["-c", "-o", obj + ".new", os.path.join(HERE, "csrc", unit + ".cu")]
         jobs.append((obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     for obj, job in jobs:
         text, _ = job.communicate()
         out += text
-        if job.returncode != 0 and os.path.exists(obj):
-            os.remove(obj)
-    if any(job.returncode for _, job in jobs):
+        if job.returncode == 0:
+            os.replace(obj + ".new", obj)       # (whole, or not there)
+        else:
+            failed = True
+            if os.path.exists(obj):
+                os.remove(obj)
+    if failed:
         raise RuntimeError("nvcc failed:\n" + out)
-    r = subprocess.run([nvcc] + NVCC_FLAGS + ["-o", LIB_PATH] + [os.path.join(objects, unit + ".o") for unit in UNITS], capture_output=True, text=True)
+    r = subprocess.run([nvcc] + NVCC_FLAGS + ["-o", LIB_PATH + ".new"] + [os.path.join(objects, unit + ".o") for unit in UNITS], capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("nvcc failed:\n" + r.stdout + r.stderr)
+    os.replace(LIB_PATH + ".new", LIB_PATH)
     if verbose:
         print(out)
-    return LIB_PATH
 
 
 class Config(C.Structure):
