@@ -422,7 +422,8 @@ int wd_kv_fork(wd_kv_cache *c, int src, int n, const int *dsts, void *stream);
  * of a tree of drafts, or what an eviction leaves. A page takes the largest scale among the pages that its tokens come from, and codes
  * of smaller ones are rounded anew. Positions inside keys (a rotary embedding) are the caller's. */
 int wd_kv_keep(wd_kv_cache *c, int seq, int first, int n, const int *index, void *stream);
-/* The first `length` tokens stay (a rejected draft); pages behind them become free. wd_kv_free: no token stays. */
+/* The first `length` tokens stay (a rejected draft); pages behind them become free. A last page that is not full keeps the scale that the tokens
+ * behind gave it, and its codes the rounding that came with it. wd_kv_free: no token stays. */
 int wd_kv_truncate(wd_kv_cache *c, int seq, int length, void *stream);
 int wd_kv_free(wd_kv_cache *c, int n, const int *seqs, void *stream);
 /* Tokens of a sequence; pages nobody holds; a sequence's pages (returns how many, writes at most cap). Negative: an error code. */
@@ -431,7 +432,9 @@ int wd_kv_free_pages(const wd_kv_cache *c);
 int wd_kv_pages(const wd_kv_cache *c, int seq, int *pages, int cap);
 /* Name of the kernels that the last wd_kv_attend ran on: one for few rows or one for prompts, whichever is expected to be through first. */
 const char *wd_kv_kernel_name(const wd_kv_cache *c);
-/* Waits for the device, returns its status word and clears it: 0, or 32 where a NaN or an infinity was appended. */
+/* Waits for the device, returns its status word and clears it: 0, or 32 where a NaN or an infinity was appended. WD_E_DEVICE: a wait inside a kernel
+ * ran out (its limit is 1.4 s), and what wd_kv_attend has answered since the last wd_kv_status is void, although the calls returned WD_OK; later calls'
+ * waits are short until the status has been asked for. Such a wait has never been seen to run out; a program that wants to know asks after a step. */
 int wd_kv_status(wd_kv_cache *c, int *status);
 
 /* ---- scoring of tokens ----------------------------------------------------------------------- */

@@ -182,12 +182,11 @@ int flush(wd_kv_cache *c, cudaStream_t s) {
         k.pool_layer = c->pool_layer;
         k.scales_layer = c->scales_layer;
         k.page_bytes = page_bytes;
-        k.n = static_cast<int>(std::min<size_t>(wd::kCopyPairs, c->copies.size() - at));
-        k.n_layers = c->cfg.n_layers;
         k.page_scales = c->cfg.n_kv_heads * 2;
-        std::memcpy(k.pair, c->copies.data() + at, static_cast<size_t>(k.n) * sizeof(int2));
+        const size_t n = std::min<size_t>(wd::kCopyPairs, c->copies.size() - at);
+        std::memcpy(k.pair, c->copies.data() + at, n * sizeof(int2));
         const unsigned x = static_cast<unsigned>(std::min<size_t>(64, (page_bytes / 16 + 1023) / 1024));
-        wd::kv_copy_kernel<<<dim3(x, k.n, k.n_layers), 256, 0, s>>>(k);
+        wd::kv_copy_kernel<<<dim3(x, static_cast<unsigned>(n), c->cfg.n_layers), 256, 0, s>>>(k);
     }
     c->copies.clear();
     for (size_t at = 0; at < c->changed.size();) {

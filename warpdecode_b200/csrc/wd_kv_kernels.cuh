@@ -261,8 +261,8 @@ struct KvCopy {
     uint8_t *pool;
     float *scales;
     size_t pool_layer, scales_layer, page_bytes;
-    int n, n_layers, page_scales;
-    int2 pair[kCopyPairs];      // from, to
+    int page_scales;
+    int2 pair[kCopyPairs];      // from, to; a block of the second index each (the third: layers)
 };
 __global__ void __launch_bounds__(256) kv_copy_kernel(const __grid_constant__ KvCopy P) {
     const int2 pr = P.pair[blockIdx.y];
