@@ -240,9 +240,9 @@ int attend_of(wd_kv_cache *c, wd::KvAttend &p, bool few, cudaStream_t s) {
 
 // Which of the two attention kernels a step takes: the one that is expected to be through first, by what each was measured to take (us):
 //   for few rows   c_f for 64 tokens of a head by 16 rows (8 of heads of 256) and worker: heads of 64 1.8, of 128 in F32 4.2, of 256 1.8
-//   for prompts    3 more, and c_p for 128 tokens by 256 rows (128 of heads of 256) and CTA: heads of 64 1.8, of 128 in F32 3.3, of 256 4.5;
+//   for prompts    3 more, and c_p for 128 tokens by 256 rows (128 of heads of 256) and CTA: heads of 64 1.8, of 128 in F32 3.4, of 256 4.2;
 //                  8 more where items are cut into runs
-// (64 rows a head of 64, 1,000 tokens: 15 against 23 us; 512 rows, 8,000 tokens: 63 against 39.)
+// (64 rows a head of 64, 1,000 tokens: 15 against 23 us; 512 rows, 8,000 tokens: 63 against 39. Heads of 32 and 96 go by the lines through these points.)
 struct Choice {
     bool prompt, split;
 };

@@ -25,8 +25,8 @@
 // hold by the last CTA to arrive, always in the workers' order.
 //
 // Bound: memory for long work. 131,089 tokens of 8 heads of 128: 58 us, 4.6 TB/s of codes (the copy rate's floor is 42); 64 sequences of 90 to 8,000
-// tokens, 8 heads of 64: 46 us, 3.9 TB/s (28): the rest is the way to the first tile and the joining of parts. Short work is a chain of latencies: 131
-// tokens, 4 heads of 64: 10 us, most of them the launch, entry -> table -> page -> tile, and code that an SM fetches for the first time.
+// tokens, 8 heads of 64: 46 us, 3.9 TB/s (28): the rest is the way to the first tile and the joining of parts (DRAM is busy for 56 and 48 % of the
+// launch, issue slots 30 and 47 %, the tensor pipe 13 and 11 %). Short work is a chain of latencies: 131 tokens, 4 heads of 64: 9 to 10 us, most of them the launch, entry -> table -> page -> tile, and code that an SM fetches for the first time.
 #pragma once
 
 #include <type_traits>
@@ -39,7 +39,7 @@ constexpr int kAttWorkers = 8, kAttThreads = 512, kAttMaxSeqs = 1024, kAttMaxRow
 // Registers a thread: the warps that compute take what those that copy give back (128 at launch).
 constexpr int kAttRegsMore = 192, kAttRegsLess = 64;
 static_assert(256 * kAttRegsMore + 256 * kAttRegsLess <= kAttThreads * 128, "more than the block was launched with: the increase would wait for ever");
-constexpr float kAttFloor = -1.0e30f;       // a maximum over nothing
+constexpr float kAttFloor = -1.0e30f;       // a maximum over nothing (scores are below 2^20)
 constexpr int kAttTop = 13, kAttScale = 6;              // exponents: of the largest P_j, of what a value scale is multiplied by (F32's largest scale is below 2^122)
 constexpr float kAttUnit = 1.0f / (1 << kAttScale);
 

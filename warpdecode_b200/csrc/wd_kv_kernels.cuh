@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(256) kv_run_kernel(const __grid_constant__ KvR
 // magnitude, from which the scale follows, then the codes (the rows come from the caches the second time). A page that held tokens before keeps its
 // scale unless the new ones need a larger one; then the codes that are there are rounded anew. Values are turned in shared memory.
 // Bound: instruction issue for a prompt (8,191 tokens of 8 heads of 128, written and read back: 52 us, 1.9 TB/s over both), the chain entry -> table ->
-// scale -> rows for one token of each of 64 sequences (with the step's begin and the reading back 18.5 us).
+// scale -> rows for one token of each of 64 sequences (with the reading back 18.5 us).
 struct KvAppend {
     uint8_t *pool;              // of the layer
     float *scales;              // of the layer

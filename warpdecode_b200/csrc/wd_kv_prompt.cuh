@@ -16,9 +16,9 @@
 // Items are dealt out heaviest first, back and forth over the CTAs (the last rows of a sequence see the most). Where there are not half as many as CTAs
 // each is cut into as many runs of its tokens as fill them, and a second kernel puts the runs' sums together.
 //
-// Bound: heads of 64 by the softmax: one warp on each scheduler takes about 1,900 cycles for 128 columns of a tile, about half of them the exponential
-// unit's. 4,000 rows behind 1,011 tokens, 32 heads over 8: of 64 187 us (530 TFLOP/s), of 128 265 us (745), of 256 436 us (905);
-// F32 rows of 64, with twice the products, 284 us.
+// Bound: heads of 64 by the softmax: the two row tiles' warps on a scheduler take about 4,400 cycles for 128 columns each, 2,048 of them the exponential
+// unit's: they run nearly one after the other. 4,000 rows behind 1,011 tokens, 32 heads over 8: of 64 193 us (510 TFLOP/s; exponential pipe 52 %, tensor pipe
+// 23 %), of 128 276 us (715; 37 and 33 %), of 256 875 us (450); F32 rows, with twice the products, of 64 301 us, of 128 420, of 256 1,317.
 #pragma once
 
 #include "wd_kv_attend.cuh"

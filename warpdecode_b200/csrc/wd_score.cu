@@ -8,10 +8,10 @@
 //
 // The alternatives are collected beside: a key is (order of the value, lowest index first) in 64 bits, a candidate is what is not below the CTA's bar,
 // and each warp has a list of candidates, which it cuts to its n_top best when it is full. The bar is the n_top-th of the maxima of groups of eight
-// threads (to seven bits behind the leading one; of 64 groups the 20th is met by 24 elements, not 20) after the first round, and what one warp finds
-// it to be after 2, 4, 8, ... rounds, so that few elements behind meet it, whatever their order; a warp that cuts its list raises it too.
+// threads after the first round, and what one warp finds it to be after 2, 4, 8, ... rounds, so that few elements behind meet it, whatever their order; a
+// warp that cuts its list raises it too.
 //
-// Bound: memory. 1,000 rows of 128,256 F32 with 20 alternatives: 105 to 116 us, 4.4 to 4.9 TB/s (a copy's rate: 80); what is missing goes to the candidates of a
+// Bound: memory. 1,000 rows of 128,256 F32 with 20 alternatives: 114 us, 4.5 TB/s (a copy's rate: 80); what is missing goes to the candidates of a
 // row's first rounds and to its end. Four rows of 151,936 with 5: 12 us of launch, the first bytes and the cluster's exchange.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
