@@ -128,3 +128,18 @@ def test_queries_whose_elements_are_far_apart(dtype, kernel, heads, count):
     got, want = run(p, q.to(t), k.to(t), v.to(t), kernel)
     values = np.abs(v.double().numpy()).max()
     assert np.abs(got - want).max() <= (2.0 ** -12 + (0.0 if dtype == "f32" else 2.0 ** -10) + 2.0 ** -14 + HALF_STEP[dtype]) * values
+
+
+@pytest.mark.parametrize("kernel,heads,count", KERNELS)
+@pytest.mark.parametrize("was", [1.0, 1e26, 1e33])
+def test_pages_of_zeros_beside_numbers(was, kernel, heads, count):
+    """Pages of zeros have a third of the weight, in a cache that has held values of another size before: the others lose nothing by it."""
+    n = 1200 + count
+    p = Pair(heads, 2, 64, 16, 0, "f32", n_pages=400, layers=1)
+    p.step([0], [100], rows=[(p.rand(100, 2, 64), p.rand(100, 2, 64) * was)])
+    p.kv.free([0])
+    p.ref[0].truncate(0, 0)
+    k, v = torch.zeros(n, 2, 64), p.rand(n, 2, 64).abs() + 0.5
+    v[torch.arange(n) // 16 % 3 == 1] = 0.0
+    got, want = run(p, torch.zeros(count, heads, 64), k, v, kernel)
+    assert np.linalg.norm(got - want) <= TOL * np.linalg.norm(want)

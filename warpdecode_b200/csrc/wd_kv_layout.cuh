@@ -25,11 +25,13 @@ constexpr int kKvStepWords = 8;         // words of a step's entry: sequence, fi
 constexpr int kKvHead = 8;              // words in front of the entries: sequences, rows, page items
 constexpr float kKvLeastScale = 7.888609052210118e-31f;     // 2^-100: keeps 1 / scale and sums of it far inside F32
 
-// whether value scales may be so far apart that a weight times the one is nothing in F32 where that times the other is of size 1; and what may stand for a
-// scale of 0 (nothing but zeros) among them: far below the largest, so that it costs no weight its place, and no farther apart than the others
-__device__ __forceinline__ bool kv_far_apart(int2 reach) { return reach.x && (reach.x - 1024) - (1024 - reach.y) > 90; }
+// Whether value scales may be so far apart that a weight times the one is nothing in F32 where that times the other is of size 1; and what stands for a
+// scale of 0 (nothing but zeros): well below the others, so that its tokens cost no weight its place, and where they are not far apart no farther than that.
+constexpr int kKvFar = 90;
+__device__ __forceinline__ bool kv_far_apart(int2 reach) { return reach.x && (reach.x - 1024) - (1024 - reach.y) > kKvFar; }
 __device__ __forceinline__ float kv_zero_scale(int2 reach) {
-    return __uint_as_float(static_cast<uint32_t>((reach.x ? max(reach.x - 1024, -40) : -40) - 60 + 127) << 23);
+    const int hi = reach.x - 1024, lo = 1024 - reach.y;
+    return reach.x == 0 || hi - lo > kKvFar ? kKvLeastScale : __uint_as_float(static_cast<uint32_t>(max(max(lo - 60, hi - kKvFar), -100) + 127) << 23);
 }
 
 enum : unsigned { kKvNonFinite = 32u };     // status bit: a NaN or an infinity was appended
