@@ -376,7 +376,7 @@ int wd_head_argmax_q8_0(void *packed_dev, int rows, int cols, const float *x_dev
  * stream: a cudaStream_t of the cache's device, NULL = its default stream. wd_kv_append, wd_kv_attend and wd_kv_read can be captured;
  * the others cannot (they are refused), but may come between replays: a replayed append or attend works on the step that is current
  * then, with the launches of the captured one (any step is answered rightly; the captured rows should be about as many), and does
- * nothing where none is.
+ * nothing where none is; a replayed read reads its tokens from the pages that the sequences have then.
  *
  * Rows: [rows][heads][head_dim] of F32, F16 or BF16 (WD_TYPE_*); a stride is the elements from one row to the next, 0 = rows lie
  * one behind the other, so that the parts of a fused q/k/v row can be used where they are. Sums, maxima and scores are F32; F32 rows

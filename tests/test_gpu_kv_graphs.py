@@ -57,3 +57,34 @@ def test_a_replay_behind_the_end_of_a_step_does_nothing(chunk, end):
     want = p.ref[0].attend(1, rows[2][:1].double().numpy(), 0.125, 0)
     assert np.linalg.norm(out[:1].double().cpu().numpy() - want) <= 2.0 ** -16 * np.linalg.norm(want)
     p.check_numbers([0, 1])
+
+
+def test_a_replayed_read_finds_the_pages_that_a_sequence_has_then():
+    p = Pair(4, 2, 64, 16, 0, "f32", layers=2)
+    p.step([0, 1], [40, 40])
+    k, v = (torch.zeros(2, 40, 2, 64, device="cuda") for _ in range(2))
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        p.kv.read(-1, [1], [0], [40], k.data_ptr(), v.data_ptr(), stream=s.cuda_stream)
+
+    def same(seq):
+        with torch.cuda.stream(s):
+            g.replay()
+        s.synchronize()
+        for layer in range(2):
+            assert np.array_equal(np.stack([k[layer].cpu().numpy(), v[layer].cpu().numpy()]), p.ref[layer].numbers(seq)[:, :40].astype(np.float32))
+
+    same(1)
+    p.kv.free([1], s.cuda_stream)
+    p.kv.fork(0, [1], s.cuda_stream)            # nothing else is called before the replay
+    same(0)
+    for r in p.ref:
+        r.truncate(1, 0)
+        r.fork(0, 1)
+    torch.cuda.synchronize()
+    p.step([1, 0], [5, 30])
+    same(1)
+    p.kv.truncate(1, 41, s.cuda_stream)
+    same(1)

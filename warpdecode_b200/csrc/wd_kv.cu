@@ -46,7 +46,7 @@ struct wd_kv_cache {
     int2 *d_reach = nullptr;
     size_t pool_layer = 0, scales_layer = 0;
     const char *last_kernel = "";           // of wd_kv_attend
-    bool graphs = false;                    // an append or an attend has been captured: replays look for the step in the device's book
+    bool graphs = false;                    // a call has been captured: replays look for the step and the pages in the device's book
     bool broken = false;                    // a launch failed half-way: mirror and device may differ
 
     bool host_only() const { return cfg.device < 0; }
@@ -133,22 +133,20 @@ int check_device(const wd_kv_cache *c) {
     return WD_OK;
 }
 
-// Changes that no kernel reads before the next begin, read or keep wait for it: pages change hands only there.
-int later(wd_kv_cache *c) {
+int flush(wd_kv_cache *c, cudaStream_t s);
+// Changes that no kernel reads before the next begin, read or keep wait for it (pages change hands only there), unless replays of captured calls may come before:
+// they look for the step and for the sequences' pages in the device's book.
+int later(wd_kv_cache *c, cudaStream_t s) {
     if (c->host_only()) {
         for (int at : c->changed) c->dirty[at] = 0;
         c->changed.clear();
+        return WD_OK;
     }
-    return WD_OK;
-}
-int flush(wd_kv_cache *c, cudaStream_t s);
-// The end of a step waits likewise, unless replays of captured calls may come before: they are not to find it any more.
-int step_ended(wd_kv_cache *c, cudaStream_t s) {
-    if (!c->graphs) return later(c);
+    if (!c->graphs) return WD_OK;
     OnDevice on(c->cfg.device);
     return flush(c, s);
 }
-// Whether the call becomes part of a graph; then the cache's steps end on the device too.
+// Whether the call becomes part of a graph; then changes do not wait.
 int note_capture(wd_kv_cache *c, cudaStream_t s) {
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
     WD_TRY_CUDA(cudaStreamIsCapturing(s, &st));
@@ -171,7 +169,7 @@ void send_words(wd_kv_cache *c, size_t from, cudaStream_t s) {
 int flush(wd_kv_cache *c, cudaStream_t s) {
     if (c->host_only()) {
         c->copies.clear();
-        return later(c);
+        return later(c, s);
     }
     c->broken = true;
     const size_t page_bytes = wd::kv_page_bytes(c->shape);
@@ -562,6 +560,7 @@ int wd_kv_read(wd_kv_cache *c, int layer, int n, const int *seqs, const int *fir
         if (!c->changed.empty())
             if (int rc = check_not_captured(c, s)) return rc;
         OnDevice on(c->cfg.device);
+        if (int rc = note_capture(c, s)) return rc;
         if (int rc = flush(c, s)) return rc;
         const size_t width = static_cast<size_t>(c->cfg.n_kv_heads) * c->cfg.head_dim;
         const int layers = layer < 0 ? c->cfg.n_layers : 1;
@@ -620,7 +619,7 @@ int wd_kv_fork(wd_kv_cache *c, int src, int n, const int *dsts, void *stream) {
                 c->set_page(dsts[i], static_cast<int>(j), from.pages[j]);
             }
         }
-        return later(c);
+        return later(c, s);
     });
 }
 
@@ -634,7 +633,7 @@ int wd_kv_truncate(wd_kv_cache *c, int seq, int length, void *stream) {
         c->changed.reserve(c->changed.size() + 3);
         c->cut(c->seqs[seq], length);
         c->end_step();
-        return step_ended(c, s);
+        return later(c, s);
     });
 }
 
@@ -648,7 +647,7 @@ int wd_kv_free(wd_kv_cache *c, int n, const int *seqs, void *stream) {
         c->changed.reserve(c->changed.size() + 3);
         for (int i = 0; i < n; ++i) c->cut(c->seqs[seqs[i]], 0);
         c->end_step();
-        return step_ended(c, s);
+        return later(c, s);
     });
 }
 
@@ -670,7 +669,7 @@ int wd_kv_keep(wd_kv_cache *c, int seq, int first, int n, const int *index, void
             c->changed.reserve(c->changed.size() + 3);
             c->cut(q, end);
             c->end_step();
-            return step_ended(c, s);
+            return later(c, s);
         }
         const int page0 = from / c->page_tokens(), pages = c->pages_for(end) - page0;
         // Into new pages, all at once, where there are enough of them; else in place, page by page, but never into a page that others hold.
@@ -748,7 +747,7 @@ int wd_kv_keep(wd_kv_cache *c, int seq, int first, int n, const int *index, void
         }
         c->cut(q, end);
         c->end_step();
-        return c->host_only() ? later(c) : flush(c, s);
+        return c->host_only() ? later(c, s) : flush(c, s);
     });
 }
 
