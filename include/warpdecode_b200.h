@@ -379,11 +379,11 @@ int wd_head_argmax_q8_0(void *packed_dev, int rows, int cols, const float *x_dev
  * nothing where none is; a replayed read reads its tokens from the pages that the sequences have then.
  *
  * Rows: [rows][heads][head_dim] of F32, F16 or BF16 (WD_TYPE_*); a stride is the elements from one row to the next, 0 = rows lie
- * one behind the other, so that the parts of a fused q/k/v row can be used where they are. Sums, maxima and scores are F32; F32 rows
- * are answered to about 2^-20 of the values' size by the kernel for few rows, to 2^-15 by the one for prompts (tensor cores cut long sums
- * of one sign off), F16 and BF16 rows to their own rounding. A weight counts down to 2^-38 of its row's largest (rows of 16 bits in the kernel
- * for prompts: 2^-34): less is rounded to one of these steps. Scores (scale q k) are taken to be below 2^20, beyond which F32 tells their
- * exponentials no longer apart; a row with larger ones may be answered with NaN. */
+ * one behind the other, so that the parts of a fused q/k/v row can be used where they are. Sums, maxima and scores are F32. F32 rows are
+ * answered to about 2^-20 of the values' size (the largest that the pages they see can hold) by the kernel for few rows, to 2^-15 by the
+ * one for prompts (tensor cores cut long sums of one sign off), F16 and BF16 rows to their own rounding. A weight counts down to 2^-38 of
+ * its row's largest (rows of 16 bits in the kernel for prompts: 2^-34): less is rounded to one of these steps. Scores (scale q k) are taken
+ * to be below 2^20, beyond which F32 tells their exponentials no longer apart; a row with larger ones may be answered with NaN. */
 #define WD_KV_INT8 0
 #define WD_KV_E4M3 1
 typedef struct {
