@@ -18,7 +18,7 @@
 //
 // Bound: heads of 64 by the softmax: the two row tiles' warps on a scheduler take about 4,400 cycles for 128 columns each, 2,048 of them the exponential
 // unit's: they run nearly one after the other. 4,000 rows behind 1,011 tokens, 32 heads over 8: of 64 193 us (510 TFLOP/s; exponential pipe 52 %, tensor pipe
-// 23 %), of 128 276 us (715; 37 and 33 %), of 256 875 us (450); F32 rows, with twice the products, of 64 301 us, of 128 420, of 256 1,317.
+// 23 %), of 128 275 us (717; 37 and 33 %), of 256 893 us (442); F32 rows, with twice the products, of 64 301 us, of 128 420, of 256 1,312.
 #pragma once
 
 #include "wd_kv_attend.cuh"
