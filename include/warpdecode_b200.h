@@ -373,7 +373,7 @@ int wd_head_argmax_q8_0(void *packed_dev, int rows, int cols, const float *x_dev
  *
  * Which sequence holds which pages is kept on the host (calls fail there, with nothing changed) and sent to the device in the
  * stream's order: calls of one cache are made from one host thread at a time and on one stream, or on streams that the caller orders.
- * stream: a cudaStream_t of the cache's device, NULL = its default stream. wd_kv_append, wd_kv_attend and wd_kv_read can be captured;
+ * stream: a cudaStream_t of the cache's device, NULL = its default stream. wd_kv_append, wd_kv_append_rope, wd_kv_attend and wd_kv_read can be captured;
  * the others cannot (they are refused), but may come between replays: a replayed append or attend works on the step that is current
  * then, with the launches of the captured one (any step is answered rightly; the captured rows should be about as many), and does
  * nothing where none is; a replayed read reads its tokens from the pages that the sequences have then.
@@ -408,6 +408,38 @@ void wd_kv_destroy(wd_kv_cache *c);
 int wd_kv_begin(wd_kv_cache *c, int n, const int *seqs, const int *counts, void *stream);
 /* Keys and values of the step's rows into a layer. The same rows again leave the cache as it is. */
 int wd_kv_append(wd_kv_cache *c, int layer, const void *k_dev, const void *v_dev, int type, int64_t k_stride, int64_t v_stride, void *stream);
+/* Rotary positions of heads: pair p of the first rotary_dim elements of a head turns by the angle position * f_p, f_p = theta^(-2p / rotary_dim), or inv_freq[p]
+ * (host, rotary_dim / 2 of them; null: from theta): (x0, x1) -> factor (x0 cos - x1 sin, x1 cos + x0 sin). With several axes (time, height, width of a picture's or a
+ * film's tokens) a token has a position on each, and the first sections[0] pairs go by the first, the next sections[1] by the second, and so on; they are
+ * rotary_dim / 2 together. Angles are made in 64 bits. The handle is host memory only, belongs to no device, and may serve several caches and threads. */
+#define WD_ROPE_HALVES 0        /* element p with element p + rotary_dim / 2 */
+#define WD_ROPE_NEIGHBOURS 1    /* element 2p with element 2p + 1 */
+typedef struct {
+    int32_t head_dim;
+    int32_t rotary_dim;     /* even, 2 to head_dim (0: head_dim); the elements behind are not turned */
+    int32_t pairs;          /* WD_ROPE_* */
+    int32_t n_axes;         /* 1 (or 0) to 4 */
+    int32_t sections[4];    /* of several axes */
+    float theta;
+    float factor;           /* 1, or what a scaled context multiplies the rotated elements by */
+} wd_rope_config;
+typedef struct wd_rope wd_rope;
+int wd_rope_create(const wd_rope_config *cfg, const double *inv_freq, wd_rope **out);
+void wd_rope_destroy(wd_rope *r);
+/* A step's rows on their way through the norms of heads and the rotation. Strides as above. */
+typedef struct {
+    const int32_t *positions_dev;       /* [rows][n_axes]; null: every token's own place in its sequence, on all axes */
+    const float *q_norm_dev, *k_norm_dev;       /* [head_dim]: x -> x w / sqrt(mean x^2 + eps) in front of the rotation; null: no norm */
+    const void *k_dev, *v_dev;
+    const void *q_dev;                  /* null, with its output: only k and v */
+    void *q_out_dev;                    /* may be q, with the same stride */
+    int64_t q_stride, q_out_stride, k_stride, v_stride;
+    float eps;                          /* positive, where there is a norm */
+    int32_t type;
+} wd_rope_rows;
+/* As wd_kv_append, k with its norm and rotation on the way (in 64 bits, rounded to F32 once, then to codes), and q with its own into q_out (in F32, rounded
+ * to the rows' type). v as it is. An infinity or a NaN in k makes numbers that are none of its pair, or with a norm of its head. Can be captured, as wd_kv_append can. */
+int wd_kv_append_rope(wd_kv_cache *c, int layer, const wd_rope *r, const wd_rope_rows *rows, void *stream);
 /* out = softmax(scale q k) v of the step's rows, each against the tokens up to its own (which must have been appended), or the last
  * `window` of them (0 = all). Row i of a sequence's n rows is the token n - 1 - i before its last. out may be q, with the same stride; they
  * do not overlap otherwise. */

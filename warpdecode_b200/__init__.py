@@ -20,11 +20,19 @@ SOURCES = [os.path.join(HERE, "csrc", f) for f in
            ("wd_engine.cu", "wd_aux_kernels.cuh", "wd_moe_kernel.cuh", "wd_moe_kernel_phases.inc", "wd_moe_fast.cuh", "wd_moe_batch.cuh", "wd_dense_decoder.cuh", "wd_dense_decoder.inc", "wd_dense_token.cuh", "wd_dense_prefill.cuh", "wd_dense_prompt_tc.cuh",
             "wd_plain_moe.cuh", "wd_plain_wide.cuh", "wd_plain_moe.inc", "wd_blocks.cuh", "wd_router.cuh",
             "wd_formats.cuh", "wd_device.cuh", "wd_dense.cuh", "wd_gguf.inc",
-            "wd_grids.h", "wd_host.h", "wd_tcgen05.cuh", "wd_kv.cu", "wd_kv_layout.cuh", "wd_kv_kernels.cuh", "wd_kv_attend.cuh", "wd_kv_prompt.cuh", "wd_score.cu")] + [
+            "wd_grids.h", "wd_host.h", "wd_tcgen05.cuh", "wd_kv.cu", "wd_kv_rope.cu", "wd_kv_host.h", "wd_kv_launch.cuh", "wd_kv_layout.cuh", "wd_kv_append.cuh", "wd_kv_kernels.cuh", "wd_kv_attend.cuh", "wd_kv_prompt.cuh", "wd_score.cu")] + [
                os.path.join(ROOT, "include", "warpdecode_b200.h")]
+_HOST = ("wd_device", "wd_host", "warpdecode")
+
+
+def _files(*starts):
+    return [s for s in SOURCES if os.path.basename(s).startswith(starts + _HOST)]
+
+
 UNITS = {"wd_engine": [s for s in SOURCES if not os.path.basename(s).startswith(("wd_kv", "wd_score"))],        # translation units, and what they include
-         "wd_kv": [s for s in SOURCES if os.path.basename(s).startswith(("wd_kv", "wd_device", "wd_tcgen05", "wd_host", "warpdecode"))],
-         "wd_score": [s for s in SOURCES if os.path.basename(s).startswith(("wd_score", "wd_device", "wd_host", "warpdecode"))]}
+         "wd_kv": _files("wd_kv.", "wd_kv_host", "wd_kv_launch", "wd_kv_layout", "wd_kv_append", "wd_kv_kernels", "wd_kv_attend", "wd_kv_prompt", "wd_tcgen05"),
+         "wd_kv_rope": _files("wd_kv_rope", "wd_kv_host", "wd_kv_layout", "wd_kv_append"),
+         "wd_score": _files("wd_score")}
 
 TYPE_F16, TYPE_BF16 = 1, 30
 KV_INT8, KV_E4M3 = 0, 1
@@ -97,6 +105,15 @@ class DenseConfig(C.Structure):
 class KvConfig(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("n_layers", "n_heads", "n_kv_heads", "head_dim", "page_tokens", "n_pages", "max_seqs", "max_context",
                                          "codes", "device")]
+
+
+class RopeConfig(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("head_dim", "rotary_dim", "pairs", "n_axes")] + [("sections", C.c_int32 * 4), ("theta", C.c_float), ("factor", C.c_float)]
+
+
+class RopeRows(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("positions", "q_norm", "k_norm", "k", "v", "q", "q_out")] + \
+               [(n, C.c_int64) for n in ("q_stride", "q_out_stride", "k_stride", "v_stride")] + [("eps", C.c_float), ("type", C.c_int32)]
 
 
 _lib = None
@@ -189,6 +206,10 @@ def lib():
         L.wd_kv_destroy.restype = None
         L.wd_kv_begin.argtypes = [vp, i, vp, vp, vp]
         L.wd_kv_append.argtypes = [vp, i, vp, vp, i, i64, i64, vp]
+        L.wd_rope_create.argtypes = [C.POINTER(RopeConfig), vp, C.POINTER(vp)]
+        L.wd_rope_destroy.argtypes = [vp]
+        L.wd_rope_destroy.restype = None
+        L.wd_kv_append_rope.argtypes = [vp, i, vp, C.POINTER(RopeRows), vp]
         L.wd_kv_attend.argtypes = [vp, i, vp, vp, i, C.c_float, i, i64, i64, vp]
         L.wd_kv_read.argtypes = [vp, i, i, vp, vp, vp, vp, vp, i, vp]
         L.wd_kv_fork.argtypes = [vp, i, i, vp, vp]
@@ -639,6 +660,35 @@ def _fit64(*numbers):
             raise ValueError("a whole number of 64 bits is wanted, not %r" % (n,))
 
 
+class Rope:
+    """Rotary positions of heads (wd_rope_*): pairs of elements turn by position * theta^(-2p / rotary_dim), or by position * inv_freq[p].
+
+    sections: how many of the rotary_dim / 2 pairs go by each of several axes (2 to 4); none: one axis. neighbours: pairs are elements 2p and 2p + 1, not p and
+    p + rotary_dim / 2."""
+
+    def __init__(self, head_dim, rotary_dim=0, theta=10000.0, sections=(), neighbours=False, factor=1.0, inv_freq=None):
+        self.h = C.c_void_p()
+        _fit(head_dim, rotary_dim, *sections)
+        if len(sections) == 1 or len(sections) > 4:
+            raise ValueError("sections of 2 to 4 axes, or none")
+        cfg = RopeConfig(head_dim, rotary_dim, int(neighbours), max(1, len(sections)), (C.c_int32 * 4)(*sections), theta, factor)
+        freq = None if inv_freq is None else np.ascontiguousarray(inv_freq, np.float64)
+        if freq is not None and freq.shape != ((rotary_dim or head_dim) // 2,):
+            raise ValueError("one frequency for each of rotary_dim / 2 pairs")
+        _check(lib().wd_rope_create(C.byref(cfg), _ptr(freq), C.byref(self.h)))
+
+    def close(self):
+        if self.h:
+            lib().wd_rope_destroy(self.h)
+            self.h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class KvCache:
     """Keys and values in 8 bits, in pages that sequences share, and attention over them (wd_kv_*). device=-1: the host's part alone.
 
@@ -664,6 +714,17 @@ class KvCache:
             _fit(layer, type)
             _fit64(k_stride, v_stride)
         rc = lib().wd_kv_append(self.h, layer, k_ptr, v_ptr, type, k_stride, v_stride, stream)
+        if rc:
+            _check(rc)
+
+    def append_rope(self, layer, rope, k_ptr, v_ptr, q_ptr=None, q_out_ptr=None, positions_ptr=None, q_norm_ptr=None, k_norm_ptr=None, eps=1e-6, type=TYPE_F32,
+                    q_stride=0, q_out_stride=0, k_stride=0, v_stride=0, stream=None):
+        """append with the norm and the rotation of k on the way, and of q into q_out. positions: int32 [rows][axes], by default the tokens' own places."""
+        if (layer | type) >> 31 or (q_stride | q_out_stride | k_stride | v_stride) >> 63:
+            _fit(layer, type)
+            _fit64(q_stride, q_out_stride, k_stride, v_stride)
+        rows = RopeRows(positions_ptr, q_norm_ptr, k_norm_ptr, k_ptr, v_ptr, q_ptr, q_out_ptr, q_stride, q_out_stride, k_stride, v_stride, eps, type)
+        rc = lib().wd_kv_append_rope(self.h, layer, rope.h, C.byref(rows), stream)
         if rc:
             _check(rc)
 

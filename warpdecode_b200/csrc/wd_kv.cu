@@ -1,137 +1,17 @@
 // Host side of the 8-bit key/value cache (wd_kv_*): which sequence holds which pages, the step, and the launches.
-#include <algorithm>
-#include <cmath>
 #include <climits>
-#include <memory>
-#include <type_traits>
+#include <cmath>
 #include <cstring>
+#include <memory>
 #include <unordered_map>
-#include <vector>
 
-#include "wd_host.h"
-#include "wd_kv_attend.cuh"
+#include "wd_kv_append.cuh"
 #include "wd_kv_kernels.cuh"
-#include "wd_kv_prompt.cuh"
+#include "wd_kv_launch.cuh"
 
-using wd_host::OnDevice;
-using wd_host::set_error;
-
-namespace {
-
-struct Sequence {
-    std::vector<int> pages;
-    int length = 0;
-};
-
-}  // namespace
-
-// The device's book (wd_kv_layout.cuh) has a mirror here; a call changes the mirror and sends the words that differ.
-struct wd_kv_cache {
-    wd_kv_config cfg{};
-    wd::KvShape shape{};
-    std::vector<Sequence> seqs;
-    std::vector<int> holders;               // of each page
-    std::vector<int> free_pages;            // last one goes first
-    std::vector<int> book;
-    std::vector<int> changed;               // words to send, each of them once
-    std::vector<char> dirty;                // those in `changed`
-    std::vector<int2> copies;               // pages to copy: from, to
-    int table_at = 0, rows = 0, max_rows = 0, items = 0;        // rows of the step, the most of one sequence's, page items
-
-    int n_sm = 0;
-    uint8_t *d_pool = nullptr;
-    float *d_scales = nullptr, *d_part = nullptr, *d_cta_part = nullptr;
-    int *d_book = nullptr, *d_index = nullptr;
-    unsigned *d_arrived = nullptr, *d_status = nullptr;
-    int2 *d_reach = nullptr;
-    size_t pool_layer = 0, scales_layer = 0;
-    const char *last_kernel = "";           // of wd_kv_attend
-    bool graphs = false;                    // a call has been captured: replays look for the step and the pages in the device's book
-    bool broken = false;                    // a launch failed half-way: mirror and device may differ
-
-    bool host_only() const { return cfg.device < 0; }
-    int page_tokens() const { return cfg.page_tokens; }
-    int pages_for(int tokens) const { return (tokens + cfg.page_tokens - 1) / cfg.page_tokens; }
-
-    void set(size_t at, int value) {
-        if (book[at] == value) return;
-        book[at] = value;
-        if (dirty[at]) return;
-        dirty[at] = 1;
-        changed.push_back(static_cast<int>(at));
-    }
-    void set_page(int seq, int i, int page) { set(table_at + static_cast<size_t>(seq) * shape.max_pages + i, page); }
-    int take_page() {
-        const int p = free_pages.back();
-        free_pages.pop_back();
-        holders[p] = 1;
-        return p;
-    }
-    void release(int page) {
-        if (--holders[page] == 0) free_pages.push_back(page);
-    }
-    void cut(Sequence &s, int length) {
-        const int keep = pages_for(length);
-        while (static_cast<int>(s.pages.size()) > keep) {
-            release(s.pages.back());
-            s.pages.pop_back();
-        }
-        s.length = length;
-    }
-    void end_step() {
-        set(0, 0);
-        set(1, 0);
-        set(2, 0);
-        rows = max_rows = items = 0;
-    }
-};
+using namespace wd_kv;
 
 namespace {
-
-int check_seq(const wd_kv_cache *c, int seq) {
-    if (seq < 0 || seq >= c->cfg.max_seqs)
-        return set_error(WD_E_INVALID, "key/value cache: sequence " + std::to_string(seq) + " of " + std::to_string(c->cfg.max_seqs));
-    return WD_OK;
-}
-
-int rows_type(int type, int *out) {
-    if (type == WD_TYPE_F32) *out = wd::kRowsF32;
-    else if (type == WD_TYPE_F16) *out = wd::kRowsF16;
-    else if (type == WD_TYPE_BF16) *out = wd::kRowsBF16;
-    else return set_error(WD_E_INVALID, "key/value cache: rows are F32, F16 or BF16");
-    return WD_OK;
-}
-size_t rows_size(int type) { return type == wd::kRowsF32 ? 4 : 2; }
-
-int check_rows(const void *p, size_t size, long long *stride, long long least, const char *what) {
-    if (!p) return set_error(WD_E_INVALID, std::string("key/value cache: ") + what + " is null");
-    if (reinterpret_cast<uintptr_t>(p) % size) return set_error(WD_E_INVALID, std::string("key/value cache: ") + what + " is not aligned to its type");
-    if (*stride == 0) *stride = least;
-    if (*stride < least) return set_error(WD_E_INVALID, std::string("key/value cache: rows of ") + what + " overlap");
-    return WD_OK;
-}
-
-// Calls that change the book on the host may not be part of a graph: a replay would repeat the change of the first time.
-int check_not_captured(const wd_kv_cache *c, cudaStream_t s) {
-    if (c->broken) return set_error(WD_E_STATE, "key/value cache: an earlier call failed on the device");
-    if (c->host_only()) return WD_OK;
-    cudaGetLastError();         // what an earlier call failed with was said then
-    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-    const cudaError_t ce = cudaStreamIsCapturing(s, &st);
-    if (ce != cudaSuccess) {
-        cudaGetLastError();
-        return set_error(WD_E_STATE, std::string("key/value cache: ") + cudaGetErrorString(ce));
-    }
-    if (st != cudaStreamCaptureStatusNone) return set_error(WD_E_STATE, "key/value cache: sequences cannot be changed, nor a step without rows taken, while a graph is captured");
-    return WD_OK;
-}
-int check_device(const wd_kv_cache *c) {
-    if (!c) return set_error(WD_E_INVALID, "key/value cache: null handle");
-    if (c->host_only()) return set_error(WD_E_STATE, "key/value cache: created without a device");
-    if (c->broken) return set_error(WD_E_STATE, "key/value cache: an earlier call failed on the device");
-    cudaGetLastError();
-    return WD_OK;
-}
 
 int flush(wd_kv_cache *c, cudaStream_t s);
 // Changes that no kernel reads before the next begin, read or keep wait for it (pages change hands only there), unless replays of captured calls may come before:
@@ -146,14 +26,6 @@ int later(wd_kv_cache *c, cudaStream_t s) {
     OnDevice on(c->cfg.device);
     return flush(c, s);
 }
-// Whether the call becomes part of a graph; then changes do not wait.
-int note_capture(wd_kv_cache *c, cudaStream_t s) {
-    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-    WD_TRY_CUDA(cudaStreamIsCapturing(s, &st));
-    if (st != cudaStreamCaptureStatusNone) c->graphs = true;
-    return WD_OK;
-}
-
 template <int N>
 void send_words(wd_kv_cache *c, size_t from, cudaStream_t s) {
     wd::KvWords<N> w;
@@ -197,95 +69,6 @@ int flush(wd_kv_cache *c, cudaStream_t s) {
     WD_TRY_CUDA(cudaGetLastError());
     c->broken = false;
     return WD_OK;
-}
-
-template <class F>
-int by_codes(const wd_kv_cache *c, F &&f) {
-    return c->shape.e4m3 ? f(std::true_type{}) : f(std::false_type{});
-}
-
-template <class F>
-int by_rows_and_codes(const wd_kv_cache *c, int rows, F &&f) {
-    return by_codes(c, [&](auto e4m3) {
-        return rows == wd::kRowsF32 ? f(0.0f, e4m3) : rows == wd::kRowsF16 ? f(__half(), e4m3) : f(__nv_bfloat16(), e4m3);
-    });
-}
-
-template <int D, int N8, bool SPLIT>
-int attend_launch(wd_kv_cache *c, wd::KvAttend &p, cudaStream_t s) {
-    using A = wd::AttendPlan<D>;
-    constexpr int kMost = 227 * 1024 - 8192;        // what a block may have, less what the kernel declares itself
-    static_assert(A::fixed_bytes(4, N8, SPLIT) + 4 * 2 * A::kSlot <= kMost, "four workers with two slots fit");
-    // keys of one tile and values of the one before should be on their way while a worker computes
-    for (p.workers = 8; p.workers > 4; p.workers /= 2)
-        if ((kMost - A::fixed_bytes(p.workers, N8, SPLIT)) / (p.workers * A::kSlot) >= 3) break;
-    p.slots = std::min(wd::kAttMaxSlots, (kMost - A::fixed_bytes(p.workers, N8, SPLIT)) / (p.workers * A::kSlot));
-    const int smem = p.workers * p.slots * A::kSlot + A::fixed_bytes(p.workers, N8, SPLIT);
-    return by_codes(c, [&](auto e4m3) {
-        auto kernel = wd::kv_attend_kernel<D, N8, SPLIT, decltype(e4m3)::value>;
-        WD_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        kernel<<<std::min(c->n_sm, wd::kAttMaxCtas), wd::kAttThreads, smem, s>>>(p);
-        WD_TRY_CUDA(cudaGetLastError());
-        return WD_OK;
-    });
-}
-template <int D>
-int attend_of(wd_kv_cache *c, wd::KvAttend &p, bool few, cudaStream_t s) {
-    if constexpr (D > 128) few = true;       // (the sums of 16 rows of 256 do not fit a warp's registers)
-    if (p.type == wd::kRowsF32) return few ? attend_launch<D, 1, true>(c, p, s) : attend_launch<D, (D > 128 ? 1 : 2), true>(c, p, s);
-    return few ? attend_launch<D, 1, false>(c, p, s) : attend_launch<D, (D > 128 ? 1 : 2), false>(c, p, s);
-}
-
-// Which of the two attention kernels a step takes: the one that is expected to be through first, by what each was measured to take (us):
-//   for few rows   c_f for 64 tokens of a head by 16 rows (8 of heads of 256) and worker: heads of 64 1.8, of 128 in F32 4.2, of 256 1.8
-//   for prompts    3 more, and c_p for 128 tokens by 256 rows (128 of heads of 256) and CTA: heads of 64 1.8, of 128 in F32 3.4, of 256 4.2;
-//                  8 more where items are cut into runs
-// (64 rows a head of 64, 1,000 tokens: 15 against 23 us; 512 rows, 8,000 tokens: 63 against 39. Heads of 32 and 96 go by the lines through these points.)
-struct Choice {
-    bool prompt, split;
-};
-Choice choose(const wd_kv_cache *c, bool f32, int window) {
-    const int g = c->cfg.n_heads / c->cfg.n_kv_heads, d = c->cfg.head_dim, h = c->cfg.n_kv_heads;
-    const int few_rows = d > 128 ? 8 : 16, item_rows = d > 128 ? 128 : 256;
-    double few = 0.0, tiles = 0.0;
-    long long items = 0;
-    int most = 0;
-    for (int i = 0; i < c->book[0]; ++i) {
-        const int *e = c->book.data() + wd::kKvHead + static_cast<size_t>(i) * wd::kKvStepWords;
-        const long long rows = static_cast<long long>(e[2]) * g;
-        if (rows == 0) continue;
-        const int seen = window ? std::min(e[3], window + item_rows / g) : e[3], n = (seen + 127) / 128;
-        const long long blocks = (rows + item_rows - 1) / item_rows;
-        few += static_cast<double>((rows + few_rows - 1) / few_rows) * h * ((seen + 63) / 64);
-        tiles += static_cast<double>(blocks) * h * n;
-        items += blocks * h;
-        most = std::max(most, n);
-    }
-    Choice r;
-    const int runs = wd::prompt_runs(c->n_sm, items, most);
-    r.split = runs > 1;
-    const double c_f = d / 36.0 * (f32 ? 1.2 : 1.0) * (d > 128 ? 0.25 : 1.0), c_p = (1.0 + d / 80.0) * (f32 ? 1.3 : 1.0);
-    const double of_few = c_f * few / (c->n_sm * (d > 128 ? 4.0 : 8.0));
-    const double of_prompt = 3.0 + (r.split ? 8.0 + c_p * most / runs : c_p * std::max<double>(most, tiles / c->n_sm));
-    r.prompt = of_prompt < of_few;
-    return r;
-}
-
-template <int D, bool SPLIT>
-int prompt_launch(wd_kv_cache *c, const wd::KvPrompt &p, cudaStream_t s) {
-    return by_codes(c, [&](auto e4m3) {
-        auto kernel = wd::kv_prompt_kernel<D, SPLIT, decltype(e4m3)::value>;
-        constexpr int smem = wd::PromptAttPlan<D, SPLIT>::kSmem;
-        WD_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        kernel<<<c->n_sm, wd::kPromptThreads, smem, s>>>(p);
-        if (p.split) wd::kv_prompt_join_kernel<D><<<2 * c->n_sm, 256, 0, s>>>(p);
-        WD_TRY_CUDA(cudaGetLastError());
-        return WD_OK;
-    });
-}
-template <int D>
-int prompt_of(wd_kv_cache *c, const wd::KvPrompt &p, cudaStream_t s) {
-    return p.type == wd::kRowsF32 ? prompt_launch<D, true>(c, p, s) : prompt_launch<D, false>(c, p, s);
 }
 
 }  // namespace
@@ -445,16 +228,7 @@ int wd_kv_append(wd_kv_cache *c, int layer, const void *k_dev, const void *v_dev
         if (int rc = check_rows(v_dev, size, &p.stride[1], width, "v")) return rc;
         OnDevice on(c->cfg.device);
         if (int rc = note_capture(c, s)) return rc;
-        p.pool = c->d_pool + layer * c->pool_layer;
-        p.scales = c->d_scales + layer * c->scales_layer;
-        p.reach = c->d_reach + static_cast<size_t>(layer) * c->cfg.n_kv_heads;
-        p.book = c->d_book;
-        p.table = c->d_book + c->table_at;
-        p.rows[0] = k_dev;
-        p.rows[1] = v_dev;
-        p.status = c->d_status;
-        p.s = c->shape;
-        for (int i = 0; i < 2; ++i) p.vec[i] = reinterpret_cast<uintptr_t>(p.rows[i]) % 16 == 0 && p.stride[i] * size % 16 == 0;
+        fill_append(c, layer, k_dev, v_dev, size, &p);
         const dim3 grid(static_cast<unsigned>(c->items), c->cfg.n_kv_heads, 2);
         const size_t smem = static_cast<size_t>(c->cfg.page_tokens) * c->cfg.head_dim;
         // few tokens a page: a warp reads them at once, and more threads would only meet at the barriers

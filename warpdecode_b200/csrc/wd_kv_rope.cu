@@ -1,0 +1,317 @@
+// Norms and rotary positions of a step's queries and keys, the keys and values into the 8-bit cache on the way (wd_rope_*, wd_kv_append_rope).
+//
+//   n = x w / sqrt(mean x^2 + eps);   pair p of a head: angle a = position f_p,  (y0, y1) = factor (n0 cos a - n1 sin a, n1 cos a + n0 sin a)
+//
+// A block takes the step's tokens that lie in one page and one kv head: its keys (blockIdx.z = 0), its values (1), or some of the query heads that share it
+// (2 and up). A warp takes a token's head, a lane the pairs lane, lane + 32, ...: the rotation's cosines are made once for all of a warp's heads of a token.
+//
+// Angles are made in turns, position (f_p / 2 pi) in 64 bits less the nearest whole number: in 32 bits the position 131,072 is off by 2^-8 radians. Queries
+// are rotated in F32. Keys in 64 bits, rounded to F32 once: then the code is the same however the sums are ordered, but for one number in 2^28, and the same
+// rows again leave the cache as it is. The rotated keys of a page wait in shared memory for the page's scale, as many tokens at a time as it holds; those
+// of a page that has more are made a second time.
+#include <cmath>
+#include <memory>
+
+#include "wd_kv_append.cuh"
+#include "wd_kv_host.h"
+
+using namespace wd_kv;
+
+struct wd_rope {
+    wd_rope_config cfg{};
+    int section_end[4] = {};
+    double turns[128] = {};         // of each pair, for a step of one in its position
+};
+
+namespace wd {
+namespace {
+
+constexpr int kRopePairs = 4;       // of a lane: heads of up to 256
+
+struct KvRope {
+    KvAppend a;
+    const void *q;
+    void *q_out;
+    long long q_stride, q_out_stride;
+    const int *positions;           // null: the tokens' own places
+    const float *q_norm, *k_norm;
+    float eps, factor;
+    int rotary, neighbours, n_axes, q_parts, held;      // held: tokens that shared memory has room for
+    int section_end[4];
+    double turns[128];
+};
+
+// The pairs of a lane: their elements, axis and frequency. Pairs behind the rotated ones are two elements that are only brought through.
+struct RopeLane {
+    int e0[kRopePairs], e1[kRopePairs], axis[kRopePairs];
+    double turns[kRopePairs];
+    bool is[kRopePairs], turned[kRopePairs];
+};
+__device__ __forceinline__ RopeLane rope_lane(const KvRope &P, int lane) {
+    RopeLane r;
+#pragma unroll
+    for (int i = 0; i < kRopePairs; ++i) {
+        const int p = lane + 32 * i, half = P.rotary / 2;
+        r.is[i] = p < P.a.s.head_dim / 2;
+        r.turned[i] = p < half;
+        r.e0[i] = r.turned[i] && !P.neighbours ? p : 2 * p;
+        r.e1[i] = r.turned[i] && !P.neighbours ? p + half : 2 * p + 1;
+        r.axis[i] = (p >= P.section_end[0]) + (p >= P.section_end[1]) + (p >= P.section_end[2]);
+        r.turns[i] = r.turned[i] ? P.turns[p] : 0.0;
+    }
+    return r;
+}
+// 2 (turns less the nearest whole number): what the functions of pi times x take
+__device__ __forceinline__ double rope_angle(const KvRope &P, const RopeLane &l, int i, int row, int place) {
+    const double a = static_cast<double>(P.positions ? P.positions[static_cast<size_t>(row) * P.n_axes + min(l.axis[i], P.n_axes - 1)] : place) * l.turns[i];
+    return 2.0 * (a - rint(a));
+}
+
+// where a float of the held rows is: 16 of them that one thread reads lie in other banks than its neighbours'
+__device__ __forceinline__ int rope_held(int e) { return (e & ~15) | ((((e >> 2) + (e >> 5)) & 3) << 2) | (e & 3); }
+
+template <class T, bool E4M3, int THREADS>
+__global__ void __launch_bounds__(THREADS) kv_rope_kernel(const __grid_constant__ KvRope P) {
+    extern __shared__ __align__(16) uint8_t rope_sm[];           // keys: rotated rows; values: the codes of the sub-blocks that the rows touch
+    __shared__ float part[THREADS / 32];
+    __shared__ int bad_any;
+    constexpr int W = THREADS / 32;
+    const int n_seq = P.a.book[0], n_items = P.a.book[2], h = blockIdx.y, D = P.a.s.head_dim, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll 1
+    for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+        const KvPagePart at = kv_page_part(P.a.book, P.a.table, P.a.s, n_seq, item);
+        const int n = at.b - at.a;
+        if (blockIdx.z == 1) {
+            kv_append_part<T, E4M3, THREADS>(P.a, at, h, 1, rope_sm, part, bad_any);
+        } else if (blockIdx.z == 0) {
+            const RopeLane l = rope_lane(P, lane);
+            const T *rows = static_cast<const T *>(P.a.rows[0]) + static_cast<size_t>(at.row) * P.a.stride[0] + static_cast<size_t>(h) * D;
+            float *held = reinterpret_cast<float *>(rope_sm);
+            auto rotate = [&](int t0, int m) {
+                for (int t = warp; t < m; t += W) {
+                    const T *x = rows + static_cast<size_t>(t0 + t) * P.a.stride[0];
+                    float x0[kRopePairs], x1[kRopePairs];
+#pragma unroll
+                    for (int i = 0; i < kRopePairs; ++i) {
+                        x0[i] = l.is[i] ? static_cast<float>(x[l.e0[i]]) : 0.0f;
+                        x1[i] = l.is[i] ? static_cast<float>(x[l.e1[i]]) : 0.0f;
+                    }
+                    double inv = 1.0;
+                    if (P.k_norm) {
+                        double sum = 0.0;
+#pragma unroll
+                        for (int i = 0; i < kRopePairs; ++i) sum += static_cast<double>(x0[i]) * x0[i] + static_cast<double>(x1[i]) * x1[i];
+#pragma unroll
+                        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                        inv = 1.0 / sqrt(sum / D + static_cast<double>(P.eps));
+                    }
+#pragma unroll
+                    for (int i = 0; i < kRopePairs; ++i) {
+                        if (!l.is[i]) continue;
+                        double n0 = x0[i], n1 = x1[i];
+                        if (P.k_norm) n0 = n0 * inv * P.k_norm[l.e0[i]], n1 = n1 * inv * P.k_norm[l.e1[i]];
+                        if (l.turned[i]) {
+                            double sn, cs;
+                            sincospi(rope_angle(P, l, i, at.row + t0 + t, at.place + t0 + t), &sn, &cs);
+                            const double f = P.factor, y0 = f * (n0 * cs - n1 * sn), y1 = f * (n1 * cs + n0 * sn);
+                            n0 = y0, n1 = y1;
+                        }
+                        held[rope_held(t * D + l.e0[i])] = static_cast<float>(n0);
+                        held[rope_held(t * D + l.e1[i])] = static_cast<float>(n1);
+                    }
+                }
+            };
+            auto load = [&](int t, int k, float *x) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float4 v = *reinterpret_cast<const float4 *>(held + rope_held(t * D + k + 4 * j));
+                    x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
+                }
+            };
+            float top = 0.0f;
+            int bad = 0;
+            for (int t0 = 0; t0 < n; t0 += P.held) {
+                if (t0 > 0) __syncthreads();
+                rotate(t0, min(P.held, n - t0));
+                __syncthreads();
+                top = kv_part_top<THREADS>(D, min(P.held, n - t0), load, top, bad);
+            }
+            const KvPartScale sc = kv_part_scale<E4M3, THREADS>(P.a, at, h, 0, top, bad, part, bad_any);
+            for (int t0 = 0; t0 < n; t0 += P.held) {
+                if (n > P.held) {
+                    __syncthreads();
+                    rotate(t0, min(P.held, n - t0));
+                    __syncthreads();
+                }
+                kv_part_codes<E4M3, THREADS>(P.a, at, h, 0, sc, nullptr, t0, min(P.held, n - t0), load);
+            }
+            kv_part_end(P.a, at, h, 0, sc.s, make_int2(0, 0));
+        } else {
+            const RopeLane l = rope_lane(P, lane);
+            const int g = P.a.s.heads / P.a.s.kv_heads, part_q = blockIdx.z - 2, h0 = h * g + g * part_q / P.q_parts, h1 = h * g + g * (part_q + 1) / P.q_parts;
+            // a warp a token; where there are fewer tokens, some warps share one's heads
+            const int share = n < W ? W / n : 1;
+            for (int t = warp / share; t < n; t += W / share) {
+                float cs[kRopePairs], sn[kRopePairs];
+#pragma unroll
+                for (int i = 0; i < kRopePairs; ++i) {
+                    cs[i] = 1.0f, sn[i] = 0.0f;
+                    if (!l.turned[i]) continue;
+                    sincospif(static_cast<float>(rope_angle(P, l, i, at.row + t, at.place + t)), &sn[i], &cs[i]);
+                    cs[i] *= P.factor, sn[i] *= P.factor;
+                }
+                const T *from = static_cast<const T *>(P.q) + static_cast<size_t>(at.row + t) * P.q_stride;
+                T *to = static_cast<T *>(P.q_out) + static_cast<size_t>(at.row + t) * P.q_out_stride;
+                for (int head = h0 + warp % share; head < h1; head += share) {
+                    const T *x = from + static_cast<size_t>(head) * D;
+                    T *y = to + static_cast<size_t>(head) * D;
+                    float x0[kRopePairs], x1[kRopePairs];
+#pragma unroll
+                    for (int i = 0; i < kRopePairs; ++i) {
+                        x0[i] = l.is[i] ? static_cast<float>(x[l.e0[i]]) : 0.0f;
+                        x1[i] = l.is[i] ? static_cast<float>(x[l.e1[i]]) : 0.0f;
+                    }
+                    if (P.q_norm) {
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < kRopePairs; ++i) sum = fmaf(x0[i], x0[i], fmaf(x1[i], x1[i], sum));
+#pragma unroll
+                        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                        float inv = __frsqrt_rn(sum / D + P.eps);
+                        if (!(sum > 1e-30f && sum < 1e38f)) {           // squares that F32 does not hold
+                            double wide = 0.0;
+#pragma unroll
+                            for (int i = 0; i < kRopePairs; ++i) wide += static_cast<double>(x0[i]) * x0[i] + static_cast<double>(x1[i]) * x1[i];
+#pragma unroll
+                            for (int o = 16; o; o >>= 1) wide += __shfl_xor_sync(0xffffffffu, wide, o);
+                            inv = static_cast<float>(1.0 / sqrt(wide / D + static_cast<double>(P.eps)));
+                        }
+#pragma unroll
+                        for (int i = 0; i < kRopePairs; ++i) {
+                            if (!l.is[i]) continue;
+                            x0[i] = x0[i] * inv * P.q_norm[l.e0[i]];
+                            x1[i] = x1[i] * inv * P.q_norm[l.e1[i]];
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < kRopePairs; ++i) {
+                        if (!l.is[i]) continue;
+                        y[l.e0[i]] = row_number<T>(l.turned[i] ? x0[i] * cs[i] - x1[i] * sn[i] : x0[i]);
+                        y[l.e1[i]] = row_number<T>(l.turned[i] ? x1[i] * cs[i] + x0[i] * sn[i] : x1[i]);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+}  // namespace
+}  // namespace wd
+
+extern "C" {
+
+int wd_rope_create(const wd_rope_config *cfg, const double *inv_freq, wd_rope **out) {
+    return wd_host::guarded([&]() -> int {
+        if (!cfg || !out) return set_error(WD_E_INVALID, "null argument");
+        *out = nullptr;
+        wd_rope_config c = *cfg;
+        if (c.rotary_dim == 0) c.rotary_dim = c.head_dim;
+        if (c.n_axes == 0) c.n_axes = 1;
+        if (c.head_dim < 2 || c.head_dim > 256) return set_error(WD_E_INVALID, "rotary positions: head_dim must be 2 to 256");
+        if (c.rotary_dim < 2 || c.rotary_dim > c.head_dim || c.rotary_dim % 2) return set_error(WD_E_INVALID, "rotary positions: rotary_dim must be even, 2 to head_dim");
+        if (c.pairs != WD_ROPE_HALVES && c.pairs != WD_ROPE_NEIGHBOURS) return set_error(WD_E_INVALID, "rotary positions: pairs must be WD_ROPE_HALVES or WD_ROPE_NEIGHBOURS");
+        if (c.n_axes < 1 || c.n_axes > 4) return set_error(WD_E_INVALID, "rotary positions: 1 to 4 axes");
+        if (!std::isfinite(c.factor) || !(inv_freq || (c.theta > 0.0f && std::isfinite(c.theta)))) return set_error(WD_E_INVALID, "rotary positions: theta must be positive, factor finite");
+        auto r = std::make_unique<wd_rope>();
+        const int pairs = c.rotary_dim / 2;
+        int end = 0;
+        for (int i = 0; i < 4; ++i) {
+            if (c.n_axes > 1 && i < c.n_axes) {
+                if (c.sections[i] < 0 || c.sections[i] > pairs - end) return set_error(WD_E_INVALID, "rotary positions: the axes' pairs must be rotary_dim / 2 together");
+                end += c.sections[i];
+            } else {
+                end = i < c.n_axes ? pairs : end;
+            }
+            r->section_end[i] = end;
+        }
+        if (end != pairs) return set_error(WD_E_INVALID, "rotary positions: the axes' pairs must be rotary_dim / 2 together");
+        for (int p = 0; p < pairs; ++p) {
+            const double f = inv_freq ? inv_freq[p] : std::pow(static_cast<double>(c.theta), -2.0 * p / c.rotary_dim);
+            if (!std::isfinite(f)) return set_error(WD_E_INVALID, "rotary positions: frequencies must be finite");
+            r->turns[p] = f / 6.283185307179586476925;
+        }
+        r->cfg = c;
+        *out = r.release();
+        return WD_OK;
+    });
+}
+
+void wd_rope_destroy(wd_rope *r) { delete r; }
+
+int wd_kv_append_rope(wd_kv_cache *c, int layer, const wd_rope *r, const wd_rope_rows *x, void *stream) {
+    return wd_host::guarded([&]() -> int {
+        if (int rc = check_device(c)) return rc;
+        if (!r || !x) return set_error(WD_E_INVALID, "null argument");
+        if (layer < 0 || layer >= c->cfg.n_layers) return set_error(WD_E_INVALID, "key/value cache: layer out of range");
+        if (r->cfg.head_dim != c->cfg.head_dim) return set_error(WD_E_INVALID, "key/value cache: rotary positions of another head_dim");
+        if ((x->q_norm_dev || x->k_norm_dev) && !(x->eps > 0.0f && std::isfinite(x->eps))) return set_error(WD_E_INVALID, "key/value cache: eps of the norms must be positive");
+        if ((x->q_dev == nullptr) != (x->q_out_dev == nullptr)) return set_error(WD_E_INVALID, "key/value cache: q needs its output, and the other way round");
+        for (const void *p : {static_cast<const void *>(x->positions_dev), static_cast<const void *>(x->q_norm_dev), static_cast<const void *>(x->k_norm_dev)})
+            if (reinterpret_cast<uintptr_t>(p) % 4) return set_error(WD_E_INVALID, "key/value cache: positions and norms are not aligned to their type");
+        int rows_of = 0;
+        if (int rc = rows_type(x->type, &rows_of)) return rc;
+        if (c->book[0] == 0) return set_error(WD_E_STATE, "key/value cache: no step has begun");
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        if (c->items == 0) return check_not_captured(c, s);
+        const size_t size = rows_size(rows_of);
+        const int D = c->cfg.head_dim, H = c->cfg.n_kv_heads, g = c->cfg.n_heads / H;
+        const long long width = static_cast<long long>(H) * D;
+        wd::KvRope p;
+        p.a.stride[0] = x->k_stride;
+        p.a.stride[1] = x->v_stride;
+        if (int rc = check_rows(x->k_dev, size, &p.a.stride[0], width, "k")) return rc;
+        if (int rc = check_rows(x->v_dev, size, &p.a.stride[1], width, "v")) return rc;
+        p.q_stride = x->q_stride;
+        p.q_out_stride = x->q_out_stride;
+        if (x->q_dev) {
+            if (int rc = check_rows(x->q_dev, size, &p.q_stride, width * g, "q")) return rc;
+            if (int rc = check_rows(x->q_out_dev, size, &p.q_out_stride, width * g, "q's output")) return rc;
+            if (x->q_dev == x->q_out_dev && p.q_stride != p.q_out_stride) return set_error(WD_E_INVALID, "key/value cache: an output over q needs q's stride");
+        }
+        OnDevice on(c->cfg.device);
+        if (int rc = note_capture(c, s)) return rc;
+        fill_append(c, layer, x->k_dev, x->v_dev, size, &p.a);
+        p.q = x->q_dev;
+        p.q_out = x->q_out_dev;
+        p.positions = x->positions_dev;
+        p.q_norm = x->q_norm_dev;
+        p.k_norm = x->k_norm_dev;
+        p.eps = x->eps;
+        p.factor = r->cfg.factor;
+        p.rotary = r->cfg.rotary_dim;
+        p.neighbours = r->cfg.pairs == WD_ROPE_NEIGHBOURS;
+        p.n_axes = r->cfg.n_axes;
+        for (int i = 0; i < 4; ++i) p.section_end[i] = r->section_end[i];
+        for (int i = 0; i < 128; ++i) p.turns[i] = r->turns[i];
+        const int most = std::min(c->max_rows, c->cfg.page_tokens);       // of a page (a replay may have more)
+        p.held = std::min(most, 16384 / D);
+        const size_t smem = std::max<size_t>(static_cast<size_t>(p.held) * D * 4, static_cast<size_t>(c->cfg.page_tokens) * D);
+        // one head of q a block where there are not enough blocks for the SMs, all that share a kv head where there are
+        p.q_parts = std::max<long long>(1, std::min<long long>(g, 4ll * c->n_sm / (static_cast<long long>(c->items) * H)));
+        const dim3 grid(static_cast<unsigned>(c->items), H, x->q_dev ? 2 + p.q_parts : 2);
+        const bool small = static_cast<long long>(most) * D <= 2048;
+        return by_rows_and_codes(c, rows_of, [&](auto t, auto e4m3) {
+            using T = decltype(t);
+            auto launch = [&](auto kernel, int threads) {
+                WD_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+                kernel<<<grid, threads, smem, s>>>(p);
+                WD_TRY_CUDA(cudaGetLastError());
+                return WD_OK;
+            };
+            return small ? launch(wd::kv_rope_kernel<T, decltype(e4m3)::value, 64>, 64) : launch(wd::kv_rope_kernel<T, decltype(e4m3)::value, 256>, 256);
+        });
+    });
+}
+
+}  // extern "C"
