@@ -481,6 +481,31 @@ int wd_kv_status(wd_kv_cache *c, int *status);
 int wd_token_logprobs(const void *logits_dev, int type, int rows, int vocab, int64_t stride, const int *tokens_dev, float *logprob_dev,
                       float *entropy_dev, int n_top, int *top_ids_dev, float *top_logprobs_dev, void *stream);
 
+/* Verification of drafted tokens (speculative decoding): the tokens that come out are distributed as if the target model alone had made them.
+ *
+ * rows rows of logits, those of n_seqs sequences one behind the other: sequence i has the rows first_dev[i] .. first_dev[i + 1] - 1 (first_dev null: equal
+ * shares; 0 <= first_dev[i] <= first_dev[i + 1] <= rows is the caller's), at most 1024 (one with more is answered as one without). A sequence's first row is the last token that is certain, its others are drafted tokens, a
+ * tree: parents_dev as in wd_kv_attend_tree (null: a chain, each row follows the one in front of it). target_dev[r] is what the target model says behind row r,
+ * draft_dev[r] (nullable, of the same type) what the draft model said there, from which the row's children were drawn, independently of one another.
+ * p and q are softmax(logits / temperature_dev[i]) (null: 1); below 1e-6: greedy, p is 1 for the largest logit (the lowest id of equals) and q is not asked for.
+ *
+ * From the first row on, a row's children are judged in order, child x with the number uniforms_dev[x] from [0, 1):
+ *   drawn from q     accepted where u S q(x) < max(p(x) - c q(x), 0), S = sum max(p - c q, 0); c is 0 at first, and each rejection adds its S to it
+ *   without draft    (tokens that were chosen, not drawn) accepted where u (1 - p(R)) < p(x), R the tokens rejected so far, x not among them
+ * The first accepted one is the next row. Where there is none, the token behind is drawn from what is left, p without R or max(p - c q, 0), by the number of the
+ * sequence's first row: the first id where the running sum is above u times the whole. A drafted token outside of the vocabulary is passed over.
+ *
+ *   path_dev[rows]       the accepted rows of each sequence from its first row's place on, counted from that row, itself (0) first; -1 behind them. With the host's
+ *                        copy: wd_kv_keep(c, seq, tokens before the step, count, path)
+ *   count_dev[n_seqs]    how many they are; 0 for a sequence without rows
+ *   next_dev[n_seqs]     the token behind them; -1 for a sequence without rows, or where a row has no distribution (a NaN, +inf, nothing but -inf)
+ *
+ * Running sums are 64 bits, so that a number that is not next to a border gives the same token however they are ordered. strides: elements from row to row,
+ * 0 = vocab. Without a workspace; runs on the device of target_dev; can be captured. */
+int wd_verify_drafts(const void *target_dev, const void *draft_dev, int type, int rows, int vocab, int64_t target_stride, int64_t draft_stride, int n_seqs,
+                     const int *first_dev, const int *tokens_dev, const int *parents_dev, const float *uniforms_dev, const float *temperature_dev, int *path_dev,
+                     int *count_dev, int *next_dev, void *stream);
+
 /* Has no counterpart in the reference. y = W x for one IQ3_S matrix like wd_matvec_host, for callers
  * that must not allocate device memory (HBM already handed to the expert pool, a latency-critical
  * token loop where cudaMalloc's device-wide synchronisation is unacceptable, memory owned by another

@@ -20,7 +20,7 @@ SOURCES = [os.path.join(HERE, "csrc", f) for f in
            ("wd_engine.cu", "wd_aux_kernels.cuh", "wd_moe_kernel.cuh", "wd_moe_kernel_phases.inc", "wd_moe_fast.cuh", "wd_moe_batch.cuh", "wd_dense_decoder.cuh", "wd_dense_decoder.inc", "wd_dense_token.cuh", "wd_dense_prefill.cuh", "wd_dense_prompt_tc.cuh",
             "wd_plain_moe.cuh", "wd_plain_wide.cuh", "wd_plain_moe.inc", "wd_blocks.cuh", "wd_router.cuh",
             "wd_formats.cuh", "wd_device.cuh", "wd_dense.cuh", "wd_gguf.inc",
-            "wd_grids.h", "wd_host.h", "wd_tcgen05.cuh", "wd_kv.cu", "wd_kv_rope.cu", "wd_kv_host.h", "wd_kv_launch.cuh", "wd_kv_layout.cuh", "wd_kv_append.cuh", "wd_kv_kernels.cuh", "wd_kv_attend.cuh", "wd_kv_prompt.cuh", "wd_score.cu")] + [
+            "wd_grids.h", "wd_host.h", "wd_tcgen05.cuh", "wd_kv.cu", "wd_kv_rope.cu", "wd_kv_host.h", "wd_kv_launch.cuh", "wd_kv_layout.cuh", "wd_kv_append.cuh", "wd_kv_kernels.cuh", "wd_kv_attend.cuh", "wd_kv_prompt.cuh", "wd_score.cu", "wd_verify.cu")] + [
                os.path.join(ROOT, "include", "warpdecode_b200.h")]
 _HOST = ("wd_device", "wd_host", "warpdecode")
 
@@ -29,10 +29,11 @@ def _files(*starts):
     return [s for s in SOURCES if os.path.basename(s).startswith(starts + _HOST)]
 
 
-UNITS = {"wd_engine": [s for s in SOURCES if not os.path.basename(s).startswith(("wd_kv", "wd_score"))],        # translation units, and what they include
+UNITS = {"wd_engine": [s for s in SOURCES if not os.path.basename(s).startswith(("wd_kv", "wd_score", "wd_verify"))],        # translation units, and what they include
          "wd_kv": _files("wd_kv.", "wd_kv_host", "wd_kv_launch", "wd_kv_layout", "wd_kv_append", "wd_kv_kernels", "wd_kv_attend", "wd_kv_prompt", "wd_tcgen05"),
          "wd_kv_rope": _files("wd_kv_rope", "wd_kv_host", "wd_kv_layout", "wd_kv_append"),
-         "wd_score": _files("wd_score")}
+         "wd_score": _files("wd_score"),
+         "wd_verify": _files("wd_verify")}
 
 TYPE_F16, TYPE_BF16 = 1, 30
 KV_INT8, KV_E4M3 = 0, 1
@@ -223,6 +224,7 @@ def lib():
         L.wd_kv_kernel_name.argtypes = [vp]
         L.wd_kv_kernel_name.restype = C.c_char_p
         L.wd_token_logprobs.argtypes = [vp, i, i, i, i64, vp, vp, vp, i, vp, vp, vp]
+        L.wd_verify_drafts.argtypes = [vp, vp, i, i, i, i64, i64, i, vp, vp, vp, vp, vp, vp, vp, vp, vp]
         L.wd_gguf_open.argtypes = [C.c_char_p, C.POINTER(vp)]
         L.wd_gguf_close.argtypes = [vp]
         L.wd_gguf_close.restype = None
@@ -813,6 +815,17 @@ def token_logprobs(logits_ptr, rows, vocab, tokens_ptr=None, logprob_ptr=None, e
     _fit(rows, vocab, n_top, type)
     _fit64(stride)
     rc = lib().wd_token_logprobs(logits_ptr, type, rows, vocab, stride, tokens_ptr, logprob_ptr, entropy_ptr, n_top, top_ids_ptr, top_logprobs_ptr, stream)
+    if rc:
+        _check(rc)
+
+
+def verify_drafts(target_ptr, rows, vocab, tokens_ptr, uniforms_ptr, path_ptr, count_ptr, next_ptr, n_seqs=1, draft_ptr=None, parents_ptr=None, first_ptr=None,
+                  temperature_ptr=None, type=TYPE_F32, target_stride=0, draft_stride=0, stream=None):
+    """Which drafted tokens the target's logits accept, given random numbers, and the token behind them, on device buffers (wd_verify_drafts)."""
+    _fit(rows, vocab, n_seqs, type)
+    _fit64(target_stride, draft_stride)
+    rc = lib().wd_verify_drafts(target_ptr, draft_ptr, type, rows, vocab, target_stride, draft_stride, n_seqs, first_ptr, tokens_ptr, parents_ptr, uniforms_ptr, temperature_ptr,
+                                path_ptr, count_ptr, next_ptr, stream)
     if rc:
         _check(rc)
 
