@@ -445,6 +445,13 @@ int wd_kv_append_rope(wd_kv_cache *c, int layer, const wd_rope *r, const wd_rope
  * do not overlap otherwise. */
 int wd_kv_attend(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, int type, float scale, int window, int64_t q_stride,
                  int64_t out_stride, void *stream);
+/* As wd_kv_attend, where the step's rows of each sequence are a tree of drafted tokens (at most 128 rows of a sequence): parents_dev[r] is the row that row r
+ * follows, counted from the sequence's first one, and lies in front of r; -1 (and what is no row in front of it): the token before the step. A row sees the
+ * tokens before the step, the rows on its way up the tree, and itself; its position is the number of tokens before the step plus its depth, and a window
+ * leaves it the last `window` positions. (A tree that is a chain, parents -1, 0, 1, ...: wd_kv_attend.) After the verification wd_kv_keep leaves the accepted
+ * path. Can be captured; parents are read when the call runs. A replay on a step with more than 128 rows of a sequence does nothing. */
+int wd_kv_attend_tree(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, const int *parents_dev, int type, float scale, int window, int64_t q_stride,
+                      int64_t out_stride, void *stream);
 /* Tokens firsts[i] .. firsts[i] + counts[i] - 1 of the sequences as numbers, one behind the other: [rows][n_kv_heads][head_dim], for
  * layer -1 [n_layers][rows][n_kv_heads][head_dim]. Either output may be null. */
 int wd_kv_read(wd_kv_cache *c, int layer, int n, const int *seqs, const int *firsts, const int *counts, void *k_dev, void *v_dev, int type, void *stream);

@@ -41,3 +41,13 @@ def test_needs_a_device():
     for kw in (dict(layer=2 ** 32), dict(type=2 ** 32), dict(q_stride=2 ** 64), dict(v_stride=2 ** 64 + 512)):
         with pytest.raises(ValueError):
             kv.append_rope(kw.pop("layer", 0), wd.Rope(64), 16, 16, **kw)
+
+
+def test_attention_of_a_tree_needs_a_device():
+    kv = wd.KvCache(2, 8, 2, 64, 12, 5, 100, page_tokens=16, device=-1)
+    kv.begin([0], [4])
+    with pytest.raises(wd.WdError, match="without a device"):
+        kv.attend_tree(0, 16, 16, 16)
+    for kw in (dict(layer=2 ** 32), dict(type=2 ** 32), dict(window=2 ** 32), dict(q_stride=2 ** 64)):
+        with pytest.raises(ValueError):
+            kv.attend_tree(kw.pop("layer", 0), 16, 16, 16, **kw)

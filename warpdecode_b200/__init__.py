@@ -20,7 +20,7 @@ SOURCES = [os.path.join(HERE, "csrc", f) for f in
            ("wd_engine.cu", "wd_aux_kernels.cuh", "wd_moe_kernel.cuh", "wd_moe_kernel_phases.inc", "wd_moe_fast.cuh", "wd_moe_batch.cuh", "wd_dense_decoder.cuh", "wd_dense_decoder.inc", "wd_dense_token.cuh", "wd_dense_prefill.cuh", "wd_dense_prompt_tc.cuh",
             "wd_plain_moe.cuh", "wd_plain_wide.cuh", "wd_plain_moe.inc", "wd_blocks.cuh", "wd_router.cuh",
             "wd_formats.cuh", "wd_device.cuh", "wd_dense.cuh", "wd_gguf.inc",
-            "wd_grids.h", "wd_host.h", "wd_tcgen05.cuh", "wd_kv.cu", "wd_kv_rope.cu", "wd_kv_host.h", "wd_kv_launch.cuh", "wd_kv_layout.cuh", "wd_kv_append.cuh", "wd_kv_kernels.cuh", "wd_kv_attend.cuh", "wd_kv_prompt.cuh", "wd_score.cu", "wd_verify.cu")] + [
+            "wd_grids.h", "wd_host.h", "wd_tcgen05.cuh", "wd_kv.cu", "wd_kv_rope.cu", "wd_kv_tree.cu", "wd_kv_host.h", "wd_kv_launch.cuh", "wd_kv_layout.cuh", "wd_kv_append.cuh", "wd_kv_kernels.cuh", "wd_kv_attend.cuh", "wd_kv_prompt.cuh", "wd_score.cu", "wd_verify.cu")] + [
                os.path.join(ROOT, "include", "warpdecode_b200.h")]
 _HOST = ("wd_device", "wd_host", "warpdecode")
 
@@ -31,6 +31,7 @@ def _files(*starts):
 
 UNITS = {"wd_engine": [s for s in SOURCES if not os.path.basename(s).startswith(("wd_kv", "wd_score", "wd_verify"))],        # translation units, and what they include
          "wd_kv": _files("wd_kv.", "wd_kv_host", "wd_kv_launch", "wd_kv_layout", "wd_kv_append", "wd_kv_kernels", "wd_kv_attend", "wd_kv_prompt", "wd_tcgen05"),
+         "wd_kv_tree": _files("wd_kv_tree", "wd_kv_host", "wd_kv_launch", "wd_kv_layout", "wd_kv_append", "wd_kv_attend", "wd_kv_prompt", "wd_tcgen05"),
          "wd_kv_rope": _files("wd_kv_rope", "wd_kv_host", "wd_kv_layout", "wd_kv_append"),
          "wd_score": _files("wd_score"),
          "wd_verify": _files("wd_verify")}
@@ -212,6 +213,7 @@ def lib():
         L.wd_rope_destroy.restype = None
         L.wd_kv_append_rope.argtypes = [vp, i, vp, C.POINTER(RopeRows), vp]
         L.wd_kv_attend.argtypes = [vp, i, vp, vp, i, C.c_float, i, i64, i64, vp]
+        L.wd_kv_attend_tree.argtypes = [vp, i, vp, vp, vp, i, C.c_float, i, i64, i64, vp]
         L.wd_kv_read.argtypes = [vp, i, i, vp, vp, vp, vp, vp, i, vp]
         L.wd_kv_fork.argtypes = [vp, i, i, vp, vp]
         L.wd_kv_keep.argtypes = [vp, i, i, i, vp, vp]
@@ -736,6 +738,15 @@ class KvCache:
             _fit(layer, type, window)
             _fit64(q_stride, out_stride)
         rc = lib().wd_kv_attend(self.h, layer, q_ptr, out_ptr, type, self.cfg.head_dim ** -0.5 if scale is None else scale, window, q_stride, out_stride, stream)
+        if rc:
+            _check(rc)
+
+    def attend_tree(self, layer, q_ptr, out_ptr, parents_ptr, type=TYPE_F32, scale=None, window=0, q_stride=0, out_stride=0, stream=None):
+        """attend where each sequence's rows are a tree of drafted tokens: parents, int32 [rows], the row that each follows, counted from its sequence's first; -1: the token before the step."""
+        if (layer | type | window) >> 31 or (q_stride | out_stride) >> 63:
+            _fit(layer, type, window)
+            _fit64(q_stride, out_stride)
+        rc = lib().wd_kv_attend_tree(self.h, layer, q_ptr, out_ptr, parents_ptr, type, self.cfg.head_dim ** -0.5 if scale is None else scale, window, q_stride, out_stride, stream)
         if rc:
             _check(rc)
 

@@ -244,68 +244,7 @@ int wd_kv_append(wd_kv_cache *c, int layer, const void *k_dev, const void *v_dev
 }
 
 int wd_kv_attend(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, int type, float scale, int window, int64_t q_stride, int64_t out_stride, void *stream) {
-    return wd_host::guarded([&]() -> int {
-        if (int rc = check_device(c)) return rc;
-        if (layer < 0 || layer >= c->cfg.n_layers) return set_error(WD_E_INVALID, "key/value cache: layer out of range");
-        if (!(scale > 0.0f && scale * 1.4426950408889634 <= 3.4028234663852886e38)) return set_error(WD_E_INVALID, "key/value cache: the scale of the scores must be positive and finite");
-        if (window < 0) return set_error(WD_E_INVALID, "key/value cache: a window is 0 (none) or at least 1");
-        wd::KvAttend p;
-        if (int rc = rows_type(type, &p.type)) return rc;
-        if (c->book[0] == 0) return set_error(WD_E_STATE, "key/value cache: no step has begun");
-        cudaStream_t s = static_cast<cudaStream_t>(stream);
-        if (c->rows == 0) return check_not_captured(c, s);
-        if (window >= c->cfg.max_context) window = 0;
-        p.q_stride = q_stride;
-        p.out_stride = out_stride;
-        const long long width = static_cast<long long>(c->cfg.n_heads) * c->cfg.head_dim;
-        if (int rc = check_rows(q_dev, rows_size(p.type), &p.q_stride, width, "q")) return rc;
-        if (int rc = check_rows(out_dev, rows_size(p.type), &p.out_stride, width, "out")) return rc;
-        if (q_dev == out_dev && p.q_stride != p.out_stride) return set_error(WD_E_INVALID, "key/value cache: out over q needs q's stride");
-        OnDevice on(c->cfg.device);
-        if (int rc = note_capture(c, s)) return rc;
-        p.pool = c->d_pool + layer * c->pool_layer;
-        p.scales = c->d_scales + layer * c->scales_layer;
-        p.book = c->d_book;
-        p.table = c->d_book + c->table_at;
-        p.q = q_dev;
-        p.out = out_dev;
-        p.part = c->d_part;
-        p.cta_part = c->d_cta_part;
-        p.arrived = c->d_arrived;
-        p.status = c->d_status;
-        p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-        p.window = window;
-        p.max_seqs = c->cfg.max_seqs;
-        p.vec = reinterpret_cast<uintptr_t>(q_dev) % 16 == 0 && p.q_stride * rows_size(p.type) % 16 == 0;
-        p.s = c->shape;
-        const long long group = static_cast<long long>(c->max_rows) * (c->cfg.n_heads / c->cfg.n_kv_heads);
-        const Choice by = choose(c, p.type == wd::kRowsF32, window);
-        c->last_kernel = by.prompt ? by.split ? "kv_prompt_kernel, kv_prompt_join_kernel" : "kv_prompt_kernel" : "kv_attend_kernel";
-        if (by.prompt) {
-            wd::KvPrompt r;
-            r.pool = p.pool, r.scales = p.scales, r.reach = c->d_reach + static_cast<size_t>(layer) * c->cfg.n_kv_heads, r.book = p.book, r.table = p.table, r.q = p.q, r.out = p.out;
-            r.q_stride = p.q_stride, r.out_stride = p.out_stride, r.status = p.status, r.scale_log2 = p.scale_log2;
-            r.type = p.type, r.window = p.window, r.s = p.s, r.part = c->d_part, r.ctas = c->n_sm;
-            r.split = by.split;         // (the kernels count the items of the step that is current when they run)
-            const size_t size = rows_size(p.type);
-            r.vec = (reinterpret_cast<uintptr_t>(q_dev) | reinterpret_cast<uintptr_t>(out_dev)) % 16 == 0 && p.q_stride * size % 16 == 0 && p.out_stride * size % 16 == 0;
-            switch (c->cfg.head_dim) {
-                case 32: return prompt_of<32>(c, r, s);
-                case 64: return prompt_of<64>(c, r, s);
-                case 96: return prompt_of<96>(c, r, s);
-                case 128: return prompt_of<128>(c, r, s);
-                default: return prompt_of<256>(c, r, s);
-            }
-        }
-        const bool few = group <= 8;
-        switch (c->cfg.head_dim) {
-            case 32: return attend_of<32>(c, p, few, s);
-            case 64: return attend_of<64>(c, p, few, s);
-            case 96: return attend_of<96>(c, p, few, s);
-            case 128: return attend_of<128>(c, p, few, s);
-            default: return attend_of<256>(c, p, few, s);
-        }
-    });
+    return wd_host::guarded([&]() -> int { return attend_call<wd::KvAttend, wd::KvPrompt>(c, layer, q_dev, out_dev, nullptr, type, scale, window, q_stride, out_stride, stream); });
 }
 
 int wd_kv_read(wd_kv_cache *c, int layer, int n, const int *seqs, const int *firsts, const int *counts, void *k_dev, void *v_dev, int type, void *stream) {

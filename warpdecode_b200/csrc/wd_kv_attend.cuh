@@ -60,6 +60,38 @@ struct KvAttend {
     KvShape s;
 };
 
+// Where the rows of each sequence are a tree of drafts: parents[row], the row in front that a row follows, counted from its sequence's first; else -1.
+constexpr int kTreeRows = 128;              // of a sequence, at most
+struct KvAttendTree : KvAttend {
+    const int *parents;
+};
+// what a row's parent is, for the walk up to the token before the step
+__device__ __forceinline__ int tree_parent(const int *parents, int row0, int i) {
+    const int p = parents[row0 + i];
+    return p >= 0 && p < i ? p : -1;
+}
+// Which of the tokens first .. first + 127 a row of a tree sees: those in front of the step (the first of which is `start`) as its window allows, and the rows on its way
+// up. With `places` the parents of the sequence's rows; `node` the row's own.
+struct TreeSight {
+    unsigned long long lo, hi;
+};
+__device__ __forceinline__ unsigned long long tree_low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
+__device__ __forceinline__ TreeSight tree_sight(const int8_t *places, int node, int start, int first, int window) {
+    TreeSight r = {0ull, 0ull};
+    int depth = 0;
+#pragma unroll 1
+    for (int a = node; a >= 0; a = places[a], ++depth) {
+        const int o = start + a - first;
+        if (window && depth >= window) continue;        // (the walk goes on: the depth is the row's position)
+        if (o >= 0 && o < 64) r.lo |= 1ull << o;
+        else if (o >= 64 && o < 128) r.hi |= 1ull << (o - 64);
+    }
+    const int end = start - first, begin = window ? min(start, start + depth - window) - first : 0;         // (the row's position is start + depth - 1)
+    r.lo |= tree_low_bits(end) & ~tree_low_bits(begin);
+    r.hi |= tree_low_bits(end - 64) & ~tree_low_bits(begin - 64);
+    return r;
+}
+
 template <int D>
 struct AttendPlan {
     static constexpr int kCw = D % 64 == 0 ? 64 : 32;
@@ -121,8 +153,9 @@ __device__ __forceinline__ int att_tiles(int length, int count, int group_rows, 
     return min(all, (min(window, length) + tokens + 62) / 64 + 1);
 }
 
-template <int D, int N8, bool SPLIT, bool E4M3>
-__global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_constant__ KvAttend P) {
+template <int D, int N8, bool SPLIT, bool E4M3, class Params>
+__global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_constant__ Params P) {
+    constexpr bool TREE = std::is_same_v<Params, KvAttendTree>;
     using A = AttendPlan<D>;
     constexpr int CW = A::kCw, LB = CW / 4, NH = LB / 8, ROWS = 8 * N8, PITCH = D + 4;
     extern __shared__ __align__(128) uint8_t att_sm[];
@@ -137,6 +170,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
     __shared__ float *job_to[kAttWorkers * 2];                  // null: the answer
     __shared__ const float *job_from[2 * kAttMaxCtas];
     __shared__ int4 step[kAttEntries];                          // the first entries of the step
+    __shared__ int8_t places[TREE ? kAttWorkers : 1][kTreeRows];
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), worker = warp & 7;
     uint8_t *ring = att_sm + worker * P.slots * A::kSlot;
     uint8_t *qs = att_sm + P.workers * P.slots * A::kSlot + worker * A::q_bytes(N8, SPLIT);
@@ -160,10 +194,11 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
         if (n == 1) e0 = make_int4(__shfl_sync(0xffffffffu, e0.x, 0), __shfl_sync(0xffffffffu, e0.y, 0), __shfl_sync(0xffffffffu, e0.z, 0), __shfl_sync(0xffffffffu, e0.w, 0));
         auto items_of = [&](const int4 &e) { return (static_cast<long long>(e.z) * g_heads + ROWS - 1) / ROWS; };
         long long tiles = 0;
-        int most = 0;
+        int most = 0, most_rows = 0;
         for (int i = n == 1 ? 0 : lane; i < n; i += 32) {
             const int4 e = entry(i);
-            const int per = att_tiles(e.w, e.z, ROWS, g_heads, P.window);
+            const int per = att_tiles(e.w, e.z, TREE ? e.z * g_heads : ROWS, g_heads, P.window);
+            most_rows = max(most_rows, e.z);
             tiles += items_of(e) * per;
             most = max(most, per);
         }
@@ -184,7 +219,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
             if (i < n) {
                 const int4 e = entry(i);
                 if (i >= 32 && i < kAttEntries) step[i] = e;
-                v = items_of(e) * (att_tiles(e.w, e.z, ROWS, g_heads, P.window) + more);
+                v = items_of(e) * (att_tiles(e.w, e.z, TREE ? e.z * g_heads : ROWS, g_heads, P.window) + more);
             }
             long long inc = v;
 #pragma unroll
@@ -195,6 +230,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
             if (i < n) prefix[i] = sum + inc - v;
             sum += __shfl_sync(0xffffffffu, inc, 31);
         }
+        if (TREE && __any_sync(0xffffffffu, most_rows > kTreeRows)) sum = 0;        // (a replay on such a step does nothing)
         if (lane == 0) {
             prefix[n] = sum;
             of_step[0] = n;
@@ -223,7 +259,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
         }
         const int4 e = lo < kAttEntries ? step[lo] : *reinterpret_cast<const int4 *>(entries + lo * kKvStepWords);
         s.seq = e.x, s.row0 = e.y, s.count = e.z, s.length = e.w;
-        const int per_item = att_tiles(s.length, s.count, ROWS, g_heads, P.window) + extra;
+        const int per_item = att_tiles(s.length, s.count, TREE ? s.count * g_heads : ROWS, g_heads, P.window) + extra;
         const long long per_head = prefix[lo + 1] - prefix[lo], base = prefix[lo] * P.s.kv_heads, in = at - base;
         auto over = [&](long long a, long long b) { return small ? static_cast<int>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : static_cast<int>(a / b); };
         s.head = over(in, per_head);
@@ -234,7 +270,7 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
         s.rows = min(ROWS, s.count * g_heads - s.item_row);
         s.next = min(s.item1, end);
         s.whole = s.item0 >= begin && s.item1 <= end;
-        const int pos0 = s.length - s.count + s.item_row / g_heads, pos1 = s.length - s.count + (s.item_row + s.rows - 1) / g_heads;
+        const int pos0 = s.length - s.count + (TREE ? 0 : s.item_row / g_heads), pos1 = s.length - s.count + (s.item_row + s.rows - 1) / g_heads;
         const int low = P.window ? max(0, pos0 - P.window + 1) >> 6 : 0, high = (pos1 >> 6) + 1;
         s.lo = min(low + max(0, static_cast<int>(at - s.item0) - extra), high);
         s.hi = min(low + max(0, static_cast<int>(s.next - s.item0) - extra), high);
@@ -389,6 +425,12 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
                 pos[n][i] = start + min(s.item_row + 8 * n + 2 * t + i, last_row) / g_heads;
             }
         }
+        if constexpr (TREE) {
+#pragma unroll
+            for (int i = lane; i < kTreeRows; i += 32)
+                if (i < s.count) places[worker][i] = static_cast<int8_t>(tree_parent(P.parents, s.row0, i));
+            __syncwarp();
+        }
 #pragma unroll 1
         for (int tile = s.lo; tile < s.hi; ++tile) {
             // tokens x rows: x[n][b][c] is token 16 b + g + 8 (c >> 1) of the tile, row 8 n + 2 t + (c & 1)
@@ -448,7 +490,21 @@ __global__ void __launch_bounds__(kAttThreads, 1) kv_attend_kernel(const __grid_
             for (int b = 0; b < 4; ++b) sc[b] = *reinterpret_cast<const float4 *>(ring + slot * A::kSlot + 64 * D + b * 16);
             pass_on();
             const int first = tile * 64;
-            if (first + 63 > pos_lo || (P.window && first <= pos_hi - P.window)) {
+            if constexpr (TREE) {
+                if (first + 63 >= start || (P.window && first <= start + s.count - 1 - P.window)) {
+#pragma unroll
+                    for (int n = 0; n < N8; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const unsigned long long sight = tree_sight(places[worker], pos[n][i] - start, start, first, P.window).lo >> g;
+#pragma unroll
+                            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h)
+                                    if (!(sight >> (16 * b + 8 * h) & 1ull)) x[n][b][2 * h + i] = -INFINITY;
+                        }
+                }
+            } else if (first + 63 > pos_lo || (P.window && first <= pos_hi - P.window)) {
 #pragma unroll
                 for (int n = 0; n < N8; ++n)
 #pragma unroll
