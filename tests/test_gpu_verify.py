@@ -163,6 +163,40 @@ def test_tokens_come_out_as_the_target_makes_them(with_draft):
     assert count.max() == 2 and (count == 2).mean() > 0.3
 
 
+@pytest.mark.parametrize("kind", ["swapped", "few", "scaled", "one"])
+@pytest.mark.parametrize("vocab", [3000, 70001])
+def test_drafts_that_are_the_target_but_for_some_tokens(kind, vocab):
+    """Most tokens' quotient of the two probabilities lies on the border between something left and nothing, or a rounding beside it."""
+    gen = np.random.default_rng(vocab)
+    lengths, heats = [2, 4, 4, 4], [1.0, 0.7, 1.0, 1.3]
+    target = gen.standard_normal((14, vocab)) * 1.5
+    draft = target.copy()
+    for r in range(14):
+        a = gen.permutation(vocab)[:20]
+        if kind == "swapped":
+            target[r, a[:10]] += 4.0
+            draft[r, a[10:]] = target[r, a[:10]]
+            draft[r, a[:10]] = target[r, a[10:]]
+        elif kind == "few":
+            draft[r, a] += gen.standard_normal(20) * 3
+        elif kind == "scaled":
+            draft[r] = target[r] + 2.0
+            draft[r, a] += gen.standard_normal(20) * 3
+        else:
+            draft[r, a[0]] += 6.0
+    target, draft = (torch.tensor(x, dtype=torch.float32) for x in (target, draft))
+    parents = np.array([-1, 0] + [-1, 0, 0, 0] * 3)
+    first = [0, 2, 6, 10, 14]
+    root = np.repeat([0, 2, 6, 10], [2, 4, 4, 4])
+    for turn in range(6):
+        # the tokens that the draft likes better than the target, so that many are turned down
+        more = [verify_oracle.softmax(draft[r].double().numpy(), 1.0) - verify_oracle.softmax(target[r].double().numpy(), 1.0) for r in range(14)]
+        tokens = np.array([int(np.argsort(-more[r])[gen.integers(0, 3)]) for r in root])
+        u = gen.random(14).astype(np.float32)
+        got = call(target.cuda(), ints(tokens), ints(parents), torch.tensor(u, device="cuda"), draft.cuda(), ints(first), torch.tensor(heats, dtype=torch.float32, device="cuda"), 4)
+        check(got, lengths, target, draft, tokens, parents, u, [float(np.float32(t)) for t in heats])
+
+
 def test_borders():
     """Numbers that lie on a border, or at the ends of [0, 1)."""
     even = torch.zeros(1, 4, device="cuda")
