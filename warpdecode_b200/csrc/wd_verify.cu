@@ -141,8 +141,9 @@ __device__ __forceinline__ int ver_pick(const double (&v)[K], double aim, double
     return from * K + __shfl_sync(0xffffffffu, place, from);
 }
 
-template <class T, bool HELD>
-__global__ void __launch_bounds__(kVerThreads, 3) verify_kernel(const __grid_constant__ VerifyParams P) {
+// (three CTAs an SM where there is no draft; with one shared memory has room for two, and they may have the registers)
+template <class T, bool HELD, bool DRAFT>
+__global__ void __launch_bounds__(kVerThreads, DRAFT ? 2 : 3) verify_kernel(const __grid_constant__ VerifyParams P) {
     extern __shared__ __align__(16) uint8_t ver_rows[];
     __shared__ VerifyShared sh;
     cg::cluster_group cluster = cg::this_cluster();
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(kVerThreads, 3) verify_kernel(const __grid_con
     auto draft_row = [&](int i) { return static_cast<const T *>(P.draft) + static_cast<size_t>(f0 + i) * P.draft_stride; };
 
     // ---- rows in shared memory: a slot is [target, draft][warps] of run_bytes; a run lies in it as in memory, from the boundary of 16 bytes in front of it on
-    auto run_place = [&](int slot, int which, int w) { return ver_rows + (static_cast<size_t>(slot) * (P.draft ? 2 : 1) + which) * kVerWarps * P.run_bytes + static_cast<size_t>(w) * P.run_bytes; };
+    auto run_place = [&](int slot, int which, int w) { return ver_rows + (static_cast<size_t>(slot) * (DRAFT ? 2 : 1) + which) * kVerWarps * P.run_bytes + static_cast<size_t>(w) * P.run_bytes; };
     auto beside = [](const T *x) { return static_cast<int>(reinterpret_cast<uintptr_t>(x) & 15u); };
     auto copy_run = [&](const T *x, uint8_t *to) {
         const T *from = x + run0;
@@ -214,7 +215,7 @@ __global__ void __launch_bounds__(kVerThreads, 3) verify_kernel(const __grid_con
         sh.parents[i] = static_cast<int16_t>(p >= 0 && p < i ? p : -1);
     }
     if (tid < 32) sh.power[tid] = P.power[tid];
-    const bool greedy = !(heat >= kVerGreedy), with_draft = P.draft && !greedy;
+    const bool greedy = !(heat >= kVerGreedy), with_draft = DRAFT && !greedy;
     const float k = greedy ? 1.44269504f : fmaxf(static_cast<float>(1.4426950408889634 / heat), 1e-30f);        // (not 0: -inf times k has to stay what it is)
     const double k32 = greedy ? 0.0 : 32 * 1.4426950408889634 / heat;
     if constexpr (HELD) {
@@ -651,9 +652,9 @@ __global__ void __launch_bounds__(kVerThreads, 3) verify_kernel(const __grid_con
     }
 }
 
-template <class T, bool HELD>
+template <class T, bool HELD, bool DRAFT>
 int verify_launch(const VerifyParams &p, size_t smem, cudaStream_t s) {
-    auto kernel = verify_kernel<T, HELD>;
+    auto kernel = verify_kernel<T, HELD, DRAFT>;
     WD_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
     if (p.ctas > 8) WD_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t cfg = {};
@@ -680,11 +681,12 @@ int verify_of(VerifyParams p, int n_sm, cudaStream_t s) {
     const long long run_bytes = static_cast<long long>(p.piece) * 32 * sizeof(T) + 16, slot = run_bytes * kVerWarps * (p.draft ? 2 : 1), most = 227 * 1024 - static_cast<long long>(sizeof(VerifyShared)) - 1024;
     if (slot > most) {
         p.slots = p.run_bytes = 0;
-        return verify_launch<T, false>(p, 0, s);
+        return p.draft ? verify_launch<T, false, true>(p, 0, s) : verify_launch<T, false, false>(p, 0, s);
     }
     p.run_bytes = static_cast<int>(run_bytes);
     p.slots = static_cast<long long>(p.n_seqs) * p.ctas <= n_sm ? static_cast<int>(std::min<long long>(kVerSlots, most / slot)) : 1;
-    return verify_launch<T, true>(p, static_cast<size_t>(slot) * p.slots, s);
+    const size_t smem = static_cast<size_t>(slot) * p.slots;
+    return p.draft ? verify_launch<T, true, true>(p, smem, s) : verify_launch<T, true, false>(p, smem, s);
 }
 
 }  // namespace
