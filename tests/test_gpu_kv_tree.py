@@ -9,7 +9,7 @@ import warpdecode_b200 as wd
 from test_gpu_kv_cache import GEOMETRY, TYPES, Pair
 
 pytestmark = pytest.mark.gpu
-FEW, PROMPT, RUNS = "kv_attend_kernel", "kv_prompt_kernel", "kv_prompt_kernel, kv_prompt_join_kernel"
+FEW, TREE = "kv_attend_kernel", "kv_tree_kernel"
 
 
 def make_tree(n, rng, kind):
@@ -91,11 +91,13 @@ def test_windows_count_positions(geometry, window):
     check(p, [2, 0, 1], counts, [x for n in counts for x in make_tree(n, rng, "any")], window=window)
 
 
-LONG = [(FEW, [8100, 70, 0, 301], [2, 1, 3, 5]), (RUNS, [8100], [128]), (RUNS, [8100, 100], [128, 3]), (PROMPT, [300, 170, 0, 255, 256, 257, 100, 290], [128] * 7 + [77])]
+SIZES = [(FEW, [8100, 70, 0, 301], [2, 1, 3, 5]), (TREE, [8100], [128]), (TREE, [8100, 100], [128, 3]), (None, [130], [64]), (None, [300, 170, 0, 255], [128] * 4),
+         (TREE, [300, 8000, 0, 255, 256, 257, 1000, 2900], [128] * 7 + [77])]
 
 
-@pytest.mark.parametrize("geometry", [(32, 1, 64, 64, 0, "bf16"), (64, 1, 128, 64, 1, "f32"), (16, 1, 256, 128, 0, "bf16"), (32, 1, 96, 32, 0, "f16"), (32, 1, 64, 16, 1, "f32"), (16, 1, 256, 64, 1, "f32")])
-@pytest.mark.parametrize("kernel,before,counts", LONG)
+@pytest.mark.parametrize("geometry", [(32, 1, 64, 64, 0, "bf16"), (64, 1, 128, 64, 1, "f32"), (16, 1, 256, 128, 0, "bf16"), (32, 1, 96, 32, 0, "f16"), (32, 1, 64, 16, 1, "f32"), (16, 1, 256, 64, 1, "f32"),
+                                      (32, 2, 32, 16, 0, "bf16"), (32, 1, 128, 128, 0, "bf16")])
+@pytest.mark.parametrize("kernel,before,counts", SIZES)
 def test_every_kernel(geometry, kernel, before, counts):
     p, rng = Pair(*geometry, n_pages=4000, max_context=9000, layers=2), random.Random(1)
     seqs = list(range(len(before)))
@@ -103,6 +105,36 @@ def test_every_kernel(geometry, kernel, before, counts):
     p.step(seqs, counts)
     check(p, seqs, counts, [x for n in counts for x in make_tree(n, rng, "any")], kernel=kernel)
     check(p, seqs, counts, [x for n in counts for x in make_tree(n, rng, "any")], window=150)
+    check(p, seqs, counts, [x for n in counts for x in make_tree(n, rng, "any")], window=1500)
+
+
+@pytest.mark.parametrize("dtype,tokens", [("f32", 70000), ("bf16", 140000)])
+def test_sums_that_are_brought_to_memory(dtype, tokens):
+    """More tiles of a CTA than one sum may hold: a few values of one sign, whose sums a tensor core would cut off."""
+    p = Pair(64, 1, 64, 128, 0, dtype, n_pages=tokens // 128 + 8, max_seqs=1, max_context=tokens + 256, layers=1)
+    gen = torch.Generator().manual_seed(7)
+    t = TYPES[dtype][0]
+    rows = lambda n: ((torch.randn(n, 1, 64, generator=gen) * 0.3).to(t), (torch.rand(n, 1, 64, generator=gen) + 0.5).to(t))  # noqa: E731
+    p.step([0], [tokens], rows=[rows(tokens)])
+    p.step([0], [128], rows=[rows(128)])
+    q = (torch.randn(128, 64, 64, generator=gen) * 0.3).to(t)
+    parents = make_tree(128, random.Random(3), "any")
+    qd, pd = q.cuda(), torch.tensor(parents, dtype=torch.int32, device="cuda")
+    out = torch.empty_like(qd)
+    torch.cuda.synchronize()
+    p.kv.attend_tree(0, qd.data_ptr(), out.data_ptr(), pd.data_ptr(), TYPES[dtype][1])
+    torch.cuda.synchronize()
+    assert p.kv.kernel_name() == TREE and p.kv.status() == 0
+    k, v = p.ref[0].numbers(0)
+    see = seen(parents, tokens, 0)
+    for r in (0, 1, 64, 127):
+        for h in (0, 37, 63):
+            x = np.where(see[r], k[:, 0] @ q[r, h].double().numpy() / 8, -np.inf)
+            w = np.exp(x - x.max())
+            want = w @ v[:, 0] / w.sum()
+            # the answer's rounding, half a step of the weights' (16 bits), and what the sums may be cut off by: 2^-13 (F32 rows 2^-15)
+            tol = 2.0 ** -14 if dtype == "f32" else 2.0 ** -8 + 2.0 ** -11 + 2.0 ** -12
+            assert np.abs(out[r, h].double().cpu().numpy() - want).max() <= tol * np.abs(want).max()
 
 
 @pytest.mark.parametrize("count", [1, 6, 128])
@@ -112,10 +144,14 @@ def test_a_chain_is_attention(count):
         p.step([0, 1], [333, 50])
         p.step([0, 1], [count, 3])
         qd, out, _ = check(p, [0, 1], [count, 3], make_tree(count, None, "chain") + [-1, 0, 1], layer=0)
-        same = torch.empty_like(out)
+        same, kernel = torch.empty_like(out), p.kv.kernel_name()
         p.kv.attend(0, qd.data_ptr(), same.data_ptr(), TYPES[p.dtype][1])
         torch.cuda.synchronize()
-        assert torch.equal(out, same)
+        if kernel == p.kv.kernel_name():
+            assert torch.equal(out, same)
+        want = p.ref[0].attend(0, qd[:count].double().cpu().numpy(), p.dim ** -0.5, 0)
+        for x in (out, same):
+            assert np.abs(x[:count].double().cpu().numpy() - want).max() <= p.tolerance(qd.cpu(), [0], layer=0) * np.abs(p.ref[0].numbers(0)[1]).max()
 
 
 def test_parents_that_are_no_row_in_front():

@@ -20,7 +20,7 @@ SOURCES = [os.path.join(HERE, "csrc", f) for f in
            ("wd_engine.cu", "wd_aux_kernels.cuh", "wd_moe_kernel.cuh", "wd_moe_kernel_phases.inc", "wd_moe_fast.cuh", "wd_moe_batch.cuh", "wd_dense_decoder.cuh", "wd_dense_decoder.inc", "wd_dense_token.cuh", "wd_dense_prefill.cuh", "wd_dense_prompt_tc.cuh",
             "wd_plain_moe.cuh", "wd_plain_wide.cuh", "wd_plain_moe.inc", "wd_blocks.cuh", "wd_router.cuh",
             "wd_formats.cuh", "wd_device.cuh", "wd_dense.cuh", "wd_gguf.inc",
-            "wd_grids.h", "wd_host.h", "wd_tcgen05.cuh", "wd_kv.cu", "wd_kv_rope.cu", "wd_kv_tree.cu", "wd_kv_host.h", "wd_kv_launch.cuh", "wd_kv_layout.cuh", "wd_kv_append.cuh", "wd_kv_kernels.cuh", "wd_kv_attend.cuh", "wd_kv_prompt.cuh", "wd_score.cu", "wd_verify.cu")] + [
+            "wd_grids.h", "wd_host.h", "wd_tcgen05.cuh", "wd_kv.cu", "wd_kv_rope.cu", "wd_kv_tree.cu", "wd_kv_tree.cuh", "wd_kv_host.h", "wd_kv_launch.cuh", "wd_kv_layout.cuh", "wd_kv_append.cuh", "wd_kv_kernels.cuh", "wd_kv_attend.cuh", "wd_kv_prompt.cuh", "wd_score.cu", "wd_verify.cu")] + [
                os.path.join(ROOT, "include", "warpdecode_b200.h")]
 _HOST = ("wd_device", "wd_host", "warpdecode")
 

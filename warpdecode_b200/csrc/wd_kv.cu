@@ -124,7 +124,7 @@ int wd_kv_create(const wd_kv_config *cfg, wd_kv_cache **out) {
         const size_t part = static_cast<size_t>(k->n_sm) * 2 * wd::kAttMaxRows * (c.head_dim + 4) * 4;     // of a CTA, or of a worker
         // (zeros are codes, so that no part of a page ever holds what is not one)
         if (alloc(&k->d_pool, k->pool_layer * c.n_layers) != cudaSuccess || alloc(&k->d_scales, k->scales_layer * c.n_layers * 4) != cudaSuccess ||
-            alloc(&k->d_part, part * wd::kAttWorkers) != cudaSuccess || alloc(&k->d_cta_part, part) != cudaSuccess || alloc(&k->d_book, words * 4) != cudaSuccess ||
+            alloc(&k->d_part, part * wd::kAttWorkers * wd::kTreeUnits / 2) != cudaSuccess || alloc(&k->d_cta_part, part) != cudaSuccess || alloc(&k->d_book, words * 4) != cudaSuccess ||
             alloc(&k->d_index, (static_cast<size_t>(c.max_context) + k->shape.max_pages) * 4) != cudaSuccess ||
             alloc(&k->d_arrived, static_cast<size_t>(k->n_sm) * 4) != cudaSuccess || alloc(&k->d_status, 16) != cudaSuccess ||
             alloc(&k->d_reach, static_cast<size_t>(c.n_layers) * c.n_kv_heads * sizeof(int2)) != cudaSuccess)
@@ -244,7 +244,26 @@ int wd_kv_append(wd_kv_cache *c, int layer, const void *k_dev, const void *v_dev
 }
 
 int wd_kv_attend(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, int type, float scale, int window, int64_t q_stride, int64_t out_stride, void *stream) {
-    return wd_host::guarded([&]() -> int { return attend_call<wd::KvAttend, wd::KvPrompt>(c, layer, q_dev, out_dev, nullptr, type, scale, window, q_stride, out_stride, stream); });
+    return wd_host::guarded([&]() -> int {
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        wd::KvAttend p;
+        int rc = WD_OK;
+        if (!attend_ready(c, layer, q_dev, out_dev, type, scale, window, q_stride, out_stride, s, p, rc)) return rc;
+        OnDevice on(c->cfg.device);
+        if (int r = note_capture(c, s)) return r;
+        const Choice by = choose(c, p.type == wd::kRowsF32, p.window);
+        if (!by.prompt) return attend_few(c, p, s);
+        c->last_kernel = by.split ? "kv_prompt_kernel, kv_prompt_join_kernel" : "kv_prompt_kernel";
+        wd::KvPrompt r;
+        fill_prompt(c, layer, p, by.split, &r);
+        switch (c->cfg.head_dim) {
+            case 32: return prompt_of<32>(c, r, s);
+            case 64: return prompt_of<64>(c, r, s);
+            case 96: return prompt_of<96>(c, r, s);
+            case 128: return prompt_of<128>(c, r, s);
+            default: return prompt_of<256>(c, r, s);
+        }
+    });
 }
 
 int wd_kv_read(wd_kv_cache *c, int layer, int n, const int *seqs, const int *firsts, const int *counts, void *k_dev, void *v_dev, int type, void *stream) {

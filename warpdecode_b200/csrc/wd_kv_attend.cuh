@@ -62,6 +62,7 @@ struct KvAttend {
 
 // Where the rows of each sequence are a tree of drafts: parents[row], the row in front that a row follows, counted from its sequence's first; else -1.
 constexpr int kTreeRows = 128;              // of a sequence, at most
+constexpr int kTreeUnits = 3;               // of 128 rows, of the parts that a CTA of the kernel on tensor cores (wd_kv_tree.cuh) has
 struct KvAttendTree : KvAttend {
     const int *parents;
 };

@@ -7,7 +7,7 @@
 
 namespace wd_kv {
 
-// (P: wd::KvAttend, or wd::KvAttendTree; R: wd::KvPrompt, or wd::KvPromptTree)
+// (P: wd::KvAttend, or wd::KvAttendTree)
 template <int D, int N8, bool SPLIT, class P>
 int attend_launch(wd_kv_cache *c, P &p, cudaStream_t s) {
     using A = wd::AttendPlan<D>;
@@ -41,7 +41,7 @@ int attend_of(wd_kv_cache *c, P &p, bool few, cudaStream_t s) {
 struct Choice {
     bool prompt, split;
 };
-inline Choice choose(const wd_kv_cache *c, bool f32, int window, bool tree) {
+inline Choice choose(const wd_kv_cache *c, bool f32, int window) {
     const int g = c->cfg.n_heads / c->cfg.n_kv_heads, d = c->cfg.head_dim, h = c->cfg.n_kv_heads;
     const int few_rows = d > 128 ? 8 : 16, item_rows = d > 128 ? 128 : 256;
     double few = 0.0, tiles = 0.0;
@@ -51,7 +51,7 @@ inline Choice choose(const wd_kv_cache *c, bool f32, int window, bool tree) {
         const int *e = c->book.data() + wd::kKvHead + static_cast<size_t>(i) * wd::kKvStepWords;
         const long long rows = static_cast<long long>(e[2]) * g;
         if (rows == 0) continue;
-        const int seen = window ? std::min(e[3], window + (tree ? e[2] : item_rows / g)) : e[3], n = (seen + 127) / 128;
+        const int seen = window ? std::min(e[3], window + item_rows / g) : e[3], n = (seen + 127) / 128;
         const long long blocks = (rows + item_rows - 1) / item_rows;
         few += static_cast<double>((rows + few_rows - 1) / few_rows) * h * ((seen + 63) / 64);
         tiles += static_cast<double>(blocks) * h * n;
@@ -68,51 +68,44 @@ inline Choice choose(const wd_kv_cache *c, bool f32, int window, bool tree) {
     return r;
 }
 
-template <int D, bool SPLIT, class R>
-int prompt_launch(wd_kv_cache *c, const R &p, cudaStream_t s) {
+template <int D, bool SPLIT>
+int prompt_launch(wd_kv_cache *c, const wd::KvPrompt &p, cudaStream_t s) {
     return by_codes(c, [&](auto e4m3) {
-        auto kernel = wd::kv_prompt_kernel<D, SPLIT, decltype(e4m3)::value, R>;
+        auto kernel = wd::kv_prompt_kernel<D, SPLIT, decltype(e4m3)::value>;
         constexpr int smem = wd::PromptAttPlan<D, SPLIT>::kSmem;
-        static_assert(smem <= 225 * 1024, "beside the 2 KB that the kernel declares itself");
         WD_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         kernel<<<c->n_sm, wd::kPromptThreads, smem, s>>>(p);
-        if (p.split) wd::kv_prompt_join_kernel<D, R><<<2 * c->n_sm, 256, 0, s>>>(p);
+        if (p.split) wd::kv_prompt_join_kernel<D><<<2 * c->n_sm, 256, 0, s>>>(p);
         WD_TRY_CUDA(cudaGetLastError());
         return WD_OK;
     });
 }
-template <int D, class R>
-int prompt_of(wd_kv_cache *c, const R &p, cudaStream_t s) {
+template <int D>
+int prompt_of(wd_kv_cache *c, const wd::KvPrompt &p, cudaStream_t s) {
     return p.type == wd::kRowsF32 ? prompt_launch<D, true>(c, p, s) : prompt_launch<D, false>(c, p, s);
 }
 
-// wd_kv_attend, or with parents wd_kv_attend_tree
-template <class A, class R>
-int attend_call(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, const int *parents_dev, int type, float scale, int window, int64_t q_stride, int64_t out_stride, void *stream) {
-    constexpr bool kTree = std::is_same_v<A, wd::KvAttendTree>;
-    if (int rc = check_device(c)) return rc;
-    if (layer < 0 || layer >= c->cfg.n_layers) return set_error(WD_E_INVALID, "key/value cache: layer out of range");
-    if (!(scale > 0.0f && scale * 1.4426950408889634 <= 3.4028234663852886e38)) return set_error(WD_E_INVALID, "key/value cache: the scale of the scores must be positive and finite");
-    if (window < 0) return set_error(WD_E_INVALID, "key/value cache: a window is 0 (none) or at least 1");
-    A p;
-    if (int rc = rows_type(type, &p.type)) return rc;
-    if (c->book[0] == 0) return set_error(WD_E_STATE, "key/value cache: no step has begun");
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (c->rows == 0) return check_not_captured(c, s);
-    if (window >= c->cfg.max_context) window = 0;
-    if constexpr (kTree) {
-        if (!parents_dev || reinterpret_cast<uintptr_t>(parents_dev) % 4) return set_error(WD_E_INVALID, "key/value cache: parents are null, or not aligned to their type");
-        if (c->max_rows > wd::kTreeRows) return set_error(WD_E_INVALID, "key/value cache: a tree has at most 128 rows");
-        p.parents = parents_dev;
-    }
-    p.q_stride = q_stride;
-    p.out_stride = out_stride;
-    const long long width = static_cast<long long>(c->cfg.n_heads) * c->cfg.head_dim;
-    if (int rc = check_rows(q_dev, rows_size(p.type), &p.q_stride, width, "q")) return rc;
-    if (int rc = check_rows(out_dev, rows_size(p.type), &p.out_stride, width, "out")) return rc;
-    if (q_dev == out_dev && p.q_stride != p.out_stride) return set_error(WD_E_INVALID, "key/value cache: out over q needs q's stride");
-    OnDevice on(c->cfg.device);
-    if (int rc = note_capture(c, s)) return rc;
+// What attention calls check, and the launch of the kernel for few rows, p; rc is set where there is nothing more to do.
+template <class P>
+bool attend_ready(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, int type, float scale, int window, int64_t q_stride, int64_t out_stride, cudaStream_t s, P &p, int &rc) {
+    auto check = [&]() -> int {
+        if (int r = check_device(c)) return r;
+        if (layer < 0 || layer >= c->cfg.n_layers) return set_error(WD_E_INVALID, "key/value cache: layer out of range");
+        if (!(scale > 0.0f && scale * 1.4426950408889634 <= 3.4028234663852886e38)) return set_error(WD_E_INVALID, "key/value cache: the scale of the scores must be positive and finite");
+        if (window < 0) return set_error(WD_E_INVALID, "key/value cache: a window is 0 (none) or at least 1");
+        if (int r = rows_type(type, &p.type)) return r;
+        if (c->book[0] == 0) return set_error(WD_E_STATE, "key/value cache: no step has begun");
+        if (c->rows == 0) return check_not_captured(c, s);
+        p.q_stride = q_stride;
+        p.out_stride = out_stride;
+        const long long width = static_cast<long long>(c->cfg.n_heads) * c->cfg.head_dim;
+        if (int r = check_rows(q_dev, rows_size(p.type), &p.q_stride, width, "q")) return r;
+        if (int r = check_rows(out_dev, rows_size(p.type), &p.out_stride, width, "out")) return r;
+        if (q_dev == out_dev && p.q_stride != p.out_stride) return set_error(WD_E_INVALID, "key/value cache: out over q needs q's stride");
+        return WD_OK;
+    };
+    rc = check();
+    if (rc || c->rows == 0) return false;
     p.pool = c->d_pool + layer * c->pool_layer;
     p.scales = c->d_scales + layer * c->scales_layer;
     p.book = c->d_book;
@@ -124,31 +117,25 @@ int attend_call(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, con
     p.arrived = c->d_arrived;
     p.status = c->d_status;
     p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-    p.window = window;
+    p.window = window >= c->cfg.max_context ? 0 : window;
     p.max_seqs = c->cfg.max_seqs;
     p.vec = reinterpret_cast<uintptr_t>(q_dev) % 16 == 0 && p.q_stride * rows_size(p.type) % 16 == 0;
     p.s = c->shape;
-    const long long group = static_cast<long long>(c->max_rows) * (c->cfg.n_heads / c->cfg.n_kv_heads);
-    const Choice by = choose(c, p.type == wd::kRowsF32, window, kTree);
-    c->last_kernel = by.prompt ? by.split ? "kv_prompt_kernel, kv_prompt_join_kernel" : "kv_prompt_kernel" : "kv_attend_kernel";
-    if (by.prompt) {
-        R r;
-        r.pool = p.pool, r.scales = p.scales, r.reach = c->d_reach + static_cast<size_t>(layer) * c->cfg.n_kv_heads, r.book = p.book, r.table = p.table, r.q = p.q, r.out = p.out;
-        r.q_stride = p.q_stride, r.out_stride = p.out_stride, r.status = p.status, r.scale_log2 = p.scale_log2;
-        r.type = p.type, r.window = p.window, r.s = p.s, r.part = c->d_part, r.ctas = c->n_sm;
-        r.split = by.split;         // (the kernels count the items of the step that is current when they run)
-        const size_t size = rows_size(p.type);
-        r.vec = (reinterpret_cast<uintptr_t>(q_dev) | reinterpret_cast<uintptr_t>(out_dev)) % 16 == 0 && p.q_stride * size % 16 == 0 && p.out_stride * size % 16 == 0;
-        if constexpr (kTree) r.parents = parents_dev;
-        switch (c->cfg.head_dim) {
-            case 32: return prompt_of<32>(c, r, s);
-            case 64: return prompt_of<64>(c, r, s);
-            case 96: return prompt_of<96>(c, r, s);
-            case 128: return prompt_of<128>(c, r, s);
-            default: return prompt_of<256>(c, r, s);
-        }
-    }
-    const bool few = group <= 8;
+    return true;
+}
+// the same for the kernels on tensor cores
+inline void fill_prompt(const wd_kv_cache *c, int layer, const wd::KvAttend &p, bool split, wd::KvPrompt *r) {
+    r->pool = p.pool, r->scales = p.scales, r->reach = c->d_reach + static_cast<size_t>(layer) * c->cfg.n_kv_heads, r->book = p.book, r->table = p.table, r->q = p.q, r->out = p.out;
+    r->q_stride = p.q_stride, r->out_stride = p.out_stride, r->status = p.status, r->scale_log2 = p.scale_log2;
+    r->type = p.type, r->window = p.window, r->s = p.s, r->part = c->d_part, r->ctas = c->n_sm;
+    r->split = split;         // (the kernels count the items of the step that is current when they run)
+    const size_t size = rows_size(p.type);
+    r->vec = (reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.out)) % 16 == 0 && p.q_stride * size % 16 == 0 && p.out_stride * size % 16 == 0;
+}
+template <class P>
+int attend_few(wd_kv_cache *c, P &p, cudaStream_t s) {
+    c->last_kernel = "kv_attend_kernel";
+    const bool few = static_cast<long long>(c->max_rows) * (c->cfg.n_heads / c->cfg.n_kv_heads) <= 8;
     switch (c->cfg.head_dim) {
         case 32: return attend_of<32>(c, p, few, s);
         case 64: return attend_of<64>(c, p, few, s);

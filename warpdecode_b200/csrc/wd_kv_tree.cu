@@ -1,11 +1,83 @@
-// Attention over the 8-bit cache where the rows of each sequence are a tree of drafted tokens (wd_kv_attend_tree): the kernels of wd_kv_attend, which look up a
-// row's way to the root where a tile of tokens reaches into the step.
+// Attention over the 8-bit cache where the rows of each sequence are a tree of drafted tokens (wd_kv_attend_tree).
 #include "wd_kv_launch.cuh"
+#include "wd_kv_tree.cuh"
 
 using namespace wd_kv;
 
+namespace {
+
+static_assert(wd::kTreeUnits * 128 <= 2 * wd::kAttMaxRows * wd::kAttWorkers * wd::kTreeUnits / 2, "the parts that a cache allocates");
+
+// Which of the two kernels a step takes, as choose() does for chains.
+//   for few rows   see choose()
+//   for trees      5 more, and c_t for 128 tokens by 128 rows and CTA; what it costs to join cut items is counted as four tiles
+Choice choose_tree(const wd_kv_cache *c, bool f32, int window) {
+    const int g = c->cfg.n_heads / c->cfg.n_kv_heads, d = c->cfg.head_dim, h = c->cfg.n_kv_heads, few_rows = d > 128 ? 8 : 16;
+    double few = 0.0;
+    long long items = 0, total = 0;
+    int most = 0;
+    for (int i = 0; i < c->book[0]; ++i) {
+        const int *e = c->book.data() + wd::kKvHead + static_cast<size_t>(i) * wd::kKvStepWords;
+        const long long rows = static_cast<long long>(e[2]) * g;
+        if (rows == 0) continue;
+        const int n = wd::tree_tiles(e[3], e[2], window, 128);
+        const long long blocks = (rows + 127) / 128;
+        few += static_cast<double>((rows + few_rows - 1) / few_rows) * h * 2 * n;
+        items += blocks * h;
+        total += blocks * h * n;
+        most = std::max(most, n);
+    }
+    Choice r;
+    const long long chunk = wd::tree_chunk(total, c->n_sm, most, 128), whole = (items + c->n_sm - 1) / c->n_sm * most;
+    r.split = whole > chunk + 4;
+    const double c_f = d / 36.0 * (f32 ? 1.2 : 1.0) * (d > 128 ? 0.25 : 1.0), c_t = (d > 128 ? 4.2 : 0.5 + d / 200.0) * (f32 ? 1.3 : 1.0);
+    r.prompt = 5.0 + c_t * static_cast<double>(r.split ? chunk + 4 : whole) < c_f * few / (c->n_sm * (d > 128 ? 4.0 : 8.0));
+    return r;
+}
+
+template <int D, bool SPLIT>
+int tree_launch(wd_kv_cache *c, const wd::KvTree &p, cudaStream_t s) {
+    return by_codes(c, [&](auto e4m3) {
+        using A = wd::TreePlan<D, SPLIT>;
+        auto kernel = wd::kv_tree_kernel<D, SPLIT, decltype(e4m3)::value>;
+        WD_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, A::kSmem));
+        kernel<<<c->n_sm, wd::kPromptThreads, A::kSmem, s>>>(p);
+        WD_TRY_CUDA(cudaGetLastError());
+        return WD_OK;
+    });
+}
+template <int D>
+int tree_of(wd_kv_cache *c, const wd::KvTree &p, cudaStream_t s) {
+    return p.type == wd::kRowsF32 ? tree_launch<D, true>(c, p, s) : tree_launch<D, false>(c, p, s);
+}
+
+}  // namespace
+
 extern "C" int wd_kv_attend_tree(wd_kv_cache *c, int layer, const void *q_dev, void *out_dev, const int *parents_dev, int type, float scale, int window, int64_t q_stride,
                                  int64_t out_stride, void *stream) {
-    return wd_host::guarded(
-        [&]() -> int { return attend_call<wd::KvAttendTree, wd::KvPromptTree>(c, layer, q_dev, out_dev, parents_dev, type, scale, window, q_stride, out_stride, stream); });
+    return wd_host::guarded([&]() -> int {
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        wd::KvAttendTree p;
+        int rc = WD_OK;
+        if (!attend_ready(c, layer, q_dev, out_dev, type, scale, window, q_stride, out_stride, s, p, rc)) return rc;
+        if (!parents_dev || reinterpret_cast<uintptr_t>(parents_dev) % 4) return set_error(WD_E_INVALID, "key/value cache: parents are null, or not aligned to their type");
+        if (c->max_rows > wd::kTreeRows) return set_error(WD_E_INVALID, "key/value cache: a tree has at most 128 rows");
+        p.parents = parents_dev;
+        OnDevice on(c->cfg.device);
+        if (int r = note_capture(c, s)) return r;
+        const Choice by = choose_tree(c, p.type == wd::kRowsF32, p.window);
+        if (!by.prompt) return attend_few(c, p, s);
+        c->last_kernel = "kv_tree_kernel";
+        wd::KvTree r;
+        fill_prompt(c, layer, p, by.split, &r);
+        r.parents = parents_dev;
+        r.arrived = c->d_arrived;
+        switch (c->cfg.head_dim) {
+            case 32: return tree_of<32>(c, r, s);
+            case 64: return tree_of<64>(c, r, s);
+            case 96: return tree_of<96>(c, r, s);
+            case 128: return tree_of<128>(c, r, s);
+            default: return tree_of<256>(c, r, s);
+        }
+    });
 }
