@@ -60,7 +60,7 @@ def check(p, seqs, counts, parents, window=0, kernel=None, layer=1):
     p.kv.attend_tree(layer, qd.data_ptr(), out.data_ptr(), pd.data_ptr(), TYPES[p.dtype][1], window=window)
     torch.cuda.synchronize()
     if kernel:
-        assert p.kv.kernel_name() == kernel
+        assert p.kv.kernel_name().startswith(kernel)
     want, got = attend(p, layer, seqs, counts, q, parents, p.dim ** -0.5, window), out.double().cpu().numpy()
     values = max(np.abs(p.ref[layer].numbers(s)[1]).max() for s in seqs)
     assert np.abs(got - want).max() <= p.tolerance(q, seqs, layer=layer) * values
@@ -124,7 +124,7 @@ def test_sums_that_are_brought_to_memory(dtype, tokens):
     torch.cuda.synchronize()
     p.kv.attend_tree(0, qd.data_ptr(), out.data_ptr(), pd.data_ptr(), TYPES[dtype][1])
     torch.cuda.synchronize()
-    assert p.kv.kernel_name() == TREE and p.kv.status() == 0
+    assert p.kv.kernel_name().startswith(TREE) and p.kv.status() == 0
     k, v = p.ref[0].numbers(0)
     see = seen(parents, tokens, 0)
     for r in (0, 1, 64, 127):

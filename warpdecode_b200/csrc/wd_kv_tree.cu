@@ -8,9 +8,12 @@ namespace {
 
 static_assert(wd::kTreeUnits * 128 <= 2 * wd::kAttMaxRows * wd::kAttWorkers * wd::kTreeUnits / 2, "the parts that a cache allocates");
 
-// Which of the two kernels a step takes, as choose() does for chains.
-//   for few rows   see choose()
-//   for trees      5 more, and c_t for 128 tokens by 128 rows and CTA; what it costs to join cut items is counted as four tiles
+// Which of the two kernels a step takes: the one that is expected to be through first, by what each was measured to take (us, d the head's size):
+//   for few rows   11, and 1.2 (heads of 256 1.6) times what choose() counts
+//   for trees      12 + d / 16 (F32 rows 3 more), and 0.85 + d^2 / 17,500 (F32 rows 1.3 times that) for 128 tokens by 128 rows and CTA; an item counts
+//                  kTreeExtra tiles more, and the second kernel, which joins items that are cut, four
+// (32 heads over 8 of 128, 16 sequences of 26 rows behind 300 to 6,000: 137 against 58 us; one of 13 rows behind 131: 12 against 16; 64 of 8 rows behind 90 to
+// 3,000, of 64: 57 against 72.)
 Choice choose_tree(const wd_kv_cache *c, bool f32, int window) {
     const int g = c->cfg.n_heads / c->cfg.n_kv_heads, d = c->cfg.head_dim, h = c->cfg.n_kv_heads, few_rows = d > 128 ? 8 : 16;
     double few = 0.0;
@@ -24,14 +27,15 @@ Choice choose_tree(const wd_kv_cache *c, bool f32, int window) {
         const long long blocks = (rows + 127) / 128;
         few += static_cast<double>((rows + few_rows - 1) / few_rows) * h * 2 * n;
         items += blocks * h;
-        total += blocks * h * n;
+        total += blocks * h * (n + wd::kTreeExtra);
         most = std::max(most, n);
     }
     Choice r;
-    const long long chunk = wd::tree_chunk(total, c->n_sm, most, 128), whole = (items + c->n_sm - 1) / c->n_sm * most;
-    r.split = whole > chunk + 4;
-    const double c_f = d / 36.0 * (f32 ? 1.2 : 1.0) * (d > 128 ? 0.25 : 1.0), c_t = (d > 128 ? 4.2 : 0.5 + d / 200.0) * (f32 ? 1.3 : 1.0);
-    r.prompt = 5.0 + c_t * static_cast<double>(r.split ? chunk + 4 : whole) < c_f * few / (c->n_sm * (d > 128 ? 4.0 : 8.0));
+    const long long chunk = wd::tree_chunk(total, c->n_sm, most, 128), whole = (items + c->n_sm - 1) / c->n_sm * (most + wd::kTreeExtra);
+    r.split = whole > chunk + wd::kTreeExtra + 4;
+    const double c_f = d / 36.0 * (f32 ? 1.2 : 1.0) * (d > 128 ? 0.4 : 1.2), c_t = (0.85 + d * d / 17500.0) * (f32 ? 1.3 : 1.0);
+    const double of_few = 11.0 + c_f * few / (c->n_sm * (d > 128 ? 4.0 : 8.0)), of_tree = 12.0 + d / 16.0 + (f32 ? 3.0 : 0.0) + c_t * static_cast<double>(r.split ? chunk : whole);
+    r.prompt = of_tree < of_few;
     return r;
 }
 
@@ -43,6 +47,17 @@ int tree_launch(wd_kv_cache *c, const wd::KvTree &p, cudaStream_t s) {
         WD_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, A::kSmem));
         kernel<<<c->n_sm, wd::kPromptThreads, A::kSmem, s>>>(p);
         WD_TRY_CUDA(cudaGetLastError());
+        if (!p.split) return WD_OK;
+        cudaLaunchConfig_t cfg = {};            // (its blocks may take their places while the last CTAs of the first kernel work)
+        cfg.gridDim = dim3(c->n_sm, 128 / wd::kTreeJoinRows<D>);
+        cfg.blockDim = dim3(256);
+        cfg.stream = s;
+        cudaLaunchAttribute a[1];
+        a[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        a[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = a;
+        cfg.numAttrs = 1;
+        WD_TRY_CUDA(cudaLaunchKernelEx(&cfg, wd::kv_tree_join_kernel<D>, p));
         return WD_OK;
     });
 }
@@ -67,11 +82,11 @@ extern "C" int wd_kv_attend_tree(wd_kv_cache *c, int layer, const void *q_dev, v
         if (int r = note_capture(c, s)) return r;
         const Choice by = choose_tree(c, p.type == wd::kRowsF32, p.window);
         if (!by.prompt) return attend_few(c, p, s);
-        c->last_kernel = "kv_tree_kernel";
+        c->last_kernel = by.split ? "kv_tree_kernel, kv_tree_join_kernel" : "kv_tree_kernel";
         wd::KvTree r;
         fill_prompt(c, layer, p, by.split, &r);
         r.parents = parents_dev;
-        r.arrived = c->d_arrived;
+        r.cuts = reinterpret_cast<int4 *>(c->d_cta_part);
         switch (c->cfg.head_dim) {
             case 32: return tree_of<32>(c, r, s);
             case 64: return tree_of<64>(c, r, s);

@@ -2,8 +2,10 @@
 // (wd_kv_prompt.cuh); which of the step's tokens a row sees is looked up on its way to the root, where a tile reaches into the step.
 //
 // A tree has few rows and a long context: an item is 128 rows of one kv head of a sequence (the G query heads of a token are neighbouring rows) against all
-// tokens that the sequence's rows see, KT = 128 at a time (64 where F32 rows of 256 leave no room). All items' tiles are numbered through and each CTA takes an
-// equal run of the numbers, whatever the sequences' lengths; the last of the CTAs that have a part of an item puts them together.
+// tokens that the sequence's rows see, KT = 128 at a time, 64 of F32 rows of 128, 32 of 256: so that there is room for two stages of operands and a tile of
+// codes on its way (F32 rows of 128, 131,000 tokens: 430 us by 128 with the codes read when they are needed, 289 by 64; of 256 631 and 463). All items' tiles are numbered through and each CTA takes an
+// equal run of the numbers, whatever the sequences' lengths; a second kernel puts together the items that several CTAs have a part of (by the last CTA that brings one it took
+// 17 us for nine parts of heads of 128, by all SMs 5).
 //
 //   warps 0 .. 3, 4 .. 7   a thread a row: scores -> weights. Both have the same rows: one takes the even tiles, the other the odd ones, each with sums and a
 //                          maximum of its own, which are put together at the item's end (heads of 256: the first alone, tensor memory has no room for two)
@@ -11,8 +13,8 @@
 //                          warps that work on scores get fewer issue slots)
 //   warp 12                issues the products
 //
-// A CTA's parts in memory are three units of 128 rows: what it has of its first item; and the sums of the two streams until an item's end, the first of which
-// then holds what it has of its last item.
+// A CTA's parts in memory are three units of 128 rows: what it has of an item that began in an earlier one's run; and the sums of the two streams until an
+// item's end, the first of which then holds what it has of an item that ends in a later one's.
 #pragma once
 
 #include "wd_kv_prompt.cuh"
@@ -21,26 +23,23 @@ namespace wd {
 
 struct KvTree : KvPrompt {
     const int *parents;         // see KvAttendTree
-    unsigned *arrived;          // [CTAs]
+    int4 *cuts;                 // [CTAs][2]: of the item that begins in a CTA's run and ends behind it: its sequence's first row, rows of a head, head, first row; CTA of its end (-1: none)
 };
 
 template <int D, bool SPLIT>
 struct TreePlan {
-    static constexpr int kStreams = D <= 128 ? 2 : 1, kKt = D == 256 ? 64 : 128, kRows = 128;
+    static constexpr int kStreams = D <= 128 ? 2 : 1, kKt = D == 256 ? 32 : D == 128 && SPLIT ? 64 : 128;
     static constexpr int kQ = 128 * D * 2, kQTile = kQ * (SPLIT ? 2 : 1);
     static constexpr int kKStep = kKt * 16, kK = D / 8 * kKStep, kVStep = D * 16 + 64, kV = kKt / 8 * kVStep;
-    // a tile's codes on their way, where there is room for them beside two stages of operands (F32 rows of 128 and more: in registers)
-    static constexpr int kCodes = 2 * kKt * D, kFit = (208 * 1024 - kQTile - kCodes) / (kK + kV), kFitBare = (208 * 1024 - kQTile) / (kK + kV);
-    static constexpr bool kAhead = kFit >= 2;
-    static constexpr int kStages = kAhead ? (kFit > 4 ? 4 : kFit) : kFitBare;
-    static constexpr int kSmem = kQTile + kStages * (kK + kV) + (kAhead ? kCodes : 0) + (kAttMaxSeqs + 2) * 8 + 1024;
+    static constexpr int kCodes = 2 * kKt * D, kFit = (209 * 1024 - kQTile - kCodes) / (kK + kV), kStages = kFit > 4 ? 4 : kFit;        // a tile's codes on their way; stages of operands
+    static constexpr int kSmem = kQTile + kStages * (kK + kV) + kCodes + (kAttMaxSeqs + 2) * 8 + kAttEntries * 16 + 1024;
     static constexpr int kColO = 128 * kStreams, kColP = kColO + kStreams * D, kWidthP = kKt / 2 * (SPLIT ? 2 : 1);
     static constexpr bool kApart = kColP + kStreams * kWidthP <= 512;
     static constexpr int kChain = (SPLIT ? 2048 : 8192) / kKt;          // tiles of a stream
     static constexpr float kTop = SPLIT ? 13.0f : 9.0f, kGrowth = 15.0f - kTop;
     static constexpr uint32_t kIdescS = 1u << 4 | (kKt >> 3) << 17 | (128 >> 4) << 24, kIdescO = 1u << 4 | (D >> 3) << 17 | (128 >> 4) << 24;
     static constexpr int kScales = 8;       // tiles whose scales are held: a stage is free four tiles behind the softmax at most
-    static_assert(kColO + kStreams * D <= 512 && kStages >= 1 && kSmem <= 220 * 1024, "plan of the memories");
+    static_assert(kColO + kStreams * D <= 512 && kStages >= 2 && kSmem <= 220 * 1024, "plan of the memories");
 };
 // Tiles that every item of a sequence has.
 __host__ __device__ inline int tree_first_tile(int length, int count, int window, int kt) {
@@ -48,19 +47,22 @@ __host__ __device__ inline int tree_first_tile(int length, int count, int window
     return window && first > 0 ? first / kt : 0;
 }
 __host__ __device__ inline int tree_tiles(int length, int count, int window, int kt) { return (length + kt - 1) / kt - tree_first_tile(length, count, window, kt); }
-// The run of a CTA: at least what joining costs (items of so many tiles stay whole).
+// The run of a CTA: two tiles of 128 tokens at least (1,000 tokens, 60 rows of 4 x 64: by four 17.1 us, by two 15.9).
 __host__ __device__ inline long long tree_chunk(long long total, int ctas, int most, int kt) {
-    const long long even = total < (1ll << 31) ? static_cast<long long>((static_cast<uint32_t>(total) + ctas - 1) / static_cast<uint32_t>(ctas)) : (total + ctas - 1) / ctas, least = 512 / kt < most ? 512 / kt : most;
+    const long long even = total < (1ll << 31) ? static_cast<long long>((static_cast<uint32_t>(total) + ctas - 1) / static_cast<uint32_t>(ctas)) : (total + ctas - 1) / ctas, least = 256 / kt < most ? 256 / kt : most;
     return even > least ? even : least;
 }
 
+// An item counts a few tiles more than it has, in front of them, for what it costs to begin and end one.
+constexpr int kTreeExtra = 6;
+
 struct TreeSegment {
     int seq, row0, count, length, head, item_row, rows, lo, hi;     // rows: of the sequence and head; lo .. hi - 1: tiles of KT tokens
-    int tiles, whole, first;    // of the item; it holds all of the item; it is the CTA's first one
-    long long item0, next;
+    bool whole, begun;          // it holds all of the item; the item began in an earlier CTA's run
+    long long tile0, tile1, next;       // numbers: of the item's tiles; the one behind the segment
 };
 // Numbers of one head in front of each sequence; behind their number that of the tiles that an item has at most. By one warp.
-__device__ __forceinline__ void tree_prefix(const KvTree &P, int kt, long long *prefix, int lane) {
+__device__ __forceinline__ void tree_prefix(const KvTree &P, int kt, long long *prefix, int4 *step, int lane) {
     const int n_seq = P.book[0], g_heads = P.s.heads / P.s.kv_heads;
     const int *entries = P.book + kKvHead;
     long long sum = 0;
@@ -70,8 +72,9 @@ __device__ __forceinline__ void tree_prefix(const KvTree &P, int kt, long long *
         long long inc = 0;
         if (i < n_seq) {
             const int4 e = *reinterpret_cast<const int4 *>(entries + i * kKvStepWords);
+            if (i < kAttEntries) step[i] = e;
             const int n = e.z > 0 ? tree_tiles(e.w, e.z, P.window, kt) : 0;
-            inc = static_cast<long long>((e.z * g_heads + 127) / 128) * n;
+            inc = static_cast<long long>((e.z * g_heads + 127) / 128) * (n + kTreeExtra);
             most = max(most, n);
             most_rows = max(most_rows, e.z);
         }
@@ -91,8 +94,8 @@ __device__ __forceinline__ void tree_prefix(const KvTree &P, int kt, long long *
         prefix[n_seq + 1] = most;
     }
 }
-// the segment of the numbers at .. end - 1 that belongs to one item
-__device__ __forceinline__ TreeSegment tree_segment(const KvTree &P, int kt, const long long *prefix, int n_seq, long long at, long long end) {
+// the segment of the numbers at .. end - 1 that belongs to one item (lo == hi where it has none of its tiles); `begin`: of the CTA's run
+__device__ __forceinline__ TreeSegment tree_segment(const KvTree &P, int kt, const long long *prefix, const int4 *step, int n_seq, long long begin, long long at, long long end) {
     TreeSegment s;
     const int H = P.s.kv_heads;
     int lo = 0, hi = n_seq - 1;
@@ -101,22 +104,23 @@ __device__ __forceinline__ TreeSegment tree_segment(const KvTree &P, int kt, con
         if (prefix[mid] * H <= at) lo = mid;
         else hi = mid - 1;
     }
-    const int4 e = *reinterpret_cast<const int4 *>(P.book + kKvHead + lo * kKvStepWords);
+    const int4 e = lo < kAttEntries ? step[lo] : *reinterpret_cast<const int4 *>(P.book + kKvHead + lo * kKvStepWords);
     s.seq = e.x, s.row0 = e.y, s.count = e.z, s.length = e.w;
     const int tiles = tree_tiles(s.length, s.count, P.window, kt), first = tree_first_tile(s.length, s.count, P.window, kt);
-    const long long in = at - prefix[lo] * H, of_head = prefix[lo + 1] - prefix[lo];
-    // (numbers that 32 bits hold are divided in 32 bits)
-    const uint32_t blocks = of_head < (1ll << 31) ? static_cast<uint32_t>(of_head) / static_cast<uint32_t>(tiles) : static_cast<uint32_t>(of_head / tiles);
-    const long long item = in < (1ll << 31) ? static_cast<long long>(static_cast<uint32_t>(in) / static_cast<uint32_t>(tiles)) : in / tiles;
-    s.item0 = prefix[lo] * H + item * tiles;
-    s.head = static_cast<int>(static_cast<uint32_t>(item) / blocks);         // (fewer items than rows of heads, which 32 bits count)
-    s.item_row = static_cast<int>(static_cast<uint32_t>(item) % blocks) * 128;
-    s.rows = s.count * (P.s.heads / H);
-    s.next = min(s.item0 + tiles, end);
-    s.lo = first + static_cast<int>(at - s.item0);
-    s.hi = first + static_cast<int>(s.next - s.item0);
-    s.tiles = tiles;
+    const uint32_t per = tiles + kTreeExtra, g_heads = P.s.heads / H, blocks = (s.count * g_heads + 127) / 128;
+    const long long in = at - prefix[lo] * H;
+    // (numbers that 32 bits hold are divided in 32 bits; there are fewer items than rows of heads, which 32 bits count)
+    const uint32_t item = in < (1ll << 31) ? static_cast<uint32_t>(in) / per : static_cast<uint32_t>(in / per);
+    s.head = static_cast<int>(item / blocks);
+    s.item_row = static_cast<int>(item % blocks) * 128;
+    s.rows = s.count * g_heads;
+    s.tile0 = prefix[lo] * H + static_cast<long long>(item) * per + kTreeExtra;
+    s.tile1 = s.tile0 + tiles;
+    s.next = min(s.tile1, end);
+    s.lo = first + static_cast<int>(max(at, s.tile0) - s.tile0);
+    s.hi = max(s.lo, first + static_cast<int>(s.next - s.tile0));
     s.whole = s.hi - s.lo == tiles;
+    s.begun = s.tile0 < begin;
     return s;
 }
 
@@ -131,9 +135,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_tree_kernel(const __grid
     __shared__ float muls[128];            // of a row's scores, what its terms were divided by too
     __shared__ int8_t places[2][kTreeRows];         // parents of a segment's rows, and of the one's behind it
     __shared__ uint32_t tmem_base;
-    __shared__ bool last_one;
     uint8_t *qs = tsm, *ks = tsm + A::kQTile, *vs = ks + ST * A::kK, *raws = vs + ST * A::kV;
-    long long *prefix = reinterpret_cast<long long *>(raws + (A::kAhead ? A::kCodes : 0));
+    int4 *step = reinterpret_cast<int4 *>(raws + A::kCodes);            // the first entries of the step
+    long long *prefix = reinterpret_cast<long long *>(step + kAttEntries);
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int n_seq = P.book[0], g_heads = P.s.heads / P.s.kv_heads, H = P.s.kv_heads;
     if (warp == 0) {
@@ -153,7 +157,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_tree_kernel(const __grid
             }
             mbar_fence_init();
         }
-        tree_prefix(P, KT, prefix, lane);
+        tree_prefix(P, KT, prefix, step, lane);
     }
     if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_base)) : "memory");
@@ -169,23 +173,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_tree_kernel(const __grid
     // the segment behind `at` (-1: the first one); false behind the last
     auto next_segment = [&](long long &at, TreeSegment &s) {
         if (P.split) {
-            if (at < 0) at = begin;
-            if (at >= end) return false;
-            s = tree_segment(P, KT, prefix, n_seq, at, end);
-            s.first = at == begin;
-            at = s.next;
-            return true;
+            for (at = at < 0 ? begin : at; at < end;) {
+                s = tree_segment(P, KT, prefix, step, n_seq, begin, at, end);
+                at = s.next;
+                if (s.lo < s.hi) return true;
+            }
+            return false;
         }
         // item number n of all: its numbers are looked for by the sequences' items
         long long n = at < 0 ? blockIdx.x : at;
         at = n + gridDim.x;
         if (total == 0) return false;
         for (int i = 0; i < n_seq; ++i) {
-            const int4 e = *reinterpret_cast<const int4 *>(P.book + kKvHead + i * kKvStepWords);
-            const long long blocks = e.z > 0 ? (e.z * g_heads + 127) / 128 : 0, items = blocks * H;
+            const int4 e = i < kAttEntries ? step[i] : *reinterpret_cast<const int4 *>(P.book + kKvHead + i * kKvStepWords);
+            const long long items = e.z > 0 ? static_cast<long long>((e.z * g_heads + 127) / 128) * H : 0;
             if (n < items) {
-                s = tree_segment(P, KT, prefix, n_seq, prefix[i] * H + n * tree_tiles(e.w, e.z, P.window, KT), total);
-                s.first = 0;
+                s = tree_segment(P, KT, prefix, step, n_seq, 0, prefix[i] * H + n * (tree_tiles(e.w, e.z, P.window, KT) + kTreeExtra), total);
                 return true;
             }
             n -= items;
@@ -267,8 +270,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_tree_kernel(const __grid
         for (int x = 0; x < X; ++x)
             if (n_p[x] > 0) tc_drain(&o_done[x], (n_p[x] - 1) & 1);
     } else if (warp >= 8 && warp < 12) {
-        // A thread's codes of a tile are asked for a tile ahead, into places of its own (of segments too: what it does with them does not depend on where they
-        // come from). Where there is no room for that it reads them when it comes to them.
+        // A thread's codes of a tile are asked for a tile ahead, into places of its own (of segments too: what it does with them does not depend on where they come from).
         const int shift = P.s.page_shift, ct = tid - 256, cw = warp - 8, g = lane >> 2, t = lane & 3;
         constexpr int KU = KT * D / 16 / 128, KB = KU < 8 ? KU : 8;         // of 16 bytes: of a thread, at once
         constexpr int VU = SUBS * (D / 32) / 4, VB = VU < 8 ? VU : 8;          // of 512 bytes (16 tokens of 32 elements of a value): of a warp, at once
@@ -339,33 +341,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_tree_kernel(const __grid
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        if constexpr (A::kAhead) {
-            ask_keys();
-            ask_values();
-        }
+        ask_keys();
+        ask_values();
         for (int n = 0; more; ++n) {
             const float4 of_tile = mine;
             const int scale_lane = lane - (tile - group) * SUBS, st = n % ST;
             const uint32_t par = (static_cast<uint32_t>(n / ST) & 1u) ^ 1u;
             uint4 u[KB], w[VB];
-            const uint8_t *kp = nullptr;
-            const uint4 *vp[A::kAhead ? 1 : VU];
-            if constexpr (!A::kAhead) {
-                kp = key_base();
-#pragma unroll
-                for (int i = 0; i < VU; ++i) vp[i] = value_at(i);
-#pragma unroll
-                for (int i = 0; i < KB; ++i) u[i] = __ldg(key_at(kp, i));
-            }
             more = next_tile();
-            if constexpr (A::kAhead) asm volatile("cp.async.wait_group 1;" ::: "memory");
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
             att_wait(&k_free[st], par, P.status);
 #pragma unroll
             for (int b = 0; b < KU; b += KB) {
-                if (A::kAhead || b > 0) {
 #pragma unroll
-                    for (int i = 0; i < KB; ++i) u[i] = A::kAhead ? raw_k[(b + i) * 128] : __ldg(key_at(kp, b + i));
-                }
+                for (int i = 0; i < KB; ++i) u[i] = raw_k[(b + i) * 128];
 #pragma unroll
                 for (int i = 0; i < KB; ++i) {
                     const int k16 = ((b + i) * 128 + ct) / KT;
@@ -382,20 +371,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_tree_kernel(const __grid
             if (cw == 0 && scale_lane >= 0 && scale_lane < SUBS) scales[n & (A::kScales - 1)][scale_lane] = of_tile;
             fence_proxy_async();
             mbar_arrive(&k_full[st]);
-            if constexpr (A::kAhead) {
-                ask_keys();
-                asm volatile("cp.async.wait_group 1;" ::: "memory");
-            } else {
-#pragma unroll
-                for (int i = 0; i < VB; ++i) w[i] = __ldg(vp[i]);
-            }
+            ask_keys();
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
             att_wait(&v_free[st], par, P.status);
 #pragma unroll
             for (int b = 0; b < VU; b += VB) {
-                if (A::kAhead || b > 0) {
 #pragma unroll
-                    for (int i = 0; i < VB; ++i) w[i] = A::kAhead ? raw_v[(b + i) * 128] : __ldg(vp[A::kAhead ? 0 : b + i]);
-                }
+                for (int i = 0; i < VB; ++i) w[i] = raw_v[(b + i) * 128];
 #pragma unroll
                 for (int i = 0; i < VB; ++i) {
                     const int unit = (b + i) * 4 + cw, s = unit / (D / 32), blk = unit % (D / 32);
@@ -411,19 +393,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_tree_kernel(const __grid
             }
             fence_proxy_async();
             mbar_arrive(&v_full[st]);
-            if constexpr (A::kAhead) ask_values();
+            ask_values();
         }
-        if constexpr (A::kAhead) asm volatile("cp.async.wait_group 0;" ::: "memory");
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else if (warp < 4 * X) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromptRegsMore));
         const int x = warp >> 2, r = tid & 127;
         const uint32_t lanes = tm + (static_cast<uint32_t>((warp & 3) * 32) << 16), sc = lanes + x * 128, oc = lanes + A::kColO + x * D, pc = A::kApart ? lanes + A::kColP + x * A::kWidthP : sc;
         int n_s = 0, n_o = 0, n = 0;            // scores, sums, and tiles of all segments so far
+        int cut_end = -1;                       // CTA in which the last item ends, where it is cut
         auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(128 * X) : "memory"); };
         for (int turn = 0; next_segment(at, it); ++turn) {
             const int row = it.item_row + r, last = it.rows - 1, start = it.length - it.count, node = min(row, last) / g_heads, tiles = it.hi - it.lo;         // (tiles of the segment)
             const bool is = row <= last;
-            if (r < it.count && x == 0) places[turn & 1][r] = static_cast<int8_t>(tree_parent(P.parents, it.row0, r));
+            const int parent = r < it.count && x == 0 ? P.parents[it.row0 + r] : -1;        // (asked for in front of q, used behind it)
             // q: a warp brings eight rows at a time, a lane eight elements in front of every 32 of row lane % 8; the row's largest magnitude, then its F16 terms; element k
             // of row r lies at (k / 8) 2048 + r 16
             auto bring = [&](const auto *q) {
@@ -477,6 +460,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_tree_kernel(const __grid
             if constexpr (SPLIT) bring(static_cast<const float *>(P.q));
             else if (P.type == kRowsF16) bring(static_cast<const __half *>(P.q));
             else bring(static_cast<const __nv_bfloat16 *>(P.q));
+            if (r < it.count && x == 0) places[turn & 1][r] = static_cast<int8_t>(parent >= 0 && parent < r ? parent : -1);
             fence_proxy_async();
             mbar_arrive(&q_full);
             meet();             // (the parents and the factors are there)
@@ -720,11 +704,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_tree_kernel(const __grid
                 }
             };
             const float inv = kAttUnit / den;
-            const int to_unit = unit + (it.first ? 0 : 1);
-            // 16 elements of a row's answer from c on
-            auto answer = [&](int of_row, int c, const float (&y)[16]) {
-                const int in = it.item_row + of_row;
-                const size_t dst = static_cast<size_t>(it.row0 + in / g_heads) * P.out_stride + (static_cast<size_t>(it.head) * g_heads + in % g_heads) * D + c;
+            const int to_unit = unit + (it.begun ? 0 : 1);
+            const size_t dst = static_cast<size_t>(it.row0 + row / g_heads) * P.out_stride + (static_cast<size_t>(it.head) * g_heads + row % g_heads) * D;
+            // 16 elements of the row's answer from c on
+            auto answer = [&](int c, const float (&y)[16]) {
                 auto put = [&](auto *o) {
                     using R = std::remove_pointer_t<decltype(o)>;
                     __align__(16) R z[16];
@@ -738,9 +721,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_tree_kernel(const __grid
                         for (int i = 0; i < 16; ++i) o[i] = z[i];
                     }
                 };
-                if constexpr (SPLIT) put(static_cast<float *>(P.out) + dst);
-                else if (P.type == kRowsF16) put(static_cast<__half *>(P.out) + dst);
-                else put(static_cast<__nv_bfloat16 *>(P.out) + dst);
+                if constexpr (SPLIT) put(static_cast<float *>(P.out) + dst + c);
+                else if (P.type == kRowsF16) put(static_cast<__half *>(P.out) + dst + c);
+                else put(static_cast<__nv_bfloat16 *>(P.out) + dst + c);
             };
 #pragma unroll 1
             for (int c = x * (D / X); c < (x + 1) * (D / X); c += 16) {
@@ -752,76 +735,76 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_tree_kernel(const __grid
                 } else if (is) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) y[i] *= inv;
-                    answer(r, c, y);
+                    answer(c, y);
                 }
                 __syncwarp();
             }
             if (is && !it.whole && x == 0) *prompt_part_end<D, 128>(P.part, to_unit, of) = make_float2(all, den);
-            if (!it.whole) {        // the last of the CTAs that have a part of the item puts them together
-                const int c0 = static_cast<int>(it.item0 / chunk), c1 = static_cast<int>((it.item0 + it.tiles - 1) / chunk);
-                __threadfence();
-                meet();
-                if (tid == 0) {
-                    const unsigned before = atomicAdd(P.arrived + c0, 1u);
-                    last_one = before == static_cast<unsigned>(c1 - c0);
-                    if (last_one) P.arrived[c0] = 0u;
-                    __threadfence();
-                }
-                meet();
-                if (last_one) {
-                    // rows by as many threads each as there are, 16 columns at a time
-                    const int rows = min(128, it.rows - it.item_row), wide = rows > 64 ? 1 : rows > 32 ? 2 : 4, t = x * 128 + r, j_row = t / (X * wide), part_of = t % (X * wide);
-                    constexpr int kLeastColumns = 16;
-                    const int columns = max(kLeastColumns, D / (X * wide));
-                    auto unit_of = [&](int k) { return k * kTreeUnits + (it.item0 > k * chunk ? 1 : 0); };
-                    if (j_row < rows) {
-#pragma unroll 1
-                        for (int c = part_of * columns; c < min(D, (part_of + 1) * columns); c += 16) {
-                            float y[16], best = kAttFloor, total_den = 0.0f;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) y[i] = 0.0f;
-#pragma unroll 1
-                            for (int k0 = c0; k0 <= c1; k0 += 4) {
-                                float2 z[4];
-                                float4 v[4][4];
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    const int from = unit_of(min(k0 + k, c1));
-                                    z[k] = __ldcg(prompt_part_end<D, 128>(P.part, from, j_row));
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) v[k][i] = __ldcg(reinterpret_cast<const float4 *>(prompt_part<D, 128>(P.part, from, j_row, c + 4 * i)));
-                                }
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    if (k0 + k > c1) break;
-                                    const float both = fmaxf(best, z[k].x), ha = ex2(0.5f * (best - both)), hb = ex2(0.5f * (z[k].x - both)), fa = ha * ha, fb = hb * hb;
-                                    best = both;
-                                    total_den = total_den * ha * ha + z[k].y * hb * hb;
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) {
-                                        y[4 * i] = fmaf(v[k][i].x, fb, y[4 * i] * fa), y[4 * i + 1] = fmaf(v[k][i].y, fb, y[4 * i + 1] * fa);
-                                        y[4 * i + 2] = fmaf(v[k][i].z, fb, y[4 * i + 2] * fa), y[4 * i + 3] = fmaf(v[k][i].w, fb, y[4 * i + 3] * fa);
-                                    }
-                                }
-                            }
-                            const float over = kAttUnit / total_den;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) y[i] *= over;
-                            answer(j_row, c, y);
-                        }
-                    }
-                }
+            if (tid == 0 && P.split && !it.begun && it.tile1 > end) {
+                P.cuts[2 * blockIdx.x] = make_int4(it.row0, it.rows, it.head, it.item_row);
+                cut_end = static_cast<int>((it.tile1 - 1) / chunk);
             }
             tc_fence_before();      // the sums have been read: the next segment's may be written once its weights are there
             meet();
         }
+        if (P.split && tid == 0) P.cuts[2 * blockIdx.x + 1] = make_int4(cut_end, 0, 0, 0);
     } else if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromptRegsMore));
     }
+    grid_dep_launch();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm) : "memory");
+}
+
+// The parts of the items that several CTAs have one of: blockIdx.x is the CTA that an item begins in, blockIdx.y some of its rows; a thread has four elements of a row.
+template <int D>
+constexpr int kTreeJoinRows = D == 96 ? 8 : 1024 / D;
+template <int D>
+__global__ void __launch_bounds__(256) kv_tree_join_kernel(const __grid_constant__ KvTree P) {
+    grid_dep_wait();
+    const int c0 = blockIdx.x, tid = threadIdx.x, r = blockIdx.y * kTreeJoinRows<D> + tid / (D / 4), c = tid % (D / 4) * 4;
+    const int4 a = P.cuts[2 * c0], b = P.cuts[2 * c0 + 1];
+    if (b.x < 0 || tid / (D / 4) >= kTreeJoinRows<D> || a.w + r >= a.y) return;
+    const int g_heads = P.s.heads / P.s.kv_heads, row = a.w + r;
+    float top = kAttFloor, den = 0.0f;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+    for (int k0 = c0; k0 <= b.x; k0 += 8) {
+        float2 z[8];
+        float4 y[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int from = min(k0 + k, b.x), unit = from * kTreeUnits + (from == c0 ? 1 : 0);       // (of the others it is the first item)
+            z[k] = *prompt_part_end<D, 128>(P.part, unit, r);
+            y[k] = *reinterpret_cast<const float4 *>(prompt_part<D, 128>(P.part, unit, r, c));
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (k0 + k > b.x) break;
+            const float both = fmaxf(top, z[k].x), ha = ex2(0.5f * (top - both)), hb = ex2(0.5f * (z[k].x - both)), fa = ha * ha, fb = hb * hb;
+            top = both;
+            den = den * ha * ha + z[k].y * hb * hb;
+            sum.x = fmaf(y[k].x, fb, sum.x * fa), sum.y = fmaf(y[k].y, fb, sum.y * fa), sum.z = fmaf(y[k].z, fb, sum.z * fa), sum.w = fmaf(y[k].w, fb, sum.w * fa);
+        }
+    }
+    const float inv = kAttUnit / den;
+    const size_t to = static_cast<size_t>(a.x + row / g_heads) * P.out_stride + (static_cast<size_t>(a.z) * g_heads + row % g_heads) * D + c;
+    auto put = [&](auto *o) {
+        using R = std::remove_pointer_t<decltype(o)>;
+        __align__(16) R v[4] = {row_number<R>(sum.x * inv), row_number<R>(sum.y * inv), row_number<R>(sum.z * inv), row_number<R>(sum.w * inv)};
+        if (P.vec) {
+            if constexpr (sizeof(R) == 4) *reinterpret_cast<uint4 *>(o) = *reinterpret_cast<const uint4 *>(v);
+            else *reinterpret_cast<uint2 *>(o) = *reinterpret_cast<const uint2 *>(v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = v[i];
+        }
+    };
+    if (P.type == kRowsF32) put(static_cast<float *>(P.out) + to);
+    else if (P.type == kRowsF16) put(static_cast<__half *>(P.out) + to);
+    else put(static_cast<__nv_bfloat16 *>(P.out) + to);
 }
 
 }  // namespace wd
