@@ -206,6 +206,227 @@ __global__ void __launch_bounds__(THREADS) kv_rope_kernel(const __grid_constant_
     }
 }
 
+// ---- many tokens of a page: a lane has eight pairs of a head, so that rows are read and written by 16 bytes ---------------------------------
+// The pairs 8 c .. 8 c + 7 of a head of D elements, c the lane's place in a group of G lanes (a power of two, some without pairs): their elements are eight at a
+// and eight at b, pair by pair (apart: the rotation's halves) or one pair behind the other.
+struct RopeEight {
+    int a, b, first;            // first: pair
+    bool is, apart, turned;     // turned: all of them, or none
+};
+__device__ __forceinline__ RopeEight rope_eight(const KvRope &P, int c) {
+    RopeEight e;
+    const int half = P.rotary / 2;
+    e.first = 8 * c;
+    e.is = 16 * c < P.a.s.head_dim;
+    e.turned = e.first < half;
+    e.apart = e.turned && !P.neighbours;
+    e.a = e.apart ? e.first : 16 * c;
+    e.b = e.apart ? half + e.first : 16 * c + 8;
+    return e;
+}
+// N numbers of 16 bytes and more at `from`
+template <class T>
+__device__ __forceinline__ void rope_get8(const T *from, float *x) {
+    constexpr int N = 16 / sizeof(T);
+    uint4 u[8 / N];
+#pragma unroll
+    for (int i = 0; i < 8 / N; ++i) u[i] = reinterpret_cast<const uint4 *>(from)[i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(reinterpret_cast<const T *>(&u[i / N])[i % N]);
+}
+template <class T>
+__device__ __forceinline__ void rope_put8(T *to, const float *x) {
+    constexpr int N = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8 / N; ++i) {
+        __align__(16) T y[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) y[j] = row_number<T>(x[i * N + j]);
+        reinterpret_cast<uint4 *>(to)[i] = *reinterpret_cast<const uint4 *>(y);
+    }
+}
+// the eight pairs' first and second elements
+template <class T>
+__device__ __forceinline__ void rope_pairs(const T *row, const RopeEight &e, float *x0, float *x1) {
+    float a[8], b[8];
+    rope_get8(row + e.a, a);
+    rope_get8(row + e.b, b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        x0[i] = e.apart ? a[i] : i < 4 ? a[2 * i] : b[2 * i - 8];
+        x1[i] = e.apart ? b[i] : i < 4 ? a[2 * i + 1] : b[2 * i - 7];
+    }
+}
+// eight pairs as they lie: at a, at b
+__device__ __forceinline__ void rope_places(const RopeEight &e, const float *y0, const float *y1, float *a, float *b) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        a[i] = e.apart ? y0[i] : i & 1 ? y1[i / 2] : y0[i / 2];
+        b[i] = e.apart ? y1[i] : i & 1 ? y1[4 + i / 2] : y0[4 + i / 2];
+    }
+}
+
+constexpr int kRopeThreads = 256;
+template <class T, bool E4M3>
+__global__ void __launch_bounds__(kRopeThreads, 2) kv_rope_rows_kernel(const __grid_constant__ KvRope P) {
+    extern __shared__ __align__(16) uint8_t rope_sm[];           // keys: rotated rows; values: the codes of the sub-blocks that the rows touch
+    __shared__ float part[kRopeThreads / 32];
+    __shared__ int bad_any;
+    const int n_seq = P.a.book[0], n_items = P.a.book[2], h = blockIdx.y, D = P.a.s.head_dim, tid = threadIdx.x;
+    const int shift = D <= 32 ? 1 : D <= 64 ? 2 : D <= 128 ? 3 : 4, G = 1 << shift, c = tid & (G - 1);
+    const unsigned group = ((1u << G) - 1) << (tid & 31 & -G);          // the lanes of a head: a warp's groups may have tokens or not
+    const RopeEight e = rope_eight(P, c);
+    double turns[8];
+    int axis[8];
+    float w0[8], w1[8];
+    const float *norm = blockIdx.z == 0 ? P.k_norm : P.q_norm;
+    if (blockIdx.z != 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int p = e.first + i;
+            turns[i] = e.is && e.turned ? P.turns[p] : 0.0;
+            axis[i] = min((p >= P.section_end[0]) + (p >= P.section_end[1]) + (p >= P.section_end[2]), P.n_axes - 1);
+            w0[i] = w1[i] = 1.0f;
+            if (norm && e.is) w0[i] = norm[e.apart ? e.a + i : 2 * p], w1[i] = norm[e.apart ? e.b + i : 2 * p + 1];
+        }
+    }
+    auto angle = [&](int i, int row, int place) {
+        const double a = static_cast<double>(P.positions ? P.positions[static_cast<size_t>(row) * P.n_axes + axis[i]] : place) * turns[i];
+        return 2.0 * (a - rint(a));
+    };
+#pragma unroll 1
+    for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+        const KvPagePart at = kv_page_part(P.a.book, P.a.table, P.a.s, n_seq, item);
+        const int n = at.b - at.a;
+        if (blockIdx.z == 1) {
+            kv_append_part<T, E4M3, kRopeThreads>(P.a, at, h, 1, rope_sm, part, bad_any);
+        } else if (blockIdx.z == 0) {
+            const T *rows = static_cast<const T *>(P.a.rows[0]) + static_cast<size_t>(at.row) * P.a.stride[0] + static_cast<size_t>(h) * D;
+            float *held = reinterpret_cast<float *>(rope_sm);
+            auto rotate = [&](int t0, int m) {
+#pragma unroll 1
+                for (int t = tid >> shift; t < m; t += kRopeThreads >> shift) {
+                    const int row = at.row + t0 + t, place = at.place + t0 + t;
+                    float x0[8], x1[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x0[i] = x1[i] = 0.0f;
+                    if (e.is) rope_pairs(rows + static_cast<size_t>(t0 + t) * P.a.stride[0], e, x0, x1);
+                    double inv = 1.0;
+                    if (P.k_norm) {
+                        double sum = 0.0, more = 0.0;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) sum = fma(static_cast<double>(x0[i]), static_cast<double>(x0[i]), sum), more = fma(static_cast<double>(x1[i]), static_cast<double>(x1[i]), more);
+                        sum += more;
+                        for (int o = G / 2; o; o >>= 1) sum += __shfl_xor_sync(group, sum, o);
+                        inv = rsqrt(sum / D + static_cast<double>(P.eps));
+                    }
+                    float a[8], b[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        double n0 = x0[i], n1 = x1[i];
+                        if (P.k_norm) n0 = n0 * inv * w0[i], n1 = n1 * inv * w1[i];
+                        if (e.turned) {
+                            double sn, cs;
+                            sincospi(angle(i, row, place), &sn, &cs);
+                            const double f = P.factor, y0 = f * (n0 * cs - n1 * sn), y1 = f * (n1 * cs + n0 * sn);
+                            n0 = y0, n1 = y1;
+                        }
+                        x0[i] = static_cast<float>(n0);
+                        x1[i] = static_cast<float>(n1);
+                    }
+                    rope_places(e, x0, x1, a, b);
+                    if (e.is) {
+#pragma unroll
+                        for (int i = 0; i < 8; i += 4) {
+                            *reinterpret_cast<float4 *>(held + rope_held(t * D + e.a + i)) = make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]);
+                            *reinterpret_cast<float4 *>(held + rope_held(t * D + e.b + i)) = make_float4(b[i], b[i + 1], b[i + 2], b[i + 3]);
+                        }
+                    }
+                }
+            };
+            auto load = [&](int t, int k, float *x) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float4 v = *reinterpret_cast<const float4 *>(held + rope_held(t * D + k + 4 * j));
+                    x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
+                }
+            };
+            float top = 0.0f;
+            int bad = 0;
+            for (int t0 = 0; t0 < n; t0 += P.held) {
+                if (t0 > 0) __syncthreads();
+                rotate(t0, min(P.held, n - t0));
+                __syncthreads();
+                top = kv_part_top<kRopeThreads>(D, min(P.held, n - t0), load, top, bad);
+            }
+            const KvPartScale sc = kv_part_scale<E4M3, kRopeThreads>(P.a, at, h, 0, top, bad, part, bad_any);
+            for (int t0 = 0; t0 < n; t0 += P.held) {
+                if (n > P.held) {
+                    __syncthreads();
+                    rotate(t0, min(P.held, n - t0));
+                    __syncthreads();
+                }
+                kv_part_codes<E4M3, kRopeThreads>(P.a, at, h, 0, sc, nullptr, t0, min(P.held, n - t0), load);
+            }
+            kv_part_end(P.a, at, h, 0, sc.s, make_int2(0, 0));
+        } else {
+            const int g = P.a.s.heads / P.a.s.kv_heads, part_q = blockIdx.z - 2, h0 = h * g + g * part_q / P.q_parts, h1 = h * g + g * (part_q + 1) / P.q_parts;
+            // where there are fewer tokens than groups, some groups share one's heads
+            const int groups = kRopeThreads >> shift, share = n < groups ? min(h1 - h0, groups / n) : 1, slot = tid >> shift;
+#pragma unroll 1
+            for (int t = slot / share; t < n; t += groups / share) {
+                float cs[8], sn[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    cs[i] = 1.0f, sn[i] = 0.0f;
+                    if (e.turned) {
+                        sincospif(static_cast<float>(angle(i, at.row + t, at.place + t)), &sn[i], &cs[i]);
+                        cs[i] *= P.factor, sn[i] *= P.factor;
+                    }
+                }
+                const T *from = static_cast<const T *>(P.q) + static_cast<size_t>(at.row + t) * P.q_stride;
+                T *to = static_cast<T *>(P.q_out) + static_cast<size_t>(at.row + t) * P.q_out_stride;
+#pragma unroll 2
+                for (int head = h0 + slot % share; head < h1; head += share) {
+                    float x0[8], x1[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x0[i] = x1[i] = 0.0f;
+                    if (e.is) rope_pairs(from + static_cast<size_t>(head) * D, e, x0, x1);
+                    if (P.q_norm) {
+                        float sum = 0.0f, more = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) sum = fmaf(x0[i], x0[i], sum), more = fmaf(x1[i], x1[i], more);
+                        sum += more;
+                        for (int o = G / 2; o; o >>= 1) sum += __shfl_xor_sync(group, sum, o);
+                        float inv = __frsqrt_rn(sum / D + P.eps);
+                        if (!(sum > 1e-30f && sum < 1e38f)) {           // squares that F32 does not hold
+                            double wide = 0.0;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) wide += static_cast<double>(x0[i]) * x0[i] + static_cast<double>(x1[i]) * x1[i];
+                            for (int o = G / 2; o; o >>= 1) wide += __shfl_xor_sync(group, wide, o);
+                            inv = static_cast<float>(1.0 / sqrt(wide / D + static_cast<double>(P.eps)));
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x0[i] = x0[i] * inv * w0[i], x1[i] = x1[i] * inv * w1[i];
+                    }
+                    float y0[8], y1[8], a[8], b[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        y0[i] = e.turned ? x0[i] * cs[i] - x1[i] * sn[i] : x0[i];
+                        y1[i] = e.turned ? x1[i] * cs[i] + x0[i] * sn[i] : x1[i];
+                    }
+                    rope_places(e, y0, y1, a, b);
+                    if (e.is) {
+                        rope_put8(to + static_cast<size_t>(head) * D + e.a, a);
+                        rope_put8(to + static_cast<size_t>(head) * D + e.b, b);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
 }  // namespace
 }  // namespace wd
 
@@ -301,6 +522,9 @@ int wd_kv_append_rope(wd_kv_cache *c, int layer, const wd_rope *r, const wd_rope
         p.q_parts = std::max<long long>(1, std::min<long long>(g, 4ll * c->n_sm / (static_cast<long long>(c->items) * H)));
         const dim3 grid(static_cast<unsigned>(c->items), H, x->q_dev ? 2 + p.q_parts : 2);
         const bool small = static_cast<long long>(most) * D <= 2048;
+        // by eights of pairs where the rows lie on boundaries of 16 bytes and no eight has some pairs that are turned and some that are not
+        bool by_eight = !small && r->cfg.rotary_dim % 16 == 0 && p.a.vec[0];
+        if (x->q_dev) by_eight &= (reinterpret_cast<uintptr_t>(x->q_dev) | reinterpret_cast<uintptr_t>(x->q_out_dev)) % 16 == 0 && p.q_stride * size % 16 == 0 && p.q_out_stride * size % 16 == 0;
         return by_rows_and_codes(c, rows_of, [&](auto t, auto e4m3) {
             using T = decltype(t);
             auto launch = [&](auto kernel, int threads) {
@@ -309,6 +533,7 @@ int wd_kv_append_rope(wd_kv_cache *c, int layer, const wd_rope *r, const wd_rope
                 WD_TRY_CUDA(cudaGetLastError());
                 return WD_OK;
             };
+            if (by_eight) return launch(wd::kv_rope_rows_kernel<T, decltype(e4m3)::value>, wd::kRopeThreads);
             return small ? launch(wd::kv_rope_kernel<T, decltype(e4m3)::value, 64>, 64) : launch(wd::kv_rope_kernel<T, decltype(e4m3)::value, 256>, 256);
         });
     });
