@@ -266,13 +266,28 @@ __device__ __forceinline__ void rope_places(const RopeEight &e, const float *y0,
     }
 }
 
+// sine and cosine of 2 pi turn, |turn| <= 1/2: those of the nearest 256th of a turn, from the table, and the series of the rest, put together; off by 2^-51
+__device__ __forceinline__ void rope_sincos(const double2 *circle, double turn, double &sn, double &cs) {
+    constexpr double magic = 6755399441055744.0;         // 1.5 2^52: what is added to it is rounded to a whole number
+    const double t = 256.0 * turn, whole = t + magic, x = (t - (whole - magic)) * (6.283185307179586476925 / 256), x2 = x * x;
+    const double2 at = circle[__double2loint(whole) & 255];
+    const double s = fma(x2 * x, fma(x2, fma(x2, -1.0 / 5040, 1.0 / 120), -1.0 / 6), x), c = x2 * fma(x2, fma(x2, -1.0 / 720, 1.0 / 24), -0.5);         // (c: less 1)
+    sn = at.y + fma(at.y, c, at.x * s);
+    cs = at.x + fma(at.x, c, -(at.y * s));
+}
+
 constexpr int kRopeThreads = 256;
 template <class T, bool E4M3>
 __global__ void __launch_bounds__(kRopeThreads, 2) kv_rope_rows_kernel(const __grid_constant__ KvRope P) {
     extern __shared__ __align__(16) uint8_t rope_sm[];           // keys: rotated rows; values: the codes of the sub-blocks that the rows touch
+    __shared__ double2 circle[256];                              // cosine and sine of a turn's 256ths
     __shared__ float part[kRopeThreads / 32];
     __shared__ int bad_any;
     const int n_seq = P.a.book[0], n_items = P.a.book[2], h = blockIdx.y, D = P.a.s.head_dim, tid = threadIdx.x;
+    if (blockIdx.z == 0) {
+        for (int i = tid; i < 256; i += kRopeThreads) sincospi(i / 128.0, &circle[i].y, &circle[i].x);
+        __syncthreads();
+    }
     const int shift = D <= 32 ? 1 : D <= 64 ? 2 : D <= 128 ? 3 : 4, G = 1 << shift, c = tid & (G - 1);
     const unsigned group = ((1u << G) - 1) << (tid & 31 & -G);          // the lanes of a head: a warp's groups may have tokens or not
     const RopeEight e = rope_eight(P, c);
@@ -290,9 +305,11 @@ __global__ void __launch_bounds__(kRopeThreads, 2) kv_rope_rows_kernel(const __g
             if (norm && e.is) w0[i] = norm[e.apart ? e.a + i : 2 * p], w1[i] = norm[e.apart ? e.b + i : 2 * p + 1];
         }
     }
-    auto angle = [&](int i, int row, int place) {
-        const double a = static_cast<double>(P.positions ? P.positions[static_cast<size_t>(row) * P.n_axes + axis[i]] : place) * turns[i];
-        return 2.0 * (a - rint(a));
+    // less whole turns; first: the position on the first axis
+    auto first_at = [&](int row, int place) { return static_cast<double>(P.positions ? P.positions[static_cast<size_t>(row) * P.n_axes] : place); };
+    auto turn_of = [&](int i, double first, int row) {
+        const double a = (P.n_axes > 1 && P.positions ? static_cast<double>(P.positions[static_cast<size_t>(row) * P.n_axes + axis[i]]) : first) * turns[i];
+        return a - rint(a);
     };
 #pragma unroll 1
     for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
@@ -306,7 +323,8 @@ __global__ void __launch_bounds__(kRopeThreads, 2) kv_rope_rows_kernel(const __g
             auto rotate = [&](int t0, int m) {
 #pragma unroll 1
                 for (int t = tid >> shift; t < m; t += kRopeThreads >> shift) {
-                    const int row = at.row + t0 + t, place = at.place + t0 + t;
+                    const int row = at.row + t0 + t;
+                    const double first = first_at(row, at.place + t0 + t);
                     float x0[8], x1[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) x0[i] = x1[i] = 0.0f;
@@ -327,7 +345,7 @@ __global__ void __launch_bounds__(kRopeThreads, 2) kv_rope_rows_kernel(const __g
                         if (P.k_norm) n0 = n0 * inv * w0[i], n1 = n1 * inv * w1[i];
                         if (e.turned) {
                             double sn, cs;
-                            sincospi(angle(i, row, place), &sn, &cs);
+                            rope_sincos(circle, turn_of(i, first, row), sn, cs);
                             const double f = P.factor, y0 = f * (n0 * cs - n1 * sn), y1 = f * (n1 * cs + n0 * sn);
                             n0 = y0, n1 = y1;
                         }
@@ -375,12 +393,13 @@ __global__ void __launch_bounds__(kRopeThreads, 2) kv_rope_rows_kernel(const __g
             const int groups = kRopeThreads >> shift, share = n < groups ? min(h1 - h0, groups / n) : 1, slot = tid >> shift;
 #pragma unroll 1
             for (int t = slot / share; t < n; t += groups / share) {
+                const double first = first_at(at.row + t, at.place + t);
                 float cs[8], sn[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     cs[i] = 1.0f, sn[i] = 0.0f;
                     if (e.turned) {
-                        sincospif(static_cast<float>(angle(i, at.row + t, at.place + t)), &sn[i], &cs[i]);
+                        sincospif(static_cast<float>(2.0 * turn_of(i, first, at.row + t)), &sn[i], &cs[i]);
                         cs[i] *= P.factor, sn[i] *= P.factor;
                     }
                 }
