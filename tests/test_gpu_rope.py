@@ -96,6 +96,40 @@ def test_codes_are_exact_and_queries_turned(shape, kind):
     assert t.p.kv.status() == 0
 
 
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 256])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rotary,neighbours,norm", [(0, False, True), (0, False, False), (0, True, True), (32, False, True), (16, True, False)])
+def test_many_tokens_of_a_page(dim, dtype, rotary, neighbours, norm):
+    g = {32: 1, 64: 3, 96: 2, 128: 7, 256: 4}[dim]
+    t = Turned(2 * g, 2, dim, 128, dim // 32 % 2, dtype, rotary=rotary, neighbours=neighbours, norm=norm, max_context=1000, n_pages=40, layers=1)
+    t.step([0], [128])
+    t.step([1, 0, 2], [67, 201, 99], own=True)
+    t.step([2, 1], [130, 1])
+    t.p.check_numbers([0, 1, 2])
+    assert t.p.kv.status() == 0
+
+
+def test_many_tokens_in_place_of_parts_of_a_fused_row():
+    t = Turned(6, 2, 96, 64, 0, "bf16", layers=1)
+    n, width = 150, 10 * 96
+    k, v, q = t.rows(n)
+    for lead in (0, 8, 3):              # (rows on boundaries of 16 bytes, and not)
+        row = torch.full((n, width + 16), 9.0, dtype=torch.bfloat16)
+        row[:, lead:lead + width] = torch.cat([x.reshape(n, -1) for x in (q, k, v)], dim=1)
+        dev, at = row.cuda(), 2 * lead
+        t.p.kv.begin([0], [n])
+        pos = t.own_places([0], [n])
+        torch.cuda.synchronize()
+        here = lambda e: dev.data_ptr() + at + 2 * e  # noqa: E731
+        t.call(0, here(6 * 96), here(8 * 96), here(0), here(0), None, q_stride=width + 16, q_out_stride=width + 16, k_stride=width + 16, v_stride=width + 16)
+        torch.cuda.synchronize()
+        got = dev.cpu()
+        t.check_q(got[:, lead:lead + 576].reshape(n, 6, 96), q, pos)
+        assert torch.equal(got[:, :lead], row[:, :lead]) and torch.equal(got[:, lead + 576:], row[:, lead + 576:])
+        t.keep_plain(0, [0], [n], k, v, pos)
+        t.p.check_numbers([0])
+
+
 def test_the_same_rows_again_leave_the_cache_as_it_is():
     t = Turned(8, 2, 128, 64, 0, "bf16", layers=1)
     t.step([0], [50])

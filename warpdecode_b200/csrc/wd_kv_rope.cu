@@ -3,12 +3,15 @@
 //   n = x w / sqrt(mean x^2 + eps);   pair p of a head: angle a = position f_p,  (y0, y1) = factor (n0 cos a - n1 sin a, n1 cos a + n0 sin a)
 //
 // A block takes the step's tokens that lie in one page and one kv head: its keys (blockIdx.z = 0), its values (1), or some of the query heads that share it
-// (2 and up). A warp takes a token's head, a lane the pairs lane, lane + 32, ...: the rotation's cosines are made once for all of a warp's heads of a token.
+// (2 and up). An angle is made once for all of a block's query heads of a token.
 //
 // Angles are made in turns, position (f_p / 2 pi) in 64 bits less the nearest whole number: in 32 bits the position 131,072 is off by 2^-8 radians. Queries
-// are rotated in F32. Keys in 64 bits, rounded to F32 once: then the code is the same however the sums are ordered, but for one number in 2^28, and the same
+// are rotated in F32. Keys in 64 bits, rounded to F32 once: then the code is the same however the sums are ordered, but for one number in 2^25, and the same
 // rows again leave the cache as it is. The rotated keys of a page wait in shared memory for the page's scale, as many tokens at a time as it holds; those
 // of a page that has more are made a second time.
+//
+// Few tokens are a chain of latencies (64 sequences, a token each, 32/8 heads of 128: 9.2 us). Many are bound by instruction issue, at two blocks an SM: 4,000 tokens of
+// 32/8 heads of 64 27 us (57 MB, 8.8 at the memory's rate), 5,003 of 128 by three axes 74, of which the codes of keys and values are 26, the keys' rotation 14 and the queries 34.
 #include <cmath>
 #include <memory>
 
@@ -70,6 +73,7 @@ __device__ __forceinline__ double rope_angle(const KvRope &P, const RopeLane &l,
 // where a float of the held rows is: 16 of them that one thread reads lie in other banks than its neighbours'
 __device__ __forceinline__ int rope_held(int e) { return (e & ~15) | ((((e >> 2) + (e >> 5)) & 3) << 2) | (e & 3); }
 
+// ---- few tokens, or rows that do not lie on boundaries of 16 bytes: a warp a token's head, a lane the pairs lane, lane + 32, ... ----------------
 template <class T, bool E4M3, int THREADS>
 __global__ void __launch_bounds__(THREADS) kv_rope_kernel(const __grid_constant__ KvRope P) {
     extern __shared__ __align__(16) uint8_t rope_sm[];           // keys: rotated rows; values: the codes of the sub-blocks that the rows touch
@@ -209,6 +213,7 @@ __global__ void __launch_bounds__(THREADS) kv_rope_kernel(const __grid_constant_
 // ---- many tokens of a page: a lane has eight pairs of a head, so that rows are read and written by 16 bytes ---------------------------------
 // The pairs 8 c .. 8 c + 7 of a head of D elements, c the lane's place in a group of G lanes (a power of two, some without pairs): their elements are eight at a
 // and eight at b, pair by pair (apart: the rotation's halves) or one pair behind the other.
+// (5,003 tokens of 128: 186 us by the kernel above, 74 by this one; by four pairs a lane a tenth to a half slower.)
 struct RopeEight {
     int a, b, first;            // first: pair
     bool is, apart, turned;     // turned: all of them, or none

@@ -13,6 +13,9 @@
 // read it, and where there are few sequences that of the rows that may be next beside it. What a CTA finds it sends to all CTAs' shared memory, where 16 bytes from
 // each complete a barrier (550 cycles; behind a barrier of the cluster it is 1,000), and every warp puts them together by the same arithmetic and comes to the same
 // decision, so that nothing is sent back.
+//
+// 64 chains of 5 rows of 151,936 F32, with a draft: 133 us (33 at the memory's rate), bound by the 64-bit terms of rejections and draws; one chain 21 to 27, 2.9 to 3.4 a
+// row and 7 a draw, bound by latency. With rows read from memory by each pass, sums met by a barrier of the cluster, and exp() for the terms 250 and 41.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
