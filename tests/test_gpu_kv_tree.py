@@ -9,7 +9,7 @@ import warpdecode_b200 as wd
 from test_gpu_kv_cache import GEOMETRY, TYPES, Pair
 
 pytestmark = pytest.mark.gpu
-FEW, TREE = "kv_attend_kernel", "kv_tree_kernel"
+FEW, TREE = "kv_attend_kernel", ("kv_tree_kernel", "kv_prompt_kernel")         # (of the second, by lengths)
 
 
 def make_tree(n, rng, kind):
@@ -106,6 +106,20 @@ def test_every_kernel(geometry, kernel, before, counts):
     check(p, seqs, counts, [x for n in counts for x in make_tree(n, rng, "any")], kernel=kernel)
     check(p, seqs, counts, [x for n in counts for x in make_tree(n, rng, "any")], window=150)
     check(p, seqs, counts, [x for n in counts for x in make_tree(n, rng, "any")], window=1500)
+
+
+@pytest.mark.parametrize("geometry", [(32, 8, 128, 64, 1, "f16"), (16, 4, 64, 64, 0, "f32"), (24, 6, 96, 32, 0, "bf16"), (16, 4, 32, 128, 1, "bf16")])
+@pytest.mark.parametrize("kernel,before,counts", [(TREE, [30000], [64]), (TREE, [20001, 15000], [61, 128]), (None, [300 + 80 * i for i in range(16)], [26] * 16)])
+def test_two_blocks_of_rows_by_one(geometry, kernel, before, counts):
+    p, rng = Pair(*geometry, n_pages=-(-sum(before) // geometry[3]) + 100, max_context=31000, max_seqs=16, layers=2), random.Random(2)
+    seqs = list(range(len(before)))
+    p.step(seqs, before)
+    p.step(seqs, counts)
+    parents = [x for n in counts for x in make_tree(n, rng, "any")]
+    check(p, seqs, counts, parents, kernel="kv_prompt_kernel" if before == [30000] and p.dim == 128 else kernel)
+    check(p, seqs, counts, parents, window=9000)
+    check(p, seqs, counts, [x for n in counts for x in make_tree(n, rng, "chain")], window=40)
+    assert p.kv.status() == 0
 
 
 @pytest.mark.parametrize("dtype,tokens", [("f32", 70000), ("bf16", 140000)])

@@ -41,7 +41,8 @@ int attend_of(wd_kv_cache *c, P &p, bool few, cudaStream_t s) {
 struct Choice {
     bool prompt, split;
 };
-inline Choice choose(const wd_kv_cache *c, bool f32, int window) {
+// tree: of wd_kv_attend_tree, whose items see all of the step; us, where asked for: what the kernel for prompts is expected to take
+inline Choice choose(const wd_kv_cache *c, bool f32, int window, bool tree = false, double *us = nullptr) {
     const int g = c->cfg.n_heads / c->cfg.n_kv_heads, d = c->cfg.head_dim, h = c->cfg.n_kv_heads;
     const int few_rows = d > 128 ? 8 : 16, item_rows = d > 128 ? 128 : 256;
     double few = 0.0, tiles = 0.0;
@@ -51,7 +52,7 @@ inline Choice choose(const wd_kv_cache *c, bool f32, int window) {
         const int *e = c->book.data() + wd::kKvHead + static_cast<size_t>(i) * wd::kKvStepWords;
         const long long rows = static_cast<long long>(e[2]) * g;
         if (rows == 0) continue;
-        const int seen = window ? std::min(e[3], window + item_rows / g) : e[3], n = (seen + 127) / 128;
+        const int seen = window ? std::min(e[3], window + (tree ? e[2] : item_rows / g)) : e[3], n = (seen + 127) / 128;
         const long long blocks = (rows + item_rows - 1) / item_rows;
         few += static_cast<double>((rows + few_rows - 1) / few_rows) * h * ((seen + 63) / 64);
         tiles += static_cast<double>(blocks) * h * n;
@@ -65,23 +66,25 @@ inline Choice choose(const wd_kv_cache *c, bool f32, int window) {
     const double of_few = c_f * few / (c->n_sm * (d > 128 ? 4.0 : 8.0));
     const double of_prompt = 3.0 + (r.split ? 8.0 + c_p * most / runs : c_p * std::max<double>(most, tiles / c->n_sm));
     r.prompt = of_prompt < of_few;
+    if (us) *us = of_prompt;
     return r;
 }
 
-template <int D, bool SPLIT>
-int prompt_launch(wd_kv_cache *c, const wd::KvPrompt &p, cudaStream_t s) {
+// (R: wd::KvPrompt, or wd::KvPromptTree)
+template <int D, bool SPLIT, class R>
+int prompt_launch(wd_kv_cache *c, const R &p, cudaStream_t s) {
     return by_codes(c, [&](auto e4m3) {
-        auto kernel = wd::kv_prompt_kernel<D, SPLIT, decltype(e4m3)::value>;
+        auto kernel = wd::kv_prompt_kernel<D, SPLIT, decltype(e4m3)::value, R>;
         constexpr int smem = wd::PromptAttPlan<D, SPLIT>::kSmem;
         WD_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         kernel<<<c->n_sm, wd::kPromptThreads, smem, s>>>(p);
-        if (p.split) wd::kv_prompt_join_kernel<D><<<2 * c->n_sm, 256, 0, s>>>(p);
+        if (p.split) wd::kv_prompt_join_kernel<D, R><<<2 * c->n_sm, 256, 0, s>>>(p);
         WD_TRY_CUDA(cudaGetLastError());
         return WD_OK;
     });
 }
-template <int D>
-int prompt_of(wd_kv_cache *c, const wd::KvPrompt &p, cudaStream_t s) {
+template <int D, class R>
+int prompt_of(wd_kv_cache *c, const R &p, cudaStream_t s) {
     return p.type == wd::kRowsF32 ? prompt_launch<D, true>(c, p, s) : prompt_launch<D, false>(c, p, s);
 }
 

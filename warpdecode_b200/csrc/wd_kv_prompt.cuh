@@ -47,6 +47,10 @@ struct KvPrompt {
     KvShape s;
 };
 
+struct KvPromptTree : KvPrompt {
+    const int *parents;         // see KvAttendTree
+};
+
 template <int D, bool SPLIT>
 struct PromptAttPlan {
     static constexpr int kTiles = D <= 128 ? 2 : 1, kKt = D == 256 && SPLIT ? 64 : 128, kRows = 128 * kTiles;
@@ -90,17 +94,20 @@ struct PromptItem {
 };
 
 // Items of one head in front of each sequence, and behind their number the most tiles of 128 tokens that one sees; by one warp.
-__device__ __forceinline__ void prompt_prefix(const KvPrompt &P, int rows, int *prefix, int lane) {
+template <class Params>
+__device__ __forceinline__ void prompt_prefix(const Params &P, int rows, int *prefix, int lane) {
+    constexpr bool TREE = std::is_same_v<Params, KvPromptTree>;
     const int n_seq = P.book[0], g_heads = P.s.heads / P.s.kv_heads;
     const int *entries = P.book + kKvHead;
-    int sum = 0, most = 0;
+    int sum = 0, most = 0, most_rows = 0;
     for (int i0 = 0; i0 < n_seq; i0 += 32) {
         const int i = i0 + lane;
         int inc = 0;
         if (i < n_seq) {
             const int4 e = *reinterpret_cast<const int4 *>(entries + i * kKvStepWords);
             inc = static_cast<int>((static_cast<long long>(e.z) * g_heads + rows - 1) / rows);
-            most = max(most, (P.window ? min(e.w, min(P.window, e.w) + rows / g_heads) : e.w) + 127 >> 7);
+            most = max(most, (P.window ? min(e.w, min(P.window, e.w) + (TREE ? e.z : rows / g_heads)) : e.w) + 127 >> 7);
+            most_rows = max(most_rows, e.z);
         }
         const int v = inc;
 #pragma unroll
@@ -112,6 +119,7 @@ __device__ __forceinline__ void prompt_prefix(const KvPrompt &P, int rows, int *
         sum += __shfl_sync(0xffffffffu, inc, 31);
     }
     most = __reduce_max_sync(0xffffffffu, most);
+    if (TREE && __any_sync(0xffffffffu, most_rows > kTreeRows)) sum = 0;        // (a replay on such a step does nothing)
     if (lane == 0) {
         prefix[n_seq] = sum;
         prefix[n_seq + 1] = most;
@@ -144,8 +152,9 @@ __device__ __forceinline__ PromptItem prompt_item(const KvPrompt &P, const int *
     return it;
 }
 
-template <int D, bool SPLIT, bool E4M3>
-__global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __grid_constant__ KvPrompt P) {
+template <int D, bool SPLIT, bool E4M3, class Params>
+__global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __grid_constant__ Params P) {
+    constexpr bool TREE = std::is_same_v<Params, KvPromptTree>;
     using A = PromptAttPlan<D, SPLIT>;
     constexpr int KT = A::kKt, T = A::kTiles, ST = A::kStages, CW = D % 64 == 0 ? 64 : 32, SUBS = KT / 16;
     constexpr int kPartP = A::kApart && !SPLIT ? 16 : 32;           // columns of the weights of 32 tokens
@@ -153,6 +162,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
     __shared__ __align__(8) uint64_t q_full[T], k_full[ST], k_free[ST], v_full[ST], v_free[ST], s_full[T], s_free[T], p_full[T], o_done[T];
     __shared__ __align__(16) float4 scales[4][SUBS];
     __shared__ uint32_t tmem_base;
+    __shared__ int8_t places[TREE ? 2 : 1][T][TREE ? kTreeRows : 1];        // of an item and the one behind it
     uint8_t *qs = psm, *ks = psm + T * A::kQTile, *vs = ks + ST * A::kK;
     int *prefix = reinterpret_cast<int *>(vs + ST * A::kV);
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -192,7 +202,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
         const long long at = static_cast<long long>(turn) * gridDim.x + (turn & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         if (at >= n_items * runs) return false;
         it = prompt_item(P, prefix, n_seq, runs > 1 ? at / runs : at, A::kRows);
-        const int start = it.length - it.count, pos0 = start + it.item_row / g_heads, pos1 = start + min(it.item_row + A::kRows - 1, it.rows - 1) / g_heads;
+        const int start = it.length - it.count, pos0 = start + (TREE ? 0 : it.item_row / g_heads), pos1 = start + min(it.item_row + A::kRows - 1, it.rows - 1) / g_heads;
         it.lo = P.window ? max(0, pos0 - P.window + 1) / KT : 0;
         it.hi = pos1 / KT + 1;
         if (runs > 1) {
@@ -419,6 +429,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
             const int pos = start + min(row, last) / g_heads;
             const int warp_row = it.item_row + x * 128 + (warp & 3) * 32, pos_lo = start + min(warp_row, last) / g_heads, pos_hi = start + min(warp_row + 31, last) / g_heads;
             const bool is = row <= last;
+            if constexpr (TREE) {
+                if (r < it.count) places[turn & 1][x][r] = static_cast<int8_t>(tree_parent(P.parents, it.row0, r));
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + x) : "memory");
+            }
             const size_t elem = (static_cast<size_t>(it.head) * g_heads + row % g_heads) * D;
             const size_t src = static_cast<size_t>(it.row0 + row / g_heads) * P.q_stride + elem;
             // q: the row's largest magnitude, then its F16 terms; element k of row r lies at (k / 8) 2048 + r 16
@@ -495,7 +509,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
                         att_wait(&s_full[x], n_s++ & 1, P.status);
                         tc_fence_after();
                         const int first = tile * KT;
-                        const bool edge = first + KT - 1 > pos_lo || (P.window && first <= pos_hi - P.window);
+                        const bool edge = TREE ? first + KT - 1 >= start || (P.window && first <= start + it.count - 1 - P.window)
+                                               : first + KT - 1 > pos_lo || (P.window && first <= pos_hi - P.window);
+                        TreeSight sight = {~0ull, ~0ull};
+                        if constexpr (TREE)
+                            if (edge) sight = tree_sight(places[turn & 1][x], pos - start, start, first, P.window);
                         if constexpr (kFar) {           // (rare: little code, few registers, the scores read twice)
                             float most = kAttFloor;
                             uint32_t u[32], hi[16], lo[16];
@@ -504,8 +522,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
                                 tc_wait_ld(u);
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) {
-                                    const int p = i & 15, token = first + c * 32 + (i & 16) + (p >> 2) * 2 + (p & 1) + ((p & 2) << 2);
-                                    if (token > pos || (P.window && token <= pos - P.window)) u[i] = 0xff800000u;
+                                    const int p = i & 15, in = (i & 16) + (p >> 2) * 2 + (p & 1) + ((p & 2) << 2), token = first + c * 32 + in;
+                                    if constexpr (TREE) {
+                                        if (!((c & 2 ? sight.hi : sight.lo) >> (c & 1) * 32 + in & 1ull)) u[i] = 0xff800000u;
+                                    } else {
+                                        if (token > pos || (P.window && token <= pos - P.window)) u[i] = 0xff800000u;
+                                    }
                                 }
                             };
 #pragma unroll 1
@@ -557,8 +579,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
                                 for (int c = 0; c < KT / 32; ++c)
 #pragma unroll
                                     for (int i = 0; i < 32; ++i) {
-                                        const int p = i & 15, token = first + c * 32 + (i & 16) + (p >> 2) * 2 + (p & 1) + ((p & 2) << 2);
-                                        if (token > pos || (P.window && token <= pos - P.window)) v[c][i] = 0xff800000u;
+                                        const int p = i & 15, in = (i & 16) + (p >> 2) * 2 + (p & 1) + ((p & 2) << 2), token = first + c * 32 + in;
+                                        if constexpr (TREE) {
+                                            if (!((c & 2 ? sight.hi : sight.lo) >> (c & 1) * 32 + in & 1ull)) v[c][i] = 0xff800000u;
+                                        } else {
+                                            if (token > pos || (P.window && token <= pos - P.window)) v[c][i] = 0xff800000u;
+                                        }
                                     }
                             }
                             float most = kAttFloor;
@@ -734,8 +760,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv_prompt_kernel(const __gr
 }
 
 // The runs' sums of each row of the items: a thread has four elements of a row, a warp 32 rows.
-template <int D>
-__global__ void __launch_bounds__(256) kv_prompt_join_kernel(const __grid_constant__ KvPrompt P) {
+template <int D, class Params>
+__global__ void __launch_bounds__(256) kv_prompt_join_kernel(const __grid_constant__ Params P) {
     constexpr int ROWS = D <= 128 ? 256 : 128, UNITS = ROWS * (D / 4);
     __shared__ int prefix[kAttMaxSeqs + 2];
     const int tid = threadIdx.x, n_seq = P.book[0], g_heads = P.s.heads / P.s.kv_heads;

@@ -17,8 +17,8 @@
 // item's end, the first of which then holds what it has of an item that ends in a later one's.
 //
 // A tile of 128 rows by 128 tokens takes a CTA 1.75 us at heads of 128, 1.1 at 64: instruction issue (codes to operands, softmax) and exponentials, not memory. 16 trees of 26 rows
-// behind 300 to 6,000 tokens, 32/8 heads of 128: 64 us (12 at the memory's rate; by the kernel of chains 145); 64 rows behind 131,025: 205 to 233 (83 at the tensor cores' rate). There
-// both row blocks of a head expand the same codes: the kernel of prompts, which does so once for 256 rows, takes 184, and more on every shorter shape.
+// behind 300 to 6,000 tokens, 32/8 heads of 128: 64 us (12 at the memory's rate; by the kernel of chains 145); 64 rows behind 131,025: 207 to 233 (83 at the tensor cores' rate). There
+// both row blocks of a head expand the same codes, which the kernel for prompts does once for 256 rows (184): choose_tree() gives it such steps.
 #pragma once
 
 #include "wd_kv_prompt.cuh"
