@@ -655,10 +655,13 @@ __global__ void __launch_bounds__(kVerThreads, DRAFT ? 2 : 3) verify_kernel(cons
     }
 }
 
+constexpr long long kVerHeld = 227 * 1024 - static_cast<long long>(sizeof(VerifyShared)) - 1024;         // bytes of rows that a CTA holds at most
+
 template <class T, bool HELD, bool DRAFT>
 int verify_launch(const VerifyParams &p, size_t smem, cudaStream_t s) {
     auto kernel = verify_kernel<T, HELD, DRAFT>;
-    WD_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    // (the attribute is the kernel's, for all threads: never what this call needs alone)
+    if (HELD) WD_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kVerHeld)));
     if (p.ctas > 8) WD_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(p.n_seqs) * p.ctas);
@@ -681,13 +684,13 @@ int verify_of(VerifyParams p, int n_sm, cudaStream_t s) {
     while (p.ctas < kVerCtas && static_cast<long long>(p.n_seqs) * p.ctas * 2 <= 8 * n_sm && p.vocab >= p.ctas * 2 * kVerThreads * 4) p.ctas *= 2;
     p.piece = static_cast<int>((static_cast<long long>(p.vocab) + p.ctas * kVerThreads - 1) / (p.ctas * kVerThreads)) | 1;
     // What shared memory holds of the rows: one row where there are many CTAs, two of them an SM; up to four where there are few.
-    const long long run_bytes = static_cast<long long>(p.piece) * 32 * sizeof(T) + 16, slot = run_bytes * kVerWarps * (p.draft ? 2 : 1), most = 227 * 1024 - static_cast<long long>(sizeof(VerifyShared)) - 1024;
-    if (slot > most) {
+    const long long run_bytes = static_cast<long long>(p.piece) * 32 * sizeof(T) + 16, slot = run_bytes * kVerWarps * (p.draft ? 2 : 1);
+    if (slot > kVerHeld) {
         p.slots = p.run_bytes = 0;
         return p.draft ? verify_launch<T, false, true>(p, 0, s) : verify_launch<T, false, false>(p, 0, s);
     }
     p.run_bytes = static_cast<int>(run_bytes);
-    p.slots = static_cast<long long>(p.n_seqs) * p.ctas <= n_sm ? static_cast<int>(std::min<long long>(kVerSlots, most / slot)) : 1;
+    p.slots = static_cast<long long>(p.n_seqs) * p.ctas <= n_sm ? static_cast<int>(std::min<long long>(kVerSlots, kVerHeld / slot)) : 1;
     const size_t smem = static_cast<size_t>(slot) * p.slots;
     return p.draft ? verify_launch<T, true, true>(p, smem, s) : verify_launch<T, true, false>(p, smem, s);
 }
