@@ -1,4 +1,5 @@
 """Calls of two host threads at once, of one kernel and other sizes: what a launch needs of a kernel belongs to the call."""
+import ctypes
 import threading
 
 import numpy as np
@@ -56,3 +57,37 @@ def test_verification_of_two_vocabularies(with_draft, dtype, type_):
     assert side_by_side(*(p[0] for p in pairs), turns=3000) == []
     for _, out, want, _ in pairs:
         assert all(torch.equal(x, y) for x, y in zip(out, want))
+
+
+@pytest.mark.parametrize("neighbours", [False, True])
+def test_rotary_append_into_two_caches(neighbours):
+    def one(dim, page, count):
+        kv = wd.KvCache(1, 2, 2, dim, 8, 1, 8 * page, page_tokens=page)
+        rope = wd.Rope(dim, neighbours=neighbours)
+        gen = torch.Generator("cuda").manual_seed(dim)
+        k, v, q = (torch.randn(count, 2, dim, generator=gen, device="cuda") for _ in range(3))
+        out, s = torch.zeros_like(q), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        kv.begin([0], [count], s.cuda_stream)
+
+        rows = wd.RopeRows(None, None, None, k.data_ptr(), v.data_ptr(), q.data_ptr(), out.data_ptr(), 0, 0, 0, 0, 1e-6, wd.TYPE_F32)
+        args, f = (kv.h, 0, rope.h, ctypes.byref(rows), s.cuda_stream), wd.lib().wd_kv_append_rope
+
+        def call():                     # (by the C entry: less of the turn is the interpreter's, which one thread has at a time)
+            if f(*args):
+                raise RuntimeError(wd.lib().wd_last_error().decode())
+
+        def read():
+            got = [torch.zeros(count, 2, dim, device="cuda") for _ in range(2)]
+            torch.cuda.synchronize()
+            kv.read(0, [0], [0], [count], *(g.data_ptr() for g in got), stream=s.cuda_stream)
+            torch.cuda.synchronize()
+            return [out.cpu().numpy()] + [g.cpu().numpy() for g in got]
+
+        call()
+        return call, read, read(), (k, v, q, kv, rope, rows)
+
+    pairs = [one(256, 128, 64), one(64, 64, 40), one(256, 128, 64), one(64, 64, 40)]
+    assert side_by_side(*(p[0] for p in pairs), turns=15000) == []
+    for _, read, want, _ in pairs:
+        assert all(np.array_equal(x, y) for x, y in zip(read(), want))

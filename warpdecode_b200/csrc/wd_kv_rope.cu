@@ -30,6 +30,7 @@ namespace wd {
 namespace {
 
 constexpr int kRopePairs = 4;       // of a lane: heads of up to 256
+constexpr int kRopeHeld = 16384;    // floats of rotated keys that a block holds at most; the codes of a page's values are no more bytes than these
 
 struct KvRope {
     KvAppend a;
@@ -564,7 +565,7 @@ int wd_kv_append_rope(wd_kv_cache *c, int layer, const wd_rope *r, const wd_rope
         for (int i = 0; i < 4; ++i) p.section_end[i] = r->section_end[i];
         for (int i = 0; i < 128; ++i) p.turns[i] = r->turns[i];
         const int most = std::min(c->max_rows, c->cfg.page_tokens);       // of a page (a replay may have more)
-        p.held = std::min(most, 16384 / D);
+        p.held = std::min(most, wd::kRopeHeld / D);
         const size_t smem = std::max<size_t>(static_cast<size_t>(p.held) * D * 4, static_cast<size_t>(c->cfg.page_tokens) * D);
         // one head of q a block where there are not enough blocks for the SMs, all that share a kv head where there are
         p.q_parts = std::max<long long>(1, std::min<long long>(g, 4ll * c->n_sm / (static_cast<long long>(c->items) * H)));
@@ -576,7 +577,8 @@ int wd_kv_append_rope(wd_kv_cache *c, int layer, const wd_rope *r, const wd_rope
         return by_rows_and_codes(c, rows_of, [&](auto t, auto e4m3) {
             using T = decltype(t);
             auto launch = [&](auto kernel, int threads) {
-                WD_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+                // (the attribute is the kernel's, for all threads and caches: never what this call needs alone)
+                WD_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, wd::kRopeHeld * 4));
                 kernel<<<grid, threads, smem, s>>>(p);
                 WD_TRY_CUDA(cudaGetLastError());
                 return WD_OK;
