@@ -353,9 +353,10 @@ __global__ void __launch_bounds__(kVerThreads, DRAFT ? 2 : 3) verify_kernel(cons
         return is;
     };
     // What is left of the target: max(p - c q, 0) zp = max(w - ratio v, 0) of the terms w and v of p and q, ratio = c zp / zq. So one pass finds zp, zq and what the
-    // first rejection leaves, although it needs them: it takes the ratio that the F32 sums give, and beside the sum of the terms v that have something left. The right
-    // ratio is less than 2^-19 of itself off that, and the sum less by the difference times that of v. Terms that something is left of by one ratio and nothing by
-    // the other are known by lying within 2^-18; where they could be felt (a draft that is the target but for a few tokens) a pass is made with the right one.
+    // first rejection leaves, although it needs them: it takes the ratio that the F32 sums give, and beside the sum of the terms v that have something left. By the right
+    // ratio the sum is less by the difference times that of v, but for terms that something is left of by one ratio and nothing by the other. Where the ratios are within
+    // 2^-19 of each other, such a term's w - ratio v is below 2^-19 ratio v, and that below 2^-18 w: those terms' v are summed too. Where they could be felt (a draft that
+    // is the target but for a few tokens), or the ratios are farther apart, a pass is made with the right one.
     auto left_of = [&](const T *x, const T *y, int i, double r) { return fmax(fma(-r, power(static_cast<float>(y[i]), sq.m), power(static_cast<float>(x[i]), sp.m)), 0.0); };
     // The whole cluster's sums (first: p, q and what is left of p; else one), the CTAs' of what a draw is made from in the slots, the warps' and the lanes' in their places.
     auto sums = [&](auto kind, double *found) {
@@ -372,7 +373,7 @@ __global__ void __launch_bounds__(kVerThreads, DRAFT ? 2 : 3) verify_kernel(cons
             b += w;
             d += v;
             e += rest > 0.0 ? v : 0.0;
-            near += (__double2hiint(rest) & 0x7fffffff) + (18 << 20) < __double2hiint(v) ? v : 0.0;
+            near += (__double2hiint(rest) & 0x7fffffff) + (18 << 20) < __double2hiint(w) ? v : 0.0;
             return fmax(rest, 0.0);
         };
         int i = lane0;
@@ -530,7 +531,7 @@ __global__ void __launch_bounds__(kVerThreads, DRAFT ? 2 : 3) verify_kernel(cons
                         bend = zp / zq - ratio;
                         over_zq = 1.0 / zq;
                         first_left = fmax(found[0] - bend * found[1], 0.0);
-                        if (fabs(bend) * found[4] > 1e-13 * first_left) {
+                        if (fabs(bend) * found[4] > 1e-13 * first_left || !(fabs(bend) <= 0x1p-19 * ratio)) {
                             ratio += bend;
                             bend = 0.0;
                             sums(Left{}, &first_left);
