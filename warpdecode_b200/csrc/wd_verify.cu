@@ -6,8 +6,8 @@
 // vocabulary's size is kept from one child to the next, and a number each decides: u S q(x) < max(p(x) - c q(x), 0).
 //
 // A cluster of CTAs goes down a sequence's tree and reads the rows on its way alone, not those of all drafts. A row's maximum and sum are F32 and decide
-// for a child that is not within 1e-4 of its border. What is nearer, and every draw, is made of sums in 64 bits: the running sums of 150,000 tokens lie 1e-7
-// apart where the unlikely ones are, and the heavy ones' F32 errors (3e-8) would choose among them.
+// for a child that is not within 1e-4 of its border, or more where a thread has very many terms. What is nearer, and every draw, is made of sums in 64 bits: the running sums
+// of 150,000 tokens lie 1e-7 apart where the unlikely ones are, and the heavy ones' F32 errors (3e-8) would choose among them.
 //
 // A warp has a run of the vocabulary, the warps of a cluster one behind the other. It copies its part of a row into shared memory, where all of the row's passes
 // read it, and where there are few sequences that of the rows that may be next beside it. What a CTA finds it sends to all CTAs' shared memory, where 16 bytes from
@@ -36,7 +36,11 @@ namespace {
 
 constexpr int kVerThreads = 256, kVerWarps = kVerThreads / 32, kVerCtas = 16, kVerRows = 1024, kVerSlots = 4;
 constexpr float kVerGreedy = 1e-6f, kVerFloor = -3.402823466e38f;
-constexpr float kVerUnsure = 1e-4f;        // F32 sums and exponentials are off by less than half of it
+// How near its border, relative to the numbers that are compared, a child is left to the sums in 64 bits. Exponents are off by three roundings of up to 120 (2^-16 of a term),
+// a lane's sum of n terms by 11 roundings of 2^-24 for every ten: four of the exponential by which it follows a larger maximum, one of that product, six of additions.
+// Together less than 3e-5 and n 2^-23 of a probability. 1e-4 is more than that up to 580 terms a lane: 2.3 million tokens by 16 CTAs, 148,000 by one.
+constexpr float kVerUnsure = 1e-4f;
+inline float ver_unsure(int piece) { return fmaxf(kVerUnsure, 3e-5f + 0x1p-23f * static_cast<float>(piece)); }
 
 struct VerifyParams {
     const void *target, *draft;
@@ -45,6 +49,7 @@ struct VerifyParams {
     const int *first, *tokens, *parents;
     const float *uniforms, *temperature;
     int *path, *count, *next;
+    float unsure;           // see ver_unsure
     double power[32];       // 2^(j / 32)
 };
 
@@ -556,7 +561,7 @@ __global__ void __launch_bounds__(kVerThreads, DRAFT ? 2 : 3) verify_kernel(cons
                 if (!dp && __shfl_sync(0xffffffffu, again, i)) continue;          // (nothing of it is left)
                 // 1: taken, 2: F32 cannot tell
                 const float l = u * static_cast<float>(left) * q;
-                int verdict = exact || !told || !(fabsf(l - p) > kVerUnsure * (p + u * q)) ? 2 : l < p ? 1 : 0;
+                int verdict = exact || !told || !(fabsf(l - p) > P.unsure * (p + u * q)) ? 2 : l < p ? 1 : 0;
                 verdict = __shfl_sync(0xffffffffu, verdict, i);
                 if (verdict == 2) {
                     if (!exact) {
@@ -684,6 +689,7 @@ int verify_of(VerifyParams p, int n_sm, cudaStream_t s) {
     p.ctas = 1;
     while (p.ctas < kVerCtas && static_cast<long long>(p.n_seqs) * p.ctas * 2 <= 8 * n_sm && p.vocab >= p.ctas * 2 * kVerThreads * 4) p.ctas *= 2;
     p.piece = static_cast<int>((static_cast<long long>(p.vocab) + p.ctas * kVerThreads - 1) / (p.ctas * kVerThreads)) | 1;
+    p.unsure = ver_unsure(p.piece);
     // What shared memory holds of the rows: one row where there are many CTAs, two of them an SM; up to four where there are few.
     const long long run_bytes = static_cast<long long>(p.piece) * 32 * sizeof(T) + 16, slot = run_bytes * kVerWarps * (p.draft ? 2 : 1);
     if (slot > kVerHeld) {
