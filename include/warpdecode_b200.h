@@ -506,6 +506,7 @@ int wd_token_logprobs(const void *logits_dev, int type, int rows, int vocab, int
  *                        copy: wd_kv_keep(c, seq, tokens before the step, count, path)
  *   count_dev[n_seqs]    how many they are; 0 for a sequence without rows
  *   next_dev[n_seqs]     the token behind them; -1 for a sequence without rows, or where a row has no distribution (a NaN, +inf, nothing but -inf)
+ * A sequence whose CTAs waited a second for one another in vain has a count of -1, and nothing but -1 in its path and as the token behind.
  *
  * Running sums are 64 bits, so that a number that is not next to a border gives the same token however they are ordered. strides: elements from row to row,
  * 0 = vocab. Without a workspace; runs on the device of target_dev; can be captured. */

@@ -22,6 +22,8 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdio>
+#include <cstdlib>
 #include <type_traits>
 
 #include "wd_device.cuh"
@@ -50,6 +52,7 @@ struct VerifyParams {
     const float *uniforms, *temperature;
     int *path, *count, *next;
     float unsure;           // see ver_unsure
+    int stop_at, stop_rank, stop_warp;      // tests: the meeting whose wait runs out, -1: none; in which CTA, in which of its warps, -1: in all
     double power[32];       // 2^(j / 32)
 };
 
@@ -100,6 +103,7 @@ struct VerifyShared {
     uint64_t full[2];
     double power[32], lane_sum[kVerWarps][32], lane_bend[kVerWarps][32];
     int rejected[kVerRows];                             // tokens
+    int gone_at;                                        // the barrier that a warp came to after a wait that ran out
     int16_t parents[kVerRows], kids[kVerWarps][32], path[kVerRows];
 };
 struct VerOne {
@@ -115,6 +119,19 @@ __device__ __forceinline__ void ver_send(uint4 *to, uint64_t *bar, int cta, uint
         " st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [a], {%3, %4, %5, %6}, [b];\n}" ::"r"(smem_u32(to)),
         "r"(smem_u32(bar)), "r"(cta), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
         : "memory");
+}
+
+// whether the barrier's phase was completed within a second
+__device__ __forceinline__ bool ver_wait(uint64_t *bar, uint32_t parity) {
+    unsigned long long t0 = 0;
+#pragma unroll 1
+    for (unsigned i = 1; !mbar_try_wait(bar, parity); ++i) {
+        if (i % 64 != 0) continue;          // (the timer is slow to read, and an ordinary wait is over before)
+        const unsigned long long t = global_timer_ns();
+        if (i == 64) t0 = t;
+        else if (t - t0 > kWaitLimitNs) return false;
+    }
+    return true;
 }
 
 enum { kSumFirst, kSumLeft, kSumTarget };   // of p, of q and of max(p - q, 0); of max(p - c q, 0); of p without the rejected tokens
@@ -223,6 +240,7 @@ __global__ void __launch_bounds__(kVerThreads, DRAFT ? 2 : 3) verify_kernel(cons
         sh.parents[i] = static_cast<int16_t>(p >= 0 && p < i ? p : -1);
     }
     if (tid < 32) sh.power[tid] = P.power[tid];
+    if (tid == 0) sh.gone_at = 0x7fffffff;
     const bool greedy = !(heat >= kVerGreedy), with_draft = DRAFT && !greedy;
     const float k = greedy ? 1.44269504f : fmaxf(static_cast<float>(1.4426950408889634 / heat), 1e-30f);        // (not 0: -inf times k has to stay what it is)
     const double k32 = greedy ? 0.0 : 32 * 1.4426950408889634 / heat;
@@ -236,32 +254,44 @@ __global__ void __launch_bounds__(kVerThreads, DRAFT ? 2 : 3) verify_kernel(cons
     // What the warps of the cluster bring, put together by `join` (of a lane's 16 bytes, whether it has any; the same in all lanes). The places of a turn are free
     // again when all have come to the next one.
     int turn = 0, meetings = 0;
-    bool lost = false;                      // a wait has run out
-    auto meet = [&](auto mine, auto join) {          // (one or three times 16 bytes)
+    // A wait that runs out in a warp (gone) is known to all of the CTA from that warp's next barrier on, whichever it is to the others (lost): the warp says which number it
+    // has before it comes there. (__syncthreads_or() takes 150 ns more than a barrier.) From then on nothing is sent or waited for. What such a warp finds is zeros.
+    bool gone = false, lost = false;
+    int barriers = 0;
+    const int stop_at = (P.stop_rank < 0 || rank == P.stop_rank) && (P.stop_warp < 0 || warp == P.stop_warp) ? P.stop_at : -1;
+    auto all_here = [&]() __attribute__((always_inline)) {
+        if (lost) return;
+        ++barriers;
+        if (gone) sh.gone_at = barriers;
+        __syncthreads();
+        lost = *static_cast<volatile int *>(&sh.gone_at) <= barriers;
+    };
+    auto meet = [&](auto mine, auto join) __attribute__((always_inline)) {          // (one or three times 16 bytes)
         constexpr int N = sizeof(mine) / 16;
+        const decltype(mine) nothing{};
+        if (lost) return nothing;
         if (lane == 0)
 #pragma unroll
             for (int i = 0; i < N; ++i) sh.warp_slot[turn][warp][i] = mine.v[i];
         if (ctas > 1 && tid == 0) mbar_expect_tx(&sh.full[turn], 16 * N * ctas);
-        __syncthreads();
+        all_here();
         auto all = mine;
         if (ctas == 1 || warp == 0) {
 #pragma unroll
             for (int i = 0; i < N; ++i) all.v[i] = sh.warp_slot[turn][lane & (kVerWarps - 1)][i];
             all = join(all, lane < kVerWarps);
         }
+        if (lost) return nothing;           // (asked behind the reading of the slots, which takes as long)
         if (ctas > 1) {
             if (meetings == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");        // (all have made their barriers)
             if (warp == 0 && lane < ctas)
 #pragma unroll
                 for (int i = 0; i < N; ++i) ver_send(&sh.slot[turn][rank][i], &sh.full[turn], lane, all.v[i]);
-            bool there = false;
-#pragma unroll 1
-            for (unsigned i = 0; i < kSpinLimit && !there && !lost; ++i) there = mbar_try_wait(&sh.full[turn], meetings >> 1 & 1);
-            lost = !__all_sync(0xffffffffu, there);
+            gone = !__all_sync(0xffffffffu, meetings != stop_at && ver_wait(&sh.full[turn], meetings >> 1 & 1));
 #pragma unroll
             for (int i = 0; i < N; ++i) all.v[i] = sh.slot[turn][lane & (kVerCtas - 1)][i];
             all = join(all, lane < ctas);
+            if (gone) all = nothing;
         }
         turn ^= 1;
         ++meetings;
@@ -279,7 +309,7 @@ __global__ void __launch_bounds__(kVerThreads, DRAFT ? 2 : 3) verify_kernel(cons
     // maxima and sums of the row, and its largest logit
     RowSum sp{}, sq{};
     int best = 0;
-    auto row_sums = [&]() {
+    auto row_sums = [&]() __attribute__((always_inline)) {
         constexpr int U = 10;
         float m[2] = {kVerFloor, kVerFloor}, s[2] = {0.0f, 0.0f}, top = none;
         int top_at = 0;
@@ -364,7 +394,7 @@ __global__ void __launch_bounds__(kVerThreads, DRAFT ? 2 : 3) verify_kernel(cons
     // is the target but for a few tokens), or the ratios are farther apart, a pass is made with the right one.
     auto left_of = [&](const T *x, const T *y, int i, double r) { return fmax(fma(-r, power(static_cast<float>(y[i]), sq.m), power(static_cast<float>(x[i]), sp.m)), 0.0); };
     // The whole cluster's sums (first: p, q and what is left of p; else one), the CTAs' of what a draw is made from in the slots, the warps' and the lanes' in their places.
-    auto sums = [&](auto kind, double *found) {
+    auto sums = [&](auto kind, double *found) __attribute__((always_inline)) {
         constexpr int KIND = decltype(kind)::value, U = KIND == kSumTarget ? 8 : 4;
         double a = 0.0, b = 0.0, d = 0.0, e = 0.0, near = 0.0;
         const T *x = run_of(0, warp, run0), *y = KIND == kSumTarget ? nullptr : run_of(1, warp, run0);
@@ -490,7 +520,7 @@ __global__ void __launch_bounds__(kVerThreads, DRAFT ? 2 : 3) verify_kernel(cons
             slot = held;
         }
         row_sums();
-        if (lost || !(sp.m < INFINITY)) break;
+        if (gone || lost || !(sp.m < INFINITY)) break;
         if (greedy) {
             const int top = best;
             if (!(sp.s > none)) break;
@@ -526,7 +556,7 @@ __global__ void __launch_bounds__(kVerThreads, DRAFT ? 2 : 3) verify_kernel(cons
             if (!dp && (todo & (todo - 1u))) again = (__match_any_sync(0xffffffffu, x) & ((1u << lane) - 1u)) != 0u;
             if (!dp && n_rejected > 0) again |= is_rejected(x);
             double exact_p = 0.0, exact_q = 1.0;
-            auto make_exact = [&]() {
+            auto make_exact = [&]() __attribute__((always_inline)) {
                 if (!exact) {
                     double found[6];
                     if (dp) {
@@ -592,14 +622,15 @@ __global__ void __launch_bounds__(kVerThreads, DRAFT ? 2 : 3) verify_kernel(cons
                     }
                 } else {
                     left = fmax(left - (exact ? __shfl_sync(0xffffffffu, exact_p, i) : static_cast<double>(__shfl_sync(0xffffffffu, p, i))), 0.0);
-                    const int gone = __shfl_sync(0xffffffffu, x, i);
-                    __syncthreads();
-                    if (tid == 0) sh.rejected[n_rejected] = gone;
-                    __syncthreads();
+                    const int out = __shfl_sync(0xffffffffu, x, i);
+                    all_here();
+                    if (tid == 0) sh.rejected[n_rejected] = out;
+                    all_here();
+                    if (lost) break;
                     ++n_rejected;
                 }
             }
-            if (to >= 0 || from >= n) break;
+            if (to >= 0 || lost || from >= n) break;
             child = children(from);
             look_up();
         }
@@ -629,7 +660,7 @@ __global__ void __launch_bounds__(kVerThreads, DRAFT ? 2 : 3) verify_kernel(cons
             const double v[1] = {sum_in(sh.slot[turn ^ 1][lane & (kVerCtas - 1)][0], lane < ctas)};
             const int owner = ver_pick(v, aim, base, lane);
             mine_to_say = max(owner, 0) == rank;
-            if (lost || !mine_to_say || owner < 0) break;
+            if (gone || lost || !mine_to_say || owner < 0) break;
         }
         if (warp > 0) break;
         const double of_warp[1] = {sum_in(sh.warp_slot[turn ^ 1][lane & (kVerWarps - 1)][0], lane < kVerWarps)};
@@ -653,13 +684,31 @@ __global__ void __launch_bounds__(kVerThreads, DRAFT ? 2 : 3) verify_kernel(cons
         break;
     }
     if constexpr (HELD) asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (mine_to_say && tid == 0) P.next[seq] = lost ? -1 : token;
+    all_here();                             // (and the path is there)
+    if (lost) {
+        // None may leave while another one could send to it: those whose waits have run out meet here (of the others none sends any more: they have left), and wait once
+        // more for what is on its way to them. Whatever the others said of the sequence before they left, it has no answer.
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+        ver_wait(&sh.full[turn ^ 1], (meetings - 1) >> 1 & 1);
+        for (int i = tid; i < n; i += kVerThreads) P.path[f0 + i] = -1;
+        if (tid == 0) P.count[seq] = P.next[seq] = -1;
+        return;
+    }
+    if (mine_to_say && tid == 0) P.next[seq] = token;
     if (rank == 0) {
-        __syncthreads();
         if (tid == 0) P.count[seq] = level;
         for (int i = tid; i < n; i += kVerThreads) P.path[f0 + i] = i < level ? sh.path[i] : -1;
     }
 }
+
+// WD_VERIFY_STOP_AT=meeting[:CTA[:warp]] (tests): the wait of a sequence's CTAs for one another that runs out
+struct VerStop {
+    int at = -1, rank = -1, warp = -1;
+    VerStop() {
+        if (const char *v = std::getenv("WD_VERIFY_STOP_AT")) std::sscanf(v, "%d:%d:%d", &at, &rank, &warp);
+    }
+};
 
 constexpr long long kVerHeld = 227 * 1024 - static_cast<long long>(sizeof(VerifyShared)) - 1024;         // bytes of rows that a CTA holds at most
 
@@ -690,6 +739,10 @@ int verify_of(VerifyParams p, int n_sm, cudaStream_t s) {
     while (p.ctas < kVerCtas && static_cast<long long>(p.n_seqs) * p.ctas * 2 <= 8 * n_sm && p.vocab >= p.ctas * 2 * kVerThreads * 4) p.ctas *= 2;
     p.piece = static_cast<int>((static_cast<long long>(p.vocab) + p.ctas * kVerThreads - 1) / (p.ctas * kVerThreads)) | 1;
     p.unsure = ver_unsure(p.piece);
+    static const VerStop stop;
+    p.stop_at = stop.at;
+    p.stop_rank = stop.rank;
+    p.stop_warp = stop.warp;
     // What shared memory holds of the rows: one row where there are many CTAs, two of them an SM; up to four where there are few.
     const long long run_bytes = static_cast<long long>(p.piece) * 32 * sizeof(T) + 16, slot = run_bytes * kVerWarps * (p.draft ? 2 : 1);
     if (slot > kVerHeld) {
