@@ -373,15 +373,15 @@ int wd_head_argmax_q8_0(void *packed_dev, int rows, int cols, const float *x_dev
  *
  * Which sequence holds which pages is kept on the host (calls fail there, with nothing changed) and sent to the device in the
  * stream's order: calls of one cache are made from one host thread at a time and on one stream, or on streams that the caller orders.
- * stream: a cudaStream_t of the cache's device, NULL = its default stream. wd_kv_append, wd_kv_append_rope, wd_kv_attend and wd_kv_read can be captured;
- * the others cannot (they are refused), but may come between replays: a replayed append or attend works on the step that is current
+ * stream: a cudaStream_t of the cache's device, NULL = its default stream. wd_kv_append, wd_kv_append_rope, wd_kv_attend, wd_kv_attend_tree and wd_kv_read can be
+ * captured; the others cannot (they are refused), but may come between replays: a replayed append or attend works on the step that is current
  * then, with the launches of the captured one (any step is answered rightly; the captured rows should be about as many), and does
  * nothing where none is; a replayed read reads its tokens from the pages that the sequences have then.
  *
  * Rows: [rows][heads][head_dim] of F32, F16 or BF16 (WD_TYPE_*); a stride is the elements from one row to the next, 0 = rows lie
  * one behind the other, so that the parts of a fused q/k/v row can be used where they are. Sums, maxima and scores are F32. F32 rows are
  * answered to about 2^-20 of the values' size (the largest that the pages they see can hold) by the kernel for few rows, to 2^-15 by the
- * one for prompts (tensor cores cut long sums of one sign off), F16 and BF16 rows to their own rounding. A weight counts down to 2^-38 of
+ * ones for prompts and trees (tensor cores cut long sums of one sign off), F16 and BF16 rows to their own rounding. A weight counts down to 2^-38 of
  * its row's largest (rows of 16 bits in the kernel for prompts: 2^-34): less is rounded to one of these steps. Scores (scale q k) are taken
  * to be below 2^20, beyond which F32 tells their exponentials no longer apart; a row with larger ones may be answered with NaN. */
 #define WD_KV_INT8 0
@@ -411,7 +411,7 @@ int wd_kv_append(wd_kv_cache *c, int layer, const void *k_dev, const void *v_dev
 /* Rotary positions of heads: pair p of the first rotary_dim elements of a head turns by the angle position * f_p, f_p = theta^(-2p / rotary_dim), or inv_freq[p]
  * (host, rotary_dim / 2 of them; null: from theta): (x0, x1) -> factor (x0 cos - x1 sin, x1 cos + x0 sin). With several axes (time, height, width of a picture's or a
  * film's tokens) a token has a position on each, and the first sections[0] pairs go by the first, the next sections[1] by the second, and so on; they are
- * rotary_dim / 2 together. Angles are made in 64 bits. The handle is host memory only, belongs to no device, and may serve several caches and threads. */
+ * rotary_dim / 2 together (runs of pairs: an order that deals the pairs out to the axes in turn cannot be said). Angles are made in 64 bits. The handle is host memory only, belongs to no device, and may serve several caches and threads. */
 #define WD_ROPE_HALVES 0        /* element p with element p + rotary_dim / 2 */
 #define WD_ROPE_NEIGHBOURS 1    /* element 2p with element 2p + 1 */
 typedef struct {
@@ -438,7 +438,9 @@ typedef struct {
     int32_t type;
 } wd_rope_rows;
 /* As wd_kv_append, k with its norm and rotation on the way (in 64 bits, rounded to F32 once, then to codes), and q with its own into q_out (in F32, rounded
- * to the rows' type). v as it is. An infinity or a NaN in k makes numbers that are none of its pair, or with a norm of its head. Can be captured, as wd_kv_append can. */
+ * to the rows' type). v as it is. What is no number of a pair is none of both its elements; with a norm a NaN makes NaNs of its whole head, an infinity zeros of the other
+ * pairs. Any alignment to the type, strides and rotary_dim are taken; prompts are two to three times as fast where the rows of k, q and its output lie on boundaries of 16 bytes
+ * and rotary_dim is a multiple of 16. Can be captured, as wd_kv_append can. */
 int wd_kv_append_rope(wd_kv_cache *c, int layer, const wd_rope *r, const wd_rope_rows *rows, void *stream);
 /* out = softmax(scale q k) v of the step's rows, each against the tokens up to its own (which must have been appended), or the last
  * `window` of them (0 = all). Row i of a sequence's n rows is the token n - 1 - i before its last. out may be q, with the same stride; they

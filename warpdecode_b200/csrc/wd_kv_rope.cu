@@ -6,12 +6,13 @@
 // (2 and up). An angle is made once for all of a block's query heads of a token.
 //
 // Angles are made in turns, position (f_p / 2 pi) in 64 bits less the nearest whole number: in 32 bits the position 131,072 is off by 2^-8 radians. Queries
-// are rotated in F32. Keys in 64 bits, rounded to F32 once: then the code is the same however the sums are ordered, but for one number in 2^25, and the same
+// are rotated in F32, by the sine of that rest rounded to F32 (off by 2^-26 of a turn at most: 1e-7 of an element). Keys in 64 bits, rounded to F32 once: then the code is the same however the sums are ordered, but for one number in 2^25, and the same
 // rows again leave the cache as it is. The rotated keys of a page wait in shared memory for the page's scale, as many tokens at a time as it holds; those
 // of a page that has more are made a second time.
 //
-// Few tokens are a chain of latencies (64 sequences, a token each, 32/8 heads of 128: 9.2 us). Many are bound by instruction issue, at two blocks an SM: 4,000 tokens of
-// 32/8 heads of 64 27 us (57 MB, 8.8 at the memory's rate), 5,003 of 128 by three axes 74, of which the codes of keys and values are 26, the keys' rotation 14 and the queries 34.
+// Few tokens are a chain of latencies (64 sequences, a token each, 32/8 heads of 128: 10.6 us). Many are bound by instruction issue and conversions of 64 bits, at two blocks an SM:
+// 4,000 tokens of 32/8 heads of 64 29 us (57 MB, 8.8 at the memory's rate), 5,003 of 128 by three axes 76, of which the codes of keys and values are 26, the keys' rotation 14 and
+// the queries 34. Every kv head's blocks make the step's angles anew, in each layer.
 #include <cmath>
 #include <memory>
 
@@ -289,7 +290,7 @@ __device__ __forceinline__ void rope_sincos(const double2 *circle, double turn, 
 }
 
 constexpr int kRopeThreads = 256;
-// (APART: all pairs are turned, and are of halves: known when it is compiled. 4,000 tokens of 32 x 64: 27 us for 29)
+// (APART: all pairs are turned, and are of halves: known when it is compiled. 4,000 tokens of 32 x 64: 7 % faster)
 template <class T, bool E4M3, bool APART>
 __global__ void __launch_bounds__(kRopeThreads, 2) kv_rope_rows_kernel(const __grid_constant__ KvRope P) {
     extern __shared__ __align__(16) uint8_t rope_sm[];           // keys: rotated rows; values: the codes of the sub-blocks that the rows touch

@@ -16,8 +16,9 @@
 // A CTA's parts in memory are three units of 128 rows: what it has of an item that began in an earlier one's run; and the sums of the two streams until an
 // item's end, the first of which then holds what it has of an item that ends in a later one's.
 //
-// A tile of 128 rows by 128 tokens takes a CTA 1.75 us at heads of 128, 1.1 at 64: instruction issue (codes to operands, softmax) and exponentials, not memory. 16 trees of 26 rows
-// behind 300 to 6,000 tokens, 32/8 heads of 128: 64 us (12 at the memory's rate; by the kernel of chains 145); 64 rows behind 131,025: 207 to 233 (83 at the tensor cores' rate). There
+// A tile of 128 rows by 128 tokens takes a CTA 1.75 us at heads of 128, 1.1 at 64. 16 trees of 26 rows behind 300 to 6,000 tokens, 32/8 heads of 128: 64 us (12 at the memory's
+// rate; by the kernel of chains 145), of which the beginnings and ends of items are as much as their tiles: latency, with issue slots 29 % busy, tensor cores 17 %, the exponentials' unit
+// 18 %, DRAM 17 %, and stalls on memory (35 %) and at the barriers between an item's parts (27 %); 64 rows behind 131,025: 207 to 233 (83 at the tensor cores' rate). There
 // both row blocks of a head expand the same codes, which the kernel for prompts does once for 256 rows (184): choose_tree() gives it such steps.
 #pragma once
 

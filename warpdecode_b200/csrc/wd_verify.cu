@@ -14,8 +14,10 @@
 // each complete a barrier (550 cycles; behind a barrier of the cluster it is 1,000), and every warp puts them together by the same arithmetic and comes to the same
 // decision, so that nothing is sent back.
 //
-// 64 chains of 5 rows of 151,936 F32, with a draft: 133 us (33 at the memory's rate), bound by the 64-bit terms of rejections and draws; one chain 21 to 27, 2.9 to 3.4 a
-// row and 7 a draw, bound by latency. With rows read from memory by each pass, sums met by a barrier of the cluster, and exp() for the terms 250 and 41.
+// 64 chains of 5 rows of 151,936 F32, with a draft: 137 to 141 us (33 at the memory's rate; DRAM 18 % busy, 1.9 instructions a cycle, the pipe of 64 bits 11 %). 14 clusters of 16 CTAs
+// run at once, and there each holds one row: a CTA waits for its part of the row, then works on it with nothing on its way, 32 us for each further accepted row (16 without a
+// draft). One chain 21 to 32, 3 to 3.5 a row and 7 a draw, bound by latency. With rows read from memory by each pass, sums met by a barrier of the cluster, and exp() for the
+// terms 250 and 41.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -166,7 +168,7 @@ __device__ __forceinline__ int ver_pick(const double (&v)[K], double aim, double
     return from * K + __shfl_sync(0xffffffffu, place, from);
 }
 
-// (three CTAs an SM where there is no draft; with one shared memory has room for two, and they may have the registers)
+// (registers for three CTAs an SM where there is no draft; with one, shared memory has room for two at most, and they may have them)
 template <class T, bool HELD, bool DRAFT>
 __global__ void __launch_bounds__(kVerThreads, DRAFT ? 2 : 3) verify_kernel(const __grid_constant__ VerifyParams P) {
     extern __shared__ __align__(16) uint8_t ver_rows[];
@@ -743,7 +745,7 @@ int verify_of(VerifyParams p, int n_sm, cudaStream_t s) {
     p.stop_at = stop.at;
     p.stop_rank = stop.rank;
     p.stop_warp = stop.warp;
-    // What shared memory holds of the rows: one row where there are many CTAs, two of them an SM; up to four where there are few.
+    // What shared memory holds of the rows: one row where there are more CTAs than SMs (up to 100 KB of it leave room for two of them an SM), up to four where there are fewer.
     const long long run_bytes = static_cast<long long>(p.piece) * 32 * sizeof(T) + 16, slot = run_bytes * kVerWarps * (p.draft ? 2 : 1);
     if (slot > kVerHeld) {
         p.slots = p.run_bytes = 0;
