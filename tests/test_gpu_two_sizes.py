@@ -9,6 +9,31 @@ from warpdecode_b200 import synth
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize("one_launch", [False, True])            # operations by a graph of kernels, or a token by one kernel
+def test_decoders(monkeypatch, one_launch):
+    monkeypatch.setenv("WD_DENSE_TOKEN_KERNEL", str(int(one_launch)))
+
+    def decoder(hidden, heads, kv, ffn, ctx):
+        d = wd.DenseDecoder(hidden, heads, kv, 64, ffn, 96, 1, ctx, 1e-5, 500000.0)
+        d.synth(11, 0.05)
+        return d
+
+    tokens = np.random.Generator(np.random.PCG64(3)).integers(0, 96, 20).astype(np.int32)
+    large = decoder(2048, 32, 8, 8192, 4000)
+    assert (large.kernel_name() == "dense_token_kernel") == one_launch
+    want, _ = large.decode(tokens, 5)
+    small = decoder(512, 8, 2, 1024, 64)
+    of_small, _ = small.decode(tokens, 5)
+    got, _ = large.decode(tokens, 5)
+    assert np.array_equal(got, want)
+    small.close()
+    large.close()
+    again = decoder(512, 8, 2, 1024, 64)
+    got, _ = again.decode(tokens, 5)
+    assert np.array_equal(got, of_small)
+    again.close()
+
+
 @pytest.mark.parametrize("tokens", [1, 4])
 def test_plain_engines(tokens):
     engines = []
