@@ -502,7 +502,9 @@ int wd_token_logprobs(const void *logits_dev, int type, int rows, int vocab, int
  *   drawn from q     accepted where u S q(x) < max(p(x) - c q(x), 0), S = sum max(p - c q, 0); c is 0 at first, and each rejection adds its S to it
  *   without draft    (tokens that were chosen, not drawn) accepted where u (1 - p(R)) < p(x), R the tokens rejected so far, x not among them
  * The first accepted one is the next row. Where there is none, the token behind is drawn from what is left, p without R or max(p - c q, 0), by the number of the
- * sequence's first row: the first id where the running sum is above u times the whole. A drafted token outside of the vocabulary is passed over.
+ * sequence's first row: the first id where the running sum is above u times the whole. A drafted token outside of the vocabulary is passed over. Probabilities below 2^-1000
+ * of the row's largest count as 0. Where nothing is left at all (a draft that is the target, and a token that it cannot have drawn), no further child is accepted and the
+ * token behind is drawn from p.
  *
  *   path_dev[rows]       the accepted rows of each sequence from its first row's place on, counted from that row, itself (0) first; -1 behind them. With the host's
  *                        copy: wd_kv_keep(c, seq, tokens before the step, count, path)

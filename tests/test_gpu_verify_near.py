@@ -29,3 +29,22 @@ def test_a_draft_that_has_one_token_for_many(vocab, gone):
             assert want == token + (np.float64(u) >= sums[token])
             path, count, following = call(target, ints([0, 0]), None, torch.tensor([u, 0.5], device="cuda"), draft)
             assert count[0] == 1 and following[0] == want
+
+
+def test_where_nothing_is_left():
+    """Target and draft are certain of one token and alike; another one that was not drawn from them is turned down, and then nothing is left: the sibling that would have been
+    accepted in front of it is not, and the token behind is the target's."""
+    x = torch.full((3, 300), -60000.0, device="cuda")
+    x[:, 17] = 1.0
+    half = torch.full((3,), 0.5, device="cuda")
+    for tokens, count in (([0, 3, 17], 1), ([0, 17, 3], 2)):
+        path, n, following = call(x, ints(tokens), ints([-1, 0, 0]), half, x.clone())
+        assert n[0] == count and following[0] == 17 and path.tolist() == ([0, -1, -1] if count == 1 else [0, 1, -1])
+
+
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_the_least_probability(with_draft):
+    """2^-995 of the largest is one, 2^-1010 is none: by the number 0 the first that is one is drawn."""
+    x = torch.full((1, 700), -700.0, device="cuda")
+    x[0, 400:], x[0, 600] = -690.0, 0.0
+    assert call(x, ints([0]), None, torch.zeros(1, device="cuda"), x.clone() if with_draft else None)[2][0] == 400
